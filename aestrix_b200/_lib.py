@@ -25,6 +25,11 @@ AEX_ERR_DEVICE = 7
 AEX_DTYPE_BF16 = 0
 AEX_DTYPE_F32 = 1
 
+AEX_FP4_MX = 0
+AEX_FP4_NV = 1
+AEX_ACT_SILU = 0
+AEX_ACT_GELU_TANH = 1
+
 _ERR_NAMES = {
     AEX_ERR_INVALID_ARG: "AEX_ERR_INVALID_ARG",
     AEX_ERR_UNSUPPORTED: "AEX_ERR_UNSUPPORTED",
@@ -69,6 +74,22 @@ class aex_attention_args(C.Structure):
         ("rope_cos", C.c_void_p),
         ("rope_sin", C.c_void_p),
         ("scale", C.c_float),
+    ]
+
+
+class aex_fp4_mm_args(C.Structure):
+    _fields_ = [
+        ("x", C.c_void_p),
+        ("x_dtype", C.c_int),
+        ("ldx", C.c_int64),
+        ("m", C.c_int),
+        ("quantize_x", C.c_int),
+        ("x_scale", C.c_float),
+        ("y", C.c_void_p),
+        ("y_dtype", C.c_int),
+        ("ldy", C.c_int64),
+        ("workspace", C.c_void_p),
+        ("workspace_bytes", C.c_size_t),
     ]
 
 
@@ -119,6 +140,23 @@ _SIGNATURES = [
     ("aex_qweight_dequantize", C.c_int, [_VP, _VP, _VP, _VP]),
     ("aex_qmm", C.c_int, [_VP, _VP, _VP, C.c_int64, C.c_int, _VP, C.c_int64, C.c_int, _VP]),
     ("aex_qmm_ex", C.c_int, [_VP, _VP, _VP, C.c_int, C.c_int64, C.c_int, _VP, C.c_int64, C.c_int, _VP]),
+    ("aex_fp4_quantize", C.c_int,
+     [_VP, _VP, C.c_int, C.c_int64, C.c_int, C.c_int, C.c_int, C.c_float, _VP, _VP, _VP]),
+    ("aex_fp4_dequantize", C.c_int,
+     [_VP, _VP, _VP, C.c_int, C.c_int, C.c_int, C.c_float, _VP, C.c_int, C.c_int64, _VP]),
+    ("aex_fp4weight_create", C.c_int,
+     [_VP, _VP, _VP, C.c_int, C.c_int, C.c_int, C.c_float, C.POINTER(_VP), _VP]),
+    ("aex_fp4weight_destroy", None, [_VP]),
+    ("aex_fp4weight_shape", C.c_int, [_VP, C.POINTER(C.c_int), C.POINTER(C.c_int)]),
+    ("aex_fp4weight_dequantize", C.c_int, [_VP, _VP, _VP, C.c_int, C.c_int64, _VP]),
+    ("aex_fp4_mm_workspace_bytes", C.c_size_t, [_VP, C.c_int, C.c_int]),
+    ("aex_fp4_mm", C.c_int, [_VP, _VP, C.POINTER(aex_fp4_mm_args), _VP]),
+    ("aex_fp4_gated_mm", C.c_int, [_VP, _VP, _VP, C.c_int, C.POINTER(aex_fp4_mm_args), _VP]),
+    ("aex_fp4_mm_dgrad", C.c_int,
+     [_VP, _VP, _VP, C.c_int64, C.c_int, _VP, C.c_int, C.c_int64, _VP]),
+    ("aex_fp4_gated_mm_dgrad_workspace_bytes", C.c_size_t, [_VP, C.c_int]),
+    ("aex_fp4_gated_mm_dgrad", C.c_int,
+     [_VP, _VP, _VP, C.c_int, _VP, C.c_int64, _VP, C.c_int64, C.c_int, _VP, C.c_int64, _VP, C.c_size_t, _VP]),
     ("aex_dit_create", C.c_int, [_VP, C.POINTER(aex_dit_config), C.POINTER(_VP)]),
     ("aex_dit_destroy", None, [_VP]),
     ("aex_dit_load_linear", C.c_int, [_VP, C.c_char_p, _VP, _VP, _VP, C.c_int, C.c_int, _VP]),

@@ -1,0 +1,197 @@
+// fp4.cuh — the microscaled 4-bit form shared by the fp4 kernels: its rounding,
+// its decoding and the tile layout ("records") the products read.
+//
+// A value is code * scale (* one f32 per tensor for nvfp4): e2m1 codes 0, 0.5,
+// 1, 1.5, 2, 3, 4, 6 with a sign bit, and per block of columns one scale byte,
+// mxfp4: 2^(byte - 127) for 32 columns (255: NaN); nvfp4: e4m3 for 16 columns
+// (bit 7 ignored, 0x7F: NaN).
+//
+// Record layout. A matrix is cut into records of 128 rows x 256 columns, zero
+// past its rows (weights only) and columns; record (rt, kb) of a matrix with
+// k_blocks = ceil(k / 256) starts at byte (rt * k_blocks + kb) * record bytes:
+//   [0, 16384)   codes, 128 bytes a row, as the tensor core's 128-byte swizzle
+//                wants them: 16-byte chunk c (columns 32c..32c+31) of row r at
+//                r * 128 + ((c ^ (r & 7)) << 4). Eight codes a 32-bit word, the
+//                nibbles of a word permuted as in the affine layout (nibble i
+//                holds column 2i for i < 4, 2(i - 4) + 1 above), so that one
+//                shift and mask yields two adjacent columns in the halves of a
+//                word. The permutation stays inside 8 columns, hence inside a
+//                block: a product of two matrices in this layout is unchanged.
+//   [16384, ..)  scale bytes in groups of 512, the order the tensor core's
+//                scale operand wants: row r, scale j of the group at
+//                (r % 32) * 16 + (r / 32) * 4 + j. nvfp4: one group per 64
+//                columns (4 groups); mxfp4: one per 128 columns (2 groups).
+// One bulk copy moves a record (both regions are contiguous), and the same
+// bytes serve the block-scaled tensor-core product, the dequantizing GEMM and
+// the small-row kernel.
+#pragma once
+#include "fp4_internal.h"
+#include "sm100.cuh"
+
+namespace aex {
+namespace fp4 {
+
+// ------------------------------------------------------------------ rounding
+// One of the two halves (16 columns) of what a thread quantizes.
+//
+// e2m1 rounding of |x| / unit to nearest, ties to the even code, decided as in
+// real arithmetic although the quotient is not exact in f32: every border lies
+// on the bf16 grid (at most 3 significant bits), so the approximate quotient
+// rounded to bf16 is the border itself whenever it is near one, and the sign
+// of the fused x - border * s * tensor_scale (border * s is exact in f32: 8 + 4
+// bits) says which side x is on; otherwise it lies on the same side of every
+// border as the quotient. The same argument holds for the e4m3 scale (borders
+// of at most 5 bits, border * 6 exact). Requires 2^-100 <= tensor_scale <=
+// 2^100, so that no residual that matters underflows.
+__device__ __forceinline__ float settle(float approx, float border_unit, float tensor_scale, float x) {
+  const float rt = __bfloat162float(__float2bfloat16_rn(approx));
+  const float e = __fmaf_rn(-(rt * border_unit), tensor_scale, x);
+  const int d = (e > 0.f) - (e < 0.f);
+  return __int_as_float(__float_as_int(rt) + d);
+}
+
+// cvt of two magnitudes to e2m1 codes in one byte (a: low nibble).
+__device__ __forceinline__ uint32_t e2m1x2(float a, float b) {
+  uint32_t r;
+  asm("{\n\t.reg .b8 t;\n\t"
+      "cvt.rn.satfinite.e2m1x2.f32 t, %2, %1;\n\t"
+      "cvt.u32.u8 %0, t;\n\t}"
+      : "=r"(r)
+      : "f"(a), "f"(b));
+  return r;
+}
+
+__device__ __forceinline__ uint32_t e4m3_sat(float v) {  // v >= 0, to nearest even, at most 448
+  uint16_t r;
+  asm("cvt.rn.satfinite.e4m3x2.f32 %0, %1, %2;" : "=h"(r) : "f"(0.f), "f"(v));
+  return r & 0xFFu;
+}
+
+// e4m3 byte -> f32 (bit 7 ignored): the bits, shifted into f32 exponent and
+// mantissa, are the value times 2^-120, subnormals included.
+__device__ __forceinline__ float e4m3_to_f32(uint32_t b) {
+  b &= 0x7Fu;
+  const float v = __uint_as_float(b << 20) * 0x1p120f;
+  return b == 0x7Fu ? __uint_as_float(0x7FC00000u) : v;
+}
+
+// E8M0 byte -> f32 (255: NaN; 0: 2^-127, subnormal).
+__device__ __forceinline__ float e8m0_to_f32(uint32_t b) {
+  return b == 0 ? __uint_as_float(0x00400000u) : __uint_as_float(b == 255u ? 0x7FC00000u : b << 23);
+}
+
+template <int kFormat>
+__device__ __forceinline__ float scale_to_f32(uint32_t b) {
+  return kFormat == AEX_FP4_MX ? e8m0_to_f32(b) : e4m3_to_f32(b);
+}
+
+// Quantizes 16 columns v of one row. The lane with the other 16 columns of an
+// mxfp4 block is this lane's neighbour (lane ^ 1); all lanes of a warp call it.
+// codes: two words in the order of the columns (kPermute: of the records).
+// inv_6ts is 1 / (6 tensor_scale) rounded to f32.
+template <int kFormat, bool kPermute>
+__device__ __forceinline__ void quantize16(const float* v, float tensor_scale, float inv_6ts, uint32_t* codes,
+                                           uint32_t* scale_byte) {
+  float amax = 0.f;
+  bool bad = false;
+#pragma unroll
+  for (int i = 0; i < 16; ++i) {
+    amax = fmaxf(amax, fabsf(v[i]));
+    bad |= !(fabsf(v[i]) <= 3.402823466e38f);  // NaN or infinity: the block's scale becomes NaN
+  }
+  if (kFormat == AEX_FP4_MX) {
+    amax = fmaxf(amax, __shfl_xor_sync(0xffffffffu, amax, 1));
+    bad |= __shfl_xor_sync(0xffffffffu, bad ? 1 : 0, 1) != 0;
+  }
+  float q[16];
+  if (kFormat == AEX_FP4_MX) {
+    // floor(log2 amax) - 2, biased: the exponent field less 2 (subnormals, and what is below 2^-125, take byte 0)
+    const int ex = static_cast<int>(__float_as_uint(amax) >> 23);
+    const int byte = max(ex - 2, 0);
+    const float inv = __uint_as_float(static_cast<uint32_t>(254 - byte) << 23);  // 2^(127 - byte), byte <= 252
+    *scale_byte = bad ? 0xFFu : static_cast<uint32_t>(byte);
+#pragma unroll
+    for (int i = 0; i < 16; ++i) q[i] = fabsf(v[i]) * inv;  // exact
+  } else {
+    const uint32_t sb = e4m3_sat(settle(amax * inv_6ts, 6.f, tensor_scale, amax));
+    *scale_byte = bad ? 0x7Fu : sb;
+    const float s = e4m3_to_f32(sb);
+    const float inv = sb ? __frcp_rn(s * tensor_scale) : 0.f;
+#pragma unroll
+    for (int i = 0; i < 16; ++i) q[i] = sb ? settle(fabsf(v[i]) * inv, s, tensor_scale, fabsf(v[i])) : 0.f;
+  }
+#pragma unroll
+  for (int i = 0; i < 16; ++i) q[i] = bad ? 0.f : copysignf(q[i], v[i]);
+#pragma unroll
+  for (int h = 0; h < 2; ++h) {
+    const float* p = q + 8 * h;
+    codes[h] = kPermute ? e2m1x2(p[0], p[2]) | (e2m1x2(p[4], p[6]) << 8) | (e2m1x2(p[1], p[3]) << 16) |
+                              (e2m1x2(p[5], p[7]) << 24)
+                        : e2m1x2(p[0], p[1]) | (e2m1x2(p[2], p[3]) << 8) | (e2m1x2(p[4], p[5]) << 16) |
+                              (e2m1x2(p[6], p[7]) << 24);
+  }
+}
+
+// ------------------------------------------------------------------ decoding
+// Columns (2j, 2j + 1) of a record word as a bf16 pair, times 2^-126: the three
+// magnitude bits of a code, placed at the border of exponent and mantissa, are
+// its value in units of 2^-126 (0.5 is a bf16 subnormal there).
+__device__ __forceinline__ uint32_t code_pair_tiny(uint32_t w, int j) {
+  const uint32_t mag = j == 0 ? w << 6 : j == 1 ? w << 2 : j == 2 ? w >> 2 : w >> 6;
+  return (mag & 0x01C001C0u) | ((w << (12 - 4 * j)) & 0x80008000u);
+}
+
+__device__ __forceinline__ uint32_t mul_bf16x2(uint32_t a, uint32_t b) {
+  uint32_t d;
+  asm("mul.rn.bf16x2 %0, %1, %2;" : "=r"(d) : "r"(a), "r"(b));
+  return d;
+}
+
+constexpr uint32_t kBf16x2_2p126 = 0x7E807E80u;  // 2^126 in both halves
+
+// The scale as the bf16 pair that decode_pair multiplies by. nvfp4: s * 2^119
+// (at most 1.75 * 2^127), so that one multiplication takes the pair from
+// 2^-126 to 2^-7 times its value, exactly (2 + 4 significant bits);
+// the products undo the 2^-7. mxfp4: 2^e itself (0: subnormal; 255: NaN).
+template <int kFormat>
+__device__ __forceinline__ uint32_t scale_pair(uint32_t byte) {
+  if (kFormat == AEX_FP4_MX) {
+    const uint32_t b = byte == 0 ? 0x0040u : byte == 255u ? 0x7FC0u : byte << 7;
+    return b | (b << 16);
+  }
+  const float s = e4m3_to_f32(byte) * 0x1p119f;
+  return __byte_perm(__float_as_uint(s), 0, 0x3232);
+}
+
+// What the decoded pairs are to be multiplied by in the end.
+template <int kFormat>
+__host__ __device__ constexpr float decode_unit() {
+  return kFormat == AEX_FP4_MX ? 1.f : 128.f;
+}
+
+template <int kFormat>
+__device__ __forceinline__ uint32_t decode_pair(uint32_t w, int j, uint32_t scale2) {
+  uint32_t p = code_pair_tiny(w, j);
+  if (kFormat == AEX_FP4_MX) p = mul_bf16x2(p, kBf16x2_2p126);  // the exponents of mxfp4 do not fit one step
+  return mul_bf16x2(p, scale2);
+}
+
+// -------------------------------------------------------------- activation
+// act(g) = g * sigmoid(z): silu z = g; gelu (tanh form) z = sqrt(8 / pi) (g + 0.044715 g^3), since
+// (1 + tanh(y)) / 2 = sigmoid(2 y).
+__device__ __forceinline__ float sigmoid_arg(float g, int activation) {
+  constexpr float kA = 1.5957691216057308f;  // sqrt(8 / pi)
+  return activation == AEX_ACT_SILU ? g : kA * fmaf(0.044715f * g * g, g, g);
+}
+__device__ __forceinline__ float sigmoid_arg_slope(float g, int activation) {
+  constexpr float kA = 1.5957691216057308f;
+  return activation == AEX_ACT_SILU ? 1.f : kA * fmaf(3.f * 0.044715f * g, g, 1.f);
+}
+
+template <bool kFast>
+__device__ __forceinline__ float sigmoid(float z) {
+  return kFast ? __fdividef(1.f, 1.f + __expf(-z)) : 1.f / (1.f + expf(-z));
+}
+
+}  // namespace fp4
+}  // namespace aex

@@ -1,0 +1,156 @@
+// fp4_api.cpp — argument checks and dispatch of the products with microscaled
+// 4-bit weights.
+#include "fp4_internal.h"
+
+namespace aex {
+namespace {
+
+int check_weight(aex_ctx* ctx, const aex_fp4weight* w, const char* name) {
+  if (!w) return set_error(ctx, AEX_ERR_INVALID_ARG, "%s is NULL", name);
+  if (w->device != ctx->device) return set_error(ctx, AEX_ERR_INVALID_ARG, "%s lives on another device", name);
+  return AEX_OK;
+}
+
+int check_pair(aex_ctx* ctx, const aex_fp4weight* g, const aex_fp4weight* u, int activation) {
+  if (int r = check_weight(ctx, g, "w_gate")) return r;
+  if (int r = check_weight(ctx, u, "w_up")) return r;
+  if (g->n != u->n || g->k != u->k || g->format != u->format)
+    return set_error(ctx, AEX_ERR_INVALID_ARG, "w_gate and w_up must have one shape and format");
+  if (activation != AEX_ACT_SILU && activation != AEX_ACT_GELU_TANH)
+    return set_error(ctx, AEX_ERR_INVALID_ARG, "activation must be AEX_ACT_SILU or AEX_ACT_GELU_TANH");
+  return AEX_OK;
+}
+
+int check_out(aex_ctx* ctx, const char* name, const void* y, int dtype, int64_t ld, int cols) {
+  if (!y) return set_error(ctx, AEX_ERR_INVALID_ARG, "%s is NULL", name);
+  if (dtype != AEX_DTYPE_BF16 && dtype != AEX_DTYPE_F32)
+    return set_error(ctx, AEX_ERR_INVALID_ARG, "%s: dtype must be AEX_DTYPE_BF16 or AEX_DTYPE_F32", name);
+  if ((reinterpret_cast<uintptr_t>(y) & (dtype == AEX_DTYPE_F32 ? 3 : 1)) || ld < cols)
+    return set_error(ctx, AEX_ERR_INVALID_ARG, "%s must be aligned to its element with a row pitch of at least %d", name,
+                     cols);
+  return AEX_OK;
+}
+
+int check_workspace(aex_ctx* ctx, const void* p, size_t have, size_t need) {
+  if (need && (!p || have < need || (reinterpret_cast<uintptr_t>(p) & 255)))
+    return set_error(ctx, AEX_ERR_INVALID_ARG, "workspace: %zu bytes, 256-byte aligned, are needed", need);
+  return AEX_OK;
+}
+
+size_t records_bytes(const aex_fp4weight* w, int m) {
+  const size_t tiles = (static_cast<size_t>(m) + fp4::kRecRows - 1) / fp4::kRecRows;
+  return tiles * w->k_blocks * fp4::rec_bytes(w->format);
+}
+
+size_t round256(size_t v) { return (v + 255) & ~size_t{255}; }
+
+int run(aex_ctx* ctx, const aex_fp4weight* w0, const aex_fp4weight* w1, int activation, const aex_fp4_mm_args* a,
+        aex_stream stream) {
+  if (!a) return set_error(ctx, AEX_ERR_INVALID_ARG, "args is NULL");
+  if (a->m <= 0) return set_error(ctx, AEX_ERR_INVALID_ARG, "m must be positive");
+  if (int r = fp4::check_matrix(ctx, "x", a->x, a->x_dtype, a->ldx, a->m, w0->k)) return r;
+  if (int r = check_out(ctx, "y", a->y, a->y_dtype, a->ldy, w0->n)) return r;
+  const bool f32 = a->x_dtype == AEX_DTYPE_F32;
+  if (a->quantize_x != 0 && a->quantize_x != 1)
+    return set_error(ctx, AEX_ERR_INVALID_ARG, "quantize_x must be 0 or 1");
+  if (a->quantize_x)
+    if (int r = fp4::check_format(ctx, w0->format, a->x_scale)) return r;
+  if (f32 && !a->quantize_x && a->m > fp4::kSmallRows)
+    return set_error(ctx, AEX_ERR_UNSUPPORTED, "f32 activations without quantize_x are supported for m <= %d",
+                     fp4::kSmallRows);
+  if (int r = check_workspace(ctx, a->workspace, a->workspace_bytes,
+                              aex_fp4_mm_workspace_bytes(w0, a->m, a->quantize_x)))
+    return r;
+  DeviceGuard dev(ctx);
+  if (dev.rc) return dev.rc;
+  fp4::Job j{};
+  j.w0 = w0;
+  j.w1 = w1;
+  j.activation = activation;
+  j.x = a->x;
+  j.x_f32 = f32;
+  j.ldx = a->ldx;
+  j.m = a->m;
+  j.quantize = a->quantize_x != 0;
+  j.x_scale = j.quantize ? a->x_scale : 1.f;
+  j.y = a->y;
+  j.y_f32 = a->y_dtype == AEX_DTYPE_F32;
+  j.ldy = a->ldy;
+  j.workspace = static_cast<uint8_t*>(a->workspace);
+  auto s = static_cast<cudaStream_t>(stream);
+  if (j.m <= fp4::kSmallRows) return fp4::run_small(ctx, j, s);
+  if (j.quantize) {
+    if (int r = fp4::quantize_records(ctx, j.x, j.x_f32, j.ldx, j.m, w0->k, w0->format, j.x_scale, j.workspace, s))
+      return r;
+    return fp4::run_block(ctx, j, s);
+  }
+  return fp4::run_gemm(ctx, j, s);
+}
+
+}  // namespace
+}  // namespace aex
+
+extern "C" {
+
+size_t aex_fp4_mm_workspace_bytes(const aex_fp4weight* w, int m, int quantize_x) {
+  if (!w || m <= aex::fp4::kSmallRows || !quantize_x) return 0;
+  return aex::records_bytes(w, m);
+}
+
+int aex_fp4_mm(aex_ctx* ctx, const aex_fp4weight* w, const aex_fp4_mm_args* args, aex_stream stream) {
+  using namespace aex;
+  if (!ctx) return set_error(ctx, AEX_ERR_INVALID_ARG, "NULL ctx");
+  if (int r = check_weight(ctx, w, "w")) return r;
+  return run(ctx, w, nullptr, AEX_ACT_SILU, args, stream);
+}
+
+int aex_fp4_gated_mm(aex_ctx* ctx, const aex_fp4weight* w_gate, const aex_fp4weight* w_up, int activation,
+                     const aex_fp4_mm_args* args, aex_stream stream) {
+  using namespace aex;
+  if (!ctx) return set_error(ctx, AEX_ERR_INVALID_ARG, "NULL ctx");
+  if (int r = check_pair(ctx, w_gate, w_up, activation)) return r;
+  return run(ctx, w_gate, w_up, activation, args, stream);
+}
+
+int aex_fp4_mm_dgrad(aex_ctx* ctx, const aex_fp4weight* w, const void* dy, int64_t lddy, int m, void* dx,
+                     int dx_dtype, int64_t lddx, aex_stream stream) {
+  using namespace aex;
+  if (!ctx) return set_error(ctx, AEX_ERR_INVALID_ARG, "NULL ctx");
+  if (int r = check_weight(ctx, w, "w")) return r;
+  if (int r = fp4::check_matrix(ctx, "dy", dy, AEX_DTYPE_BF16, lddy, m, w->n)) return r;
+  if (int r = check_out(ctx, "dx", dx, dx_dtype, lddx, w->k)) return r;
+  DeviceGuard dev(ctx);
+  if (dev.rc) return dev.rc;
+  return fp4::run_dgrad(ctx, w, nullptr, dy, lddy, nullptr, 0, m, w->tensor_scale, dx, dx_dtype == AEX_DTYPE_F32, lddx,
+                        static_cast<cudaStream_t>(stream));
+}
+
+size_t aex_fp4_gated_mm_dgrad_workspace_bytes(const aex_fp4weight* w_gate, int m) {
+  if (!w_gate || m <= 0) return 0;
+  // dg and du, bf16, rows padded to 16 bytes
+  return 2 * aex::round256(static_cast<size_t>(m) * ((static_cast<size_t>(w_gate->n) + 7) / 8 * 8) * 2);
+}
+
+int aex_fp4_gated_mm_dgrad(aex_ctx* ctx, const aex_fp4weight* w_gate, const aex_fp4weight* w_up, int activation,
+                           const void* x, int64_t ldx, const void* dh, int64_t lddh, int m, void* dx, int64_t lddx,
+                           void* workspace, size_t workspace_bytes, aex_stream stream) {
+  using namespace aex;
+  if (!ctx) return set_error(ctx, AEX_ERR_INVALID_ARG, "NULL ctx");
+  if (int r = check_pair(ctx, w_gate, w_up, activation)) return r;
+  if (int r = fp4::check_matrix(ctx, "x", x, AEX_DTYPE_BF16, ldx, m, w_gate->k)) return r;
+  if (int r = fp4::check_matrix(ctx, "dh", dh, AEX_DTYPE_BF16, lddh, m, w_gate->n)) return r;
+  if (int r = check_out(ctx, "dx", dx, AEX_DTYPE_BF16, lddx, w_gate->k)) return r;
+  const size_t need = aex_fp4_gated_mm_dgrad_workspace_bytes(w_gate, m);
+  if (int r = check_workspace(ctx, workspace, workspace_bytes, need)) return r;
+  DeviceGuard dev(ctx);
+  if (dev.rc) return dev.rc;
+  auto s = static_cast<cudaStream_t>(stream);
+  // The tensor scales go into dg and du, so that one accumulator takes both products.
+  const int64_t ld = (static_cast<int64_t>(w_gate->n) + 7) / 8 * 8;
+  auto* dg = static_cast<uint16_t*>(workspace);
+  auto* du = dg + need / 4;
+  if (int r = fp4::run_gated_grad(ctx, w_gate, w_up, activation, x, ldx, m, dh, lddh, dg, du, ld, s)) return r;
+  return fp4::run_dgrad(ctx, w_gate, w_up, dg, ld, du, ld, m, 1.f, dx, false, lddx, s);
+}
+
+}  // extern "C"

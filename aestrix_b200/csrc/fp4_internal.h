@@ -1,0 +1,99 @@
+// fp4_internal.h — host-side pieces shared by the translation units of the
+// microscaled 4-bit operators.
+#pragma once
+#ifdef __CUDACC__
+#define AEX_HD __host__ __device__
+#else
+#define AEX_HD
+#endif
+#include "internal.h"
+
+struct aex_fp4weight {
+  int device = 0;
+  int n = 0, k = 0;
+  int format = AEX_FP4_NV;
+  float tensor_scale = 1.f;
+  int n_tiles = 0;           // ceil(n / 128)
+  int k_blocks = 0;          // ceil(k / 256)
+  uint8_t* records = nullptr;
+  size_t bytes = 0;
+};
+
+namespace aex {
+
+// Makes the context's device current and puts the caller's back on leaving.
+struct DeviceGuard {
+  int prev = -1, rc = AEX_OK;
+  bool switched = false;
+  explicit DeviceGuard(aex_ctx* ctx) {
+    cudaError_t e = cudaGetDevice(&prev);
+    if (e == cudaSuccess && prev != ctx->device) {
+      e = cudaSetDevice(ctx->device);
+      switched = e == cudaSuccess;
+    }
+    if (e != cudaSuccess) rc = cuda_error(ctx, e, "selecting the context's device");
+  }
+  ~DeviceGuard() {
+    if (switched) cudaSetDevice(prev);
+  }
+  DeviceGuard(const DeviceGuard&) = delete;
+  DeviceGuard& operator=(const DeviceGuard&) = delete;
+};
+
+namespace fp4 {
+
+constexpr int kRecRows = 128;
+constexpr int kRecK = 256;
+constexpr int kRecCodes = kRecRows * kRecK / 2;  // 16384
+
+AEX_HD constexpr int block_of(int format) { return format == AEX_FP4_MX ? 32 : 16; }
+AEX_HD constexpr int rec_scales(int format) { return kRecRows * kRecK / block_of(format); }
+AEX_HD constexpr int rec_bytes(int format) { return kRecCodes + rec_scales(format); }
+
+// Byte offset of row r's scale group g (4 consecutive scales) inside a record.
+AEX_HD constexpr int scale_off(int r, int g) {
+  return kRecCodes + g * 512 + (r & 31) * 16 + (r >> 5) * 4;
+}
+
+
+int check_format(aex_ctx* ctx, int format, float tensor_scale);
+// A row-major matrix that is read or written in 16-byte vectors.
+int check_matrix(aex_ctx* ctx, const char* name, const void* p, int dtype, int64_t ld, int rows, int cols);
+
+// x [m, k] -> records (columns padded to whole records with zeros; rows past m left as they are).
+int quantize_records(aex_ctx* ctx, const void* x, bool f32, int64_t ldx, int m, int k, int format, float ts,
+                     uint8_t* records, cudaStream_t s);
+
+// One product (w1 NULL) or gated projection act(x w0^T) * (x w1^T).
+struct Job {
+  const aex_fp4weight* w0;
+  const aex_fp4weight* w1;
+  int activation;
+  const void* x;
+  bool x_f32;
+  int64_t ldx;
+  int m;
+  bool quantize;
+  float x_scale;
+  void* y;
+  bool y_f32;
+  int64_t ldy;
+  uint8_t* workspace;  // records of the quantized x
+};
+// Up to kSmallRows rows; no workspace.
+constexpr int kSmallRows = 16;
+int run_small(aex_ctx* ctx, const Job& j, cudaStream_t s);
+// Any number of bf16 rows: dequantizing GEMM.
+int run_gemm(aex_ctx* ctx, const Job& j, cudaStream_t s);
+// Quantized rows (records in j.workspace): block-scaled GEMM.
+int run_block(aex_ctx* ctx, const Job& j, cudaStream_t s);
+// dx = alpha (d0 . W0 + d1 . W1) (w1, d1 NULL: one product), d bf16 [m, n].
+int run_dgrad(aex_ctx* ctx, const aex_fp4weight* w0, const aex_fp4weight* w1, const void* d0, int64_t ld0,
+              const void* d1, int64_t ld1, int m, float alpha, void* dx, bool dx_f32, int64_t lddx, cudaStream_t s);
+// dg = ts_g dh u act'(g), du = ts_u dh act(g), bf16 [m, n] at row pitch ld, g and u from x.
+int run_gated_grad(aex_ctx* ctx, const aex_fp4weight* wg, const aex_fp4weight* wu, int activation, const void* x,
+                   int64_t ldx, int m, const void* dh, int64_t lddh, uint16_t* dg, uint16_t* du, int64_t ld,
+                   cudaStream_t s);
+
+}  // namespace fp4
+}  // namespace aex

@@ -1,0 +1,385 @@
+// fp4_quant.cu — to the microscaled 4-bit form and back, and the weight handle
+// of the fp4 products.
+//
+// All three kernels are streams (HBM-bound): a thread owns 16 columns of a row,
+// which is one nvfp4 block or, with its neighbouring lane, one mxfp4 block, so
+// the block's largest magnitude needs no shared memory and every element is
+// read and written once.
+#include <algorithm>
+#include <new>
+
+#include "fp4.cuh"
+#include "fp4_internal.h"
+
+namespace aex {
+namespace fp4 {
+
+constexpr int kThreads = 256;
+
+// 16 elements of a row (16-byte aligned) as f32.
+template <bool kF32>
+__device__ __forceinline__ void load16(const void* x, int64_t at, float* v) {
+  if (kF32) {
+    const float4* p = reinterpret_cast<const float4*>(static_cast<const float*>(x) + at);
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      const float4 f = __ldg(p + i);
+      v[4 * i] = f.x;
+      v[4 * i + 1] = f.y;
+      v[4 * i + 2] = f.z;
+      v[4 * i + 3] = f.w;
+    }
+  } else {
+    const uint4* p = reinterpret_cast<const uint4*>(static_cast<const uint16_t*>(x) + at);
+#pragma unroll
+    for (int i = 0; i < 2; ++i) {
+      const uint4 u = __ldg(p + i);
+      const uint32_t w[4] = {u.x, u.y, u.z, u.w};
+#pragma unroll
+      for (int j = 0; j < 4; ++j) {
+        v[8 * i + 2 * j] = bf16lo_to_f32(w[j]);
+        v[8 * i + 2 * j + 1] = bf16hi_to_f32(w[j]);
+      }
+    }
+  }
+}
+
+// x [rows, k] -> codes [rows, k/2] and scales [rows, k/block] (kRecords: the
+// record layout in `codes`, columns padded with zeros to whole records; rows
+// past the last are left as they are). `upr` units of 16 columns a row (even);
+// rows * upr < 2^31 (the host slices).
+template <int kFormat, bool kF32, bool kRecords>
+__global__ void __launch_bounds__(kThreads) quantize_kernel(const void* __restrict__ x, int64_t ldx, int rows, int k,
+                                                            uint32_t upr, float tensor_scale, float inv_6ts,
+                                                            uint8_t* __restrict__ codes,
+                                                            uint8_t* __restrict__ scales) {
+  const uint32_t u = blockIdx.x * kThreads + threadIdx.x;
+  const uint32_t row = u / upr, c = u % upr;  // an mxfp4 pair (u even, u + 1) is one row's
+  const bool live = row < static_cast<uint32_t>(rows);
+  const int col = static_cast<int>(c) * 16;
+  float v[16];
+#pragma unroll
+  for (int i = 0; i < 16; ++i) v[i] = 0.f;
+  if (live && col < k) load16<kF32>(x, static_cast<int64_t>(row) * ldx + col, v);
+  uint32_t w[2], sb;
+  quantize16<kFormat, kRecords>(v, tensor_scale, inv_6ts, w, &sb);
+  if (!live) return;
+  if (kRecords) {
+    const int r = static_cast<int>(row % kRecRows);
+    uint8_t* rec = codes + (static_cast<size_t>(row / kRecRows) * (upr / 16) + c / 16) * rec_bytes(kFormat);
+    const int cu = static_cast<int>(c % 16);  // unit inside the record
+    *reinterpret_cast<uint2*>(rec + r * 128 + (((cu >> 1) ^ (r & 7)) << 4) + (cu & 1) * 8) = make_uint2(w[0], w[1]);
+    if (kFormat == AEX_FP4_NV)
+      rec[scale_off(r, cu >> 2) + (cu & 3)] = static_cast<uint8_t>(sb);
+    else if (!(cu & 1))
+      rec[scale_off(r, cu >> 3) + ((cu >> 1) & 3)] = static_cast<uint8_t>(sb);
+  } else {
+    reinterpret_cast<uint2*>(codes)[u] = make_uint2(w[0], w[1]);
+    if (kFormat == AEX_FP4_NV)
+      scales[u] = static_cast<uint8_t>(sb);
+    else if (!(u & 1))
+      scales[u >> 1] = static_cast<uint8_t>(sb);
+  }
+}
+
+// Two codes' product with the block scale is exact in f32 (2 + 4 bits); the
+// tensor scale is then one rounding for an f32 output. For bf16 that f32 is
+// rounded to odd first, so that the second rounding sees which side of a tie
+// the product is on.
+template <bool kF32>
+__device__ __forceinline__ float scaled(float cs, float tensor_scale) {
+  if (kF32) return cs * tensor_scale;
+  const float p = __fmul_rz(cs, tensor_scale);
+  return __fmaf_rn(cs, tensor_scale, -p) != 0.f && fabsf(p) <= 3.402823466e38f
+             ? __uint_as_float(__float_as_uint(p) | 1u)
+             : p;
+}
+
+// Codes -> values, out [rows, k] (row pitch ldo). kRecords: from the record
+// layout. One thread per 16 columns.
+template <int kFormat, bool kF32, bool kRecords>
+__global__ void __launch_bounds__(kThreads) dequantize_kernel(const uint8_t* __restrict__ codes,
+                                                              const uint8_t* __restrict__ scales, int rows,
+                                                              uint32_t upr, int k_blocks, float tensor_scale,
+                                                              void* __restrict__ out, int64_t ldo) {
+  const uint32_t u = blockIdx.x * kThreads + threadIdx.x;
+  const uint32_t row = u / upr, c = u % upr;
+  if (row >= static_cast<uint32_t>(rows)) return;
+  uint2 w;
+  uint32_t sb;
+  if (kRecords) {
+    const int r = static_cast<int>(row % kRecRows), cu = static_cast<int>(c % 16);
+    const uint8_t* rec =
+        codes + (static_cast<size_t>(row / kRecRows) * k_blocks + c / 16) * rec_bytes(kFormat);
+    w = *reinterpret_cast<const uint2*>(rec + r * 128 + (((cu >> 1) ^ (r & 7)) << 4) + (cu & 1) * 8);
+    sb = kFormat == AEX_FP4_NV ? rec[scale_off(r, cu >> 2) + (cu & 3)] : rec[scale_off(r, cu >> 3) + ((cu >> 1) & 3)];
+  } else {
+    w = __ldg(reinterpret_cast<const uint2*>(codes) + u);
+    sb = __ldg(scales + (kFormat == AEX_FP4_NV ? u : u >> 1));
+  }
+  const float s = scale_to_f32<kFormat>(sb);
+  float v[16];
+#pragma unroll
+  for (int h = 0; h < 2; ++h) {
+    const uint32_t word = h ? w.y : w.x;
+#pragma unroll
+    for (int i = 0; i < 8; ++i) {
+      const int nib = kRecords ? ((i & 1) ? 4 + (i >> 1) : (i >> 1)) : i;
+      const uint32_t cd = word >> (4 * nib);
+      const float mag = __uint_as_float((cd & 7u) << 22) * 0x1p126f;
+      v[8 * h + i] = scaled<kF32>(__uint_as_float(__float_as_uint(mag) | ((cd & 8u) << 28)) * s, tensor_scale);
+    }
+  }
+  const int64_t at = static_cast<int64_t>(row) * ldo + static_cast<int64_t>(c) * 16;
+  if (kF32) {
+    float4* o = reinterpret_cast<float4*>(static_cast<float*>(out) + at);
+#pragma unroll
+    for (int i = 0; i < 4; ++i) o[i] = make_float4(v[4 * i], v[4 * i + 1], v[4 * i + 2], v[4 * i + 3]);
+  } else {
+    uint4* o = reinterpret_cast<uint4*>(static_cast<uint16_t*>(out) + at);
+#pragma unroll
+    for (int i = 0; i < 2; ++i)
+      o[i] = make_uint4(pack_bf16x2(v[8 * i], v[8 * i + 1]), pack_bf16x2(v[8 * i + 2], v[8 * i + 3]),
+                        pack_bf16x2(v[8 * i + 4], v[8 * i + 5]), pack_bf16x2(v[8 * i + 6], v[8 * i + 7]));
+  }
+}
+
+__device__ __forceinline__ uint32_t nibble_compress(uint32_t x) {  // 4 bytes < 16 -> 4 nibbles
+  x = (x | (x >> 4)) & 0x00FF00FFu;
+  return (x | (x >> 8)) & 0x0000FFFFu;
+}
+__device__ __forceinline__ uint32_t permute_word(uint32_t w) {
+  return nibble_compress(w & 0x0F0F0F0Fu) | (nibble_compress((w >> 4) & 0x0F0F0F0Fu) << 16);
+}
+
+// Rows as stored (codes, scales) -> records, zero past n and k. One CTA per
+// record, a thread per 16 columns at a time.
+template <int kFormat>
+__global__ void __launch_bounds__(kThreads) records_kernel(const uint8_t* __restrict__ codes,
+                                                           const uint8_t* __restrict__ scales, int n, int k,
+                                                           int k_blocks, uint8_t* __restrict__ records) {
+  const int rt = static_cast<int>(blockIdx.x / k_blocks), kb = static_cast<int>(blockIdx.x % k_blocks);
+  uint8_t* rec = records + static_cast<size_t>(blockIdx.x) * rec_bytes(kFormat);
+  constexpr int kBlock = block_of(kFormat);
+  for (int i = threadIdx.x; i < kRecRows * 16; i += kThreads) {
+    const int r = i >> 4, cu = i & 15;
+    const int64_t row = static_cast<int64_t>(rt) * kRecRows + r;
+    const int col = kb * kRecK + cu * 16;
+    uint2 w = make_uint2(0, 0);
+    uint32_t sb = 0;
+    if (row < n && col < k) {
+      w = __ldg(reinterpret_cast<const uint2*>(codes + row * (k / 2) + col / 2));
+      sb = scales[row * (k / kBlock) + col / kBlock];
+      if (kFormat == AEX_FP4_NV) sb &= 0x7Fu;
+    }
+    *reinterpret_cast<uint2*>(rec + r * 128 + (((cu >> 1) ^ (r & 7)) << 4) + (cu & 1) * 8) =
+        make_uint2(permute_word(w.x), permute_word(w.y));
+    if (kFormat == AEX_FP4_NV)
+      rec[scale_off(r, cu >> 2) + (cu & 3)] = static_cast<uint8_t>(sb);
+    else if (!(cu & 1))
+      rec[scale_off(r, cu >> 3) + ((cu >> 1) & 3)] = static_cast<uint8_t>(sb);
+  }
+}
+
+namespace {
+
+template <int kFormat, bool kF32, bool kRecords>
+int launch_quantize(aex_ctx* ctx, const void* x, int64_t ldx, int rows, int k, float ts, uint8_t* codes,
+                    uint8_t* scales, cudaStream_t s) {
+  const uint32_t upr = kRecords ? static_cast<uint32_t>((k + kRecK - 1) / kRecK * 16) : static_cast<uint32_t>(k / 16);
+  // 32-bit unit indices: slices of whole 128-row tiles below 2^31 units each
+  const int64_t step = std::max<int64_t>(kRecRows, (int64_t{1} << 30) / upr / kRecRows * kRecRows);
+  const float inv = static_cast<float>(1.0 / (6.0 * static_cast<double>(ts)));
+  for (int64_t r0 = 0; r0 < rows; r0 += step) {
+    const int nr = static_cast<int>(std::min<int64_t>(step, rows - r0));
+    const uint32_t blocks = static_cast<uint32_t>((static_cast<int64_t>(nr) * upr + kThreads - 1) / kThreads);
+    const uint8_t* xs = static_cast<const uint8_t*>(x) + r0 * ldx * (kF32 ? 4 : 2);
+    uint8_t* cs = kRecords ? codes + static_cast<size_t>(r0 / kRecRows) * (upr / 16) * rec_bytes(kFormat)
+                           : codes + static_cast<size_t>(r0) * upr * 8;
+    uint8_t* ss = kRecords ? nullptr : scales + static_cast<size_t>(r0) * (k / block_of(kFormat));
+    quantize_kernel<kFormat, kF32, kRecords><<<blocks, kThreads, 0, s>>>(xs, ldx, nr, k, upr, ts, inv, cs, ss);
+    if (int r = check_launch(ctx, "fp4 quantize_kernel")) return r;
+  }
+  return AEX_OK;
+}
+
+template <int kFormat, bool kF32, bool kRecords>
+int launch_dequantize(aex_ctx* ctx, const uint8_t* codes, const uint8_t* scales, int rows, int k, float ts, void* out,
+                      int64_t ldo, cudaStream_t s) {
+  const uint32_t upr = static_cast<uint32_t>(k / 16);
+  const int k_blocks = (k + kRecK - 1) / kRecK;
+  const int64_t step = std::max<int64_t>(kRecRows, (int64_t{1} << 30) / upr / kRecRows * kRecRows);
+  for (int64_t r0 = 0; r0 < rows; r0 += step) {
+    const int nr = static_cast<int>(std::min<int64_t>(step, rows - r0));
+    const uint32_t blocks = static_cast<uint32_t>((static_cast<int64_t>(nr) * upr + kThreads - 1) / kThreads);
+    const uint8_t* cs = kRecords ? codes + static_cast<size_t>(r0 / kRecRows) * k_blocks * rec_bytes(kFormat)
+                                 : codes + static_cast<size_t>(r0) * upr * 8;
+    const uint8_t* ss = kRecords ? nullptr : scales + static_cast<size_t>(r0) * (k / block_of(kFormat));
+    dequantize_kernel<kFormat, kF32, kRecords><<<blocks, kThreads, 0, s>>>(
+        cs, ss, nr, upr, k_blocks, ts, static_cast<uint8_t*>(out) + r0 * ldo * (kF32 ? 4 : 2), ldo);
+    if (int r = check_launch(ctx, "fp4 dequantize_kernel")) return r;
+  }
+  return AEX_OK;
+}
+
+template <bool kRecords>
+int dispatch_dequantize(aex_ctx* ctx, const uint8_t* codes, const uint8_t* scales, int rows, int k, int format,
+                        float ts, void* out, int out_dtype, int64_t ldo, cudaStream_t s) {
+  const bool f32 = out_dtype == AEX_DTYPE_F32;
+  if (format == AEX_FP4_MX)
+    return f32 ? launch_dequantize<AEX_FP4_MX, true, kRecords>(ctx, codes, scales, rows, k, ts, out, ldo, s)
+               : launch_dequantize<AEX_FP4_MX, false, kRecords>(ctx, codes, scales, rows, k, ts, out, ldo, s);
+  return f32 ? launch_dequantize<AEX_FP4_NV, true, kRecords>(ctx, codes, scales, rows, k, ts, out, ldo, s)
+             : launch_dequantize<AEX_FP4_NV, false, kRecords>(ctx, codes, scales, rows, k, ts, out, ldo, s);
+}
+
+}  // namespace
+
+int check_format(aex_ctx* ctx, int format, float tensor_scale) {
+  if (format != AEX_FP4_MX && format != AEX_FP4_NV)
+    return set_error(ctx, AEX_ERR_INVALID_ARG, "format must be AEX_FP4_MX or AEX_FP4_NV");
+  if (format == AEX_FP4_MX && tensor_scale != 1.f)
+    return set_error(ctx, AEX_ERR_INVALID_ARG, "mxfp4 has no tensor scale: it must be 1");
+  if (!(tensor_scale >= 0x1p-100f && tensor_scale <= 0x1p100f))
+    return set_error(ctx, AEX_ERR_INVALID_ARG, "tensor_scale must lie in [2^-100, 2^100]");
+  return AEX_OK;
+}
+
+int check_matrix(aex_ctx* ctx, const char* name, const void* p, int dtype, int64_t ld, int rows, int cols) {
+  if (!p) return set_error(ctx, AEX_ERR_INVALID_ARG, "%s is NULL", name);
+  if (dtype != AEX_DTYPE_BF16 && dtype != AEX_DTYPE_F32)
+    return set_error(ctx, AEX_ERR_INVALID_ARG, "%s: dtype must be AEX_DTYPE_BF16 or AEX_DTYPE_F32", name);
+  if (rows <= 0) return set_error(ctx, AEX_ERR_INVALID_ARG, "%s: the number of rows must be positive", name);
+  if ((reinterpret_cast<uintptr_t>(p) & 15) || ld < cols || ld % (dtype == AEX_DTYPE_F32 ? 4 : 8))
+    return set_error(ctx, AEX_ERR_INVALID_ARG,
+                     "%s must be 16-byte aligned, its row pitch at least %d elements and a multiple of 16 bytes", name,
+                     cols);
+  return AEX_OK;
+}
+
+int quantize_records(aex_ctx* ctx, const void* x, bool f32, int64_t ldx, int m, int k, int format, float ts,
+                     uint8_t* records, cudaStream_t s) {
+  if (format == AEX_FP4_MX)
+    return f32 ? launch_quantize<AEX_FP4_MX, true, true>(ctx, x, ldx, m, k, ts, records, nullptr, s)
+               : launch_quantize<AEX_FP4_MX, false, true>(ctx, x, ldx, m, k, ts, records, nullptr, s);
+  return f32 ? launch_quantize<AEX_FP4_NV, true, true>(ctx, x, ldx, m, k, ts, records, nullptr, s)
+             : launch_quantize<AEX_FP4_NV, false, true>(ctx, x, ldx, m, k, ts, records, nullptr, s);
+}
+
+}  // namespace fp4
+}  // namespace aex
+
+extern "C" {
+
+int aex_fp4_quantize(aex_ctx* ctx, const void* x, int x_dtype, int64_t ldx, int rows, int k, int format,
+                     float tensor_scale, uint8_t* codes, uint8_t* scales, aex_stream stream) {
+  using namespace aex;
+  if (!ctx) return set_error(ctx, AEX_ERR_INVALID_ARG, "NULL ctx");
+  if (int r = fp4::check_format(ctx, format, tensor_scale)) return r;
+  if (k <= 0 || k % 32) return set_error(ctx, AEX_ERR_INVALID_ARG, "k must be a positive multiple of 32 (k=%d)", k);
+  if (int r = fp4::check_matrix(ctx, "x", x, x_dtype, ldx, rows, k)) return r;
+  if (!codes || !scales || (reinterpret_cast<uintptr_t>(codes) & 15))
+    return set_error(ctx, AEX_ERR_INVALID_ARG, "codes (16-byte aligned) and scales must not be NULL");
+  DeviceGuard dev(ctx);
+  if (dev.rc) return dev.rc;
+  auto s = static_cast<cudaStream_t>(stream);
+  const bool f32 = x_dtype == AEX_DTYPE_F32;
+  if (format == AEX_FP4_MX)
+    return f32 ? fp4::launch_quantize<AEX_FP4_MX, true, false>(ctx, x, ldx, rows, k, tensor_scale, codes, scales, s)
+               : fp4::launch_quantize<AEX_FP4_MX, false, false>(ctx, x, ldx, rows, k, tensor_scale, codes, scales, s);
+  return f32 ? fp4::launch_quantize<AEX_FP4_NV, true, false>(ctx, x, ldx, rows, k, tensor_scale, codes, scales, s)
+             : fp4::launch_quantize<AEX_FP4_NV, false, false>(ctx, x, ldx, rows, k, tensor_scale, codes, scales, s);
+}
+
+int aex_fp4_dequantize(aex_ctx* ctx, const uint8_t* codes, const uint8_t* scales, int rows, int k, int format,
+                       float tensor_scale, void* out, int out_dtype, int64_t ldo, aex_stream stream) {
+  using namespace aex;
+  if (!ctx) return set_error(ctx, AEX_ERR_INVALID_ARG, "NULL ctx");
+  if (int r = fp4::check_format(ctx, format, tensor_scale)) return r;
+  if (k <= 0 || k % 32) return set_error(ctx, AEX_ERR_INVALID_ARG, "k must be a positive multiple of 32 (k=%d)", k);
+  if (!codes || !scales || (reinterpret_cast<uintptr_t>(codes) & 15))
+    return set_error(ctx, AEX_ERR_INVALID_ARG, "codes (16-byte aligned) and scales must not be NULL");
+  if (int r = fp4::check_matrix(ctx, "out", out, out_dtype, ldo, rows, k)) return r;
+  DeviceGuard dev(ctx);
+  if (dev.rc) return dev.rc;
+  return fp4::dispatch_dequantize<false>(ctx, codes, scales, rows, k, format, tensor_scale, out, out_dtype, ldo,
+                                         static_cast<cudaStream_t>(stream));
+}
+
+int aex_fp4weight_create(aex_ctx* ctx, const uint8_t* codes, const uint8_t* scales, int n, int k, int format,
+                         float tensor_scale, aex_fp4weight** out, aex_stream stream) {
+  using namespace aex;
+  if (!ctx || !out) return set_error(ctx, AEX_ERR_INVALID_ARG, "NULL ctx/out");
+  *out = nullptr;
+  if (int r = fp4::check_format(ctx, format, tensor_scale)) return r;
+  if (n <= 0 || k <= 0 || k % 32)
+    return set_error(ctx, AEX_ERR_INVALID_ARG, "n must be positive and k a positive multiple of 32 (n=%d k=%d)", n, k);
+  if (!codes || !scales || (reinterpret_cast<uintptr_t>(codes) & 15))
+    return set_error(ctx, AEX_ERR_INVALID_ARG, "codes (16-byte aligned) and scales must not be NULL");
+  const int64_t n_tiles = (static_cast<int64_t>(n) + fp4::kRecRows - 1) / fp4::kRecRows;
+  const int64_t k_blocks = (static_cast<int64_t>(k) + fp4::kRecK - 1) / fp4::kRecK;
+  if (n_tiles * k_blocks > 0x7FFFFFFF)
+    return set_error(ctx, AEX_ERR_UNSUPPORTED, "fp4 weight of %d x %d is too large", n, k);
+  DeviceGuard dev(ctx);
+  if (dev.rc) return dev.rc;
+  auto* w = new (std::nothrow) aex_fp4weight();
+  if (!w) return set_error(ctx, AEX_ERR_OOM, "host allocation failed");
+  w->device = ctx->device;
+  w->n = n;
+  w->k = k;
+  w->format = format;
+  w->tensor_scale = tensor_scale;
+  w->n_tiles = static_cast<int>(n_tiles);
+  w->k_blocks = static_cast<int>(k_blocks);
+  w->bytes = static_cast<size_t>(n_tiles * k_blocks) * fp4::rec_bytes(format);
+  cudaError_t e = cudaMalloc(&w->records, w->bytes);
+  if (e != cudaSuccess) {
+    delete w;
+    return cuda_error(ctx, e, "cudaMalloc(fp4 records)");
+  }
+  const auto blocks = static_cast<unsigned>(n_tiles * k_blocks);
+  auto s = static_cast<cudaStream_t>(stream);
+  if (format == AEX_FP4_MX)
+    fp4::records_kernel<AEX_FP4_MX><<<blocks, fp4::kThreads, 0, s>>>(codes, scales, n, k, w->k_blocks, w->records);
+  else
+    fp4::records_kernel<AEX_FP4_NV><<<blocks, fp4::kThreads, 0, s>>>(codes, scales, n, k, w->k_blocks, w->records);
+  if (int r = check_launch(ctx, "fp4 records_kernel")) {
+    cudaFree(w->records);
+    delete w;
+    return r;
+  }
+  *out = w;
+  return AEX_OK;
+}
+
+void aex_fp4weight_destroy(aex_fp4weight* w) {
+  if (!w) return;
+  int cur = -1;
+  cudaGetDevice(&cur);
+  cudaSetDevice(w->device);
+  cudaDeviceSynchronize();
+  cudaFree(w->records);
+  if (cur >= 0) cudaSetDevice(cur);
+  delete w;
+}
+
+int aex_fp4weight_shape(const aex_fp4weight* w, int* n, int* k) {
+  if (!w || !n || !k) return AEX_ERR_INVALID_ARG;
+  *n = w->n;
+  *k = w->k;
+  return AEX_OK;
+}
+
+int aex_fp4weight_dequantize(aex_ctx* ctx, const aex_fp4weight* w, void* out, int out_dtype, int64_t ldo,
+                             aex_stream stream) {
+  using namespace aex;
+  if (!ctx || !w) return set_error(ctx, AEX_ERR_INVALID_ARG, "NULL argument");
+  if (ctx->device != w->device) return set_error(ctx, AEX_ERR_INVALID_ARG, "weight lives on another device");
+  if (int r = fp4::check_matrix(ctx, "out", out, out_dtype, ldo, w->n, w->k)) return r;
+  DeviceGuard dev(ctx);
+  if (dev.rc) return dev.rc;
+  return fp4::dispatch_dequantize<true>(ctx, w->records, nullptr, w->n, w->k, w->format, w->tensor_scale, out,
+                                        out_dtype, ldo, static_cast<cudaStream_t>(stream));
+}
+
+}  // extern "C"

@@ -205,6 +205,105 @@ int aex_qmm(aex_ctx* ctx, const aex_qweight* w, const void* x, int64_t ldx, int 
 int aex_qmm_ex(aex_ctx* ctx, const aex_qweight* w, const void* x, int x_dtype, int64_t ldx, int m, void* y,
                int64_t ldy, int y_dtype, aex_stream stream);
 
+/* ------------------------------------- microscaled 4-bit floating point */
+
+/* The other 4-bit forms an MLX pack comes in (mode "mxfp4" and "nvfp4"; the
+ * reference loads the affine one above): e2m1 codes, two to a byte with the
+ * even column in the low nibble (the uint32 words of a pack, unchanged), and
+ * one scale byte per block of columns.
+ *   AEX_FP4_MX  blocks of 32, E8M0 scale 2^(byte - 127), 255 is NaN; no tensor
+ *               scale (pass 1).
+ *   AEX_FP4_NV  blocks of 16, e4m3 scale (bit 7 ignored, 0x7F is NaN), times
+ *               one f32 per tensor in [2^-100, 2^100].
+ * k is a multiple of 32 throughout; codes are 16-byte aligned. None of these
+ * calls uses memory of the context: what a call needs is in its arguments, so
+ * calls on different streams, and graphs that hold them, do not touch one
+ * another. They leave the calling thread's current device as it was. No output
+ * may overlap an input or the workspace. */
+#define AEX_FP4_MX 0
+#define AEX_FP4_NV 1
+#define AEX_ACT_SILU 0
+#define AEX_ACT_GELU_TANH 1
+
+typedef struct aex_fp4weight aex_fp4weight;
+
+/* x [rows, k] (bf16 or f32, 16-byte aligned, row pitch ldx elements, a
+ * multiple of 16 bytes) -> codes [rows, k/2] and scales [rows, k/block], both
+ * contiguous. A block's scale: AEX_FP4_MX 2^(floor(log2 amax) - 2), byte 0 for
+ * amax below 2^-125; AEX_FP4_NV amax / (6 tensor_scale) rounded to e4m3 (to
+ * nearest even, at most 448). Codes: x / (scale * tensor_scale) to the nearest
+ * e2m1 value, ties to the even code, at most 6; both roundings are those of
+ * the exact quotient. A block with scale 0 has codes 0; a block that holds an
+ * infinity or NaN gets a NaN scale. No reference counterpart (its packs are
+ * quantized offline). */
+int aex_fp4_quantize(aex_ctx* ctx, const void* x, int x_dtype, int64_t ldx, int rows, int k, int format,
+                     float tensor_scale, uint8_t* codes, uint8_t* scales, aex_stream stream);
+
+/* out [rows, k] (bf16 or f32, 16-byte aligned, row pitch ldo) = code * scale *
+ * tensor_scale, rounded once. The microscaled sibling of aex_dequantize_mlx. */
+int aex_fp4_dequantize(aex_ctx* ctx, const uint8_t* codes, const uint8_t* scales, int rows, int k, int format,
+                       float tensor_scale, void* out, int out_dtype, int64_t ldo, aex_stream stream);
+
+/* Lay a weight [n, k] out for the products below (device pointers as
+ * aex_fp4_quantize writes them, or as they stand in a pack). The handle owns
+ * its device memory until aex_fp4weight_destroy; the arrays may be freed once
+ * the stream has passed the call. The microscaled sibling of
+ * aex_qweight_create. */
+int aex_fp4weight_create(aex_ctx* ctx, const uint8_t* codes, const uint8_t* scales, int n, int k, int format,
+                         float tensor_scale, aex_fp4weight** out, aex_stream stream);
+void aex_fp4weight_destroy(aex_fp4weight* w);
+int aex_fp4weight_shape(const aex_fp4weight* w, int* n, int* k);
+/* out [n, k] as aex_fp4_dequantize. */
+int aex_fp4weight_dequantize(aex_ctx* ctx, const aex_fp4weight* w, void* out, int out_dtype, int64_t ldo,
+                             aex_stream stream);
+
+/* Activations and result of one product. */
+typedef struct aex_fp4_mm_args {
+  const void* x;       /* [m, k], 16-byte aligned */
+  int x_dtype;         /* AEX_DTYPE_BF16, or AEX_DTYPE_F32 where m <= 16 or quantize_x */
+  int64_t ldx;         /* row pitch in elements, a multiple of 16 bytes, >= k */
+  int m;
+  int quantize_x;      /* 1: x goes through aex_fp4_quantize's rounding in the weight's format first */
+  float x_scale;       /* its tensor scale (AEX_FP4_NV; 1 for AEX_FP4_MX); unused without quantize_x */
+  void* y;             /* [m, n], aligned to its element */
+  int y_dtype;         /* AEX_DTYPE_BF16 or AEX_DTYPE_F32 */
+  int64_t ldy;         /* row pitch in elements, >= n */
+  void* workspace;     /* aex_fp4_mm_workspace_bytes, 256-byte aligned; NULL where that is 0. Its contents need
+                        * not survive between calls; calls that may overlap must not share it */
+  size_t workspace_bytes;
+} aex_fp4_mm_args;
+
+/* Workspace of aex_fp4_mm and aex_fp4_gated_mm for m rows. 0 for bad arguments. */
+size_t aex_fp4_mm_workspace_bytes(const aex_fp4weight* w, int m, int quantize_x);
+
+/* y[m, n] = x[m, k] . W[n, k]^T, f32 accumulation, one rounding at the end.
+ * The microscaled sibling of aex_qmm_ex. */
+int aex_fp4_mm(aex_ctx* ctx, const aex_fp4weight* w, const aex_fp4_mm_args* args, aex_stream stream);
+
+/* y[m, n] = act(x . Wg^T) * (x . Wu^T), the gated feed-forward projection:
+ * both products, the activation (AEX_ACT_SILU, or AEX_ACT_GELU_TANH
+ * g (1 + tanh(sqrt(2/pi) (g + 0.044715 g^3))) / 2) and the product in one
+ * kernel, f32 until the one rounding of y. Wg and Wu have one shape and format.
+ * Reference: linear_in -> silu(g) * u, Sources/ImarelloDiT/FeedForward.swift:11-24. */
+int aex_fp4_gated_mm(aex_ctx* ctx, const aex_fp4weight* w_gate, const aex_fp4weight* w_up, int activation,
+                     const aex_fp4_mm_args* args, aex_stream stream);
+
+/* Gradient of aex_fp4_mm (without quantize_x) with respect to x: dx[m, k] =
+ * dy[m, n] . W[n, k]. dy bf16, 16-byte aligned, row pitch lddy a multiple of 8
+ * elements; dx bf16 or f32, aligned to its element, row pitch lddx. A 4-bit
+ * weight is frozen: it has no gradient. */
+int aex_fp4_mm_dgrad(aex_ctx* ctx, const aex_fp4weight* w, const void* dy, int64_t lddy, int m, void* dx,
+                     int dx_dtype, int64_t lddx, aex_stream stream);
+
+/* Gradient of aex_fp4_gated_mm (without quantize_x) with respect to x, from
+ * dh[m, n]: g and u are computed again from x (nothing is kept from the forward
+ * pass), dg = dh u act'(g) and du = dh act(g), each rounded to bf16 as operands
+ * of dx = dg . Wg + du . Wu (f32 accumulation). x, dh bf16 as dy above; dx bf16. */
+size_t aex_fp4_gated_mm_dgrad_workspace_bytes(const aex_fp4weight* w_gate, int m);
+int aex_fp4_gated_mm_dgrad(aex_ctx* ctx, const aex_fp4weight* w_gate, const aex_fp4weight* w_up, int activation,
+                           const void* x, int64_t ldx, const void* dh, int64_t lddh, int m, void* dx, int64_t lddx,
+                           void* workspace, size_t workspace_bytes, aex_stream stream);
+
 /* ------------------------------------------------------------ DiT engine */
 
 /* The FLUX.2-klein transformer denoise step on one device: the direct

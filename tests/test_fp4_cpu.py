@@ -1,0 +1,111 @@
+"""CPU side of the microscaled 4-bit operators: the float64 checker against values worked out by
+hand, and the refusals that need no device."""
+import ctypes as C
+
+import numpy as np
+import pytest
+import torch
+
+from aestrix_b200 import _lib, fp4
+from oracle import fp4_ref as R
+
+
+def test_checker_known_values():
+    # mxfp4: amax 5 -> 2^(2 - 2) = 1; codes to nearest, ties to the even code
+    x = np.zeros((1, 32))
+    x[0, :9] = [5.0, 0.25, 0.26, 0.75, -1.25, 1.75, 2.5, 3.5, -0.1]
+    codes, scales = R.quantize(x, "mxfp4")
+    assert scales[0, 0] == 127
+    assert list(codes[0, :9]) == [6, 0, 1, 2, 8 | 2, 4, 4, 6, 8]
+    # nvfp4: amax 6 * 448 -> the largest scale; a block of zeros -> scale 0
+    x = np.zeros((1, 32))
+    x[0, 0] = 6 * 448.0
+    x[0, 1] = 448.0 * 0.75
+    codes, scales = R.quantize(x, "nvfp4")
+    assert list(scales[0]) == [0x7E, 0] and list(codes[0, :2]) == [7, 2]
+    assert R.values(codes, scales, "nvfp4")[0, 1] == 448.0
+    # rounding of the scale to e4m3: 17 lies half-way between 16 and 18 and goes to the even mantissa
+    x[0, 0], x[0, 1] = 6 * 17.0, 0.0
+    assert R.scale_values(R.quantize(x, "nvfp4")[1], "nvfp4")[0, 0] == 16.0
+    # the tensor's scale divides out
+    a, b = R.quantize(x, "nvfp4"), R.quantize(x * 0.125, "nvfp4", 0.125)
+    assert np.array_equal(a[0], b[0]) and np.array_equal(a[1], b[1])
+
+
+def test_checker_e4m3_and_packing():
+    assert R.E4M3[1] == 2.0**-9 and R.E4M3[8] == 2.0**-6 and R.E4M3[126] == 448.0
+    assert (np.diff(R.E4M3) > 0).all()
+    t = torch.arange(127, dtype=torch.uint8).view(torch.float8_e4m3fn).double().numpy()
+    assert np.array_equal(t, R.E4M3)
+    codes = np.arange(32, dtype=np.uint8).reshape(1, 32) % 16
+    assert R.pack(codes)[0, 0] == 0x10
+    assert np.array_equal(R.unpack(R.pack(codes)), codes)
+
+
+def test_checker_keeps_a_nan_to_its_block():
+    x = np.ones((1, 64))
+    x[0, 40] = np.nan
+    for mode in ("mxfp4", "nvfp4"):
+        v = R.values(*R.quantize(x, mode), mode)
+        bad = np.isnan(v[0])
+        lo = 40 // R.BLOCK[mode] * R.BLOCK[mode]
+        assert bad[lo:lo + R.BLOCK[mode]].all() and bad.sum() == R.BLOCK[mode]
+
+
+@pytest.mark.parametrize("act", ["silu", "gelu_tanh"])
+def test_checker_activation_slope(act):
+    g = np.linspace(-9, 9, 181)
+    h = 1e-6
+    slope = (R.act(g + h, act)[0] - R.act(g - h, act)[0]) / (2 * h)
+    assert np.abs(slope - R.act(g, act)[1]).max() < 1e-8
+    assert np.abs(R.act(g, act)[1]).max() < 1.2  # the bound the gated tests use
+
+
+def test_refusals_without_a_device():
+    x = torch.zeros(4, 64, dtype=torch.bfloat16)
+    with pytest.raises(ValueError, match="mode"):
+        fp4.quantize(x, "int4")
+    with pytest.raises(TypeError, match="CUDA"):
+        fp4.quantize(x)
+    with pytest.raises(TypeError):
+        fp4.quantize(x.to(torch.float16))
+    with pytest.raises(TypeError):
+        fp4.quantize(x.view(2, 2, 64))
+    codes, scales = torch.zeros(4, 32, dtype=torch.uint8), torch.zeros(4, 4, dtype=torch.uint8)
+    with pytest.raises(TypeError, match="CUDA"):
+        fp4.dequantize(codes, scales, "nvfp4")
+    with pytest.raises(TypeError, match="CUDA"):
+        fp4.FP4Weight(codes, scales, "nvfp4")
+    with pytest.raises(TypeError, match="FP4Weight"):
+        fp4.fp4_mm(x, codes)
+    with pytest.raises(TypeError, match="FP4Weight"):
+        fp4.fp4_gated_mm(x, None, None)
+    with pytest.raises(TypeError, match="FP4Weight"):
+        fp4.fp4_mm_dgrad(x, codes)
+    with pytest.raises(TypeError, match="FP4Weight"):
+        fp4.fp4_gated_mm_dgrad(x, x, None, None)
+
+
+def test_c_entry_points_refuse_null():
+    L, bad = _lib.lib(), _lib.AEX_ERR_INVALID_ARG
+    a = _lib.aex_fp4_mm_args()
+    h = C.c_void_p()
+    assert L.aex_fp4_quantize(None, None, 0, 32, 1, 32, 0, 1.0, None, None, None) == bad
+    assert L.aex_fp4_dequantize(None, None, None, 1, 32, 0, 1.0, None, 0, 32, None) == bad
+    assert L.aex_fp4weight_create(None, None, None, 1, 32, 0, 1.0, C.byref(h), None) == bad and not h.value
+    assert L.aex_fp4weight_dequantize(None, None, None, 0, 32, None) == bad
+    assert L.aex_fp4weight_shape(None, None, None) == bad
+    assert L.aex_fp4_mm(None, None, C.byref(a), None) == bad
+    assert L.aex_fp4_gated_mm(None, None, None, 0, C.byref(a), None) == bad
+    assert L.aex_fp4_mm_dgrad(None, None, None, 8, 1, None, 0, 32, None) == bad
+    assert L.aex_fp4_gated_mm_dgrad(None, None, None, 0, None, 32, None, 8, 1, None, 32, None, 0, None) == bad
+    assert L.aex_fp4_mm_workspace_bytes(None, 100, 1) == 0
+    assert L.aex_fp4_gated_mm_dgrad_workspace_bytes(None, 100) == 0
+    L.aex_fp4weight_destroy(None)
+
+
+def test_args_struct_matches_the_header():
+    """The ctypes structure has the C structure's layout (offsets worked out from the header's types)."""
+    f = _lib.aex_fp4_mm_args
+    assert [getattr(f, n).offset for n, _ in f._fields_] == [0, 8, 16, 24, 28, 32, 40, 48, 56, 64, 72]
+    assert C.sizeof(f) == 80
