@@ -32,8 +32,6 @@ namespace aex {
 namespace fp4 {
 
 // ------------------------------------------------------------------ rounding
-// One of the two halves (16 columns) of what a thread quantizes.
-//
 // e2m1 rounding of |x| / unit to nearest, ties to the even code, decided as in
 // real arithmetic although the quotient is not exact in f32: every border lies
 // on the bf16 grid (at most 3 significant bits), so the approximate quotient
@@ -85,51 +83,53 @@ __device__ __forceinline__ float scale_to_f32(uint32_t b) {
   return kFormat == AEX_FP4_MX ? e8m0_to_f32(b) : e4m3_to_f32(b);
 }
 
-// Quantizes 16 columns v of one row. The lane with the other 16 columns of an
-// mxfp4 block is this lane's neighbour (lane ^ 1); all lanes of a warp call it.
-// codes: two words in the order of the columns (kPermute: of the records).
+// Scale byte and code magnitudes of kN (8 or 16) columns v of one row; the
+// block's other columns are with this lane's neighbours (lane ^ 1, and for a
+// fourth part lane ^ 2); all lanes of a warp call it. q: v over the block's
+// unit, settled on its side of every border, ready for the conversion to e2m1.
 // inv_6ts is 1 / (6 tensor_scale) rounded to f32.
-template <int kFormat, bool kPermute>
-__device__ __forceinline__ void quantize16(const float* v, float tensor_scale, float inv_6ts, uint32_t* codes,
-                                           uint32_t* scale_byte) {
+template <int kFormat, int kN>
+__device__ __forceinline__ uint32_t quantize_cols(const float* v, float tensor_scale, float inv_6ts, float* q) {
   float amax = 0.f;
   bool bad = false;
 #pragma unroll
-  for (int i = 0; i < 16; ++i) {
+  for (int i = 0; i < kN; ++i) {
     amax = fmaxf(amax, fabsf(v[i]));
     bad |= !(fabsf(v[i]) <= 3.402823466e38f);  // NaN or infinity: the block's scale becomes NaN
   }
-  if (kFormat == AEX_FP4_MX) {
-    amax = fmaxf(amax, __shfl_xor_sync(0xffffffffu, amax, 1));
-    bad |= __shfl_xor_sync(0xffffffffu, bad ? 1 : 0, 1) != 0;
+#pragma unroll
+  for (int o = 1; o < block_of(kFormat) / kN; o <<= 1) {
+    amax = fmaxf(amax, __shfl_xor_sync(0xffffffffu, amax, o));
+    bad |= __shfl_xor_sync(0xffffffffu, bad ? 1 : 0, o) != 0;
   }
-  float q[16];
+  uint32_t byte;
   if (kFormat == AEX_FP4_MX) {
     // floor(log2 amax) - 2, biased: the exponent field less 2 (subnormals, and what is below 2^-125, take byte 0)
-    const int ex = static_cast<int>(__float_as_uint(amax) >> 23);
-    const int byte = max(ex - 2, 0);
-    const float inv = __uint_as_float(static_cast<uint32_t>(254 - byte) << 23);  // 2^(127 - byte), byte <= 252
-    *scale_byte = bad ? 0xFFu : static_cast<uint32_t>(byte);
+    const int ex = max(static_cast<int>(__float_as_uint(amax) >> 23) - 2, 0);
+    const float inv = __uint_as_float(static_cast<uint32_t>(254 - ex) << 23);  // 2^(127 - ex), ex <= 252
+    byte = bad ? 0xFFu : static_cast<uint32_t>(ex);
 #pragma unroll
-    for (int i = 0; i < 16; ++i) q[i] = fabsf(v[i]) * inv;  // exact
+    for (int i = 0; i < kN; ++i) q[i] = fabsf(v[i]) * inv;  // exact
   } else {
     const uint32_t sb = e4m3_sat(settle(amax * inv_6ts, 6.f, tensor_scale, amax));
-    *scale_byte = bad ? 0x7Fu : sb;
+    byte = bad ? 0x7Fu : sb;
     const float s = e4m3_to_f32(sb);
     const float inv = sb ? __frcp_rn(s * tensor_scale) : 0.f;
 #pragma unroll
-    for (int i = 0; i < 16; ++i) q[i] = sb ? settle(fabsf(v[i]) * inv, s, tensor_scale, fabsf(v[i])) : 0.f;
+    for (int i = 0; i < kN; ++i) q[i] = sb ? settle(fabsf(v[i]) * inv, s, tensor_scale, fabsf(v[i])) : 0.f;
   }
 #pragma unroll
-  for (int i = 0; i < 16; ++i) q[i] = bad ? 0.f : copysignf(q[i], v[i]);
-#pragma unroll
-  for (int h = 0; h < 2; ++h) {
-    const float* p = q + 8 * h;
-    codes[h] = kPermute ? e2m1x2(p[0], p[2]) | (e2m1x2(p[4], p[6]) << 8) | (e2m1x2(p[1], p[3]) << 16) |
-                              (e2m1x2(p[5], p[7]) << 24)
-                        : e2m1x2(p[0], p[1]) | (e2m1x2(p[2], p[3]) << 8) | (e2m1x2(p[4], p[5]) << 16) |
-                              (e2m1x2(p[6], p[7]) << 24);
-  }
+  for (int i = 0; i < kN; ++i) q[i] = bad ? 0.f : copysignf(q[i], v[i]);
+  return byte;
+}
+
+// Eight code magnitudes as one word, in the order of the columns or (kPermute) of the records.
+template <bool kPermute>
+__device__ __forceinline__ uint32_t code_word(const float* p) {
+  return kPermute ? e2m1x2(p[0], p[2]) | (e2m1x2(p[4], p[6]) << 8) | (e2m1x2(p[1], p[3]) << 16) |
+                        (e2m1x2(p[5], p[7]) << 24)
+                  : e2m1x2(p[0], p[1]) | (e2m1x2(p[2], p[3]) << 8) | (e2m1x2(p[4], p[5]) << 16) |
+                        (e2m1x2(p[6], p[7]) << 24);
 }
 
 // ------------------------------------------------------------------ decoding

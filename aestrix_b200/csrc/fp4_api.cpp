@@ -55,9 +55,9 @@ int run(aex_ctx* ctx, const aex_fp4weight* w0, const aex_fp4weight* w1, int acti
     return set_error(ctx, AEX_ERR_INVALID_ARG, "quantize_x must be 0 or 1");
   if (a->quantize_x)
     if (int r = fp4::check_format(ctx, w0->format, a->x_scale)) return r;
-  if (f32 && !a->quantize_x && a->m > fp4::kSmallRows)
+  if (f32 && !a->quantize_x && a->m > fp4::kSmallRowsF32)
     return set_error(ctx, AEX_ERR_UNSUPPORTED, "f32 activations without quantize_x are supported for m <= %d",
-                     fp4::kSmallRows);
+                     fp4::kSmallRowsF32);
   if (int r = check_workspace(ctx, a->workspace, a->workspace_bytes,
                               aex_fp4_mm_workspace_bytes(w0, a->m, a->quantize_x)))
     return r;

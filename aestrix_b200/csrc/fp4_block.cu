@@ -310,7 +310,8 @@ int launch_block(aex_ctx* ctx, const Job& j, cudaStream_t s) {
   p.o.vec = vec_ok(j.y, j.ldy, j.y_f32);
   p.status = ctx->d_status;
   auto kern = block_kernel<kFormat, kGated>;
-  AEX_CUDA_TRY(ctx, cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, kBSmem));
+  static SmemOptIn opt_in;
+  if (int r = opt_in(ctx, reinterpret_cast<const void*>(kern), kBSmem)) return r;
   cudaLaunchConfig_t cfg{};
   cfg.blockDim = dim3(kBThreads, 1, 1);
   cfg.dynamicSmemBytes = kBSmem;

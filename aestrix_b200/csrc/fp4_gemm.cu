@@ -425,7 +425,8 @@ int launch_gemm(aex_ctx* ctx, const CUtensorMap& tm0, const CUtensorMap& tm1, Ge
   p.tiles = static_cast<int>(tiles);
   p.status = ctx->d_status;
   auto kern = gemm_kernel<kFormat, kMode>;
-  AEX_CUDA_TRY(ctx, cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, kGSmem));
+  static SmemOptIn opt_in;
+  if (int r = opt_in(ctx, reinterpret_cast<const void*>(kern), kGSmem)) return r;
   cudaLaunchConfig_t cfg{};
   cfg.blockDim = dim3(kGThreads, 1, 1);
   cfg.dynamicSmemBytes = kGSmem;

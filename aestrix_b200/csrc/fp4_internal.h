@@ -6,6 +6,8 @@
 #else
 #define AEX_HD
 #endif
+#include <atomic>
+
 #include "internal.h"
 
 struct aex_fp4weight {
@@ -38,6 +40,18 @@ struct DeviceGuard {
   }
   DeviceGuard(const DeviceGuard&) = delete;
   DeviceGuard& operator=(const DeviceGuard&) = delete;
+};
+
+// cudaFuncSetAttribute(maximum dynamic shared memory), once per kernel and device: it costs a good part of a launch.
+struct SmemOptIn {
+  std::atomic<uint64_t> done{0};
+  int operator()(aex_ctx* ctx, const void* kernel, int bytes) {
+    const uint64_t bit = uint64_t{1} << (ctx->device & 63);
+    if (ctx->device < 64 && (done.load(std::memory_order_acquire) & bit)) return AEX_OK;
+    AEX_CUDA_TRY(ctx, cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, bytes));
+    done.fetch_or(bit, std::memory_order_release);
+    return AEX_OK;
+  }
 };
 
 namespace fp4 {
@@ -80,8 +94,10 @@ struct Job {
   int64_t ldy;
   uint8_t* workspace;  // records of the quantized x
 };
-// Up to kSmallRows rows; no workspace.
-constexpr int kSmallRows = 16;
+// The few-rows kernel takes up to 48 columns of its 8-column operand: rows that are bf16 or quantized, or f32 rows at
+// three columns each. No workspace.
+constexpr int kSmallRows = 32;
+constexpr int kSmallRowsF32 = 16;
 int run_small(aex_ctx* ctx, const Job& j, cudaStream_t s);
 // Any number of bf16 rows: dequantizing GEMM.
 int run_gemm(aex_ctx* ctx, const Job& j, cudaStream_t s);

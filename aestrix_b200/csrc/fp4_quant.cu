@@ -61,8 +61,9 @@ __global__ void __launch_bounds__(kThreads) quantize_kernel(const void* __restri
 #pragma unroll
   for (int i = 0; i < 16; ++i) v[i] = 0.f;
   if (live && col < k) load16<kF32>(x, static_cast<int64_t>(row) * ldx + col, v);
-  uint32_t w[2], sb;
-  quantize16<kFormat, kRecords>(v, tensor_scale, inv_6ts, w, &sb);
+  float q[16];
+  const uint32_t sb = quantize_cols<kFormat, 16>(v, tensor_scale, inv_6ts, q);
+  const uint32_t w[2] = {code_word<kRecords>(q), code_word<kRecords>(q + 8)};
   if (!live) return;
   if (kRecords) {
     const int r = static_cast<int>(row % kRecRows);

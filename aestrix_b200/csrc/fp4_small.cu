@@ -1,23 +1,39 @@
-// fp4_small.cu — products of few rows (at most 16) with microscaled 4-bit
-// weights: y = x W^T, or act(x Wg^T) * (x Wu^T).
+// fp4_small.cu — products of few rows (at most 32; f32 rows 16) with microscaled
+// 4-bit weights: y = x W^T, or act(x Wg^T) * (x Wu^T).
 //
 // HBM-bound: the weight is read once. A CTA owns 128 weight rows (one column of
 // records; the gated form one of each weight) and one K split of a
 // thread-block cluster; a producer warp streams its records through a ring of
-// shared-memory slots by bulk copies, eight compute warps take 16 rows each.
-// The codes are decoded to bf16 pairs in registers (value * scale is exact:
-// at most 6 significant bits) and multiplied on the tensor cores by
+// shared-memory slots by bulk copies, sixteen compute warps take 16 rows of
+// every other record each (eight, with every record, left the SM's schedulers
+// idle over half of the time: two warps each). The number of slots is even, or
+// enough for every record: a slot's records then all belong to one of the two
+// halves of the warps, which so sees every phase of the slot's barriers.
+// The codes are decoded in registers and multiplied on the tensor cores by
 // mma.sync.m16n8k16 with the activations as the 8-column operand: at 1 to 8
-// rows the work on a decoded pair is the same, and the decoding (2.5 integer
-// and 1 multiply instructions per pair) is what the issue slots go to. tcgen05
-// would need its operand written back to shared memory, which at these row
-// counts costs more than the product.
-// Sums: the tensor core's f32 accumulators truncate, so each 256-column block
-// is summed there (16 steps) and then added to f32 registers; the K splits are
-// added in rank order through distributed shared memory (no atomics).
-// f32 activations enter as three bf16 columns (the top, middle and low 8 bits
-// of the significand, by truncation: their sum is x exactly), so the products
-// stay exact. Quantized activations are rounded while they are staged.
+// rows the work on a decoded pair is the same, and the decoding is what the
+// issue slots go to. (tcgen05 would need its operand written back to shared
+// memory, which at these row counts costs more than the product.)
+//
+// Decoding to f16, not bf16: a pair of e2m1 codes becomes an f16 pair in one
+// conversion, against four integer operations to a bf16 pair (measured on one
+// SM sub-partition: two cycles each). So the activations have to be f16 too.
+// Each row's 256 columns of a record are scaled by a power of two that puts the
+// largest magnitude into [2^14, 2^15); 11 bits of significand down to 2^-24
+// then hold bf16 values over 31 binades exactly. Whether they do is checked
+// value by value as they are staged; a record's columns for which they do not
+// (or that hold an infinity or NaN) are staged as bf16 and take the integer
+// decoding, which covers every value. Both products are exact.
+// f32 rows take three columns: 11 + 11 + 2 bits of the significand, each with a
+// scale of its own (bf16: 8 + 8 + 8 bits, by truncation).
+// Scales: nvfp4, 16 columns: into the decoded pair (2 + 4 bits, exact in f16);
+// mxfp4, 32 columns: exponents that f16 does not hold, so one column block is
+// summed over two products and enters the f32 sum times its scale.
+// Sums: the tensor core's f32 accumulators truncate, so a record is summed
+// there (16 steps) and then added to f32 registers; the K splits are added in
+// rank order through distributed shared memory (no atomics).
+#include <cuda_fp16.h>
+
 #include <algorithm>
 
 #include "fp4.cuh"
@@ -26,9 +42,9 @@
 namespace aex {
 namespace fp4 {
 
-constexpr int kSmWarps = 8;
-constexpr int kSmCompute = kSmWarps * 32;
-constexpr int kSmThreads = kSmCompute + 32;
+// Compute warps: sixteen for up to 16 activation columns, eight beyond (registers: 8 kT sums and more a thread).
+__host__ __device__ constexpr int sm_warps(int kT) { return kT <= 2 ? 16 : 8; }
+__host__ __device__ constexpr int sm_threads(int kT) { return sm_warps(kT) * 32 + 32; }
 constexpr int kSmMaxSplit = 8;
 constexpr size_t kSmXBudget = 68 * 1024;  // staged activations of one phase
 
@@ -53,170 +69,374 @@ struct SmallParams {
 
 __host__ __device__ constexpr int sm_slot_bytes(int format, bool gated) { return rec_bytes(format) * (gated ? 2 : 1); }
 
-__device__ __forceinline__ void mma_bf16(float* c, uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0,
-                                         uint32_t b1) {
-  asm volatile(
-      "mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
-      : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
-      : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
+// d (+)= a b, one 16 x 8 x 16 product; pa, pb: the pairs of rows g and g + 8.
+template <bool kBf16>
+__device__ __forceinline__ void mma16816(float* d, const uint32_t* pa, const uint32_t* pb, uint32_t b0, uint32_t b1) {
+  if (kBf16)
+    asm volatile(
+        "mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
+        : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
+        : "r"(pa[0]), "r"(pb[0]), "r"(pa[1]), "r"(pb[1]), "r"(b0), "r"(b1));
+  else
+    asm volatile(
+        "mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
+        : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
+        : "r"(pa[0]), "r"(pb[0]), "r"(pa[1]), "r"(pb[1]), "r"(b0), "r"(b1));
+}
+template <bool kBf16>
+__device__ __forceinline__ void mma16816_first(float* d, const uint32_t* pa, const uint32_t* pb, uint32_t b0,
+                                               uint32_t b1) {
+  if (kBf16)
+    asm volatile(
+        "{\n\t.reg .f32 z;\n\tmov.f32 z, 0f00000000;\n\t"
+        "mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {z,z,z,z};\n\t}"
+        : "=f"(d[0]), "=f"(d[1]), "=f"(d[2]), "=f"(d[3])
+        : "r"(pa[0]), "r"(pb[0]), "r"(pa[1]), "r"(pb[1]), "r"(b0), "r"(b1));
+  else
+    asm volatile(
+        "{\n\t.reg .f32 z;\n\tmov.f32 z, 0f00000000;\n\t"
+        "mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {z,z,z,z};\n\t}"
+        : "=f"(d[0]), "=f"(d[1]), "=f"(d[2]), "=f"(d[3])
+        : "r"(pa[0]), "r"(pb[0]), "r"(pa[1]), "r"(pb[1]), "r"(b0), "r"(b1));
 }
 
-// The 16-byte unit u (8 columns) of a 256-column block sits at unit sm_pos(u)
-// of its staged column: the four lanes of a row quad read units 8t + 4h + w
-// (t the lane) together, so those four are neighbours.
-__device__ __forceinline__ int sm_pos(int u) { return ((u & 7) << 2) | (u >> 3); }
+__device__ __forceinline__ uint4 lds128(uint32_t a) {
+  uint4 v;
+  asm volatile("ld.shared.v4.u32 {%0,%1,%2,%3}, [%4];" : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w) : "r"(a) : "memory");
+  return v;
+}
+__device__ __forceinline__ uint32_t lds32(uint32_t a) {
+  uint32_t v;
+  asm volatile("ld.shared.u32 %0, [%1];" : "=r"(v) : "r"(a) : "memory");
+  return v;
+}
+__device__ __forceinline__ float lds_f32(uint32_t a) { return __uint_as_float(lds32(a)); }
 
-// Stages columns [k0, k0 + 256 nkb) of the m rows; `pitch` bytes per column.
+// The eight codes of a word as four f16 pairs: byte b of a record word holds
+// columns (0, 2), (4, 6), (1, 3), (5, 7) of its eight. An operand only has to
+// pair the same columns on both sides, so the staged activations follow.
+__device__ __forceinline__ void decode_f16(uint32_t w, uint32_t* d) {
+  asm("{\n\t.reg .b8 t0, t1, t2, t3;\n\t"
+      "mov.b32 {t0, t1, t2, t3}, %4;\n\t"
+      "cvt.rn.f16x2.e2m1x2 %0, t0;\n\tcvt.rn.f16x2.e2m1x2 %1, t1;\n\t"
+      "cvt.rn.f16x2.e2m1x2 %2, t2;\n\tcvt.rn.f16x2.e2m1x2 %3, t3;\n\t}"
+      : "=r"(d[0]), "=r"(d[1]), "=r"(d[2]), "=r"(d[3])
+      : "r"(w));
+}
+
+__device__ __forceinline__ uint32_t mul_f16x2(uint32_t a, uint32_t b) {
+  uint32_t d;
+  asm("mul.rn.f16x2 %0, %1, %2;" : "=r"(d) : "r"(a), "r"(b));
+  return d;
+}
+
+// Two e4m3 bytes (the low half of v) as an f16 pair.
+__device__ __forceinline__ uint32_t e4m3_pair_f16(uint32_t v) {
+  uint32_t d;
+  asm("{\n\t.reg .b16 t, u;\n\tmov.b32 {t, u}, %1;\n\tcvt.rn.f16x2.e4m3x2 %0, t;\n\t}" : "=r"(d) : "r"(v));
+  return d;
+}
+
+__device__ __forceinline__ uint32_t f16_bits(float v) { return __half_as_ushort(__float2half_rn(v)); }
+__device__ __forceinline__ float f16_value(uint32_t b) { return __half2float(__ushort_as_half(static_cast<uint16_t>(b))); }
+
+// The eight halves h of adjacent columns as the 16 bytes the lanes multiply by:
+// in the order of decode_f16's pairs, or (wide) of adjacent columns.
+__device__ __forceinline__ uint4 operand16(const uint32_t* h, bool wide) {
+  return wide ? make_uint4(h[0] | h[1] << 16, h[2] | h[3] << 16, h[4] | h[5] << 16, h[6] | h[7] << 16)
+              : make_uint4(h[0] | h[2] << 16, h[4] | h[6] << 16, h[1] | h[3] << 16, h[5] | h[7] << 16);
+}
+
+// Where a lane quad finds its operand: the 16-byte unit u (8 columns) of a
+// record's 256 columns sits at unit sm_pos(u) of its staged column, so that the
+// four lanes of a quad read neighbours. mxfp4: lane t takes word t of a chunk
+// of 32 columns, the natural order; nvfp4: words of chunks 2t and 2t + 1.
 template <int kFormat>
-__device__ __forceinline__ void sm_stage(const SmallParams& p, uint8_t* xs, int pitch, int k0, int nkb, int t) {
-  if (p.quantize) {
-    const int upr = nkb * 16, items = p.m * upr;
-    for (int i0 = 0; i0 < items; i0 += kSmCompute) {
-      const int i = i0 + t;
-      const int mr = i / upr, c = i % upr, col = k0 + c * 16;
-      float v[16];
+__device__ __forceinline__ int sm_pos(int u) {
+  return kFormat == AEX_FP4_MX ? u : ((u & 7) << 2) | (u >> 3);
+}
+
+// Staged activations of a phase: columns of `pitch` bytes at xs, then per
+// column and record the factor that undoes its scale; *wide: a bit per record.
+struct SmStage {
+  uint8_t* xs;
+  float* factor;  // [kb_phase][cols]
+  uint32_t* wide;
+  int pitch, cols, parts;
+};
+
+// One warp per row and record: lane l stages columns 8l..8l+7. `only`: the
+// records to stage as bf16 (0: all, as f16, noting in *wide which need bf16).
+template <int kFormat>
+__device__ __forceinline__ void sm_stage(const SmallParams& p, const SmStage& st, int kb0, int nkb, uint32_t only,
+                                         int warp, int warps, int lane) {
+  for (int i = warp; i < p.m * nkb; i += warps) {
+    const int b = i / p.m, mr = i % p.m;
+    if (only && !((only >> b) & 1u)) continue;
+    const int col = (kb0 + b) * kRecK + lane * 8;
+    float v[8];
 #pragma unroll
-      for (int e = 0; e < 16; ++e) v[e] = 0.f;
-      if (i < items && col < p.k) {
-        if (p.x_f32) {
-          const float4* s = reinterpret_cast<const float4*>(static_cast<const float*>(p.x) + mr * p.ldx + col);
+    for (int e = 0; e < 8; ++e) v[e] = 0.f;
+    if (col < p.k) {
+      if (p.x_f32) {
+        const float4* s = reinterpret_cast<const float4*>(static_cast<const float*>(p.x) + mr * p.ldx + col);
+        const float4 f0 = __ldg(s), f1 = __ldg(s + 1);
+        v[0] = f0.x, v[1] = f0.y, v[2] = f0.z, v[3] = f0.w, v[4] = f1.x, v[5] = f1.y, v[6] = f1.z, v[7] = f1.w;
+      } else {
+        const uint4 u = __ldg(reinterpret_cast<const uint4*>(static_cast<const uint16_t*>(p.x) + mr * p.ldx + col));
+        const uint32_t w[4] = {u.x, u.y, u.z, u.w};
 #pragma unroll
-          for (int e = 0; e < 4; ++e) {
-            const float4 f = __ldg(s + e);
-            v[4 * e] = f.x;
-            v[4 * e + 1] = f.y;
-            v[4 * e + 2] = f.z;
-            v[4 * e + 3] = f.w;
-          }
-        } else {
-          const uint4* s = reinterpret_cast<const uint4*>(static_cast<const uint16_t*>(p.x) + mr * p.ldx + col);
-#pragma unroll
-          for (int e = 0; e < 2; ++e) {
-            const uint4 u = __ldg(s + e);
-            const uint32_t w[4] = {u.x, u.y, u.z, u.w};
-#pragma unroll
-            for (int j = 0; j < 4; ++j) {
-              v[8 * e + 2 * j] = bf16lo_to_f32(w[j]);
-              v[8 * e + 2 * j + 1] = bf16hi_to_f32(w[j]);
-            }
-          }
+        for (int j = 0; j < 4; ++j) {
+          v[2 * j] = bf16lo_to_f32(w[j]);
+          v[2 * j + 1] = bf16hi_to_f32(w[j]);
         }
-      }
-      uint32_t w[2], sb;
-      quantize16<kFormat, true>(v, p.x_scale, p.inv_6ts, w, &sb);
-      if (i < items) {
-        const uint32_t s2 = scale_pair<kFormat>(sb);
-        uint8_t* dst = xs + mr * pitch + (c >> 4) * 512;
-#pragma unroll
-        for (int h = 0; h < 2; ++h)
-          *reinterpret_cast<uint4*>(dst + sm_pos((c & 15) * 2 + h) * 16) =
-              make_uint4(decode_pair<kFormat>(w[h], 0, s2), decode_pair<kFormat>(w[h], 1, s2),
-                         decode_pair<kFormat>(w[h], 2, s2), decode_pair<kFormat>(w[h], 3, s2));
       }
     }
-  } else {
-    const int upr = nkb * 32, items = p.m * upr;
-    for (int i = t; i < items; i += kSmCompute) {
-      const int mr = i / upr, c = i % upr, col = k0 + c * 8;
-      const int off = (c >> 5) * 512 + sm_pos(c & 31) * 16;
-      if (p.x_f32) {
-        float f[8] = {0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f};
-        if (col < p.k) {
-          const float4* s = reinterpret_cast<const float4*>(static_cast<const float*>(p.x) + mr * p.ldx + col);
-          const float4 a = __ldg(s), b = __ldg(s + 1);
-          f[0] = a.x, f[1] = a.y, f[2] = a.z, f[3] = a.w, f[4] = b.x, f[5] = b.y, f[6] = b.z, f[7] = b.w;
-        }
-        uint32_t hi[8], mid[8], lo[8];
+    if (p.quantize) {
+      float q[8];
+      const float s = scale_to_f32<kFormat>(quantize_cols<kFormat, 8>(v, p.x_scale, p.inv_6ts, q));
+      uint32_t d[4];
+      decode_f16(code_word<false>(q), d);
+#pragma unroll
+      for (int j = 0; j < 4; ++j) {
+        v[2 * j] = f16_value(d[j] & 0xFFFFu) * s;  // exact
+        v[2 * j + 1] = f16_value(d[j] >> 16) * s;
+      }
+    }
+    uint8_t* dst = st.xs + (mr * st.parts) * st.pitch + b * 512 + sm_pos<kFormat>(lane) * 16;
+    uint32_t h[8];
+    if (only) {
+#pragma unroll 1
+      for (int part = 0; part < st.parts; ++part) {
 #pragma unroll
         for (int e = 0; e < 8; ++e) {
-          const uint32_t u = __float_as_uint(f[e]);
-          hi[e] = u & 0xFFFF0000u;
-          const float r1 = f[e] - __uint_as_float(hi[e]);
-          mid[e] = __float_as_uint(r1) & 0xFFFF0000u;
-          lo[e] = __float_as_uint(r1 - __uint_as_float(mid[e])) & 0xFFFF0000u;
-          if ((u & 0x7F800000u) == 0x7F800000u) {  // infinity, NaN: the top column alone carries it
-            if (u & 0x007FFFFFu) hi[e] = 0x7FC00000u;
-            mid[e] = lo[e] = 0u;
-          }
+          // the top 8 bits, exactly what there is where x has no more; an infinity or NaN is in the first part alone
+          const uint32_t u = __float_as_uint(v[e]);
+          const bool special = (u & 0x7F800000u) == 0x7F800000u;
+          h[e] = special && (u & 0x007FFFFFu) ? 0x7FC0u : u >> 16;
+          v[e] = special ? 0.f : v[e] - __uint_as_float(u & 0xFFFF0000u);
         }
-#pragma unroll
-        for (int part = 0; part < 3; ++part) {
-          const uint32_t* b = part == 0 ? hi : part == 1 ? mid : lo;
-          *reinterpret_cast<uint4*>(xs + (3 * mr + part) * pitch + off) =
-              make_uint4(__byte_perm(b[0], b[1], 0x7632), __byte_perm(b[2], b[3], 0x7632),
-                         __byte_perm(b[4], b[5], 0x7632), __byte_perm(b[6], b[7], 0x7632));
-        }
-      } else {
-        uint4 u = make_uint4(0, 0, 0, 0);
-        if (col < p.k)
-          u = __ldg(reinterpret_cast<const uint4*>(static_cast<const uint16_t*>(p.x) + mr * p.ldx + col));
-        *reinterpret_cast<uint4*>(xs + mr * pitch + off) = u;
+        *reinterpret_cast<uint4*>(dst + part * st.pitch) = operand16(h, true);
+        if (lane == 0) st.factor[b * st.cols + mr * st.parts + part] = kFormat == AEX_FP4_NV ? 128.f : 1.f;
       }
+      continue;
     }
+    uint32_t top = 0;
+#pragma unroll
+    for (int e = 0; e < 8; ++e) top = max(top, __float_as_uint(v[e]) & 0x7FFFFFFFu);
+    top = __reduce_max_sync(0xffffffffu, top);
+    // 2^k takes the largest into [2^14, 2^15); outside 2^-48 .. 2^62 (and for what is not finite) bf16
+    const int e0 = top ? static_cast<int>(top >> 23) - 127 : 14;
+    bool exact = e0 >= -48 && e0 <= 62;
+    const int k = exact ? 14 - e0 : 0;
+    const float up = __uint_as_float(static_cast<uint32_t>(127 + k) << 23);
+    float r[8];
+#pragma unroll
+    for (int e = 0; e < 8; ++e) {
+      r[e] = v[e] * up;
+      exact &= !(r[e] == 0.f && v[e] != 0.f);
+    }
+    float down = __uint_as_float(static_cast<uint32_t>(127 - k) << 23);
+#pragma unroll 1
+    for (int part = 0; part < st.parts; ++part) {
+#pragma unroll
+      for (int e = 0; e < 8; ++e) {
+        h[e] = f16_bits(r[e]);
+        r[e] = (r[e] - f16_value(h[e])) * 2048.f;  // what is left, to the next part's scale
+      }
+      *reinterpret_cast<uint4*>(dst + part * st.pitch) = operand16(h, false);
+      if (lane == 0) st.factor[b * st.cols + mr * st.parts + part] = down;
+      down *= 1.f / 2048.f;
+    }
+#pragma unroll
+    for (int e = 0; e < 8; ++e) exact &= r[e] == 0.f;
+    if (!__all_sync(0xffffffffu, exact) && lane == 0) atomicOr(st.wide, 1u << b);
   }
 }
 
-// One record against the staged columns of its block: acc += (16 rows of this
-// warp) x (8 kT columns). xb: this lane's column (of tile 0) and quad position.
-template <int kFormat, int kT>
-__device__ __forceinline__ void sm_record(const uint4* codes, const uint32_t* scales, const uint8_t* xb, int pitch,
-                                          int cols, int g, int t, float (*acc)[4]) {
+// One record against the staged columns: acc += (16 rows of this warp) x (8 kT
+// columns). codes: nvfp4, chunks 2t and 2t + 1 of row g, then of row g + 8;
+// mxfp4, [chunk / 2] words of (chunk, row). xb: per 8 columns this lane's column
+// and its place in a quad; fb: per 8 columns the factors of this lane's two.
+template <int kFormat, int kT, bool kWide>
+__device__ __forceinline__ void sm_record(const uint4* codes, const uint32_t* scales, const uint32_t* xb, uint32_t off,
+                                          const uint32_t (*fb)[2], uint32_t foff, float (*acc)[4]) {
   float c[kT][4];
+  if (kFormat == AEX_FP4_NV) {
+    float d[kT][4];  // a second chain of sums: the products of one chain wait for one another
 #pragma unroll
-  for (int i = 0; i < kT; ++i) c[i][0] = c[i][1] = c[i][2] = c[i][3] = 0.f;
+    for (int h = 0; h < 2; ++h) {
+      // the two blocks of chunk 2t + h, both rows
+      const uint32_t fa = kWide ? 0 : e4m3_pair_f16(scales[0] >> (16 * h));
+      const uint32_t fc = kWide ? 0 : e4m3_pair_f16(scales[1] >> (16 * h));
+      const uint32_t wa[4] = {codes[h].x, codes[h].y, codes[h].z, codes[h].w};
+      const uint32_t wb[4] = {codes[2 + h].x, codes[2 + h].y, codes[2 + h].z, codes[2 + h].w};
 #pragma unroll
-  for (int h = 0; h < 2; ++h) {
-    const uint32_t wa[4] = {codes[h].x, codes[h].y, codes[h].z, codes[h].w};
-    const uint32_t wb[4] = {codes[2 + h].x, codes[2 + h].y, codes[2 + h].z, codes[2 + h].w};
+      for (int w = 0; w < 4; ++w) {
+        uint32_t pa[4], pb[4];
+        if (kWide) {
+          const int sh = 16 * h + 8 * (w >> 1);
+          const uint32_t sa = scale_pair<kFormat>((scales[0] >> sh) & 0xFFu);
+          const uint32_t sb = scale_pair<kFormat>((scales[1] >> sh) & 0xFFu);
 #pragma unroll
-    for (int w = 0; w < 4; ++w) {
-      // nvfp4: scales of columns 32h + 16(w / 2) in byte 2h + w / 2; mxfp4: byte h of the lane's pair
-      const int sh = kFormat == AEX_FP4_NV ? 8 * (2 * h + (w >> 1)) : 8 * (2 * (t & 1) + h);
-      const uint32_t sa = scale_pair<kFormat>((scales[0] >> sh) & 0xFFu);
-      const uint32_t sb = scale_pair<kFormat>((scales[1] >> sh) & 0xFFu);
+          for (int j = 0; j < 4; ++j) {
+            pa[j] = decode_pair<kFormat>(wa[w], j, sa);
+            pb[j] = decode_pair<kFormat>(wb[w], j, sb);
+          }
+        } else {
+          const uint32_t sel = (w >> 1) ? 0x3232u : 0x1010u;
+          const uint32_t sa = __byte_perm(fa, 0, sel), sb = __byte_perm(fc, 0, sel);
+          decode_f16(wa[w], pa);
+          decode_f16(wb[w], pb);
+#pragma unroll
+          for (int j = 0; j < 4; ++j) {
+            pa[j] = mul_f16x2(pa[j], sa);
+            pb[j] = mul_f16x2(pb[j], sb);
+          }
+        }
+#pragma unroll
+        for (int i = 0; i < kT; ++i) {
+          const uint4 b = lds128(xb[i] + off + (h * 4 + w) * 64);
+          if (h == 0 && w == 0) {
+            mma16816_first<kWide>(c[i], pa, pb, b.x, b.y);
+            mma16816_first<kWide>(d[i], pa + 2, pb + 2, b.z, b.w);
+          } else {
+            mma16816<kWide>(c[i], pa, pb, b.x, b.y);
+            mma16816<kWide>(d[i], pa + 2, pb + 2, b.z, b.w);
+          }
+        }
+      }
+    }
+#pragma unroll
+    for (int i = 0; i < kT; ++i)
+#pragma unroll
+      for (int e = 0; e < 4; ++e) c[i][e] += d[i][e];
+  } else {
+#pragma unroll
+    for (int ch = 0; ch < 8; ++ch) {
+      const uint4 q = codes[ch >> 1];
+      const uint32_t wa = (ch & 1) ? q.z : q.x, wb = (ch & 1) ? q.w : q.y;
+      // the scale byte as 2^(byte - 127): 0 is the subnormal, 255 infinity, which the multiplication makes NaN
+      const uint32_t sel = 0x0444u | (static_cast<uint32_t>(ch & 3) << 12);
+      float sa = __uint_as_float(max(__byte_perm(scales[2 * (ch >> 2)], 0, sel) >> 1, 0x00400000u));
+      float sb = __uint_as_float(max(__byte_perm(scales[2 * (ch >> 2) + 1], 0, sel) >> 1, 0x00400000u));
+      sa = fmaf(sa, 0.f, sa);
+      sb = fmaf(sb, 0.f, sb);
       uint32_t pa[4], pb[4];
+      if (kWide) {
 #pragma unroll
-      for (int j = 0; j < 4; ++j) {
-        pa[j] = decode_pair<kFormat>(wa[w], j, sa);
-        pb[j] = decode_pair<kFormat>(wb[w], j, sb);
+        for (int j = 0; j < 4; ++j) {
+          pa[j] = mul_bf16x2(code_pair_tiny(wa, j), kBf16x2_2p126);
+          pb[j] = mul_bf16x2(code_pair_tiny(wb, j), kBf16x2_2p126);
+        }
+      } else {
+        decode_f16(wa, pa);
+        decode_f16(wb, pb);
       }
 #pragma unroll
       for (int i = 0; i < kT; ++i) {
-        uint4 b = make_uint4(0, 0, 0, 0);
-        if (8 * i + g < cols) b = *reinterpret_cast<const uint4*>(xb + 8 * i * pitch + (h * 4 + w) * 64);
-        mma_bf16(c[i], pa[0], pb[0], pa[1], pb[1], b.x, b.y);
-        mma_bf16(c[i], pa[2], pb[2], pa[3], pb[3], b.z, b.w);
+        const uint4 b = lds128(xb[i] + off + ch * 64);
+        float d[4];
+        mma16816_first<kWide>(d, pa, pb, b.x, b.y);
+        mma16816<kWide>(d, pa + 2, pb + 2, b.z, b.w);
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+          const float s = e < 2 ? sa : sb;
+          c[i][e] = ch == 0 ? d[e] * s : fmaf(d[e], s, c[i][e]);
+        }
       }
     }
   }
 #pragma unroll
-  for (int i = 0; i < kT; ++i)
+  for (int i = 0; i < kT; ++i) {
+    const float f0 = lds_f32(fb[i][0] + foff), f1 = lds_f32(fb[i][1] + foff);
+    acc[i][0] = fmaf(c[i][0], f0, acc[i][0]);
+    acc[i][1] = fmaf(c[i][1], f1, acc[i][1]);
+    acc[i][2] = fmaf(c[i][2], f0, acc[i][2]);
+    acc[i][3] = fmaf(c[i][3], f1, acc[i][3]);
+  }
+}
+
+__device__ __forceinline__ uint4 ldmatrix_x4(uint32_t addr) {
+  uint4 r;
+  asm volatile("ldmatrix.sync.aligned.m8n8.x4.shared.b16 {%0,%1,%2,%3}, [%4];"
+               : "=r"(r.x), "=r"(r.y), "=r"(r.z), "=r"(r.w)
+               : "r"(addr)
+               : "memory");
+  return r;
+}
+
+// Where this lane finds its codes and scales in a record (rows row0 + g and row0 + g + 8).
+struct SmLane {
+  uint32_t code[4], scale;
+};
+template <int kFormat>
+__device__ __forceinline__ SmLane sm_lane(int row0, int g, int t, int lane) {
+  SmLane o;
+  if (kFormat == AEX_FP4_NV) {
 #pragma unroll
-    for (int e = 0; e < 4; ++e) acc[i][e] += c[i][e];
+    for (int h = 0; h < 2; ++h) o.code[h] = o.code[2 + h] = (row0 + g) * 128 + (((2 * t + h) ^ g) << 4);
+    o.scale = scale_off(row0 + g, t);
+  } else {
+    // matrix i of four (8 rows x 16 bytes, addresses from lanes 8i..8i+7): chunk c + (i >> 1), row half i & 1;
+    // lane (g, t) receives word t of row g of each
+    const int row = row0 + (lane & 7) + ((lane >> 3) & 1) * 8;
+#pragma unroll
+    for (int c2 = 0; c2 < 4; ++c2) o.code[c2] = row * 128 + (((2 * c2 + (lane >> 4)) ^ (row & 7)) << 4);
+    o.scale = scale_off(row0 + g, 0);
+  }
+  return o;
+}
+template <int kFormat>
+__device__ __forceinline__ void sm_load(uint32_t rec, const SmLane& o, uint4* codes, uint32_t* scales) {
+  if (kFormat == AEX_FP4_NV) {
+#pragma unroll
+    for (int h = 0; h < 2; ++h) {
+      codes[h] = lds128(rec + o.code[h]);
+      codes[2 + h] = lds128(rec + o.code[h] + 8 * 128);
+    }
+    scales[0] = lds32(rec + o.scale);
+    scales[1] = lds32(rec + o.scale + 8 * 16);  // row + 8: in the same group of 32 rows
+  } else {
+#pragma unroll
+    for (int c2 = 0; c2 < 4; ++c2) codes[c2] = ldmatrix_x4(rec + o.code[c2]);
+#pragma unroll
+    for (int q = 0; q < 4; ++q) scales[q] = lds32(rec + o.scale + (q >> 1) * 512 + (q & 1) * 8 * 16);
+  }
 }
 
 template <int kFormat, int kT, bool kGated>
-__global__ void __launch_bounds__(kSmThreads) small_kernel(const __grid_constant__ SmallParams p) {
+__global__ void __launch_bounds__(sm_threads(kT)) small_kernel(const __grid_constant__ SmallParams p) {
   extern __shared__ __align__(128) uint8_t smem[];
   constexpr int kSlot = sm_slot_bytes(kFormat, kGated);
   constexpr int kRec = rec_bytes(kFormat);
+  constexpr int kSmWarps = sm_warps(kT), kSmCompute = kSmWarps * 32, kSmThreads = sm_threads(kT);
+  constexpr int kWays = kSmWarps / 8;  // the warps that share 16 rows take turns at the records
   const int slots = p.slots;
   uint8_t* ring = smem;
   uint64_t* full = reinterpret_cast<uint64_t*>(smem + slots * kSlot);
   uint64_t* empty = full + slots;
-  uint8_t* xs = reinterpret_cast<uint8_t*>(full) + 128;  // at most 8 slots
   __shared__ int abort_flag;
+  __shared__ uint32_t wide;
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
   const int rt = blockIdx.x, split = blockIdx.y;
   const int kb0 = split * p.kb_per_split;
   const int nkb = max(0, min(p.k_blocks, kb0 + p.kb_per_split) - kb0);
   const int parts = p.x_f32 && !p.quantize ? 3 : 1;
   const int cols = p.m * parts;
+  SmStage st;
+  st.xs = reinterpret_cast<uint8_t*>(full) + 128;  // at most 8 slots
+  st.pitch = p.kb_phase * 512 + 64;
+  st.factor = reinterpret_cast<float*>(st.xs + cols * st.pitch);
+  st.wide = &wide;
+  st.cols = cols;
+  st.parts = parts;
   if (tid == 0) {
     abort_flag = 0;
+    wide = 0;
     for (int s = 0; s < slots; ++s) {
       mbar_init(&full[s], 1);
-      mbar_init(&empty[s], kSmWarps);
+      mbar_init(&empty[s], 8);
     }
     fence_barrier_init();
   }
@@ -246,41 +466,67 @@ __global__ void __launch_bounds__(kSmThreads) small_kernel(const __grid_constant
     __syncwarp();
   } else {
     const int g = lane >> 2, t = lane & 3;
-    const int pitch = p.kb_phase * 512 + 64;
-    const int row = warp * 16 + g;  // and row + 8
+    const int row0 = (warp & 7) * 16, odd = warp >> 3;
+    const SmLane at = sm_lane<kFormat>(row0, g, t, lane);
+    // A column past the last reads the last one's: its sums are not stored.
+    uint32_t xb[kT], fb[kT][2];
+#pragma unroll
+    for (int i = 0; i < kT; ++i) {
+      xb[i] = smem_u32(st.xs) + min(8 * i + g, cols - 1) * st.pitch + t * 16;
+#pragma unroll
+      for (int e = 0; e < 2; ++e) fb[i][e] = smem_u32(st.factor) + min(8 * i + 2 * t + e, cols - 1) * 4;
+    }
+    const uint32_t ring0 = smem_u32(ring), full0 = smem_u32(full), empty0 = smem_u32(empty);
     bool ok = true;
-    for (int b = 0; b < nkb; ++b) {
-      const int in_phase = b % p.kb_phase;
+    uint32_t wide_now = 0;
+    // slot s and its phase bit, and the record's place in the staged columns, advance with b
+    uint32_t s = 0, ph = 0;
+    int in_phase = 0;
+#pragma unroll 1
+    for (int b = 0; b < nkb; ++b, ++in_phase) {
+      if (in_phase == p.kb_phase) in_phase = 0;
       if (in_phase == 0) {
-        if (b) asm volatile("bar.sync 1, %0;" ::"n"(kSmCompute) : "memory");  // the previous columns are used
-        sm_stage<kFormat>(p, xs, pitch, (kb0 + b) * kRecK, min(p.kb_phase, nkb - b), tid);
+        const int count = min(p.kb_phase, nkb - b);
+        if (b) {
+          asm volatile("bar.sync 1, %0;" ::"n"(kSmCompute) : "memory");  // the previous columns are used
+          if (tid == 0) wide = 0;
+          asm volatile("bar.sync 1, %0;" ::"n"(kSmCompute) : "memory");
+        }
+        sm_stage<kFormat>(p, st, kb0 + b, count, 0, warp, kSmWarps, lane);
         asm volatile("bar.sync 1, %0;" ::"n"(kSmCompute) : "memory");
-      }
-      const int s = b % slots;
-      if (ok) ok = mbar_wait_warp(&full[s], (b / slots) & 1, &abort_flag, p.status, kDevTimeoutTma);
-      if (!ok) continue;  // the barriers above still see every warp
-      const uint8_t* xb = xs + g * pitch + in_phase * 512 + t * 16;
-      uint4 codes[kGated ? 8 : 4];
-      uint32_t sc[kGated ? 4 : 2];
-#pragma unroll
-      for (int q = 0; q < (kGated ? 2 : 1); ++q) {
-        const uint8_t* rec = ring + s * kSlot + q * kRec;
-#pragma unroll
-        for (int r8 = 0; r8 < 2; ++r8) {
-          const uint8_t* rp = rec + (row + 8 * r8) * 128;
-          codes[4 * q + 2 * r8] = *reinterpret_cast<const uint4*>(rp + (((2 * t) ^ g) << 4));
-          codes[4 * q + 2 * r8 + 1] = *reinterpret_cast<const uint4*>(rp + (((2 * t + 1) ^ g) << 4));
-          sc[2 * q + r8] = *reinterpret_cast<const uint32_t*>(
-              rec + scale_off(row + 8 * r8, kFormat == AEX_FP4_NV ? t : t >> 1));
+        wide_now = *reinterpret_cast<volatile uint32_t*>(&wide);
+        if (wide_now) {
+          sm_stage<kFormat>(p, st, kb0 + b, count, wide_now, warp, kSmWarps, lane);
+          asm volatile("bar.sync 1, %0;" ::"n"(kSmCompute) : "memory");
         }
       }
-      __syncwarp();
-      if (lane == 0) mbar_arrive_addr(smem_u32(&empty[s]));  // the warp's reads of the slot are done
-      sm_record<kFormat, kT>(codes, sc, xb, pitch, cols, g, t, acc0);
-      if (kGated) sm_record<kFormat, kT>(codes + 4, sc + 2, xb, pitch, cols, g, t, acc1);
+      const uint32_t cs = s, cph = ph;
+      if (++s == static_cast<uint32_t>(slots)) {
+        s = 0;
+        ph ^= 1;
+      }
+      if (kWays == 2 && (b & 1) != odd) continue;
+      if (ok) ok = mbar_wait_warp_addr(full0 + 8 * cs, cph, &abort_flag, p.status, kDevTimeoutTma);
+      if (!ok) continue;  // the barriers above still see every warp
+      const uint32_t off = in_phase * 512, foff = in_phase * cols * 4;
+      const bool narrow = !((wide_now >> in_phase) & 1u);
+#pragma unroll
+      for (int q = 0; q < (kGated ? 2 : 1); ++q) {
+        uint4 codes[4];
+        uint32_t sc[kFormat == AEX_FP4_NV ? 2 : 4];
+        sm_load<kFormat>(ring0 + cs * kSlot + q * kRec, at, codes, sc);
+        if (q == (kGated ? 1 : 0)) {
+          __syncwarp();
+          if (lane == 0) mbar_arrive_addr(empty0 + 8 * cs);  // the warp's reads of the slot are done
+        }
+        if (narrow)
+          sm_record<kFormat, kT, false>(codes, sc, xb, off, fb, foff, q ? acc1 : acc0);
+        else
+          sm_record<kFormat, kT, true>(codes, sc, xb, off, fb, foff, q ? acc1 : acc0);
+      }
     }
   }
-  __syncthreads();  // every copy has landed and been read: the ring becomes the partial sums [cols][128]
+  __syncthreads();  // every copy has landed and been read: the ring becomes the partial sums [ways][cols][128]
   if (abort_flag) {
     // A wait ran out: the copies in flight land before the ring is written or the CTA exits.
     for (int b = max(0, issued - slots); b < issued; ++b) {
@@ -292,15 +538,15 @@ __global__ void __launch_bounds__(kSmThreads) small_kernel(const __grid_constant
     __syncthreads();
   }
   float* part0 = reinterpret_cast<float*>(ring);
-  float* part1 = part0 + cols * kRecRows;
+  float* part1 = part0 + kWays * cols * kRecRows;
   if (warp < kSmWarps) {
-    const int g = lane >> 2, t = lane & 3, row = warp * 16 + g;
+    const int g = lane >> 2, t = lane & 3, row = (warp & 7) * 16 + g, odd = warp >> 3;
 #pragma unroll
     for (int i = 0; i < kT; ++i)
 #pragma unroll
       for (int e = 0; e < 4; ++e) {
-        const int c = 8 * i + 2 * t + (e & 1), r = row + (e >> 1) * 8;
-        if (c < cols) {
+        const int c0 = 8 * i + 2 * t + (e & 1), c = odd * cols + c0, r = row + (e >> 1) * 8;
+        if (c0 < cols) {
           part0[c * kRecRows + r] = acc0[i][e];
           if (kGated) part1[c * kRecRows + r] = acc1[i][e];
         }
@@ -315,8 +561,8 @@ __global__ void __launch_bounds__(kSmThreads) small_kernel(const __grid_constant
     if (col >= p.n) continue;
     float v0 = 0.f, v1 = 0.f;
     for (int c = 0; c < nsplit; ++c)
-      for (int q = 0; q < parts; ++q) {
-        const uint32_t off = ((mr * parts + q) * kRecRows + r) * 4;
+      for (int q = 0; q < kWays * parts; ++q) {
+        const uint32_t off = (((q % kWays) * cols + mr * parts + q / kWays) * kRecRows + r) * 4;
         v0 += ld_shared_cluster_f32(mapa_shared(a0 + off, c));
         if (kGated) v1 += ld_shared_cluster_f32(mapa_shared(a1 + off, c));
       }
@@ -354,7 +600,7 @@ int launch_small(aex_ctx* ctx, const Job& j, cudaStream_t s) {
   p.k = w->k;
   p.n = w->n;
   p.k_blocks = w->k_blocks;
-  const double unit = decode_unit<kFormat>() * (j.quantize ? decode_unit<kFormat>() * static_cast<double>(j.x_scale) : 1.0);
+  const double unit = j.quantize ? static_cast<double>(j.x_scale) : 1.0;
   p.alpha0 = static_cast<float>(unit * w->tensor_scale);
   p.alpha1 = kGated ? static_cast<float>(unit * j.w1->tensor_scale) : 0.f;
   p.activation = j.activation;
@@ -366,38 +612,36 @@ int launch_small(aex_ctx* ctx, const Job& j, cudaStream_t s) {
   auto kern = small_kernel<kFormat, kT, kGated>;
   constexpr int kSlot = sm_slot_bytes(kFormat, kGated);
   constexpr int kMaxSmem = 226 * 1024;
-  AEX_CUDA_TRY(ctx, cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, kMaxSmem));
-  // K split: the largest whose CTAs run in one wave (more copies in flight per
-  // weight row), else the one of the fewest waves.
-  int best_split = 0, best_slots = 0, best_phase = 0;
-  int64_t best_waves = 0;
-  size_t best_smem = 0;
+  static SmemOptIn opt_in;
+  if (int r = opt_in(ctx, reinterpret_cast<const void*>(kern), kMaxSmem)) return r;
+  // K split: the one that leaves the busiest SM the fewest records (CTAs that share an SM share its schedulers), the
+  // smallest of those (less to add up). 72 row tiles of 16 records (B200, one row): split 2, 144 CTAs.
+  int best_split = 1;
+  int64_t best_load = INT64_MAX;
   for (int sp = 1; sp <= std::min(kSmMaxSplit, w->k_blocks); ++sp) {
     const int kb = (w->k_blocks + sp - 1) / sp;
     if ((w->k_blocks + kb - 1) / kb != sp) continue;  // an empty split
-    const int slots = std::min(kb, 4);
-    int phase = kb;
-    while (phase > 1 && static_cast<size_t>(cols) * (phase * 512 + 64) > kSmXBudget) phase = (phase + 1) / 2;
-    // the partial sums take the ring's place
-    const size_t partial = static_cast<size_t>(cols) * kRecRows * 4 * (kGated ? 2 : 1);
-    size_t smem = static_cast<size_t>(slots) * kSlot + 128 + static_cast<size_t>(cols) * (phase * 512 + 64);
-    smem = std::max(smem, partial);
-    const int64_t per_sm = std::max<int64_t>(1, std::min<int64_t>(4, (227 * 1024) / (smem + 1024)));
-    const int64_t waves = (static_cast<int64_t>(w->n_tiles) * sp + per_sm * ctx->sm_count - 1) / (per_sm * ctx->sm_count);
-    if (!best_split || waves <= best_waves) {
+    const int64_t load = (static_cast<int64_t>(w->n_tiles) * sp + ctx->sm_count - 1) / ctx->sm_count * kb;
+    if (load < best_load) {
       best_split = sp;
-      best_waves = waves;
-      best_slots = slots;
-      best_phase = phase;
-      best_smem = smem;
+      best_load = load;
     }
   }
+  const int kb = (w->k_blocks + best_split - 1) / best_split;
+  const int best_slots = std::min(kb, kGated ? 4 : 6);
+  int best_phase = std::min(kb, 32);  // a bit each in the mask of wide records
+  while (best_phase > 1 && static_cast<size_t>(cols) * (best_phase * 516 + 64) > kSmXBudget)
+    best_phase = (best_phase + 1) / 2;
+  // the partial sums take the ring's place
+  const size_t best_smem =
+      std::max(static_cast<size_t>(best_slots) * kSlot + 128 + static_cast<size_t>(cols) * (best_phase * 516 + 64),
+               static_cast<size_t>(cols) * kRecRows * 4 * (sm_warps(kT) / 8) * (kGated ? 2 : 1));
   p.kb_per_split = (w->k_blocks + best_split - 1) / best_split;
   p.kb_phase = best_phase;
   p.slots = best_slots;
   cudaLaunchConfig_t cfg{};
   cfg.gridDim = dim3(w->n_tiles, best_split, 1);
-  cfg.blockDim = dim3(kSmThreads, 1, 1);
+  cfg.blockDim = dim3(sm_threads(kT), 1, 1);
   cfg.dynamicSmemBytes = best_smem;
   cfg.stream = s;
   cudaLaunchAttribute attr[1];
@@ -416,7 +660,8 @@ int pick_tiles(aex_ctx* ctx, const Job& j, cudaStream_t s) {
   const int cols = j.m * (j.x_f32 && !j.quantize ? 3 : 1);
   if (cols <= 8) return launch_small<kFormat, 1, kGated>(ctx, j, s);
   if (cols <= 16) return launch_small<kFormat, 2, kGated>(ctx, j, s);
-  return launch_small<kFormat, 6, kGated>(ctx, j, s);  // 17..48 columns: f32 rows
+  if (cols <= 32) return launch_small<kFormat, 4, kGated>(ctx, j, s);
+  return launch_small<kFormat, 6, kGated>(ctx, j, s);  // 33..48 columns: f32 rows
 }
 
 }  // namespace

@@ -34,23 +34,32 @@ _DTYPES = {torch.bfloat16: _lib.AEX_DTYPE_BF16, torch.float32: _lib.AEX_DTYPE_F3
 
 
 def _mode(mode):
-    if mode not in MODES:
+    fmt = MODES.get(mode)
+    if fmt is None:
         raise ValueError(f"mode must be one of {sorted(MODES)}")
-    return MODES[mode]
+    return fmt
 
 
-def _matrix(name, t, dtypes=(torch.bfloat16, torch.float32), cols=None):
+# A few-rows product takes some microseconds on the device, so the checks before it count: they go
+# by get_device() and plain integers, not by torch.device objects.
+
+def _matrix(name, t, dtypes, cols=None, device=None):
+    """The checks of a 2-D input with contiguous rows; its AEX_DTYPE (None for uint8), and device index."""
     if not isinstance(t, torch.Tensor) or t.dtype not in dtypes or t.dim() != 2:
         raise TypeError(f"{name} must be a 2-D tensor of {' or '.join(str(d) for d in dtypes)}")
-    if not t.is_cuda:
+    at = t.get_device()
+    if at < 0:
         raise TypeError(f"{name} must be a CUDA tensor")
-    if cols is not None and t.shape[1] != cols:
-        raise ValueError(f"{name} must have {cols} columns, has {t.shape[1]}")
-    if t.shape[0] < 1:
+    if device is not None and at != device:
+        raise ValueError(f"{name} is on cuda:{at}, not on cuda:{device}")
+    rows, have = t.shape
+    if cols is not None and have != cols:
+        raise ValueError(f"{name} must have {cols} columns, has {have}")
+    if rows < 1:
         raise ValueError(f"{name} has no rows")
-    if t.stride(1) != 1 and t.shape[1] != 1:
+    if t.stride(1) != 1 and have != 1:
         raise ValueError(f"{name} must have contiguous rows")
-    return t
+    return at
 
 
 def _pitch(t):
@@ -58,45 +67,55 @@ def _pitch(t):
     return t.stride(0) if t.shape[0] > 1 else -(-t.shape[1] // 8) * 8
 
 
-def _empty(shape, dtype, device, stream):
-    """A tensor that belongs to the stream its kernels run on, as one made under torch.cuda.stream(stream)."""
+def _empty(shape, dtype, like, stream):
+    """A tensor on like's device that belongs to the stream its kernels run on, as one made under
+    torch.cuda.stream(stream)."""
     if stream is None:
-        return torch.empty(shape, dtype=dtype, device=device)
+        return like.new_empty(shape, dtype=dtype)
     with torch.cuda.stream(stream):
-        return torch.empty(shape, dtype=dtype, device=device)
+        return like.new_empty(shape, dtype=dtype)
 
 
-def _out(out, rows, cols, dtype, like, stream):
+def _out(out, rows, cols, dtype, like, device, stream):
     if out is None:
         if dtype not in _DTYPES:
             raise TypeError("out_dtype must be torch.bfloat16 or torch.float32")
-        return _empty((rows, cols), dtype, like.device, stream)
-    _matrix("out", out)
-    if tuple(out.shape) != (rows, cols) or out.device != like.device:
-        raise ValueError(f"out must be [{rows}, {cols}] on {like.device}")
+        return _empty((rows, cols), dtype, like, stream)
+    _matrix("out", out, _DTYPES, cols, device)
+    if out.shape[0] != rows:
+        raise ValueError(f"out must have {rows} rows, has {out.shape[0]}")
     return out
 
 
-def _same_device(device, **tensors):
-    for name, t in tensors.items():
-        if t.device != device:
-            raise ValueError(f"{name} is on {t.device}, not on {device}")
+_OPEN = {}  # device index -> (library, default context), looked up without the binding's locks
+
+
+def _handles(ctx, device):
+    if ctx is not None:
+        return _lib.lib(), ctx
+    got = _OPEN.get(device)
+    if got is None:
+        got = _OPEN[device] = (_lib.lib(), _lib.context(device))
+    return got
 
 
 def _stream(stream, device):
-    return (stream or torch.cuda.current_stream(device)).cuda_stream
+    return stream.cuda_stream if stream is not None else torch._C._cuda_getCurrentRawStream(device)
+
+
+_UINT8 = (torch.uint8,)
+_BF16 = (torch.bfloat16,)
 
 
 def _check_codes(codes, scales, mode):
-    for name, t in (("codes", codes), ("scales", scales)):
-        _matrix(name, t, (torch.uint8,))
-        if not t.is_contiguous():
-            raise ValueError(f"{name} must be contiguous")
-    _same_device(codes.device, scales=scales)
+    device = _matrix("codes", codes, _UINT8)
+    _matrix("scales", scales, _UINT8, device=device)
+    if not codes.is_contiguous() or not scales.is_contiguous():
+        raise ValueError("codes and scales must be contiguous")
     rows, k = codes.shape[0], codes.shape[1] * 2
     if tuple(scales.shape) != (rows, k // BLOCK[mode]) or k % 32:
         raise ValueError(f"codes [rows, k/2] and scales [rows, k/{BLOCK[mode]}] with k a multiple of 32")
-    return rows, k
+    return rows, k, device
 
 
 def quantize(x, mode="nvfp4", tensor_scale=1.0, ctx=None, stream=None):
@@ -105,16 +124,17 @@ def quantize(x, mode="nvfp4", tensor_scale=1.0, ctx=None, stream=None):
     and codes are those of the exact quotients, ties to even; a block that holds an infinity or NaN
     gets a NaN scale."""
     fmt = _mode(mode)
-    _matrix("x", x)
+    device = _matrix("x", x, _DTYPES)
     rows, k = x.shape
     if k % 32 or k == 0:
         raise ValueError("the number of columns must be a positive multiple of 32")
-    ctx = ctx or _lib.context(x.device.index or 0)
-    codes = _empty((rows, k // 2), torch.uint8, x.device, stream)
-    scales = _empty((rows, k // BLOCK[mode]), torch.uint8, x.device, stream)
-    ctx.check(_lib.lib().aex_fp4_quantize(ctx.handle, x.data_ptr(), _DTYPES[x.dtype], _pitch(x), rows, k, fmt,
-                                          tensor_scale, codes.data_ptr(), scales.data_ptr(),
-                                          _stream(stream, x.device)))
+    lib, ctx = _handles(ctx, device)
+    codes = _empty((rows, k // 2), torch.uint8, x, stream)
+    scales = _empty((rows, k // BLOCK[mode]), torch.uint8, x, stream)
+    rc = lib.aex_fp4_quantize(ctx.handle, x.data_ptr(), _DTYPES[x.dtype], _pitch(x), rows, k, fmt,
+                              tensor_scale, codes.data_ptr(), scales.data_ptr(), _stream(stream, device))
+    if rc:
+        ctx.check(rc)
     return codes, scales
 
 
@@ -122,12 +142,13 @@ def dequantize(codes, scales, mode="nvfp4", tensor_scale=1.0, out_dtype=torch.bf
                stream=None):
     """[rows, k] code * scale * tensor_scale, rounded once to bf16 or f32."""
     fmt = _mode(mode)
-    rows, k = _check_codes(codes, scales, mode)
-    out = _out(out, rows, k, out_dtype, codes, stream)
-    ctx = ctx or _lib.context(codes.device.index or 0)
-    ctx.check(_lib.lib().aex_fp4_dequantize(ctx.handle, codes.data_ptr(), scales.data_ptr(), rows, k, fmt,
-                                            tensor_scale, out.data_ptr(), _DTYPES[out.dtype], _pitch(out),
-                                            _stream(stream, codes.device)))
+    rows, k, device = _check_codes(codes, scales, mode)
+    out = _out(out, rows, k, out_dtype, codes, device, stream)
+    lib, ctx = _handles(ctx, device)
+    rc = lib.aex_fp4_dequantize(ctx.handle, codes.data_ptr(), scales.data_ptr(), rows, k, fmt, tensor_scale,
+                                out.data_ptr(), _DTYPES[out.dtype], _pitch(out), _stream(stream, device))
+    if rc:
+        ctx.check(rc)
     return out
 
 
@@ -137,15 +158,15 @@ class FP4Weight:
 
     def __init__(self, codes, scales, mode="nvfp4", tensor_scale=1.0, ctx=None, stream=None):
         fmt = _mode(mode)
-        self.n, self.k = _check_codes(codes, scales, mode)
+        self.n, self.k, self.index = _check_codes(codes, scales, mode)
         self.mode = mode
         self.tensor_scale = tensor_scale
         self.device = codes.device
-        self.ctx = ctx or _lib.context(codes.device.index or 0)
+        self.lib, self.ctx = _handles(ctx, self.index)
         h = C.c_void_p()
-        self.ctx.check(_lib.lib().aex_fp4weight_create(self.ctx.handle, codes.data_ptr(), scales.data_ptr(), self.n,
-                                                       self.k, fmt, tensor_scale, C.byref(h),
-                                                       _stream(stream, codes.device)))
+        self.ctx.check(self.lib.aex_fp4weight_create(self.ctx.handle, codes.data_ptr(), scales.data_ptr(), self.n,
+                                                     self.k, fmt, tensor_scale, C.byref(h),
+                                                     _stream(stream, self.index)))
         self.handle = h
 
     def close(self):
@@ -160,11 +181,16 @@ class FP4Weight:
             pass
 
     def dequantize(self, out_dtype=torch.bfloat16, stream=None):
+        _open(self)
         if out_dtype not in _DTYPES:
             raise TypeError("out_dtype must be torch.bfloat16 or torch.float32")
-        out = _empty((self.n, self.k), out_dtype, self.device, stream)
-        self.ctx.check(_lib.lib().aex_fp4weight_dequantize(self.ctx.handle, self.handle, out.data_ptr(),
-                                                           _DTYPES[out_dtype], self.k, _stream(stream, self.device)))
+        if stream is None:
+            out = torch.empty(self.n, self.k, dtype=out_dtype, device=self.device)
+        else:
+            with torch.cuda.stream(stream):
+                out = torch.empty(self.n, self.k, dtype=out_dtype, device=self.device)
+        self.ctx.check(self.lib.aex_fp4weight_dequantize(self.ctx.handle, self.handle, out.data_ptr(),
+                                                         _DTYPES[out_dtype], self.k, _stream(stream, self.index)))
         return out
 
     def __call__(self, x, **kw):
@@ -179,31 +205,34 @@ def _open(*weights):
             raise ValueError("the weight is closed")
 
 
-def _args(x, w, quantize_x, x_scale, out, stream):
-    a = _lib.aex_fp4_mm_args()
-    a.x, a.x_dtype, a.ldx, a.m = x.data_ptr(), _DTYPES[x.dtype], _pitch(x), x.shape[0]
-    a.quantize_x, a.x_scale = int(bool(quantize_x)), x_scale
-    a.y, a.y_dtype, a.ldy = out.data_ptr(), _DTYPES[out.dtype], out.stride(0) if a.m > 1 else w.n
-    a.workspace_bytes = _lib.lib().aex_fp4_mm_workspace_bytes(w.handle, a.m, a.quantize_x)
-    ws = _empty((a.workspace_bytes,), torch.uint8, x.device, stream) if a.workspace_bytes else None
-    a.workspace = None if ws is None else ws.data_ptr()
-    return a, ws
+def _product(x, w, w_up, activation, quantize_x, x_scale, out_dtype, out, stream):
+    device = w.index
+    _matrix("x", x, _DTYPES, w.k, device)
+    m = x.shape[0]
+    out = _out(out, m, w.n, out_dtype, x, device, stream)
+    q = 1 if quantize_x else 0
+    n_ws = w.lib.aex_fp4_mm_workspace_bytes(w.handle, m, q) if q else 0
+    ws = _empty((n_ws,), torch.uint8, x, stream) if n_ws else None
+    a = _lib.aex_fp4_mm_args(x.data_ptr(), _DTYPES[x.dtype], _pitch(x), m, q, x_scale, out.data_ptr(),
+                             _DTYPES[out.dtype], out.stride(0) if m > 1 else w.n, ws.data_ptr() if n_ws else None,
+                             n_ws)
+    if w_up is None:
+        rc = w.lib.aex_fp4_mm(w.ctx.handle, w.handle, a, _stream(stream, device))
+    else:
+        rc = w.lib.aex_fp4_gated_mm(w.ctx.handle, w.handle, w_up.handle, activation, a, _stream(stream, device))
+    if rc:
+        w.ctx.check(rc)
+    return out
 
 
 def fp4_mm(x, w: FP4Weight, quantize_x=False, x_scale=1.0, out_dtype=torch.bfloat16, out=None, stream=None):
     """y[m, n] = x[m, k] . W[n, k]^T, f32 sums, rounded once to bf16 or f32. x is bf16, or f32 for m <= 16.
     With quantize_x, x (bf16 or f32, any m) goes through :func:`quantize`'s rounding in the weight's
     mode first, with x_scale as its tensor scale, and both operands are multiplied in 4 bits. f32
-    results of more than 16 rows carry the tensor core's truncating f32 sums (about 1e-5 of their
+    results of more than 32 rows carry the tensor core's truncating f32 sums (about 1e-5 of their
     size at k = 9216, as the affine linears' do)."""
     _open(w)
-    _matrix("x", x, cols=w.k)
-    _same_device(w.device, x=x)
-    out = _out(out, x.shape[0], w.n, out_dtype, x, stream)
-    a, ws = _args(x, w, quantize_x, x_scale, out, stream)
-    w.ctx.check(_lib.lib().aex_fp4_mm(w.ctx.handle, w.handle, C.byref(a), _stream(stream, w.device)))
-    del ws
-    return out
+    return _product(x, w, None, 0, quantize_x, x_scale, out_dtype, out, stream)
 
 
 def fp4_gated_mm(x, w_gate: FP4Weight, w_up: FP4Weight, activation="silu", quantize_x=False, x_scale=1.0,
@@ -211,28 +240,22 @@ def fp4_gated_mm(x, w_gate: FP4Weight, w_up: FP4Weight, activation="silu", quant
     """h[m, n] = act(x . Wg^T) * (x . Wu^T): both projections, the activation ("silu" or "gelu_tanh") and
     the product in one kernel, rounded once. x, quantize_x and x_scale as :func:`fp4_mm`."""
     _open(w_gate, w_up)
-    if activation not in ACTIVATIONS:
+    act = ACTIVATIONS.get(activation)
+    if act is None:
         raise ValueError(f"activation must be one of {sorted(ACTIVATIONS)}")
-    _matrix("x", x, cols=w_gate.k)
-    _same_device(w_gate.device, x=x)
-    out = _out(out, x.shape[0], w_gate.n, out_dtype, x, stream)
-    a, ws = _args(x, w_gate, quantize_x, x_scale, out, stream)
-    w_gate.ctx.check(_lib.lib().aex_fp4_gated_mm(w_gate.ctx.handle, w_gate.handle, w_up.handle,
-                                                 ACTIVATIONS[activation], C.byref(a),
-                                                 _stream(stream, w_gate.device)))
-    del ws
-    return out
+    return _product(x, w_gate, w_up, act, quantize_x, x_scale, out_dtype, out, stream)
 
 
 def fp4_mm_dgrad(dy, w: FP4Weight, out_dtype=torch.bfloat16, out=None, stream=None):
     """dx[m, k] = dy[m, n] . W[n, k], the gradient of :func:`fp4_mm` (without quantize_x); dy bf16."""
     _open(w)
-    _matrix("dy", dy, (torch.bfloat16,), cols=w.n)
-    _same_device(w.device, dy=dy)
-    out = _out(out, dy.shape[0], w.k, out_dtype, dy, stream)
-    w.ctx.check(_lib.lib().aex_fp4_mm_dgrad(w.ctx.handle, w.handle, dy.data_ptr(), _pitch(dy), dy.shape[0],
-                                            out.data_ptr(), _DTYPES[out.dtype], _pitch(out),
-                                            _stream(stream, w.device)))
+    _matrix("dy", dy, _BF16, w.n, w.index)
+    m = dy.shape[0]
+    out = _out(out, m, w.k, out_dtype, dy, w.index, stream)
+    rc = w.lib.aex_fp4_mm_dgrad(w.ctx.handle, w.handle, dy.data_ptr(), _pitch(dy), m, out.data_ptr(),
+                                _DTYPES[out.dtype], out.stride(0) if m > 1 else w.k, _stream(stream, w.index))
+    if rc:
+        w.ctx.check(rc)
     return out
 
 
@@ -241,21 +264,24 @@ def fp4_gated_mm_dgrad(dh, x, w_gate: FP4Weight, w_up: FP4Weight, activation="si
     """dx[m, k] of :func:`fp4_gated_mm` (without quantize_x) from dh[m, n] and the forward pass's x; both
     bf16, dx bf16. The projections are computed again; nothing need be kept from the forward pass."""
     _open(w_gate, w_up)
-    if activation not in ACTIVATIONS:
+    act = ACTIVATIONS.get(activation)
+    if act is None:
         raise ValueError(f"activation must be one of {sorted(ACTIVATIONS)}")
-    _matrix("x", x, (torch.bfloat16,), cols=w_gate.k)
-    _matrix("dh", dh, (torch.bfloat16,), cols=w_gate.n)
-    _same_device(w_gate.device, x=x, dh=dh)
-    if dh.shape[0] != x.shape[0]:
+    w = w_gate
+    _matrix("x", x, _BF16, w.k, w.index)
+    _matrix("dh", dh, _BF16, w.n, w.index)
+    m = x.shape[0]
+    if dh.shape[0] != m:
         raise ValueError("dh and x must have the same number of rows")
-    out = _out(out, x.shape[0], w_gate.k, out_dtype, x, stream)
-    if out.dtype != torch.bfloat16:
+    if (out.dtype if out is not None else out_dtype) != torch.bfloat16:
         raise TypeError("the gradient is bfloat16")
-    n = _lib.lib().aex_fp4_gated_mm_dgrad_workspace_bytes(w_gate.handle, x.shape[0])
-    ws = _empty((n,), torch.uint8, x.device, stream)
-    w_gate.ctx.check(_lib.lib().aex_fp4_gated_mm_dgrad(
-        w_gate.ctx.handle, w_gate.handle, w_up.handle, ACTIVATIONS[activation], x.data_ptr(), _pitch(x),
-        dh.data_ptr(), _pitch(dh), x.shape[0], out.data_ptr(), _pitch(out), ws.data_ptr(), n,
-        _stream(stream, w_gate.device)))
-    del ws
+    out = _out(out, m, w.k, out_dtype, x, w.index, stream)
+    n_ws = w.lib.aex_fp4_gated_mm_dgrad_workspace_bytes(w.handle, m)
+    ws = _empty((n_ws,), torch.uint8, x, stream)
+    rc = w.lib.aex_fp4_gated_mm_dgrad(w.ctx.handle, w.handle, w_up.handle, act, x.data_ptr(), _pitch(x),
+                                      dh.data_ptr(), _pitch(dh), m, out.data_ptr(),
+                                      out.stride(0) if m > 1 else w.k, ws.data_ptr(), n_ws,
+                                      _stream(stream, w.index))
+    if rc:
+        w.ctx.check(rc)
     return out
