@@ -150,10 +150,12 @@ _SIGNATURES = [
     ("aex_fp4weight_shape", C.c_int, [_VP, C.POINTER(C.c_int), C.POINTER(C.c_int)]),
     ("aex_fp4weight_dequantize", C.c_int, [_VP, _VP, _VP, C.c_int, C.c_int64, _VP]),
     ("aex_fp4_mm_workspace_bytes", C.c_size_t, [_VP, C.c_int, C.c_int]),
+    ("aex_fp4_gated_mm_workspace_bytes", C.c_size_t, [_VP, C.c_int, C.c_int]),
+    ("aex_fp4_mm_dgrad_workspace_bytes", C.c_size_t, [_VP, C.c_int]),
     ("aex_fp4_mm", C.c_int, [_VP, _VP, C.POINTER(aex_fp4_mm_args), _VP]),
     ("aex_fp4_gated_mm", C.c_int, [_VP, _VP, _VP, C.c_int, C.POINTER(aex_fp4_mm_args), _VP]),
     ("aex_fp4_mm_dgrad", C.c_int,
-     [_VP, _VP, _VP, C.c_int64, C.c_int, _VP, C.c_int, C.c_int64, _VP]),
+     [_VP, _VP, _VP, C.c_int64, C.c_int, _VP, C.c_int, C.c_int64, _VP, C.c_size_t, _VP]),
     ("aex_fp4_gated_mm_dgrad_workspace_bytes", C.c_size_t, [_VP, C.c_int]),
     ("aex_fp4_gated_mm_dgrad", C.c_int,
      [_VP, _VP, _VP, C.c_int, _VP, C.c_int64, _VP, C.c_int64, C.c_int, _VP, C.c_int64, _VP, C.c_size_t, _VP]),

@@ -169,6 +169,10 @@ __host__ __device__ constexpr float decode_unit() {
   return kFormat == AEX_FP4_MX ? 1.f : 128.f;
 }
 
+// mxfp4 scales of at most 2 (byte <= 128) take the pair to its value in one
+// multiplication: 2^(byte - 127 + 126) is a bf16.
+__device__ __forceinline__ uint32_t mx_scale_from_tiny(uint32_t byte) { return (byte + 126u) * 0x00800080u; }
+
 template <int kFormat>
 __device__ __forceinline__ uint32_t decode_pair(uint32_t w, int j, uint32_t scale2) {
   uint32_t p = code_pair_tiny(w, j);

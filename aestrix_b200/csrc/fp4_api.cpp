@@ -37,12 +37,22 @@ int check_workspace(aex_ctx* ctx, const void* p, size_t have, size_t need) {
   return AEX_OK;
 }
 
+size_t round256(size_t v) { return (v + 255) & ~size_t{255}; }
+
 size_t records_bytes(const aex_fp4weight* w, int m) {
   const size_t tiles = (static_cast<size_t>(m) + fp4::kRecRows - 1) / fp4::kRecRows;
-  return tiles * w->k_blocks * fp4::rec_bytes(w->format);
+  return round256(tiles * w->k_blocks * fp4::rec_bytes(w->format));
 }
 
-size_t round256(size_t v) { return (v + 255) & ~size_t{255}; }
+// The workspace of a product: records of the quantized x, then the pieces of split tiles.
+size_t mm_workspace(const aex_fp4weight* w, bool gated, int m, bool quantize) {
+  if (m <= fp4::kSmallRows) return 0;
+  return quantize ? records_bytes(w, m) + fp4::plan_block(w, gated, m).bytes : fp4::plan_gemm(w, gated, m).bytes;
+}
+
+int check_tiles(aex_ctx* ctx, const fp4::TilePlan& p) {
+  return p.clusters ? AEX_OK : set_error(ctx, AEX_ERR_UNSUPPORTED, "the product has too many output tiles");
+}
 
 int run(aex_ctx* ctx, const aex_fp4weight* w0, const aex_fp4weight* w1, int activation, const aex_fp4_mm_args* a,
         aex_stream stream) {
@@ -58,8 +68,11 @@ int run(aex_ctx* ctx, const aex_fp4weight* w0, const aex_fp4weight* w1, int acti
   if (f32 && !a->quantize_x && a->m > fp4::kSmallRowsF32)
     return set_error(ctx, AEX_ERR_UNSUPPORTED, "f32 activations without quantize_x are supported for m <= %d",
                      fp4::kSmallRowsF32);
-  if (int r = check_workspace(ctx, a->workspace, a->workspace_bytes,
-                              aex_fp4_mm_workspace_bytes(w0, a->m, a->quantize_x)))
+  const bool gated = w1 != nullptr;
+  if (a->m > fp4::kSmallRows)
+    if (int r = check_tiles(ctx, a->quantize_x ? fp4::plan_block(w0, gated, a->m) : fp4::plan_gemm(w0, gated, a->m)))
+      return r;
+  if (int r = check_workspace(ctx, a->workspace, a->workspace_bytes, mm_workspace(w0, gated, a->m, a->quantize_x)))
     return r;
   DeviceGuard dev(ctx);
   if (dev.rc) return dev.rc;
@@ -76,14 +89,16 @@ int run(aex_ctx* ctx, const aex_fp4weight* w0, const aex_fp4weight* w1, int acti
   j.y = a->y;
   j.y_f32 = a->y_dtype == AEX_DTYPE_F32;
   j.ldy = a->ldy;
-  j.workspace = static_cast<uint8_t*>(a->workspace);
   auto s = static_cast<cudaStream_t>(stream);
   if (j.m <= fp4::kSmallRows) return fp4::run_small(ctx, j, s);
   if (j.quantize) {
-    if (int r = fp4::quantize_records(ctx, j.x, j.x_f32, j.ldx, j.m, w0->k, w0->format, j.x_scale, j.workspace, s))
+    j.x_records = static_cast<uint8_t*>(a->workspace);
+    j.pieces = j.x_records + records_bytes(w0, j.m);
+    if (int r = fp4::quantize_records(ctx, j.x, j.x_f32, j.ldx, j.m, w0->k, w0->format, j.x_scale, j.x_records, s))
       return r;
     return fp4::run_block(ctx, j, s);
   }
+  j.pieces = a->workspace;
   return fp4::run_gemm(ctx, j, s);
 }
 
@@ -93,8 +108,11 @@ int run(aex_ctx* ctx, const aex_fp4weight* w0, const aex_fp4weight* w1, int acti
 extern "C" {
 
 size_t aex_fp4_mm_workspace_bytes(const aex_fp4weight* w, int m, int quantize_x) {
-  if (!w || m <= aex::fp4::kSmallRows || !quantize_x) return 0;
-  return aex::records_bytes(w, m);
+  return w && m > 0 ? aex::mm_workspace(w, false, m, quantize_x != 0) : 0;
+}
+
+size_t aex_fp4_gated_mm_workspace_bytes(const aex_fp4weight* w_gate, int m, int quantize_x) {
+  return w_gate && m > 0 ? aex::mm_workspace(w_gate, true, m, quantize_x != 0) : 0;
 }
 
 int aex_fp4_mm(aex_ctx* ctx, const aex_fp4weight* w, const aex_fp4_mm_args* args, aex_stream stream) {
@@ -112,23 +130,32 @@ int aex_fp4_gated_mm(aex_ctx* ctx, const aex_fp4weight* w_gate, const aex_fp4wei
   return run(ctx, w_gate, w_up, activation, args, stream);
 }
 
+size_t aex_fp4_mm_dgrad_workspace_bytes(const aex_fp4weight* w, int m) {
+  return w && m > 0 ? aex::fp4::plan_dgrad(w, false, m).bytes : 0;
+}
+
 int aex_fp4_mm_dgrad(aex_ctx* ctx, const aex_fp4weight* w, const void* dy, int64_t lddy, int m, void* dx,
-                     int dx_dtype, int64_t lddx, aex_stream stream) {
+                     int dx_dtype, int64_t lddx, void* workspace, size_t workspace_bytes, aex_stream stream) {
   using namespace aex;
   if (!ctx) return set_error(ctx, AEX_ERR_INVALID_ARG, "NULL ctx");
   if (int r = check_weight(ctx, w, "w")) return r;
   if (int r = fp4::check_matrix(ctx, "dy", dy, AEX_DTYPE_BF16, lddy, m, w->n)) return r;
   if (int r = check_out(ctx, "dx", dx, dx_dtype, lddx, w->k)) return r;
+  const fp4::TilePlan plan = fp4::plan_dgrad(w, false, m);
+  if (int r = check_tiles(ctx, plan)) return r;
+  if (int r = check_workspace(ctx, workspace, workspace_bytes, plan.bytes)) return r;
   DeviceGuard dev(ctx);
   if (dev.rc) return dev.rc;
   return fp4::run_dgrad(ctx, w, nullptr, dy, lddy, nullptr, 0, m, w->tensor_scale, dx, dx_dtype == AEX_DTYPE_F32, lddx,
-                        static_cast<cudaStream_t>(stream));
+                        workspace, static_cast<cudaStream_t>(stream));
 }
 
+// dg and du, bf16, rows padded to 16 bytes, then the pieces of whichever of the two products has more.
 size_t aex_fp4_gated_mm_dgrad_workspace_bytes(const aex_fp4weight* w_gate, int m) {
   if (!w_gate || m <= 0) return 0;
-  // dg and du, bf16, rows padded to 16 bytes
-  return 2 * aex::round256(static_cast<size_t>(m) * ((static_cast<size_t>(w_gate->n) + 7) / 8 * 8) * 2);
+  const size_t d = aex::round256(static_cast<size_t>(m) * ((static_cast<size_t>(w_gate->n) + 7) / 8 * 8) * 2);
+  const size_t p0 = aex::fp4::plan_gemm(w_gate, true, m).bytes, p1 = aex::fp4::plan_dgrad(w_gate, true, m).bytes;
+  return 2 * d + (p0 > p1 ? p0 : p1);
 }
 
 int aex_fp4_gated_mm_dgrad(aex_ctx* ctx, const aex_fp4weight* w_gate, const aex_fp4weight* w_up, int activation,
@@ -140,6 +167,8 @@ int aex_fp4_gated_mm_dgrad(aex_ctx* ctx, const aex_fp4weight* w_gate, const aex_
   if (int r = fp4::check_matrix(ctx, "x", x, AEX_DTYPE_BF16, ldx, m, w_gate->k)) return r;
   if (int r = fp4::check_matrix(ctx, "dh", dh, AEX_DTYPE_BF16, lddh, m, w_gate->n)) return r;
   if (int r = check_out(ctx, "dx", dx, AEX_DTYPE_BF16, lddx, w_gate->k)) return r;
+  if (int r = check_tiles(ctx, fp4::plan_gemm(w_gate, true, m))) return r;
+  if (int r = check_tiles(ctx, fp4::plan_dgrad(w_gate, true, m))) return r;
   const size_t need = aex_fp4_gated_mm_dgrad_workspace_bytes(w_gate, m);
   if (int r = check_workspace(ctx, workspace, workspace_bytes, need)) return r;
   DeviceGuard dev(ctx);
@@ -147,10 +176,13 @@ int aex_fp4_gated_mm_dgrad(aex_ctx* ctx, const aex_fp4weight* w_gate, const aex_
   auto s = static_cast<cudaStream_t>(stream);
   // The tensor scales go into dg and du, so that one accumulator takes both products.
   const int64_t ld = (static_cast<int64_t>(w_gate->n) + 7) / 8 * 8;
-  auto* dg = static_cast<uint16_t*>(workspace);
-  auto* du = dg + need / 4;
-  if (int r = fp4::run_gated_grad(ctx, w_gate, w_up, activation, x, ldx, m, dh, lddh, dg, du, ld, s)) return r;
-  return fp4::run_dgrad(ctx, w_gate, w_up, dg, ld, du, ld, m, 1.f, dx, false, lddx, s);
+  const size_t d = round256(static_cast<size_t>(m) * ld * 2);
+  auto* ws = static_cast<uint8_t*>(workspace);
+  auto* dg = reinterpret_cast<uint16_t*>(ws);
+  auto* du = reinterpret_cast<uint16_t*>(ws + d);
+  void* pieces = ws + 2 * d;
+  if (int r = fp4::run_gated_grad(ctx, w_gate, w_up, activation, x, ldx, m, dh, lddh, dg, du, ld, pieces, s)) return r;
+  return fp4::run_dgrad(ctx, w_gate, w_up, dg, ld, du, ld, m, 1.f, dx, false, lddx, pieces, s);
 }
 
 }  // extern "C"

@@ -13,11 +13,17 @@
 //   warp 0   producer (both CTAs)
 //   warp 1   even CTA: MMA issuer; odd CTA: forwards "landed" to the even CTA
 //   warp 2   tensor-memory allocation
-//   warps 4-7 epilogue (tensor-memory lane quadrant = warp % 4)
+//   warps 4-11 epilogue (tensor-memory lane quadrant = warp % 4; half of the
+//            columns each)
+// Tensor memory holds 512 columns, two accumulators of 256 and the scales of a
+// step (48) do not fit: the accumulators overlap by 48 columns, [0, 256) and
+// [208, 464). The epilogue reads those first and hands them back (`ovl`), so
+// that the next tile's products wait for a fifth of the epilogue only (with one
+// accumulator they waited for all of it: 157 us for the largest listed case).
 // Barriers per 256-column step (stage s): the copies land on each CTA's full[s];
 // the odd CTA's forwarder arrives on the even CTA's peer[s]; the MMA thread
 // waits for both, issues the copies of scales and four products, and commits to
-// the even CTA's empty[s], whose producer forwards it to the odd CTA's.
+// both CTAs' empty[s]. Tiles are dealt out as in the dequantizing GEMM.
 #include <algorithm>
 
 #include "fp4_internal.h"
@@ -26,7 +32,7 @@
 namespace aex {
 namespace fp4 {
 
-constexpr int kBThreads = 256;
+constexpr int kBThreads = 384;
 constexpr int kBStages = 5;
 constexpr int kBOffB = kRecCodes;
 constexpr int kBOffSfa = 2 * kRecCodes;
@@ -34,13 +40,16 @@ constexpr int kBOffSfb = kBOffSfa + 2048;
 constexpr int kBStage = kBOffSfb + 2 * 2048;  // 38 KB
 static_assert(kBStage % 1024 == 0, "operand tiles start on 1024-byte boundaries");
 constexpr int kBOffBar = kBStages * kBStage;
-// full[S], peer[S], empty[S], accf, acce, drain
-constexpr int kBNumBars = 3 * kBStages + 3;
+// full[S], peer[S], empty[S], accf[2], acce[2], ovl, drain
+constexpr int kBNumBars = 3 * kBStages + 6;
 constexpr int kBSmem = kBOffBar + kBNumBars * 8 + 16 + 1024;
 static_assert(kBSmem <= 232448, "fp4 block GEMM exceeds the shared-memory limit");
-// tensor memory: the accumulator, then the scales of a stage
-constexpr uint32_t kBSfa = 256;       // 4 columns per group of 128 rows x 4 scales
-constexpr uint32_t kBSfb = kBSfa + 16;  // 8 columns per group of 256 rows x 4 scales
+// tensor memory: the accumulators, then the scales of a step
+constexpr uint32_t kBAcc1 = 208;
+constexpr int kBOvl = 256 - kBAcc1;      // columns that both accumulators use
+constexpr uint32_t kBSfa = kBAcc1 + 256;  // 4 columns per group of 128 rows x 4 scales
+constexpr uint32_t kBSfb = kBSfa + 16;    // 8 columns per group of 256 rows x 4 scales
+static_assert(kBSfb + 32 == 512, "tensor memory");
 
 struct BlockParams {
   const uint8_t* x;
@@ -49,7 +58,7 @@ struct BlockParams {
   int k_blocks;
   int x_tiles;  // records along the rows of x
   int n_tiles;  // records along the rows of a weight
-  int m_tiles, tiles;
+  TileWork work;
   TileOut o;
   int* status;
 };
@@ -103,8 +112,9 @@ __global__ void __launch_bounds__(kBThreads, 1) block_kernel(const __grid_consta
   uint64_t* peer = full + kBStages;
   uint64_t* empty = peer + kBStages;
   uint64_t* accf = empty + kBStages;
-  uint64_t* acce = accf + 1;
-  uint64_t* drain = acce + 1;
+  uint64_t* acce = accf + 2;
+  uint64_t* ovl = acce + 2;
+  uint64_t* drain = ovl + 1;
   uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(full + kBNumBars);
   __shared__ int abort_flag;
   constexpr int kRec = rec_bytes(kFormat);
@@ -124,8 +134,11 @@ __global__ void __launch_bounds__(kBThreads, 1) block_kernel(const __grid_consta
       mbar_init(&peer[s], 1);
       mbar_init(&empty[s], 1);
     }
-    mbar_init(accf, 1);
-    mbar_init(acce, 2 * 4);
+    for (int b = 0; b < 2; ++b) {
+      mbar_init(&accf[b], 1);
+      mbar_init(&acce[b], 2 * 8);
+    }
+    mbar_init(ovl, 2 * 4);
     mbar_init(drain, 1);
     fence_barrier_init();
   }
@@ -142,12 +155,12 @@ __global__ void __launch_bounds__(kBThreads, 1) block_kernel(const __grid_consta
     if (lane == 0) {
       // -------------------------------------------------------- producer
       const uint32_t empty0 = smem_u32(&empty[0]);
-      const uint32_t peer_empty0 = mapa_shared(empty0, 1);
       uint32_t s = 0, ph = 0;
       int g = 0;
       bool ok = true;
-      for (int t = cluster; t < p.tiles && ok; t += clusters) {
-        const int mt = t % p.m_tiles, nt = t / p.m_tiles;
+      TilePiece t;
+      for (int i = 0; ok && p.work.piece(cluster, clusters, p.k_blocks, i, &t); ++i) {
+        const int mt = t.mt, nt = t.nt;
         const size_t step = static_cast<size_t>(kRec);
         // past the last tile of rows or outputs: any record, its results are not stored
         const uint8_t* xa = p.x + static_cast<size_t>(min(2 * mt + static_cast<int>(rank), p.x_tiles - 1)) * p.k_blocks * step;
@@ -159,13 +172,10 @@ __global__ void __launch_bounds__(kBThreads, 1) block_kernel(const __grid_consta
           b0 = p.w0 + static_cast<size_t>(2 * nt) * p.k_blocks * step;
           b1 = p.w0 + static_cast<size_t>(min(2 * nt + 1, p.n_tiles - 1)) * p.k_blocks * step;
         }
-        for (int k = 0; k < p.k_blocks; ++k, ++g) {
-          if (g >= kBStages) {
-            if (!mbar_wait_cl(empty0 + 8 * s, ph ^ 1, &abort_flag, p.status, kDevTimeoutTma)) {
-              ok = false;
-              break;
-            }
-            if (rank == 0) mbar_arrive_cluster(peer_empty0 + 8 * s);
+        for (int k = t.r0; k < t.r1; ++k, ++g) {
+          if (g >= kBStages && !mbar_wait_cl(empty0 + 8 * s, ph ^ 1, &abort_flag, p.status, kDevTimeoutTma)) {
+            ok = false;
+            break;
           }
           uint8_t* st = smem + s * kBStage;
           const size_t at = static_cast<size_t>(k) * step;
@@ -196,8 +206,9 @@ __global__ void __launch_bounds__(kBThreads, 1) block_kernel(const __grid_consta
       const uint32_t lead = mapa_shared(smem_u32(&peer[0]), 0);
       uint32_t s = 0, ph = 0;
       bool ok = true;
-      for (int t = cluster; t < p.tiles && ok; t += clusters)
-        for (int k = 0; k < p.k_blocks; ++k) {
+      TilePiece t;
+      for (int i = 0; ok && p.work.piece(cluster, clusters, p.k_blocks, i, &t); ++i)
+        for (int k = t.r0; k < t.r1; ++k) {
           if (!mbar_wait_cl(smem_u32(&full[s]), ph, &abort_flag, p.status, kDevTimeoutTma)) {
             ok = false;
             break;
@@ -216,15 +227,19 @@ __global__ void __launch_bounds__(kBThreads, 1) block_kernel(const __grid_consta
       const uint64_t dsa0 = sdesc_scales(s0 + kBOffSfa);
       const uint64_t dsb0 = sdesc_scales(s0 + kBOffSfb);
       uint32_t s = 0, ph = 0;
-      int i = 0;
       bool ok = true;
-      for (int t = cluster; t < p.tiles && ok; t += clusters, ++i) {
-        if (i >= 1 && !mbar_wait_cl(smem_u32(acce), (i + 1) & 1, &abort_flag, p.status, kDevTimeoutMma)) {
+      TilePiece t;
+      for (int i = 0; ok && p.work.piece(cluster, clusters, p.k_blocks, i, &t); ++i) {
+        // this accumulator's previous tile is read, and of the other's the columns they share
+        const int b = i & 1;
+        if ((i >= 2 && !mbar_wait_cl(smem_u32(&acce[b]), ((i >> 1) + 1) & 1, &abort_flag, p.status, kDevTimeoutMma)) ||
+            (i >= 1 && !mbar_wait_cl(smem_u32(ovl), (i + 1) & 1, &abort_flag, p.status, kDevTimeoutMma))) {
           ok = false;
           break;
         }
         tc_fence_after();
-        for (int k = 0; k < p.k_blocks; ++k) {
+        const uint32_t d = tmem + b * kBAcc1;
+        for (int k = t.r0; k < t.r1; ++k) {
           if (!mbar_wait_cl(smem_u32(&full[s]), ph, &abort_flag, p.status, kDevTimeoutMma) ||
               !mbar_wait_cl(smem_u32(&peer[s]), ph, &abort_flag, p.status, kDevTimeoutMma)) {
             ok = false;
@@ -243,18 +258,17 @@ __global__ void __launch_bounds__(kBThreads, 1) block_kernel(const __grid_consta
             // mxfp4: a group's four scales serve two products, the second takes bytes 2 and 3
             const int gq = kFormat == AEX_FP4_MX ? kk >> 1 : kk;
             const uint32_t idesc = idesc_fp4(256, 256, kFormat == AEX_FP4_MX, kFormat == AEX_FP4_MX ? (kk & 1) * 2 : 0);
-            umma_fp4_pair<kFormat>(tmem, da0 + off + kk * 2, db0 + off + kk * 2, idesc, tmem + kBSfa + 4 * gq,
-                                   tmem + kBSfb + 8 * gq, (k > 0 || kk > 0) ? 1u : 0u);
+            umma_fp4_pair<kFormat>(d, da0 + off + kk * 2, db0 + off + kk * 2, idesc, tmem + kBSfa + 4 * gq,
+                                   tmem + kBSfb + 8 * gq, (k > t.r0 || kk > 0) ? 1u : 0u);
           }
-          umma_commit_pair(smem_u32(&empty[s]));
+          umma_commit_both(smem_u32(&empty[s]));
           if (++s == kBStages) {
             s = 0;
             ph ^= 1;
           }
         }
         if (!ok) break;
-        umma_commit_pair(smem_u32(accf));
-        umma_commit_pair(mapa_shared(smem_u32(accf), 1));
+        umma_commit_both(smem_u32(&accf[b]));
       }
       umma_commit_pair(smem_u32(drain));
       int no_abort = 0;
@@ -262,16 +276,75 @@ __global__ void __launch_bounds__(kBThreads, 1) block_kernel(const __grid_consta
     }
   } else if (warp >= 4) {
     // ------------------------------------------------------------ epilogue
-    const int quad = warp & 3;
-    int i = 0;
-    for (int t = cluster; t < p.tiles; t += clusters, ++i) {
-      if (!mbar_wait_warp_cl(smem_u32(accf), i & 1, &abort_flag, p.status, kDevTimeoutEpilogue)) break;
+    const int quad = warp & 3, half = (warp - 4) >> 2;
+    const uint32_t ovl_lead = mapa_shared(smem_u32(ovl), 0);
+    TilePiece t;
+    for (int i = 0; p.work.piece(cluster, clusters, p.k_blocks, i, &t); ++i) {
+      const int b = i & 1;
+      if (!mbar_wait_warp_cl(smem_u32(&accf[b]), (i >> 1) & 1, &abort_flag, p.status, kDevTimeoutEpilogue)) break;
       tc_fence_after();
-      const int64_t row = static_cast<int64_t>(t % p.m_tiles) * 256 + rank * 128 + quad * 32 + lane;
-      tile_rows<kGated>(p.o, row, t / p.m_tiles, tmem + (static_cast<uint32_t>(quad * 32) << 16));
+      const int in_tile = static_cast<int>(rank) * 128 + quad * 32 + lane;
+      const int64_t row = static_cast<int64_t>(t.mt) * 256 + in_tile;
+      const bool live = row < p.o.m;
+      const uint32_t tbase = tmem + (static_cast<uint32_t>(quad * 32) << 16) + b * kBAcc1;
+      // The shared columns are the last of accumulator 0, in half 1, and the first of accumulator 1, in half 0.
+      const bool mine = half != b;
+      const int o0 = b ? 0 : static_cast<int>(kBAcc1);  // first shared column of this accumulator
+      float sh[kBOvl];
+      if (mine) {
+        tmem_read<kBOvl>(tbase + o0, sh);
+        tc_fence_before();
+        __syncwarp();
+        if (lane == 0) mbar_arrive_cluster(ovl_lead);
+      }
+      if (kGated && t.slot < 0) {
+        // outputs [64 half, ..): the shared columns are up columns 80..127 (accumulator 0) or gate columns 0..47
+        if (mine) {
+#pragma unroll
+          for (int e = 0; e < kBOvl; e += 16) {
+            const int c = (b ? 0 : static_cast<int>(kBAcc1) - 128) + e;
+            float v[16];
+            tmem_read<16>(tbase + (b ? 128 : 0) + c, v);
+            if (live) finish<true, 16>(p.o, row, t.nt, c, b ? sh + e : v, b ? v : sh + e);
+          }
+        }
+        const int c0 = mine && half == 0 ? kBOvl : 64 * half;
+        const int c1 = mine && half == 1 ? static_cast<int>(kBAcc1) - 128 : 64 * half + 64;
+#pragma unroll 1
+        for (int c = c0; c < c1; c += 16) {
+          uint32_t g[16], u[16];
+          tmem_ld16(tbase + c, g);
+          tmem_ld16(tbase + 128 + c, u);
+          tmem_wait_ld();
+          if (live) finish<true, 16>(p.o, row, t.nt, c, reinterpret_cast<float*>(g), reinterpret_cast<float*>(u));
+        }
+      } else {
+        float* dst = p.work.pieces + (t.slot < 0 ? 0 : static_cast<size_t>(t.slot) * p.work.rows * 256 + in_tile);
+        auto emit = [&](int c, const float* v) {
+          if (!live) return;
+          if (t.slot < 0) {
+            finish<false, 16>(p.o, row, t.nt, c, v, nullptr);
+          } else {
+#pragma unroll
+            for (int e = 0; e < 16; ++e) dst[static_cast<size_t>(c + e) * p.work.rows] = v[e];
+          }
+        };
+        if (mine) {
+#pragma unroll
+          for (int e = 0; e < kBOvl; e += 16) emit(o0 + e, sh + e);
+        }
+        const int c0 = mine && half == 0 ? kBOvl : 128 * half;
+        const int c1 = mine && half == 1 ? static_cast<int>(kBAcc1) : 128 * half + 128;
+#pragma unroll 1
+        for (int c = c0; c < c1; c += 16) {
+          float v[16];
+          tmem_read<16>(tbase + c, v);
+          emit(c, v);
+        }
+      }
       tc_fence_before();
       __syncwarp();
-      if (lane == 0) mbar_arrive_cluster(mapa_shared(smem_u32(acce), 0));
+      if (lane == 0) mbar_arrive_cluster(mapa_shared(smem_u32(&acce[b]), 0));
     }
   }
   tc_fence_before();
@@ -283,22 +356,32 @@ __global__ void __launch_bounds__(kBThreads, 1) block_kernel(const __grid_consta
   }
 }
 
+template <bool kGated>
+__global__ void __launch_bounds__(256) block_join_kernel(const __grid_constant__ BlockParams p, int clusters) {
+  join_tile<kGated>(p.work, p.k_blocks, clusters, p.o.m,
+                    [&](int64_t row, int nt, int c, const float* v, const float* u) {
+                      finish<kGated, 8>(p.o, row, nt, c, v, u);
+                    });
+}
+
 namespace {
 
 template <int kFormat, bool kGated>
 int launch_block(aex_ctx* ctx, const Job& j, cudaStream_t s) {
   const aex_fp4weight* w = j.w0;
+  const TilePlan plan = plan_block(w, kGated, j.m);
   BlockParams p{};
-  p.x = j.workspace;
+  p.x = j.x_records;
   p.w0 = w->records;
   p.w1 = kGated ? j.w1->records : nullptr;
   p.k_blocks = w->k_blocks;
   p.x_tiles = (j.m - 1) / kRecRows + 1;
   p.n_tiles = w->n_tiles;
-  p.m_tiles = (j.m - 1) / 256 + 1;
-  const int64_t tiles = static_cast<int64_t>(p.m_tiles) * (kGated ? w->n_tiles : (w->n_tiles + 1) / 2);
-  if (tiles > 0x3FFFFFFF) return set_error(ctx, AEX_ERR_UNSUPPORTED, "fp4 GEMM: %lld output tiles", (long long)tiles);
-  p.tiles = static_cast<int>(tiles);
+  p.work.m_tiles = plan.m_tiles;
+  p.work.whole = plan.whole;
+  p.work.split = plan.split;
+  p.work.rows = plan.rows;
+  p.work.pieces = static_cast<float*>(j.pieces);
   p.o.m = j.m;
   p.o.cols = w->n;
   p.o.alpha0 = static_cast<float>(static_cast<double>(j.x_scale) * w->tensor_scale);
@@ -312,30 +395,23 @@ int launch_block(aex_ctx* ctx, const Job& j, cudaStream_t s) {
   auto kern = block_kernel<kFormat, kGated>;
   static SmemOptIn opt_in;
   if (int r = opt_in(ctx, reinterpret_cast<const void*>(kern), kBSmem)) return r;
-  cudaLaunchConfig_t cfg{};
-  cfg.blockDim = dim3(kBThreads, 1, 1);
-  cfg.dynamicSmemBytes = kBSmem;
-  cfg.stream = s;
-  cudaLaunchAttribute attr[1];
-  attr[0].id = cudaLaunchAttributeClusterDimension;
-  attr[0].val.clusterDim.x = 2;
-  attr[0].val.clusterDim.y = 1;
-  attr[0].val.clusterDim.z = 1;
-  cfg.attrs = attr;
-  cfg.numAttrs = 1;
-  if (ctx->fp4_clusters <= 0) {
-    cfg.gridDim = dim3(2 * (ctx->sm_count / 2), 1, 1);
-    int n = 0;
-    AEX_CUDA_TRY(ctx, cudaOccupancyMaxActiveClusters(&n, kern, &cfg));
-    if (n <= 0) return set_error(ctx, AEX_ERR_UNSUPPORTED, "the fp4 CTA-pair GEMM cannot be resident on this device");
-    ctx->fp4_clusters = n;
+  if (int r = launch_pairs(ctx, reinterpret_cast<const void*>(kern), plan.clusters, kBThreads, kBSmem, s, &p)) return r;
+  if (plan.split) {
+    constexpr int kGroups = kGated ? 16 : 32;
+    block_join_kernel<kGated><<<(plan.split * plan.rows * kGroups + 255) / 256, 256, 0, s>>>(p, plan.clusters);
+    return check_launch(ctx, "fp4 block_join_kernel");
   }
-  cfg.gridDim = dim3(2 * std::min(p.tiles, ctx->fp4_clusters), 1, 1);
-  AEX_CUDA_TRY(ctx, cudaLaunchKernelEx(&cfg, kern, p));
-  return check_launch(ctx, "fp4 block_kernel");
+  return AEX_OK;
 }
 
+// What a join costs, in records of the main loop (about 3 us).
+constexpr int kJoinBlock = 12;
+
 }  // namespace
+
+TilePlan plan_block(const aex_fp4weight* w, bool gated, int m) {
+  return plan_tiles(w->clusters, m, gated ? w->n_tiles : (w->n_tiles + 1) / 2, w->k_blocks, kJoinBlock);
+}
 
 int run_block(aex_ctx* ctx, const Job& j, cudaStream_t s) {
   if (j.w0->format == AEX_FP4_MX)

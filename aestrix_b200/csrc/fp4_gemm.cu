@@ -20,14 +20,23 @@
 //   warp 1      MMA issuer (even CTA only)
 //   warp 2      tensor-memory allocation
 //   warp 3      producer of the records (one bulk copy each)
-//   warps 4-7   epilogue (tensor-memory lane quadrant = warp % 4)
-//   warps 8-15  decode: two groups of four warps, alternate K steps
-// Barriers per step (stage s): the A box lands on afull[s]; a decode warp waits
-// for it and for its record, writes its part of B and arrives on the even
-// CTA's bready[s] (both CTAs' four warps of a group); the MMA thread waits for
-// that, issues four MMAs and commits to the even CTA's empty[s], whose A
-// producer forwards it to the odd CTA. A record is released (rempty) by all
-// eight decode warps.
+//   warps 4-11  epilogue (tensor-memory lane quadrant = warp % 4; half of the
+//               columns each)
+//   warps 12-27 decode: four groups of four warps, two per unit (below); with
+//               two groups a unit took 1.05 us, nearly all of it one group's
+//               latency
+// A unit of the pipeline is two K steps, decoded by two groups; the next unit by
+// the other two. Barriers: an A box lands on afull (five places); the decode
+// warps write their step's part of B and arrive on the even CTA's bready (three
+// units; both CTAs' sixteen warps, and the odd CTA's warp 1 for its A boxes);
+// the MMA thread waits for that and for its own boxes, issues eight MMAs and
+// commits once, to `done` of both CTAs, which frees the unit's A and B. `done`
+// has six barriers, a multiple of both rings' units and even, so that each wait
+// knows its phase although a group sees every other unit. A record is released
+// (rempty) by the decode warps that read it.
+// Tiles that would leave a last wave of the clusters mostly empty are split
+// along K evenly over all clusters; their f32 pieces go to the workspace and
+// join_kernel adds them in order and applies the epilogue.
 #include <algorithm>
 
 #include "fp4_internal.h"
@@ -36,42 +45,48 @@
 namespace aex {
 namespace fp4 {
 
-constexpr int kGThreads = 512;
-constexpr int kGStages = 5;
-constexpr int kGRecs = 3;
+constexpr int kGThreads = 896;
+constexpr int kGA = 5;      // places for A boxes, one K step each
+constexpr int kGB = 3;      // units (two steps) of decoded B
+constexpr int kGDone = 6;
+constexpr int kGRecs = 2;
 constexpr int kGTile = 128 * 64 * 2;  // one operand of one CTA and step
-constexpr int kGStage = 2 * kGTile;
+constexpr int kGOffB = kGA * kGTile;
 constexpr int kGRecSlot = rec_bytes(AEX_FP4_NV);
-constexpr int kGOffRec = kGStages * kGStage;
+constexpr int kGOffRec = kGOffB + kGB * 2 * kGTile;
 constexpr int kGOffBar = kGOffRec + kGRecs * kGRecSlot;
-// afull[S], bready[S], empty[S], rfull[R], rempty[R], accf[2], acce[2], drain
-constexpr int kGNumBars = 3 * kGStages + 2 * kGRecs + 5;
+// afull[A], bready[B], done[6], rfull[R], rempty[R], accf[2], acce[2], drain
+constexpr int kGNumBars = kGA + kGB + kGDone + 2 * kGRecs + 5;
 constexpr int kGSmem = kGOffBar + kGNumBars * 8 + 16 + 1024;
 static_assert(kGSmem <= 232448, "fp4 GEMM exceeds the shared-memory limit");
 
 enum GemmMode : int { kPlain = 0, kGatedFwd = 1, kGatedGrad = 2, kDgrad = 3 };
 
-struct GemmParams {
-  const uint8_t* w0;
-  const uint8_t* w1;
-  int k_blocks;  // records along the columns of a weight
-  int n_tiles;   // records along its rows
-  int m_tiles, tiles;
-  int recs;      // records per tile and CTA (dgrad: of both weights)
-  TileOut o;
-  // gated gradient
+// The gated projection's gradients in place of its result.
+struct GradOut {
   float fold0, fold1;  // the tensor scales that dg and du take on
   const uint16_t* dh;
   int64_t lddh;
   uint16_t* dg;
   uint16_t* du;
   int64_t ldg;
+};
+
+struct GemmParams {
+  const uint8_t* w0;
+  const uint8_t* w1;
+  int k_blocks;  // records along the columns of a weight
+  int n_tiles;   // records along its rows
+  int recs;      // records per tile and CTA (dgrad: of both weights)
+  TileWork work;
+  TileOut o;
+  GradOut grad;
   int* status;
 };
 
 // dg, du of 8 columns (col a multiple of 8) from g, u (already scaled).
-__device__ __forceinline__ void grad8(const GemmParams& p, int64_t row, int col, const float* g, const float* u) {
-  const int left = p.o.cols - col;
+__device__ __forceinline__ void grad8(const TileOut& o, const GradOut& p, int64_t row, int col, const float* g, const float* u) {
+  const int left = o.cols - col;
   if (left <= 0) return;
   const uint16_t* src = p.dh + row * p.lddh + col;
   uint32_t d[4];
@@ -91,9 +106,9 @@ __device__ __forceinline__ void grad8(const GemmParams& p, int64_t row, int col,
     for (int e = 0; e < 2; ++e) {
       const float gi = g[2 * i + e], ui = u[2 * i + e];
       const float dv = e ? bf16hi_to_f32(d[i]) : bf16lo_to_f32(d[i]);
-      const float sg = sigmoid<true>(sigmoid_arg(gi, p.o.activation));
+      const float sg = sigmoid<true>(sigmoid_arg(gi, o.activation));
       const float act = gi * sg;
-      a[e] = dv * ui * fmaf(act * (1.f - sg), sigmoid_arg_slope(gi, p.o.activation), sg) * p.fold0;
+      a[e] = dv * ui * fmaf(act * (1.f - sg), sigmoid_arg_slope(gi, o.activation), sg) * p.fold0;
       b[e] = dv * act * p.fold1;
     }
     og[i] = pack_bf16x2(a[0], a[1]);
@@ -112,9 +127,9 @@ __global__ void __launch_bounds__(kGThreads, 1)
   uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
   uint64_t* bars = reinterpret_cast<uint64_t*>(smem + kGOffBar);
   uint64_t* afull = bars;
-  uint64_t* bready = afull + kGStages;
-  uint64_t* empty = bready + kGStages;
-  uint64_t* rfull = empty + kGStages;
+  uint64_t* bready = afull + kGA;
+  uint64_t* done = bready + kGB;
+  uint64_t* rfull = done + kGDone;
   uint64_t* rempty = rfull + kGRecs;
   uint64_t* accf = rempty + kGRecs;
   uint64_t* acce = accf + 2;
@@ -123,7 +138,7 @@ __global__ void __launch_bounds__(kGThreads, 1)
   __shared__ int abort_flag;
   constexpr bool kBack = kMode == kDgrad;
   constexpr int kRec = rec_bytes(kFormat);
-  constexpr int kSteps = kBack ? 2 : 4;  // K steps per record
+  constexpr int kUnits = kBack ? 1 : 2;  // units (two K steps) per record
 
   const int warp = static_cast<int>(warp_id_uniform());
   const int lane = static_cast<int>(lane_id());
@@ -133,18 +148,16 @@ __global__ void __launch_bounds__(kGThreads, 1)
 
   if (threadIdx.x == 0) {
     abort_flag = 0;
-    for (int s = 0; s < kGStages; ++s) {
-      mbar_init(&afull[s], 1);
-      mbar_init(&bready[s], 2 * 4);
-      mbar_init(&empty[s], 1);
-    }
+    for (int s = 0; s < kGA; ++s) mbar_init(&afull[s], 1);
+    for (int s = 0; s < kGB; ++s) mbar_init(&bready[s], 2 * 8 + 1);
+    for (int s = 0; s < kGDone; ++s) mbar_init(&done[s], 1);
     for (int s = 0; s < kGRecs; ++s) {
       mbar_init(&rfull[s], 1);
-      mbar_init(&rempty[s], 8);
+      mbar_init(&rempty[s], kBack ? 8 : 16);
     }
     for (int b = 0; b < 2; ++b) {
       mbar_init(&accf[b], 1);
-      mbar_init(&acce[b], 2 * 4);
+      mbar_init(&acce[b], 2 * 8);
     }
     mbar_init(drain, 1);
     fence_barrier_init();
@@ -158,57 +171,58 @@ __global__ void __launch_bounds__(kGThreads, 1)
     if (kBack) prefetch_tmap(&tm1);
   }
   tc_fence_before();
-  cluster_sync_all();
+  __syncthreads();
+  // The producers touch this CTA's barriers alone: they start at once and take part in the cluster's barrier when done.
+  cluster_arrive();
+  if (warp != 0 && warp != 3) cluster_wait();
   tc_fence_after();
   const uint32_t tmem = *tmem_slot;
-  const int steps = p.recs * kSteps;
 
   if (warp == 0) {
     if (lane == 0) {
       // ------------------------------------------------------ A producer
-      const uint32_t empty0 = smem_u32(&empty[0]);
-      const uint32_t peer_empty0 = mapa_shared(empty0, 1);
-      uint32_t s = 0, ph = 0;
-      int g = 0;
+      const uint32_t done0 = smem_u32(&done[0]);
+      int g = 0;  // K steps so far
       bool ok = true;
-      for (int t = cluster; t < p.tiles && ok; t += clusters) {
-        const int row0 = (t % p.m_tiles) * 256 + static_cast<int>(rank) * 128;
-        for (int k = 0; k < steps; ++k, ++g) {
-          if (g >= kGStages) {
-            if (!mbar_wait_cl(empty0 + 8 * s, ph ^ 1, &abort_flag, p.status, kDevTimeoutTma)) {
+      TilePiece t;
+      for (int i = 0; ok && p.work.piece(cluster, clusters, p.recs, i, &t); ++i) {
+        const int row0 = t.mt * 256 + static_cast<int>(rank) * 128;
+        for (int k = t.r0 * kUnits * 2; k < t.r1 * kUnits * 2; ++k, ++g) {
+          if (g >= kGA) {
+            const int u = (g - kGA) >> 1;  // the unit that used this place
+            if (!mbar_wait_cl(done0 + 8 * (u % kGDone), (u / kGDone) & 1, &abort_flag, p.status, kDevTimeoutTma)) {
               ok = false;
               break;
             }
-            if (rank == 0) mbar_arrive_cluster(peer_empty0 + 8 * s);
           }
+          const int s = g % kGA;
           mbar_arrive_expect_tx(&afull[s], kGTile);
           // dgrad: the second weight's rows follow the first's (p.n_tiles records of two steps)
           const bool second = kBack && k >= 2 * p.n_tiles;
-          tma_load_2d(smem + s * kGStage, second ? &tm1 : &tm0, &afull[s], (second ? k - 2 * p.n_tiles : k) * 64, row0);
-          if (++s == kGStages) {
-            s = 0;
-            ph ^= 1;
-          }
+          tma_load_2d(smem + s * kGTile, second ? &tm1 : &tm0, &afull[s], (second ? k - 2 * p.n_tiles : k) * 64, row0);
         }
       }
       if (!ok) {
-        for (int j = (g > kGStages ? g - kGStages : 0); j < g; ++j) {
-          const uint32_t a = smem_u32(&afull[j % kGStages]);
+        // The copies in flight land before the CTA can exit.
+        for (int j = (g > kGA ? g - kGA : 0); j < g; ++j) {
+          const uint32_t a = smem_u32(&afull[j % kGA]);
           const uint64_t t0 = globaltimer_ns();
-          while (!mbar_try_wait(a, (j / kGStages) & 1) && globaltimer_ns() - t0 < kWaitTimeoutNs) {
+          while (!mbar_try_wait(a, (j / kGA) & 1) && globaltimer_ns() - t0 < kWaitTimeoutNs) {
           }
         }
       }
     }
+    __syncwarp();
+    cluster_wait();
   } else if (warp == 3) {
     if (lane == 0) {
       // ------------------------------------------------- record producer
       uint32_t s = 0, ph = 0;
       int g = 0;
       bool ok = true;
-      for (int t = cluster; t < p.tiles && ok; t += clusters) {
-        const int nt = t / p.m_tiles;
-        for (int i = 0; i < p.recs; ++i, ++g) {
+      TilePiece t;
+      for (int i = 0; ok && p.work.piece(cluster, clusters, p.recs, i, &t); ++i) {
+        for (int r = t.r0; r < t.r1; ++r, ++g) {
           if (g >= kGRecs && !mbar_wait(&rempty[s], ph ^ 1, &abort_flag, p.status, kDevTimeoutProducer)) {
             ok = false;
             break;
@@ -216,16 +230,16 @@ __global__ void __launch_bounds__(kGThreads, 1)
           const uint8_t* w = p.w0;
           int rt, kb;
           if (kBack) {
-            const bool second = i >= p.n_tiles;
+            const bool second = r >= p.n_tiles;
             if (second) w = p.w1;
-            rt = second ? i - p.n_tiles : i;
-            kb = nt;
+            rt = second ? r - p.n_tiles : r;
+            kb = t.nt;
           } else {
-            kb = i;
+            kb = r;
             if (kMode == kPlain) {
-              rt = min(2 * nt + static_cast<int>(rank), p.n_tiles - 1);  // an odd last tile: columns nobody stores
+              rt = min(2 * t.nt + static_cast<int>(rank), p.n_tiles - 1);  // an odd last tile: columns nobody stores
             } else {
-              rt = nt;
+              rt = t.nt;
               if (rank) w = p.w1;
             }
           }
@@ -247,20 +261,41 @@ __global__ void __launch_bounds__(kGThreads, 1)
         }
       }
     }
+    __syncwarp();
+    cluster_wait();
   } else if (warp == 1) {
-    if (lane == 0 && rank == 0) {
+    if (lane == 0 && rank == 1) {
+      // ------------------------------------- "A landed" of the odd CTA
+      const uint32_t afull0 = smem_u32(&afull[0]);
+      const uint32_t lead = mapa_shared(smem_u32(&bready[0]), 0);
+      uint32_t as = 0, aph = 0, bs = 0;
+      bool ok = true;
+      TilePiece t;
+      for (int i = 0; ok && p.work.piece(cluster, clusters, p.recs, i, &t); ++i)
+        for (int u = t.r0 * kUnits; u < t.r1 * kUnits && ok; ++u) {
+#pragma unroll
+          for (int h = 0; h < 2; ++h) {
+            ok = ok && mbar_wait_cl(afull0 + 8 * as, aph, &abort_flag, p.status, kDevTimeoutTma);
+            if (++as == kGA) {
+              as = 0;
+              aph ^= 1;
+            }
+          }
+          if (ok) mbar_arrive_cluster(lead + 8 * bs);
+          if (++bs == kGB) bs = 0;
+        }
+    } else if (lane == 0) {
       // ------------------------------------------------------------- MMA
       constexpr uint32_t kIdesc = idesc_bf16_f32(256, 256, false, kBack);
       constexpr uint32_t kBStep = kBack ? 128 : 2;  // 16 K rows of an MN-major tile: 2 KB; of a K-major one: 32 B
       const uint32_t s0 = smem_u32(smem);
-      const uint32_t bready0 = smem_u32(&bready[0]);
-      const uint32_t empty0 = smem_u32(&empty[0]);
+      const uint32_t bready0 = smem_u32(&bready[0]), afull0 = smem_u32(&afull[0]), done0 = smem_u32(&done[0]);
       const uint64_t da0 = sdesc_sw128(s0, 16, 1024);
-      const uint64_t db0 = sdesc_sw128(s0 + kGTile, kBack ? 8192 : 16, 1024);
-      uint32_t s = 0, ph = 0;
-      int i = 0;
+      const uint64_t db0 = sdesc_sw128(s0 + kGOffB, kBack ? 8192 : 16, 1024);
+      uint32_t as = 0, aph = 0, bs = 0, bph = 0, ds = 0;
       bool ok = true;
-      for (int t = cluster; t < p.tiles && ok; t += clusters, ++i) {
+      TilePiece t;
+      for (int i = 0; ok && p.work.piece(cluster, clusters, p.recs, i, &t); ++i) {
         const int b = i & 1;
         if (i >= 2 && !mbar_wait_cl(smem_u32(&acce[b]), ((i >> 1) + 1) & 1, &abort_flag, p.status, kDevTimeoutMma)) {
           ok = false;
@@ -268,62 +303,73 @@ __global__ void __launch_bounds__(kGThreads, 1)
         }
         tc_fence_after();
         const uint32_t d = tmem + b * 256;
-        for (int k = 0; k < steps; ++k) {
-          if (!mbar_wait_cl(bready0 + 8 * s, ph, &abort_flag, p.status, kDevTimeoutMma)) {
+        const int n = (t.r1 - t.r0) * kUnits;
+        for (int u = 0; u < n; ++u) {
+          if (!mbar_wait_cl(bready0 + 8 * bs, bph, &abort_flag, p.status, kDevTimeoutMma)) {
             ok = false;
             break;
           }
-          tc_fence_after();
-          const uint64_t off = (s * kGStage) >> 4;
 #pragma unroll
-          for (int kk = 0; kk < 4; ++kk)
-            umma_ss_pair(d, da0 + off + kk * 2, db0 + off + kk * kBStep, kIdesc, (k > 0 || kk > 0) ? 1u : 0u);
-          umma_commit_pair(empty0 + 8 * s);
-          if (++s == kGStages) {
-            s = 0;
-            ph ^= 1;
+          for (int h = 0; h < 2; ++h) {
+            if (!mbar_wait_cl(afull0 + 8 * as, aph, &abort_flag, p.status, kDevTimeoutMma)) {
+              ok = false;
+              break;
+            }
+            tc_fence_after();
+            const uint64_t da = da0 + ((as * kGTile) >> 4), db = db0 + (((2 * bs + h) * kGTile) >> 4);
+#pragma unroll
+            for (int kk = 0; kk < 4; ++kk)
+              umma_ss_pair(d, da + kk * 2, db + kk * kBStep, kIdesc, (u > 0 || h > 0 || kk > 0) ? 1u : 0u);
+            if (++as == kGA) {
+              as = 0;
+              aph ^= 1;
+            }
+          }
+          if (!ok) break;
+          umma_commit_both(done0 + 8 * ds);
+          if (++ds == kGDone) ds = 0;
+          if (++bs == kGB) {
+            bs = 0;
+            bph ^= 1;
           }
         }
         if (!ok) break;
-        umma_commit_pair(smem_u32(&accf[b]));
-        umma_commit_pair(mapa_shared(smem_u32(&accf[b]), 1));
+        umma_commit_both(smem_u32(&accf[b]));
       }
       // Waited for on abort too: no MMA is in flight at the teardown.
       umma_commit_pair(smem_u32(drain));
       int no_abort = 0;
       mbar_wait_cl(smem_u32(drain), 0, &no_abort, p.status, kDevTimeoutMma);
     }
-  } else if (warp >= 4 && warp < 8) {
+  } else if (warp >= 4 && warp < 12) {
     // ------------------------------------------------------------ epilogue
-    const int quad = warp & 3;
-    int i = 0;
-    for (int t = cluster; t < p.tiles; t += clusters, ++i) {
-      const int nt = t / p.m_tiles;
+    const int quad = warp & 3, half = (warp - 4) >> 2;
+    TilePiece t;
+    for (int i = 0; p.work.piece(cluster, clusters, p.recs, i, &t); ++i) {
       const int b = i & 1;
       if (!mbar_wait_warp_cl(smem_u32(&accf[b]), (i >> 1) & 1, &abort_flag, p.status, kDevTimeoutEpilogue)) break;
       tc_fence_after();
-      const int64_t row = static_cast<int64_t>(t % p.m_tiles) * 256 + rank * 128 + quad * 32 + lane;
+      const int in_tile = static_cast<int>(rank) * 128 + quad * 32 + lane;
+      const int64_t row = static_cast<int64_t>(t.mt) * 256 + in_tile;
       const uint32_t tbase = tmem + (static_cast<uint32_t>(quad * 32) << 16) + b * 256;
-      if (kMode != kGatedGrad) {
-        tile_rows<kMode == kGatedFwd>(p.o, row, nt, tbase);
+      if (t.slot >= 0) {
+        store_piece(p.work, t.slot, in_tile, row < p.o.m, half, tbase);
+      } else if (kMode != kGatedGrad) {
+        tile_half<kMode == kGatedFwd>(p.o, row, t.nt, half, tbase);
       } else {
 #pragma unroll 1
-        for (int c0 = 0; c0 < 128; c0 += 32) {
-          uint32_t gr[32], ur[32];
-          tmem_ld32(tbase + c0, gr);
-          tmem_ld32(tbase + 128 + c0, ur);
-          tmem_wait_ld();
+        for (int c = 64 * half; c < 64 * half + 64; c += 16) {
+          float g[16], u[16];
+          tmem_read<16>(tbase + c, g);
+          tmem_read<16>(tbase + 128 + c, u);
           if (row < p.o.m) {
 #pragma unroll
-            for (int e = 0; e < 32; e += 8) {
-              float g[8], u[8];
-#pragma unroll
-              for (int i = 0; i < 8; ++i) {
-                g[i] = __uint_as_float(gr[e + i]) * p.o.alpha0;
-                u[i] = __uint_as_float(ur[e + i]) * p.o.alpha1;
-              }
-              grad8(p, row, nt * 128 + c0 + e, g, u);
+            for (int e = 0; e < 16; ++e) {
+              g[e] *= p.o.alpha0;
+              u[e] *= p.o.alpha1;
             }
+            grad8(p.o, p.grad, row, t.nt * 128 + c, g, u);
+            grad8(p.o, p.grad, row, t.nt * 128 + c + 8, g + 8, u + 8);
           }
         }
       }
@@ -331,36 +377,39 @@ __global__ void __launch_bounds__(kGThreads, 1)
       __syncwarp();
       if (lane == 0) mbar_arrive_cluster(mapa_shared(smem_u32(&acce[b]), 0));
     }
-  } else if (warp >= 8) {
+  } else if (warp >= 12) {
     // -------------------------------------------------------------- decode
-    const int group = (warp - 8) >> 2;
-    const int dt = ((warp - 8) & 3) * 32 + lane;
-    const uint32_t afull0 = smem_u32(&afull[0]);
+    const int group = ((warp - 12) >> 2) & 1, turn = (warp - 12) >> 3;
+    const int dt = (warp & 3) * 32 + lane;
+    const uint32_t done0 = smem_u32(&done[0]);
     const uint32_t bready_lead0 = mapa_shared(smem_u32(&bready[0]), 0);
-    uint32_t s = 0, ph = 0, rs = 0, rph = 0;
+    uint32_t bs = 0, ds = kGDone - kGB, dph = 1, rs = 0, rph = 0;  // ds: the unit kGB before this one
+    int g = 0;                                                     // units so far
     bool ok = true;
-    for (int t = cluster; t < p.tiles && ok; t += clusters) {
-      for (int k = 0; k < steps; ++k) {
-        const uint32_t cs = s, cph = ph, crs = rs, crph = rph;
-        if (++s == kGStages) {
-          s = 0;
-          ph ^= 1;
+    TilePiece t;
+    for (int i = 0; ok && p.work.piece(cluster, clusters, p.recs, i, &t); ++i) {
+      const int n = (t.r1 - t.r0) * kUnits;
+      for (int u = 0; u < n; ++u, ++g) {
+        const uint32_t cb = bs, cds = ds, cdph = dph, crs = rs, crph = rph;
+        if (++bs == kGB) bs = 0;
+        if (++ds == kGDone) {
+          ds = 0;
+          dph ^= 1;
         }
-        const bool last_of_rec = (k & (kSteps - 1)) == kSteps - 1;
-        if (last_of_rec && ++rs == kGRecs) {
+        if ((u & (kUnits - 1)) == kUnits - 1 && ++rs == kGRecs) {
           rs = 0;
           rph ^= 1;
         }
-        if ((k & 1) != group) continue;  // steps per tile are even: the groups keep alternating
-        if (!mbar_wait_warp(&rfull[crs], crph, &abort_flag, p.status, kDevTimeoutProducer) ||
-            !mbar_wait_warp_cl(afull0 + 8 * cs, cph, &abort_flag, p.status, kDevTimeoutProducer)) {
+        if ((g & 1) != turn) continue;
+        const int k = 2 * u + group;  // this group's step, from the piece's first
+        if (!mbar_wait_warp(&rfull[crs], crph, &abort_flag, p.status, kDevTimeoutProducer)) {
           ok = false;
           break;
         }
         const uint8_t* rec = smem + kGOffRec + crs * kGRecSlot;
         // r: row of the record; cp: its 64-column part; dst: that row in B
         int r, cp;
-        uint8_t* dst = smem + cs * kGStage + kGTile;
+        uint8_t* dst = smem + kGOffB + (2 * cb + group) * kGTile;
         if (kBack) {
           r = (k & 1) * 64 + (dt & 63);
           cp = 2 * static_cast<int>(rank) + (dt >> 6);
@@ -378,23 +427,35 @@ __global__ void __launch_bounds__(kGThreads, 1)
           sc = *reinterpret_cast<const uint32_t*>(rec + scale_off(r, cp));
         else
           sc = *reinterpret_cast<const uint16_t*>(rec + scale_off(r, cp >> 1) + (cp & 1) * 2);
-        // This warp's last read of the record: group 1 takes its last step, group 0 the one before.
-        if ((k & (kSteps - 1)) >= kSteps - 2) {
-          __syncwarp();
-          if (lane == 0) mbar_arrive_addr(smem_u32(&rempty[crs]));
+        __syncwarp();
+        if (lane == 0) mbar_arrive_addr(smem_u32(&rempty[crs]));  // this warp's only read of the record
+        if (g >= kGB && !mbar_wait_warp_cl(done0 + 8 * cds, cdph, &abort_flag, p.status, kDevTimeoutMma)) {
+          ok = false;
+          break;
         }
         const uint32_t ws[8] = {c0.x, c0.y, c0.z, c0.w, c1.x, c1.y, c1.z, c1.w};
+        if (kFormat == AEX_FP4_MX && (sc & 0xFFu) <= 128u && (sc >> 8) <= 128u) {
 #pragma unroll
-        for (int j = 0; j < 8; ++j) {
-          // nvfp4: a scale every two words, mxfp4: every four
-          const uint32_t s2 = scale_pair<kFormat>((sc >> (kFormat == AEX_FP4_NV ? 8 * (j >> 1) : 8 * (j >> 2))) & 0xFFu);
-          *reinterpret_cast<uint4*>(dst + ((j ^ sw) << 4)) =
-              make_uint4(decode_pair<kFormat>(ws[j], 0, s2), decode_pair<kFormat>(ws[j], 1, s2),
-                         decode_pair<kFormat>(ws[j], 2, s2), decode_pair<kFormat>(ws[j], 3, s2));
+          for (int j = 0; j < 8; ++j) {
+            const uint32_t s2 = mx_scale_from_tiny(j < 4 ? sc & 0xFFu : sc >> 8);
+            *reinterpret_cast<uint4*>(dst + ((j ^ sw) << 4)) =
+                make_uint4(mul_bf16x2(code_pair_tiny(ws[j], 0), s2), mul_bf16x2(code_pair_tiny(ws[j], 1), s2),
+                           mul_bf16x2(code_pair_tiny(ws[j], 2), s2), mul_bf16x2(code_pair_tiny(ws[j], 3), s2));
+          }
+        } else {
+#pragma unroll
+          for (int j = 0; j < 8; ++j) {
+            // nvfp4: a scale every two words, mxfp4: every four
+            const uint32_t s2 =
+                scale_pair<kFormat>((sc >> (kFormat == AEX_FP4_NV ? 8 * (j >> 1) : 8 * (j >> 2))) & 0xFFu);
+            *reinterpret_cast<uint4*>(dst + ((j ^ sw) << 4)) =
+                make_uint4(decode_pair<kFormat>(ws[j], 0, s2), decode_pair<kFormat>(ws[j], 1, s2),
+                           decode_pair<kFormat>(ws[j], 2, s2), decode_pair<kFormat>(ws[j], 3, s2));
+          }
         }
         fence_async_shared();
         __syncwarp();
-        if (lane == 0) mbar_arrive_cluster(bready_lead0 + 8 * cs);
+        if (lane == 0) mbar_arrive_cluster(bready_lead0 + 8 * cb);
       }
     }
   }
@@ -407,6 +468,24 @@ __global__ void __launch_bounds__(kGThreads, 1)
   }
 }
 
+template <int kMode>
+__global__ void __launch_bounds__(256) join_kernel(const __grid_constant__ GemmParams p, int clusters) {
+  constexpr bool kGated = kMode == kGatedFwd || kMode == kGatedGrad;
+  join_tile<kGated>(p.work, p.recs, clusters, p.o.m, [&](int64_t row, int nt, int c, const float* v, const float* u) {
+    if (kMode == kGatedGrad) {
+      float g[8], h[8];
+#pragma unroll
+      for (int e = 0; e < 8; ++e) {
+        g[e] = v[e] * p.o.alpha0;
+        h[e] = u[e] * p.o.alpha1;
+      }
+      grad8(p.o, p.grad, row, nt * 128 + c, g, h);
+    } else {
+      finish<kGated, 8>(p.o, row, nt, c, v, u);
+    }
+  });
+}
+
 namespace {
 
 int x_map(aex_ctx* ctx, CUtensorMap* tm, const void* x, int64_t ldx, int rows, int cols) {
@@ -417,45 +496,33 @@ int x_map(aex_ctx* ctx, CUtensorMap* tm, const void* x, int64_t ldx, int rows, i
 }
 
 template <int kFormat, int kMode>
-int launch_gemm(aex_ctx* ctx, const CUtensorMap& tm0, const CUtensorMap& tm1, GemmParams p, int64_t col_tiles,
-                cudaStream_t s) {
-  p.m_tiles = (p.o.m - 1) / 256 + 1;
-  const int64_t tiles = p.m_tiles * col_tiles;
-  if (tiles > 0x3FFFFFFF) return set_error(ctx, AEX_ERR_UNSUPPORTED, "fp4 GEMM: %lld output tiles", (long long)tiles);
-  p.tiles = static_cast<int>(tiles);
+int launch_gemm(aex_ctx* ctx, const CUtensorMap& tm0, const CUtensorMap& tm1, GemmParams p, const TilePlan& plan,
+                void* pieces, cudaStream_t s) {
+  p.work.m_tiles = plan.m_tiles;
+  p.work.whole = plan.whole;
+  p.work.split = plan.split;
+  p.work.rows = plan.rows;
+  p.work.pieces = static_cast<float*>(pieces);
   p.status = ctx->d_status;
   auto kern = gemm_kernel<kFormat, kMode>;
   static SmemOptIn opt_in;
   if (int r = opt_in(ctx, reinterpret_cast<const void*>(kern), kGSmem)) return r;
-  cudaLaunchConfig_t cfg{};
-  cfg.blockDim = dim3(kGThreads, 1, 1);
-  cfg.dynamicSmemBytes = kGSmem;
-  cfg.stream = s;
-  cudaLaunchAttribute attr[1];
-  attr[0].id = cudaLaunchAttributeClusterDimension;
-  attr[0].val.clusterDim.x = 2;
-  attr[0].val.clusterDim.y = 1;
-  attr[0].val.clusterDim.z = 1;
-  cfg.attrs = attr;
-  cfg.numAttrs = 1;
-  // One CTA per SM (shared memory); clusters of two that fit at once.
-  if (ctx->fp4_clusters <= 0) {
-    cfg.gridDim = dim3(2 * (ctx->sm_count / 2), 1, 1);
-    int n = 0;
-    AEX_CUDA_TRY(ctx, cudaOccupancyMaxActiveClusters(&n, kern, &cfg));
-    if (n <= 0) return set_error(ctx, AEX_ERR_UNSUPPORTED, "the fp4 CTA-pair GEMM cannot be resident on this device");
-    ctx->fp4_clusters = n;
+  if (int r = launch_pairs(ctx, reinterpret_cast<const void*>(kern), plan.clusters, kGThreads, kGSmem, s,
+                           const_cast<CUtensorMap*>(&tm0), const_cast<CUtensorMap*>(&tm1), &p))
+    return r;
+  if (plan.split) {
+    constexpr int kGroups = kMode == kGatedFwd || kMode == kGatedGrad ? 16 : 32;
+    join_kernel<kMode><<<(plan.split * plan.rows * kGroups + 255) / 256, 256, 0, s>>>(p, plan.clusters);
+    return check_launch(ctx, "fp4 join_kernel");
   }
-  cfg.gridDim = dim3(2 * std::min(p.tiles, ctx->fp4_clusters), 1, 1);
-  AEX_CUDA_TRY(ctx, cudaLaunchKernelEx(&cfg, kern, tm0, tm1, p));
-  return check_launch(ctx, "fp4 gemm_kernel");
+  return AEX_OK;
 }
 
 template <int kMode>
 int by_format(aex_ctx* ctx, int format, const CUtensorMap& tm0, const CUtensorMap& tm1, const GemmParams& p,
-              int64_t col_tiles, cudaStream_t s) {
-  return format == AEX_FP4_MX ? launch_gemm<AEX_FP4_MX, kMode>(ctx, tm0, tm1, p, col_tiles, s)
-                              : launch_gemm<AEX_FP4_NV, kMode>(ctx, tm0, tm1, p, col_tiles, s);
+              const TilePlan& plan, void* pieces, cudaStream_t s) {
+  return format == AEX_FP4_MX ? launch_gemm<AEX_FP4_MX, kMode>(ctx, tm0, tm1, p, plan, pieces, s)
+                              : launch_gemm<AEX_FP4_NV, kMode>(ctx, tm0, tm1, p, plan, pieces, s);
 }
 
 GemmParams weight_params(const aex_fp4weight* w0, const aex_fp4weight* w1) {
@@ -471,16 +538,47 @@ float unit_of(int format) {
   return format == AEX_FP4_MX ? decode_unit<AEX_FP4_MX>() : decode_unit<AEX_FP4_NV>();
 }
 
+// What a join costs, in records of the main loop (about 3 us).
+constexpr int kJoinForward = 3, kJoinBackward = 6;
+
 }  // namespace
+
+TilePlan plan_gemm(const aex_fp4weight* w, bool gated, int m) {
+  return plan_tiles(w->clusters, m, gated ? w->n_tiles : (w->n_tiles + 1) / 2, w->k_blocks, kJoinForward);
+}
+TilePlan plan_dgrad(const aex_fp4weight* w, bool two, int m) {
+  return plan_tiles(w->clusters, m, w->k_blocks, w->n_tiles * (two ? 2 : 1), kJoinBackward);
+}
+
+int gemm_clusters(aex_ctx* ctx, int* out) {
+  auto kern = gemm_kernel<AEX_FP4_NV, kPlain>;
+  AEX_CUDA_TRY(ctx, cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, kGSmem));
+  cudaLaunchConfig_t cfg{};
+  cfg.gridDim = dim3(2 * (ctx->sm_count / 2), 1, 1);
+  cfg.blockDim = dim3(kGThreads, 1, 1);
+  cfg.dynamicSmemBytes = kGSmem;
+  cudaLaunchAttribute attr[1];
+  attr[0].id = cudaLaunchAttributeClusterDimension;
+  attr[0].val.clusterDim.x = 2;
+  attr[0].val.clusterDim.y = 1;
+  attr[0].val.clusterDim.z = 1;
+  cfg.attrs = attr;
+  cfg.numAttrs = 1;
+  int n = 0;
+  AEX_CUDA_TRY(ctx, cudaOccupancyMaxActiveClusters(&n, kern, &cfg));
+  if (n <= 0) return set_error(ctx, AEX_ERR_UNSUPPORTED, "the fp4 CTA-pair GEMM cannot be resident on this device");
+  *out = n;
+  return AEX_OK;
+}
 
 int run_gemm(aex_ctx* ctx, const Job& j, cudaStream_t s) {
   const aex_fp4weight* w = j.w0;
   CUtensorMap tm;
   if (int r = x_map(ctx, &tm, j.x, j.ldx, j.m, w->k)) return r;
   GemmParams p = weight_params(w, j.w1);
+  p.recs = w->k_blocks;
   p.o.m = j.m;
   p.o.cols = w->n;
-  p.recs = w->k_blocks;
   p.o.alpha0 = unit_of(w->format) * w->tensor_scale;
   p.o.alpha1 = j.w1 ? unit_of(w->format) * j.w1->tensor_scale : 0.f;
   p.o.activation = j.activation;
@@ -488,49 +586,51 @@ int run_gemm(aex_ctx* ctx, const Job& j, cudaStream_t s) {
   p.o.ldy = j.ldy;
   p.o.y_f32 = j.y_f32;
   p.o.vec = vec_ok(j.y, j.ldy, j.y_f32);
-  return j.w1 ? by_format<kGatedFwd>(ctx, w->format, tm, tm, p, w->n_tiles, s)
-              : by_format<kPlain>(ctx, w->format, tm, tm, p, (w->n_tiles + 1) / 2, s);
+  const TilePlan plan = plan_gemm(w, j.w1 != nullptr, j.m);
+  return j.w1 ? by_format<kGatedFwd>(ctx, w->format, tm, tm, p, plan, j.pieces, s)
+              : by_format<kPlain>(ctx, w->format, tm, tm, p, plan, j.pieces, s);
 }
 
 int run_gated_grad(aex_ctx* ctx, const aex_fp4weight* wg, const aex_fp4weight* wu, int activation, const void* x,
                    int64_t ldx, int m, const void* dh, int64_t lddh, uint16_t* dg, uint16_t* du, int64_t ld,
-                   cudaStream_t s) {
+                   void* pieces, cudaStream_t s) {
   CUtensorMap tm;
   if (int r = x_map(ctx, &tm, x, ldx, m, wg->k)) return r;
   GemmParams p = weight_params(wg, wu);
+  p.recs = wg->k_blocks;
   p.o.m = m;
   p.o.cols = wg->n;
-  p.recs = wg->k_blocks;
   p.o.alpha0 = unit_of(wg->format) * wg->tensor_scale;
   p.o.alpha1 = unit_of(wg->format) * wu->tensor_scale;
-  p.fold0 = wg->tensor_scale;
-  p.fold1 = wu->tensor_scale;
   p.o.activation = activation;
-  p.dh = static_cast<const uint16_t*>(dh);
-  p.lddh = lddh;
-  p.dg = dg;
-  p.du = du;
-  p.ldg = ld;
-  return by_format<kGatedGrad>(ctx, wg->format, tm, tm, p, wg->n_tiles, s);
+  p.grad.fold0 = wg->tensor_scale;
+  p.grad.fold1 = wu->tensor_scale;
+  p.grad.dh = static_cast<const uint16_t*>(dh);
+  p.grad.lddh = lddh;
+  p.grad.dg = dg;
+  p.grad.du = du;
+  p.grad.ldg = ld;
+  return by_format<kGatedGrad>(ctx, wg->format, tm, tm, p, plan_gemm(wg, true, m), pieces, s);
 }
 
 int run_dgrad(aex_ctx* ctx, const aex_fp4weight* w0, const aex_fp4weight* w1, const void* d0, int64_t ld0,
-              const void* d1, int64_t ld1, int m, float alpha, void* dx, bool dx_f32, int64_t lddx, cudaStream_t s) {
+              const void* d1, int64_t ld1, int m, float alpha, void* dx, bool dx_f32, int64_t lddx, void* pieces,
+              cudaStream_t s) {
   CUtensorMap tm0, tm1;
   if (int r = x_map(ctx, &tm0, d0, ld0, m, w0->n)) return r;
   tm1 = tm0;
   if (w1)
     if (int r = x_map(ctx, &tm1, d1, ld1, m, w1->n)) return r;
   GemmParams p = weight_params(w0, w1);
+  p.recs = w0->n_tiles * (w1 ? 2 : 1);
   p.o.m = m;
   p.o.cols = w0->k;
-  p.recs = w0->n_tiles * (w1 ? 2 : 1);
   p.o.alpha0 = unit_of(w0->format) * alpha;
   p.o.y = dx;
   p.o.ldy = lddx;
   p.o.y_f32 = dx_f32;
   p.o.vec = vec_ok(dx, lddx, dx_f32);
-  return by_format<kDgrad>(ctx, w0->format, tm0, tm1, p, w0->k_blocks, s);
+  return by_format<kDgrad>(ctx, w0->format, tm0, tm1, p, plan_dgrad(w0, w1 != nullptr, m), pieces, s);
 }
 
 }  // namespace fp4

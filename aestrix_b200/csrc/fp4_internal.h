@@ -17,6 +17,7 @@ struct aex_fp4weight {
   float tensor_scale = 1.f;
   int n_tiles = 0;           // ceil(n / 128)
   int k_blocks = 0;          // ceil(k / 256)
+  int clusters = 0;          // CTA pairs of the GEMMs that the device holds at once (one CTA per SM)
   uint8_t* records = nullptr;
   size_t bytes = 0;
 };
@@ -92,8 +93,59 @@ struct Job {
   void* y;
   bool y_f32;
   int64_t ldy;
-  uint8_t* workspace;  // records of the quantized x
+  uint8_t* x_records;  // workspace: the quantized x, and the pieces of split tiles
+  void* pieces;
 };
+
+// How a GEMM's 256 x 256 output tiles go to `clusters` CTA pairs (TileWork).
+struct TilePlan {
+  int clusters = 0;  // of the launch
+  int m_tiles = 0, whole = 0, split = 0;
+  int rows = 0;       // of a piece
+  size_t bytes = 0;   // of all pieces
+};
+
+// `recs` records along K per tile. Tiles that do not fill a last wave of the clusters are split when the wave's
+// records, dealt out over all clusters, and a join (in records) take less than the wave.
+inline TilePlan plan_tiles(int clusters, int m, int64_t col_tiles, int recs, int join) {
+  TilePlan p;
+  p.m_tiles = (m - 1) / 256 + 1;
+  const int64_t tiles = p.m_tiles * col_tiles;
+  const int64_t left = tiles % clusters;
+  const int64_t shared = (left * recs + clusters - 1) / clusters;
+  if (tiles > 0x3FFFFFFF) return p;  // refused by the caller
+  p.split = left && shared + join < recs && left * recs * clusters < 0x7FFFFFFF ? static_cast<int>(left) : 0;
+  p.whole = static_cast<int>(tiles) - p.split;
+  p.clusters = p.split || tiles > clusters ? clusters : static_cast<int>(tiles);
+  p.rows = m < 256 ? m : 256;
+  if (p.split) p.bytes = static_cast<size_t>(clusters + p.split) * p.rows * 256 * sizeof(float);
+  return p;
+}
+TilePlan plan_gemm(const aex_fp4weight* w, bool gated, int m);
+TilePlan plan_dgrad(const aex_fp4weight* w, bool two, int m);
+TilePlan plan_block(const aex_fp4weight* w, bool gated, int m);
+int gemm_clusters(aex_ctx* ctx, int* out);
+
+// One launch of CTA pairs.
+template <typename... Args>
+int launch_pairs(aex_ctx* ctx, const void* kernel, int clusters, int threads, int smem, cudaStream_t s, Args*... args) {
+  cudaLaunchConfig_t cfg{};
+  cfg.gridDim = dim3(2 * clusters, 1, 1);
+  cfg.blockDim = dim3(threads, 1, 1);
+  cfg.dynamicSmemBytes = smem;
+  cfg.stream = s;
+  cudaLaunchAttribute attr[1];
+  attr[0].id = cudaLaunchAttributeClusterDimension;
+  attr[0].val.clusterDim.x = 2;
+  attr[0].val.clusterDim.y = 1;
+  attr[0].val.clusterDim.z = 1;
+  cfg.attrs = attr;
+  cfg.numAttrs = 1;
+  void* argv[] = {args...};
+  AEX_CUDA_TRY(ctx, cudaLaunchKernelExC(&cfg, kernel, argv));
+  return check_launch(ctx, "fp4 GEMM");
+}
+
 // The few-rows kernel takes up to 48 columns of its 8-column operand: rows that are bf16 or quantized, or f32 rows at
 // three columns each. No workspace.
 constexpr int kSmallRows = 32;
@@ -101,15 +153,16 @@ constexpr int kSmallRowsF32 = 16;
 int run_small(aex_ctx* ctx, const Job& j, cudaStream_t s);
 // Any number of bf16 rows: dequantizing GEMM.
 int run_gemm(aex_ctx* ctx, const Job& j, cudaStream_t s);
-// Quantized rows (records in j.workspace): block-scaled GEMM.
+// Quantized rows (x_records): block-scaled GEMM.
 int run_block(aex_ctx* ctx, const Job& j, cudaStream_t s);
 // dx = alpha (d0 . W0 + d1 . W1) (w1, d1 NULL: one product), d bf16 [m, n].
 int run_dgrad(aex_ctx* ctx, const aex_fp4weight* w0, const aex_fp4weight* w1, const void* d0, int64_t ld0,
-              const void* d1, int64_t ld1, int m, float alpha, void* dx, bool dx_f32, int64_t lddx, cudaStream_t s);
+              const void* d1, int64_t ld1, int m, float alpha, void* dx, bool dx_f32, int64_t lddx, void* pieces,
+              cudaStream_t s);
 // dg = ts_g dh u act'(g), du = ts_u dh act(g), bf16 [m, n] at row pitch ld, g and u from x.
 int run_gated_grad(aex_ctx* ctx, const aex_fp4weight* wg, const aex_fp4weight* wu, int activation, const void* x,
                    int64_t ldx, int m, const void* dh, int64_t lddh, uint16_t* dg, uint16_t* du, int64_t ld,
-                   cudaStream_t s);
+                   void* pieces, cudaStream_t s);
 
 }  // namespace fp4
 }  // namespace aex

@@ -323,6 +323,8 @@ int aex_fp4weight_create(aex_ctx* ctx, const uint8_t* codes, const uint8_t* scal
     return set_error(ctx, AEX_ERR_UNSUPPORTED, "fp4 weight of %d x %d is too large", n, k);
   DeviceGuard dev(ctx);
   if (dev.rc) return dev.rc;
+  int clusters = 0;
+  if (int r = fp4::gemm_clusters(ctx, &clusters)) return r;
   auto* w = new (std::nothrow) aex_fp4weight();
   if (!w) return set_error(ctx, AEX_ERR_OOM, "host allocation failed");
   w->device = ctx->device;
@@ -331,6 +333,7 @@ int aex_fp4weight_create(aex_ctx* ctx, const uint8_t* codes, const uint8_t* scal
   w->format = format;
   w->tensor_scale = tensor_scale;
   w->n_tiles = static_cast<int>(n_tiles);
+  w->clusters = clusters;
   w->k_blocks = static_cast<int>(k_blocks);
   w->bytes = static_cast<size_t>(n_tiles * k_blocks) * fp4::rec_bytes(format);
   cudaError_t e = cudaMalloc(&w->records, w->bytes);

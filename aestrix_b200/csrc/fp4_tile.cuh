@@ -13,94 +13,213 @@ struct TileOut {
   void* y;
   int64_t ldy;
   int y_f32;
-  int vec;  // rows of y are whole 16-byte vectors
+  int vec;  // vec_ok
 };
 
-// 32 columns [col, col + 32) of one row.
-template <bool kF32>
-__device__ __forceinline__ void store32(const TileOut& p, int64_t row, int col, const float* v) {
-  if (kF32) {
-    float* o = static_cast<float*>(p.y) + row * p.ldy + col;
-    if (p.vec && col + 32 <= p.cols) {
-#pragma unroll
-      for (int i = 0; i < 32; i += 4)
-        *reinterpret_cast<float4*>(o + i) = make_float4(v[i], v[i + 1], v[i + 2], v[i + 3]);
-    } else {
-#pragma unroll
-      for (int i = 0; i < 32; ++i)
-        if (col + i < p.cols) o[i] = v[i];
-    }
-  } else {
-    uint16_t* o = static_cast<uint16_t*>(p.y) + row * p.ldy + col;
-    uint32_t pk[16];
-#pragma unroll
-    for (int i = 0; i < 16; ++i) pk[i] = pack_bf16x2(v[2 * i], v[2 * i + 1]);
-    if (p.vec && col + 32 <= p.cols) {
-#pragma unroll
-      for (int i = 0; i < 16; i += 4)
-        *reinterpret_cast<uint4*>(o + 2 * i) = make_uint4(pk[i], pk[i + 1], pk[i + 2], pk[i + 3]);
-    } else {
-#pragma unroll
-      for (int i = 0; i < 32; ++i)
-        if (col + i < p.cols) o[i] = static_cast<uint16_t>((i & 1) ? pk[i >> 1] >> 16 : pk[i >> 1] & 0xFFFFu);
-    }
-  }
-}
+// One cluster's share of an output tile: records [r0, r1) along K of tile
+// (mt, nt); slot >= 0: a piece of a split tile, -1: the whole of it.
+struct TilePiece {
+  int mt, nt, r0, r1, slot;
+};
 
-// A row's 256 accumulator columns starting at tensor-memory address tbase, as
-// columns [256 nt, ..) of y, or (gated) 128 of the gate and 128 of the up
-// projection as columns [128 nt, ..).
-template <bool kGated>
-__device__ __forceinline__ void tile_rows(const TileOut& p, int64_t row, int nt, uint32_t tbase) {
-  if (!kGated) {
-#pragma unroll 1
-    for (int c0 = 0; c0 < 256; c0 += 32) {
-      uint32_t r[32];
-      tmem_ld32(tbase + c0, r);
-      tmem_wait_ld();
-      const int col = nt * 256 + c0;
-      if (row < p.m && col < p.cols) {
-        float v[32];
-#pragma unroll
-        for (int e = 0; e < 32; ++e) v[e] = __uint_as_float(r[e]) * p.alpha0;
-        if (p.y_f32)
-          store32<true>(p, row, col, v);
-        else
-          store32<false>(p, row, col, v);
-      }
-    }
-  } else {
-#pragma unroll 1
-    for (int c0 = 0; c0 < 128; c0 += 32) {
-      uint32_t gr[32], ur[32];
-      tmem_ld32(tbase + c0, gr);
-      tmem_ld32(tbase + 128 + c0, ur);
-      tmem_wait_ld();
-      const int col = nt * 128 + c0;
-      if (row < p.m && col < p.cols) {
-        float v[32];
-        if (p.y_f32) {
-#pragma unroll
-          for (int e = 0; e < 32; ++e) {
-            const float g = __uint_as_float(gr[e]) * p.alpha0, u = __uint_as_float(ur[e]) * p.alpha1;
-            v[e] = g * sigmoid<false>(sigmoid_arg(g, p.activation)) * u;
-          }
-          store32<true>(p, row, col, v);
-        } else {
-#pragma unroll
-          for (int e = 0; e < 32; ++e) {
-            const float g = __uint_as_float(gr[e]) * p.alpha0, u = __uint_as_float(ur[e]) * p.alpha1;
-            v[e] = g * sigmoid<true>(sigmoid_arg(g, p.activation)) * u;
-          }
-          store32<false>(p, row, col, v);
+// The output tiles and who computes them. Tiles are numbered with the rows'
+// tiles fastest. The first `whole` go to the clusters in turn, one cluster
+// each; the records of the `split` others are dealt out evenly, in order, so
+// that a cluster gets at most the end of one tile and the start of the next.
+// The piece of split tile r that cluster c computes has slot c + r (from one
+// piece to the next, either c or r goes up by one).
+struct TileWork {
+  int m_tiles, whole, split;
+  int rows;  // rows of a slot
+  float* pieces;
+
+  // First record of cluster c's share; split * recs * clusters < 2^31 (plan_tiles), since 64-bit divisions at the
+  // start of every role cost over a microsecond.
+  __device__ int start(int c, int clusters, int recs) const { return split * recs * c / clusters; }
+  // The i-th piece of cluster c; false past the last.
+  __device__ bool piece(int c, int clusters, int recs, int i, TilePiece* t) const {
+    int n = 0;
+    t->r0 = 0;
+    t->r1 = recs;
+    t->slot = -1;
+    if (split > 0) {
+      const int u0 = start(c, clusters, recs), u1 = start(c + 1, clusters, recs);
+      if (u1 > u0) {
+        const int first = u0 / recs, last = (u1 - 1) / recs;
+        n = last - first + 1;
+        if (i < n) {
+          const int r = first + i;
+          if (i == 0) t->r0 = u0 - r * recs;
+          if (r == last) t->r1 = u1 - r * recs;
+          t->slot = c + r;
+          t->mt = (whole + r) % m_tiles;
+          t->nt = (whole + r) / m_tiles;
+          return true;
         }
       }
     }
+    const int at = c + (i - n) * clusters;
+    if (at >= whole) return false;
+    t->mt = at % m_tiles;
+    t->nt = at / m_tiles;
+    return true;
+  }
+};
+
+__device__ __forceinline__ void st_global_32(void* p, const uint32_t* v) {
+  asm volatile("st.global.v8.b32 [%0], {%1,%2,%3,%4,%5,%6,%7,%8};" ::"l"(p), "r"(v[0]), "r"(v[1]), "r"(v[2]), "r"(v[3]),
+               "r"(v[4]), "r"(v[5]), "r"(v[6]), "r"(v[7])
+               : "memory");
+}
+
+// kN (8 or 16) columns [c, c + kN) of a tile's row from their f32 sums (gated:
+// v of the gate, u of the up projection), columns 256 nt + c (gated: 128 nt + c)
+// of y. Each lane writes a row of its own: whole 32-byte sectors where y allows.
+template <bool kGated, int kN>
+__device__ __forceinline__ void finish(const TileOut& p, int64_t row, int nt, int c, const float* v, const float* u) {
+  const int col = nt * (kGated ? 128 : 256) + c;
+  if (col >= p.cols) return;
+  float o[kN];
+  if (!kGated) {
+#pragma unroll
+    for (int e = 0; e < kN; ++e) o[e] = v[e] * p.alpha0;
+  } else if (p.y_f32) {
+#pragma unroll
+    for (int e = 0; e < kN; ++e) {
+      const float g = v[e] * p.alpha0;
+      o[e] = g * sigmoid<false>(sigmoid_arg(g, p.activation)) * (u[e] * p.alpha1);
+    }
+  } else if (p.activation == AEX_ACT_SILU) {
+#pragma unroll
+    for (int e = 0; e < kN; ++e) {
+      const float g = v[e] * p.alpha0;
+      o[e] = g * sigmoid<true>(g) * (u[e] * p.alpha1);
+    }
+  } else {
+#pragma unroll
+    for (int e = 0; e < kN; ++e) {
+      const float g = v[e] * p.alpha0;
+      o[e] = g * sigmoid<true>(sigmoid_arg(g, AEX_ACT_GELU_TANH)) * (u[e] * p.alpha1);
+    }
+  }
+  if (p.y_f32) {
+    float* y = static_cast<float*>(p.y) + row * p.ldy + col;
+    if (p.vec && col + kN <= p.cols) {
+#pragma unroll
+      for (int e = 0; e < kN; e += 4) *reinterpret_cast<float4*>(y + e) = make_float4(o[e], o[e + 1], o[e + 2], o[e + 3]);
+    } else {
+#pragma unroll
+      for (int e = 0; e < kN; ++e)
+        if (col + e < p.cols) y[e] = o[e];
+    }
+  } else {
+    uint16_t* y = static_cast<uint16_t*>(p.y) + row * p.ldy + col;
+    uint32_t pk[kN / 2];
+#pragma unroll
+    for (int e = 0; e < kN / 2; ++e) pk[e] = pack_bf16x2(o[2 * e], o[2 * e + 1]);
+    if (kN == 16 && p.vec == 2 && col + kN <= p.cols) {
+      st_global_32(y, pk);
+    } else if (p.vec && col + kN <= p.cols) {
+#pragma unroll
+      for (int e = 0; e < kN / 2; e += 4)
+        *reinterpret_cast<uint4*>(y + 2 * e) = make_uint4(pk[e], pk[e + 1], pk[e + 2], pk[e + 3]);
+    } else {
+#pragma unroll
+      for (int e = 0; e < kN; ++e)
+        if (col + e < p.cols) y[e] = static_cast<uint16_t>((e & 1) ? pk[e >> 1] >> 16 : pk[e >> 1] & 0xFFFFu);
+    }
   }
 }
 
+// Reads kN accumulator columns (16 at a time) from tensor memory.
+template <int kN>
+__device__ __forceinline__ void tmem_read(uint32_t taddr, float* v) {
+  uint32_t r[kN];
+#pragma unroll
+  for (int e = 0; e < kN; e += 16) tmem_ld16(taddr + e, r + e);
+  tmem_wait_ld();
+#pragma unroll
+  for (int e = 0; e < kN; ++e) v[e] = __uint_as_float(r[e]);
+}
+
+// Half of a row's 256 accumulator columns starting at tensor-memory address
+// tbase: columns [128 half, ..) or (gated) outputs [64 half, ..).
+template <bool kGated>
+__device__ __forceinline__ void tile_half(const TileOut& p, int64_t row, int nt, int half, uint32_t tbase) {
+  if (!kGated) {
+#pragma unroll 1
+    for (int c = 128 * half; c < 128 * half + 128; c += 32) {
+      float v[32];
+      tmem_read<32>(tbase + c, v);
+      if (row < p.m) {
+        finish<false, 16>(p, row, nt, c, v, nullptr);
+        finish<false, 16>(p, row, nt, c + 16, v + 16, nullptr);
+      }
+    }
+  } else {
+#pragma unroll 1
+    for (int c = 64 * half; c < 64 * half + 64; c += 16) {
+      uint32_t g[16], u[16];
+      tmem_ld16(tbase + c, g);
+      tmem_ld16(tbase + 128 + c, u);
+      tmem_wait_ld();
+      if (row < p.m) finish<true, 16>(p, row, nt, c, reinterpret_cast<float*>(g), reinterpret_cast<float*>(u));
+    }
+  }
+}
+
+// ------------------------------------------------------------- split tiles
+// Half of the raw accumulators of a piece's row `in_tile` into its slot, columns
+// first (a warp's 32 rows of a column are one 128-byte line).
+__device__ __forceinline__ void store_piece(const TileWork& w, int slot, int in_tile, bool live, int half,
+                                            uint32_t tbase) {
+  float* dst = w.pieces + static_cast<size_t>(slot) * w.rows * 256 + in_tile;
+#pragma unroll 1
+  for (int c = 128 * half; c < 128 * half + 128; c += 32) {
+    float v[32];
+    tmem_read<32>(tbase + c, v);
+    if (live) {
+#pragma unroll
+      for (int e = 0; e < 32; ++e) dst[static_cast<size_t>(c + e) * w.rows] = v[e];
+    }
+  }
+}
+
+// Adds the pieces of the split tiles in the order of the clusters that wrote
+// them and hands eight columns of a row at a time to `emit(row, nt, c, v, u)`
+// (gated: v of columns [c, c + 8), u of [128 + c, ..)). One thread each.
+template <bool kGated, typename F>
+__device__ __forceinline__ void join_tile(const TileWork& w, int recs, int clusters, int m, F emit) {
+  constexpr int kGroups = kGated ? 16 : 32;
+  const int idx = static_cast<int>(blockIdx.x * blockDim.x + threadIdx.x);
+  const int in_tile = idx % w.rows, c8 = idx / w.rows % kGroups * 8, r = idx / (kGroups * w.rows);
+  if (r >= w.split) return;
+  const int t = w.whole + r;
+  const int64_t row = static_cast<int64_t>(t % w.m_tiles) * 256 + in_tile;
+  if (row >= m) return;
+  const int lo = r * recs, hi = lo + recs;
+  int c = r * clusters / w.split;
+  while (c > 0 && w.start(c, clusters, recs) > lo) --c;
+  while (w.start(c + 1, clusters, recs) <= lo) ++c;
+  float v[8], u[8];
+#pragma unroll
+  for (int e = 0; e < 8; ++e) v[e] = u[e] = 0.f;
+  for (; c < clusters && w.start(c, clusters, recs) < hi; ++c) {
+    if (w.start(c, clusters, recs) == w.start(c + 1, clusters, recs)) continue;  // nothing fell to this cluster
+    const float* src = w.pieces + (static_cast<size_t>(c + r) * 256 + c8) * w.rows + in_tile;
+#pragma unroll
+    for (int e = 0; e < 8; ++e) {
+      v[e] += src[static_cast<size_t>(e) * w.rows];
+      if (kGated) u[e] += src[static_cast<size_t>(128 + e) * w.rows];
+    }
+  }
+  emit(row, t / w.m_tiles, c8, v, u);
+}
+
+// 2: rows of whole 32-byte sectors, 1: of 16-byte vectors, 0: neither.
 inline int vec_ok(const void* y, int64_t ldy, bool f32) {
-  return (reinterpret_cast<uintptr_t>(y) & 15) == 0 && (ldy * (f32 ? 4 : 2)) % 16 == 0;
+  const uint64_t bits = reinterpret_cast<uintptr_t>(y) | static_cast<uint64_t>(ldy * (f32 ? 4 : 2));
+  return bits % 32 == 0 ? 2 : bits % 16 == 0 ? 1 : 0;
 }
 
 }  // namespace fp4

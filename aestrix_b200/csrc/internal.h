@@ -19,7 +19,6 @@ struct aex_ctx {
   void* scratch = nullptr;  // grown on demand by entry points that need workspace
   size_t scratch_bytes = 0;
   int pair_clusters = 0;    // co-resident 2-CTA clusters of the pair GEMM (0 = not yet queried)
-  int fp4_clusters = 0;     // the same of the microscaled GEMMs (one CTA per SM as well)
   std::string last_error;
 };
 

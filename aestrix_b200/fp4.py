@@ -205,13 +205,19 @@ def _open(*weights):
             raise ValueError("the weight is closed")
 
 
+_SMALL_ROWS = 16  # up to here a product needs no workspace, and the library need not be asked
+
+
 def _product(x, w, w_up, activation, quantize_x, x_scale, out_dtype, out, stream):
     device = w.index
     _matrix("x", x, _DTYPES, w.k, device)
     m = x.shape[0]
     out = _out(out, m, w.n, out_dtype, x, device, stream)
     q = 1 if quantize_x else 0
-    n_ws = w.lib.aex_fp4_mm_workspace_bytes(w.handle, m, q) if q else 0
+    n_ws = 0
+    if m > _SMALL_ROWS:
+        need = w.lib.aex_fp4_mm_workspace_bytes if w_up is None else w.lib.aex_fp4_gated_mm_workspace_bytes
+        n_ws = need(w.handle, m, q)
     ws = _empty((n_ws,), torch.uint8, x, stream) if n_ws else None
     a = _lib.aex_fp4_mm_args(x.data_ptr(), _DTYPES[x.dtype], _pitch(x), m, q, x_scale, out.data_ptr(),
                              _DTYPES[out.dtype], out.stride(0) if m > 1 else w.n, ws.data_ptr() if n_ws else None,
@@ -252,8 +258,11 @@ def fp4_mm_dgrad(dy, w: FP4Weight, out_dtype=torch.bfloat16, out=None, stream=No
     _matrix("dy", dy, _BF16, w.n, w.index)
     m = dy.shape[0]
     out = _out(out, m, w.k, out_dtype, dy, w.index, stream)
+    n_ws = w.lib.aex_fp4_mm_dgrad_workspace_bytes(w.handle, m)
+    ws = _empty((n_ws,), torch.uint8, dy, stream) if n_ws else None
     rc = w.lib.aex_fp4_mm_dgrad(w.ctx.handle, w.handle, dy.data_ptr(), _pitch(dy), m, out.data_ptr(),
-                                _DTYPES[out.dtype], out.stride(0) if m > 1 else w.k, _stream(stream, w.index))
+                                _DTYPES[out.dtype], out.stride(0) if m > 1 else w.k, ws.data_ptr() if n_ws else None,
+                                n_ws, _stream(stream, w.index))
     if rc:
         w.ctx.check(rc)
     return out

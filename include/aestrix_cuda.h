@@ -268,13 +268,15 @@ typedef struct aex_fp4_mm_args {
   void* y;             /* [m, n], aligned to its element */
   int y_dtype;         /* AEX_DTYPE_BF16 or AEX_DTYPE_F32 */
   int64_t ldy;         /* row pitch in elements, >= n */
-  void* workspace;     /* aex_fp4_mm_workspace_bytes, 256-byte aligned; NULL where that is 0. Its contents need
-                        * not survive between calls; calls that may overlap must not share it */
+  void* workspace;     /* aex_fp4_mm_workspace_bytes / aex_fp4_gated_mm_workspace_bytes, 256-byte aligned; NULL
+                        * where that is 0. Its contents need not survive between calls; calls that may overlap
+                        * must not share it */
   size_t workspace_bytes;
 } aex_fp4_mm_args;
 
-/* Workspace of aex_fp4_mm and aex_fp4_gated_mm for m rows. 0 for bad arguments. */
+/* Workspace of a call for m rows. 0 for bad arguments. */
 size_t aex_fp4_mm_workspace_bytes(const aex_fp4weight* w, int m, int quantize_x);
+size_t aex_fp4_gated_mm_workspace_bytes(const aex_fp4weight* w_gate, int m, int quantize_x);
 
 /* y[m, n] = x[m, k] . W[n, k]^T, f32 accumulation, one rounding at the end.
  * The microscaled sibling of aex_qmm_ex. */
@@ -292,8 +294,9 @@ int aex_fp4_gated_mm(aex_ctx* ctx, const aex_fp4weight* w_gate, const aex_fp4wei
  * dy[m, n] . W[n, k]. dy bf16, 16-byte aligned, row pitch lddy a multiple of 8
  * elements; dx bf16 or f32, aligned to its element, row pitch lddx. A 4-bit
  * weight is frozen: it has no gradient. */
+size_t aex_fp4_mm_dgrad_workspace_bytes(const aex_fp4weight* w, int m);
 int aex_fp4_mm_dgrad(aex_ctx* ctx, const aex_fp4weight* w, const void* dy, int64_t lddy, int m, void* dx,
-                     int dx_dtype, int64_t lddx, aex_stream stream);
+                     int dx_dtype, int64_t lddx, void* workspace, size_t workspace_bytes, aex_stream stream);
 
 /* Gradient of aex_fp4_gated_mm (without quantize_x) with respect to x, from
  * dh[m, n]: g and u are computed again from x (nothing is kept from the forward

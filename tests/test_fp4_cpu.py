@@ -97,9 +97,11 @@ def test_c_entry_points_refuse_null():
     assert L.aex_fp4weight_shape(None, None, None) == bad
     assert L.aex_fp4_mm(None, None, C.byref(a), None) == bad
     assert L.aex_fp4_gated_mm(None, None, None, 0, C.byref(a), None) == bad
-    assert L.aex_fp4_mm_dgrad(None, None, None, 8, 1, None, 0, 32, None) == bad
+    assert L.aex_fp4_mm_dgrad(None, None, None, 8, 1, None, 0, 32, None, 0, None) == bad
     assert L.aex_fp4_gated_mm_dgrad(None, None, None, 0, None, 32, None, 8, 1, None, 32, None, 0, None) == bad
     assert L.aex_fp4_mm_workspace_bytes(None, 100, 1) == 0
+    assert L.aex_fp4_gated_mm_workspace_bytes(None, 100, 1) == 0
+    assert L.aex_fp4_mm_dgrad_workspace_bytes(None, 100) == 0
     assert L.aex_fp4_gated_mm_dgrad_workspace_bytes(None, 100) == 0
     L.aex_fp4weight_destroy(None)
 
