@@ -48,17 +48,6 @@ __device__ __forceinline__ float settle(float approx, float border_unit, float t
   return __int_as_float(__float_as_int(rt) + d);
 }
 
-// cvt of two magnitudes to e2m1 codes in one byte (a: low nibble).
-__device__ __forceinline__ uint32_t e2m1x2(float a, float b) {
-  uint32_t r;
-  asm("{\n\t.reg .b8 t;\n\t"
-      "cvt.rn.satfinite.e2m1x2.f32 t, %2, %1;\n\t"
-      "cvt.u32.u8 %0, t;\n\t}"
-      : "=r"(r)
-      : "f"(a), "f"(b));
-  return r;
-}
-
 __device__ __forceinline__ uint32_t e4m3_sat(float v) {  // v >= 0, to nearest even, at most 448
   uint16_t r;
   asm("cvt.rn.satfinite.e4m3x2.f32 %0, %1, %2;" : "=h"(r) : "f"(0.f), "f"(v));
@@ -83,56 +72,113 @@ __device__ __forceinline__ float scale_to_f32(uint32_t b) {
   return kFormat == AEX_FP4_MX ? e8m0_to_f32(b) : e4m3_to_f32(b);
 }
 
-// Scale byte and code magnitudes of kN (8 or 16) columns v of one row; the
-// block's other columns are with this lane's neighbours (lane ^ 1, and for a
-// fourth part lane ^ 2); all lanes of a warp call it. q: v over the block's
-// unit, settled on its side of every border, ready for the conversion to e2m1.
-// inv_6ts is 1 / (6 tensor_scale) rounded to f32.
-template <int kFormat, int kN>
-__device__ __forceinline__ uint32_t quantize_cols(const float* v, float tensor_scale, float inv_6ts, float* q) {
-  float amax = 0.f;
-  bool bad = false;
+// Eight values as one word of codes, in the order of the columns or (kPermute) of the records.
+template <bool kPermute>
+__device__ __forceinline__ uint32_t code_word(const float* p) {
+  uint32_t w;
+  asm("{\n\t.reg .b8 b0, b1, b2, b3;\n\t"
+      "cvt.rn.satfinite.e2m1x2.f32 b0, %2, %1;\n\tcvt.rn.satfinite.e2m1x2.f32 b1, %4, %3;\n\t"
+      "cvt.rn.satfinite.e2m1x2.f32 b2, %6, %5;\n\tcvt.rn.satfinite.e2m1x2.f32 b3, %8, %7;\n\t"
+      "mov.b32 %0, {b0, b1, b2, b3};\n\t}"
+      : "=r"(w)
+      : "f"(p[0]), "f"(p[kPermute ? 2 : 1]), "f"(p[kPermute ? 4 : 2]), "f"(p[kPermute ? 6 : 3]),
+        "f"(p[kPermute ? 1 : 4]), "f"(p[kPermute ? 3 : 5]), "f"(p[kPermute ? 5 : 6]), "f"(p[7]));
+  return w;
+}
+
+__device__ __forceinline__ float rcp_approx(float x) {
+  float y;
+  asm("rcp.approx.f32 %0, %1;" : "=f"(y) : "f"(x));
+  return y;
+}
+
+// Codes and scale byte of kN (8 or 16) columns v of one row; the block's other
+// columns are with this lane's neighbours (lane ^ 1, and for a fourth part
+// lane ^ 2); all lanes of a warp call it. top: the bits of the largest |v| of
+// these columns (an infinity or NaN among them: at least 0x7F800000, which makes
+// the block's scale a NaN and its codes 0). inv_6ts is 1 / (6 tensor_scale)
+// rounded to f32.
+// mxfp4: v over a power of two is exact. nvfp4, tensor_scale a power of two: the
+// unit has 4 significant bits, and a quotient that is rounded correctly (a
+// reciprocal rounded to nearest, one residual) is a border only if v is. Any
+// other tensor_scale: v is multiplied by the reciprocal 2^-21 above and below;
+// the approximations are off by at most 2^-22, so where both give the same code
+// it is the quotient's, and where not (a value in some hundred thousand) the
+// border is settled exactly. (Settling every value cost 21 us for 4608 x 4096.)
+template <int kFormat, int kN, bool kPermute>
+__device__ __forceinline__ uint32_t quantize_cols(const float* v, uint32_t top, float tensor_scale, float inv_6ts,
+                                                  uint32_t* codes) {
 #pragma unroll
-  for (int i = 0; i < kN; ++i) {
-    amax = fmaxf(amax, fabsf(v[i]));
-    bad |= !(fabsf(v[i]) <= 3.402823466e38f);  // NaN or infinity: the block's scale becomes NaN
-  }
-#pragma unroll
-  for (int o = 1; o < block_of(kFormat) / kN; o <<= 1) {
-    amax = fmaxf(amax, __shfl_xor_sync(0xffffffffu, amax, o));
-    bad |= __shfl_xor_sync(0xffffffffu, bad ? 1 : 0, o) != 0;
-  }
-  uint32_t byte;
+  for (int o = 1; o < block_of(kFormat) / kN; o <<= 1) top = max(top, __shfl_xor_sync(0xffffffffu, top, o));
+  const bool bad = top >= 0x7F800000u;
+  const float amax = bad ? 0.f : __uint_as_float(top);
+  float q[kN];
   if (kFormat == AEX_FP4_MX) {
     // floor(log2 amax) - 2, biased: the exponent field less 2 (subnormals, and what is below 2^-125, take byte 0)
     const int ex = max(static_cast<int>(__float_as_uint(amax) >> 23) - 2, 0);
     const float inv = __uint_as_float(static_cast<uint32_t>(254 - ex) << 23);  // 2^(127 - ex), ex <= 252
-    byte = bad ? 0xFFu : static_cast<uint32_t>(ex);
 #pragma unroll
-    for (int i = 0; i < kN; ++i) q[i] = fabsf(v[i]) * inv;  // exact
-  } else {
-    const uint32_t sb = e4m3_sat(settle(amax * inv_6ts, 6.f, tensor_scale, amax));
-    byte = bad ? 0x7Fu : sb;
-    const float s = e4m3_to_f32(sb);
-    const float inv = sb ? __frcp_rn(s * tensor_scale) : 0.f;
+    for (int i = 0; i < kN; ++i) q[i] = v[i] * inv;
 #pragma unroll
-    for (int i = 0; i < kN; ++i) q[i] = sb ? settle(fabsf(v[i]) * inv, s, tensor_scale, fabsf(v[i])) : 0.f;
+    for (int h = 0; h < kN / 8; ++h) codes[h] = bad ? 0u : code_word<kPermute>(q + 8 * h);
+    return bad ? 0xFFu : static_cast<uint32_t>(ex);
   }
+  const uint32_t sb = e4m3_sat(settle(amax * inv_6ts, 6.f, tensor_scale, amax));
+  const float s = e4m3_to_f32(sb), unit = s * tensor_scale;
+  if ((__float_as_uint(tensor_scale) & 0x007FFFFFu) == 0) {
+    const float inv = __frcp_rn(unit);
 #pragma unroll
-  for (int i = 0; i < kN; ++i) q[i] = bad ? 0.f : copysignf(q[i], v[i]);
-  return byte;
-}
-
-// Eight code magnitudes as one word, in the order of the columns or (kPermute) of the records.
-template <bool kPermute>
-__device__ __forceinline__ uint32_t code_word(const float* p) {
-  return kPermute ? e2m1x2(p[0], p[2]) | (e2m1x2(p[4], p[6]) << 8) | (e2m1x2(p[1], p[3]) << 16) |
-                        (e2m1x2(p[5], p[7]) << 24)
-                  : e2m1x2(p[0], p[1]) | (e2m1x2(p[2], p[3]) << 8) | (e2m1x2(p[4], p[5]) << 16) |
-                        (e2m1x2(p[6], p[7]) << 24);
+    for (int i = 0; i < kN; ++i) {
+      const float r = v[i] * inv;
+      q[i] = fmaf(fmaf(-r, unit, v[i]), inv, r);
+      if (!(fabsf(r) < 8.f)) q[i] = r;  // beyond the largest code (the residual of a huge one may be no number)
+    }
+#pragma unroll
+    for (int h = 0; h < kN / 8; ++h) codes[h] = code_word<kPermute>(q + 8 * h);
+  } else {
+    const float inv = rcp_approx(unit);
+    const float up = inv * (1.f + 0x1p-21f), down = inv * (1.f - 0x1p-21f);
+    bool near = false;
+#pragma unroll
+    for (int h = 0; h < kN / 8; ++h) {
+      float a[8], b[8];
+#pragma unroll
+      for (int i = 0; i < 8; ++i) {
+        a[i] = v[8 * h + i] * up;
+        b[i] = v[8 * h + i] * down;
+      }
+      codes[h] = code_word<kPermute>(a);
+      near |= codes[h] != code_word<kPermute>(b);
+    }
+    if (near && sb) {
+#pragma unroll
+      for (int i = 0; i < kN; ++i) q[i] = copysignf(settle(fabsf(v[i]) * inv, s, tensor_scale, fabsf(v[i])), v[i]);
+#pragma unroll
+      for (int h = 0; h < kN / 8; ++h) codes[h] = code_word<kPermute>(q + 8 * h);
+    }
+  }
+  if (bad || sb == 0) {
+#pragma unroll
+    for (int i = 0; i < kN; ++i) q[i] = bad ? 0.f : copysignf(0.f, v[i]);
+#pragma unroll
+    for (int h = 0; h < kN / 8; ++h) codes[h] = code_word<kPermute>(q + 8 * h);
+  }
+  return bad ? 0x7Fu : sb;
 }
 
 // ------------------------------------------------------------------ decoding
+// The eight codes of a word as four f16 pairs: byte b of a record word holds
+// columns (0, 2), (4, 6), (1, 3), (5, 7) of its eight. (In the
+// order of the columns: byte b holds columns 2b and 2b + 1.)
+__device__ __forceinline__ void decode_f16(uint32_t w, uint32_t* d) {
+  asm("{\n\t.reg .b8 t0, t1, t2, t3;\n\t"
+      "mov.b32 {t0, t1, t2, t3}, %4;\n\t"
+      "cvt.rn.f16x2.e2m1x2 %0, t0;\n\tcvt.rn.f16x2.e2m1x2 %1, t1;\n\t"
+      "cvt.rn.f16x2.e2m1x2 %2, t2;\n\tcvt.rn.f16x2.e2m1x2 %3, t3;\n\t}"
+      : "=r"(d[0]), "=r"(d[1]), "=r"(d[2]), "=r"(d[3])
+      : "r"(w));
+}
+
 // Columns (2j, 2j + 1) of a record word as a bf16 pair, times 2^-126: the three
 // magnitude bits of a code, placed at the border of exponent and mantissa, are
 // its value in units of 2^-126 (0.5 is a bf16 subnormal there).
@@ -145,6 +191,23 @@ __device__ __forceinline__ uint32_t mul_bf16x2(uint32_t a, uint32_t b) {
   uint32_t d;
   asm("mul.rn.bf16x2 %0, %1, %2;" : "=r"(d) : "r"(a), "r"(b));
   return d;
+}
+
+__device__ __forceinline__ void st_global_32(void* p, const uint32_t* v) {
+  asm volatile("st.global.v8.b32 [%0], {%1,%2,%3,%4,%5,%6,%7,%8};" ::"l"(p), "r"(v[0]), "r"(v[1]), "r"(v[2]), "r"(v[3]),
+               "r"(v[4]), "r"(v[5]), "r"(v[6]), "r"(v[7])
+               : "memory");
+}
+
+// Arrives (lane 0) on the barrier at `bar` once the loads that `v` was made of
+// have returned in every lane of the warp. Program order is not enough: a load
+// whose value is used only after a later wait was seen to be carried out after
+// the arrive, and read what the producer had copied into the slot by then (the
+// address depends on the loaded values by way of a zero that only the host
+// knows to be one).
+__device__ __forceinline__ void arrive_after_loads(uint32_t bar, uint32_t v, uint32_t zero, int lane) {
+  const uint32_t all = __reduce_or_sync(0xffffffffu, v);
+  if (lane == 0) mbar_arrive_addr(bar + (all & zero));
 }
 
 constexpr uint32_t kBf16x2_2p126 = 0x7E807E80u;  // 2^126 in both halves

@@ -127,6 +127,7 @@ __global__ void __launch_bounds__(kBThreads, 1) block_kernel(const __grid_consta
   const int cluster = static_cast<int>(blockIdx.x >> 1);
   const int clusters = static_cast<int>(gridDim.x >> 1);
 
+  launch_dependents();
   if (threadIdx.x == 0) {
     abort_flag = 0;
     for (int s = 0; s < kBStages; ++s) {
@@ -150,6 +151,7 @@ __global__ void __launch_bounds__(kBThreads, 1) block_kernel(const __grid_consta
   cluster_sync_all();
   tc_fence_after();
   const uint32_t tmem = *tmem_slot;
+  wait_dependency();  // x's records are written
 
   if (warp == 0) {
     if (lane == 0) {
@@ -319,15 +321,12 @@ __global__ void __launch_bounds__(kBThreads, 1) block_kernel(const __grid_consta
           if (live) finish<true, 16>(p.o, row, t.nt, c, reinterpret_cast<float*>(g), reinterpret_cast<float*>(u));
         }
       } else {
-        float* dst = p.work.pieces + (t.slot < 0 ? 0 : static_cast<size_t>(t.slot) * p.work.rows * 256 + in_tile);
         auto emit = [&](int c, const float* v) {
           if (!live) return;
-          if (t.slot < 0) {
+          if (t.slot < 0)
             finish<false, 16>(p.o, row, t.nt, c, v, nullptr);
-          } else {
-#pragma unroll
-            for (int e = 0; e < 16; ++e) dst[static_cast<size_t>(c + e) * p.work.rows] = v[e];
-          }
+          else
+            store_piece16(p.work, t.slot, in_tile, c, v);
         };
         if (mine) {
 #pragma unroll
@@ -357,7 +356,7 @@ __global__ void __launch_bounds__(kBThreads, 1) block_kernel(const __grid_consta
 }
 
 template <bool kGated>
-__global__ void __launch_bounds__(256) block_join_kernel(const __grid_constant__ BlockParams p, int clusters) {
+__global__ void __launch_bounds__(kJoinThreads) block_join_kernel(const __grid_constant__ BlockParams p, int clusters) {
   join_tile<kGated>(p.work, p.k_blocks, clusters, p.o.m,
                     [&](int64_t row, int nt, int c, const float* v, const float* u) {
                       finish<kGated, 8>(p.o, row, nt, c, v, u);
@@ -395,22 +394,21 @@ int launch_block(aex_ctx* ctx, const Job& j, cudaStream_t s) {
   auto kern = block_kernel<kFormat, kGated>;
   static SmemOptIn opt_in;
   if (int r = opt_in(ctx, reinterpret_cast<const void*>(kern), kBSmem)) return r;
-  if (int r = launch_pairs(ctx, reinterpret_cast<const void*>(kern), plan.clusters, kBThreads, kBSmem, s, &p)) return r;
-  if (plan.split) {
-    constexpr int kGroups = kGated ? 16 : 32;
-    block_join_kernel<kGated><<<(plan.split * plan.rows * kGroups + 255) / 256, 256, 0, s>>>(p, plan.clusters);
-    return check_launch(ctx, "fp4 block_join_kernel");
-  }
+  if (int r = launch_pairs(ctx, reinterpret_cast<const void*>(kern), plan.clusters, kBThreads, kBSmem, true, s, &p))
+    return r;
+  if (plan.split)
+    return launch_after(ctx, reinterpret_cast<const void*>(block_join_kernel<kGated>), join_blocks(p.work, kGated),
+                        kJoinThreads, s, &p, const_cast<int*>(&plan.clusters));
   return AEX_OK;
 }
 
-// What a join costs, in records of the main loop (about 3 us).
-constexpr int kJoinBlock = 12;
+// Microseconds of the main loop per record (B200).
+constexpr double kBlockUs = 0.37;
 
 }  // namespace
 
 TilePlan plan_block(const aex_fp4weight* w, bool gated, int m) {
-  return plan_tiles(w->clusters, m, gated ? w->n_tiles : (w->n_tiles + 1) / 2, w->k_blocks, kJoinBlock);
+  return plan_tiles(w->clusters, m, gated ? w->n_tiles : (w->n_tiles + 1) / 2, w->k_blocks, kBlockUs);
 }
 
 int run_block(aex_ctx* ctx, const Job& j, cudaStream_t s) {

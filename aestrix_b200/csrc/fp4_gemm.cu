@@ -81,6 +81,7 @@ struct GemmParams {
   TileWork work;
   TileOut o;
   GradOut grad;
+  uint32_t zero;  // 0 (arrive_after_loads)
   int* status;
 };
 
@@ -146,6 +147,7 @@ __global__ void __launch_bounds__(kGThreads, 1)
   const int cluster = static_cast<int>(blockIdx.x >> 1);
   const int clusters = static_cast<int>(gridDim.x >> 1);
 
+  launch_dependents();
   if (threadIdx.x == 0) {
     abort_flag = 0;
     for (int s = 0; s < kGA; ++s) mbar_init(&afull[s], 1);
@@ -427,8 +429,9 @@ __global__ void __launch_bounds__(kGThreads, 1)
           sc = *reinterpret_cast<const uint32_t*>(rec + scale_off(r, cp));
         else
           sc = *reinterpret_cast<const uint16_t*>(rec + scale_off(r, cp >> 1) + (cp & 1) * 2);
-        __syncwarp();
-        if (lane == 0) mbar_arrive_addr(smem_u32(&rempty[crs]));  // this warp's only read of the record
+        // this warp's only read of the record
+        arrive_after_loads(smem_u32(&rempty[crs]), c0.x | c0.y | c0.z | c0.w | c1.x | c1.y | c1.z | c1.w | sc, p.zero,
+                           lane);
         if (g >= kGB && !mbar_wait_warp_cl(done0 + 8 * cds, cdph, &abort_flag, p.status, kDevTimeoutMma)) {
           ok = false;
           break;
@@ -469,7 +472,7 @@ __global__ void __launch_bounds__(kGThreads, 1)
 }
 
 template <int kMode>
-__global__ void __launch_bounds__(256) join_kernel(const __grid_constant__ GemmParams p, int clusters) {
+__global__ void __launch_bounds__(kJoinThreads) join_kernel(const __grid_constant__ GemmParams p, int clusters) {
   constexpr bool kGated = kMode == kGatedFwd || kMode == kGatedGrad;
   join_tile<kGated>(p.work, p.recs, clusters, p.o.m, [&](int64_t row, int nt, int c, const float* v, const float* u) {
     if (kMode == kGatedGrad) {
@@ -507,14 +510,13 @@ int launch_gemm(aex_ctx* ctx, const CUtensorMap& tm0, const CUtensorMap& tm1, Ge
   auto kern = gemm_kernel<kFormat, kMode>;
   static SmemOptIn opt_in;
   if (int r = opt_in(ctx, reinterpret_cast<const void*>(kern), kGSmem)) return r;
-  if (int r = launch_pairs(ctx, reinterpret_cast<const void*>(kern), plan.clusters, kGThreads, kGSmem, s,
+  if (int r = launch_pairs(ctx, reinterpret_cast<const void*>(kern), plan.clusters, kGThreads, kGSmem, false, s,
                            const_cast<CUtensorMap*>(&tm0), const_cast<CUtensorMap*>(&tm1), &p))
     return r;
-  if (plan.split) {
-    constexpr int kGroups = kMode == kGatedFwd || kMode == kGatedGrad ? 16 : 32;
-    join_kernel<kMode><<<(plan.split * plan.rows * kGroups + 255) / 256, 256, 0, s>>>(p, plan.clusters);
-    return check_launch(ctx, "fp4 join_kernel");
-  }
+  if (plan.split)
+    return launch_after(ctx, reinterpret_cast<const void*>(join_kernel<kMode>),
+                        join_blocks(p.work, kMode == kGatedFwd || kMode == kGatedGrad), kJoinThreads, s, &p,
+                        const_cast<int*>(&plan.clusters));
   return AEX_OK;
 }
 
@@ -538,16 +540,16 @@ float unit_of(int format) {
   return format == AEX_FP4_MX ? decode_unit<AEX_FP4_MX>() : decode_unit<AEX_FP4_NV>();
 }
 
-// What a join costs, in records of the main loop (about 3 us).
-constexpr int kJoinForward = 3, kJoinBackward = 6;
+// Microseconds of the main loop per record: four K steps forward, two backward (B200).
+constexpr double kForwardUs = 1.5, kBackwardUs = 0.75;
 
 }  // namespace
 
 TilePlan plan_gemm(const aex_fp4weight* w, bool gated, int m) {
-  return plan_tiles(w->clusters, m, gated ? w->n_tiles : (w->n_tiles + 1) / 2, w->k_blocks, kJoinForward);
+  return plan_tiles(w->clusters, m, gated ? w->n_tiles : (w->n_tiles + 1) / 2, w->k_blocks, kForwardUs);
 }
 TilePlan plan_dgrad(const aex_fp4weight* w, bool two, int m) {
-  return plan_tiles(w->clusters, m, w->k_blocks, w->n_tiles * (two ? 2 : 1), kJoinBackward);
+  return plan_tiles(w->clusters, m, w->k_blocks, w->n_tiles * (two ? 2 : 1), kBackwardUs);
 }
 
 int gemm_clusters(aex_ctx* ctx, int* out) {

@@ -105,20 +105,25 @@ struct TilePlan {
   size_t bytes = 0;   // of all pieces
 };
 
-// `recs` records along K per tile. Tiles that do not fill a last wave of the clusters are split when the wave's
-// records, dealt out over all clusters, and a join (in records) take less than the wave.
-inline TilePlan plan_tiles(int clusters, int m, int64_t col_tiles, int recs, int join) {
+// `recs` records along K per tile, `rec_us` microseconds each in the main loop. Tiles that do not fill a last wave of
+// the clusters are split when that wave's records, dealt out over all clusters, and the join take less than the wave.
+// The join: 3 us, and the pieces written and read (B200, measured: 4 us for 6 MB, 8 us for 20 MB; 77 rows through
+// 7680 -> 4096 51 us whole, 22 us split; 512 rows back through 4096 -> 7680 30.8 us whole, 32.0 us split).
+inline TilePlan plan_tiles(int clusters, int m, int64_t col_tiles, int recs, double rec_us) {
   TilePlan p;
   p.m_tiles = (m - 1) / 256 + 1;
+  p.rows = m < 256 ? m : 256;
   const int64_t tiles = p.m_tiles * col_tiles;
-  const int64_t left = tiles % clusters;
-  const int64_t shared = (left * recs + clusters - 1) / clusters;
   if (tiles > 0x3FFFFFFF) return p;  // refused by the caller
-  p.split = left && shared + join < recs && left * recs * clusters < 0x7FFFFFFF ? static_cast<int>(left) : 0;
+  const int64_t left = tiles % clusters;
+  const size_t bytes = static_cast<size_t>(clusters + left) * ((p.rows + 31) / 32 * 32) * 256 * sizeof(float);
+  const double saved = rec_us * static_cast<double>(recs - (left * recs + clusters - 1) / clusters);
+  if (left && saved > 3.0 + 2.0 * static_cast<double>(bytes) / 6.5e6 && left * recs * clusters < 0x7FFFFFFF) {
+    p.split = static_cast<int>(left);
+    p.bytes = bytes;
+  }
   p.whole = static_cast<int>(tiles) - p.split;
   p.clusters = p.split || tiles > clusters ? clusters : static_cast<int>(tiles);
-  p.rows = m < 256 ? m : 256;
-  if (p.split) p.bytes = static_cast<size_t>(clusters + p.split) * p.rows * 256 * sizeof(float);
   return p;
 }
 TilePlan plan_gemm(const aex_fp4weight* w, bool gated, int m);
@@ -126,24 +131,43 @@ TilePlan plan_dgrad(const aex_fp4weight* w, bool two, int m);
 TilePlan plan_block(const aex_fp4weight* w, bool gated, int m);
 int gemm_clusters(aex_ctx* ctx, int* out);
 
-// One launch of CTA pairs.
+// One launch of CTA pairs; `after`: set up while the stream's previous kernel runs (the kernel waits for it itself).
 template <typename... Args>
-int launch_pairs(aex_ctx* ctx, const void* kernel, int clusters, int threads, int smem, cudaStream_t s, Args*... args) {
+int launch_pairs(aex_ctx* ctx, const void* kernel, int clusters, int threads, int smem, bool after, cudaStream_t s,
+                 Args*... args) {
   cudaLaunchConfig_t cfg{};
   cfg.gridDim = dim3(2 * clusters, 1, 1);
   cfg.blockDim = dim3(threads, 1, 1);
   cfg.dynamicSmemBytes = smem;
   cfg.stream = s;
-  cudaLaunchAttribute attr[1];
+  cudaLaunchAttribute attr[2];
   attr[0].id = cudaLaunchAttributeClusterDimension;
   attr[0].val.clusterDim.x = 2;
   attr[0].val.clusterDim.y = 1;
   attr[0].val.clusterDim.z = 1;
+  attr[1].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  attr[1].val.programmaticStreamSerializationAllowed = 1;
+  cfg.attrs = attr;
+  cfg.numAttrs = after ? 2 : 1;
+  void* argv[] = {args...};
+  AEX_CUDA_TRY(ctx, cudaLaunchKernelExC(&cfg, kernel, argv));
+  return check_launch(ctx, "fp4 GEMM");
+}
+// A plain grid that is set up while the stream's previous kernel runs and waits for it itself.
+template <typename... Args>
+int launch_after(aex_ctx* ctx, const void* kernel, int blocks, int threads, cudaStream_t s, Args*... args) {
+  cudaLaunchConfig_t cfg{};
+  cfg.gridDim = dim3(blocks, 1, 1);
+  cfg.blockDim = dim3(threads, 1, 1);
+  cfg.stream = s;
+  cudaLaunchAttribute attr[1];
+  attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  attr[0].val.programmaticStreamSerializationAllowed = 1;
   cfg.attrs = attr;
   cfg.numAttrs = 1;
   void* argv[] = {args...};
   AEX_CUDA_TRY(ctx, cudaLaunchKernelExC(&cfg, kernel, argv));
-  return check_launch(ctx, "fp4 GEMM");
+  return check_launch(ctx, "fp4 join");
 }
 
 // The few-rows kernel takes up to 48 columns of its 8-column operand: rows that are bf16 or quantized, or f32 rows at

@@ -5,6 +5,8 @@
 // which is one nvfp4 block or, with its neighbouring lane, one mxfp4 block, so
 // the block's largest magnitude needs no shared memory and every element is
 // read and written once.
+#include <cuda_fp16.h>
+
 #include <algorithm>
 #include <new>
 
@@ -16,32 +18,60 @@ namespace fp4 {
 
 constexpr int kThreads = 256;
 
-// 16 elements of a row (16-byte aligned) as f32.
-template <bool kF32>
-__device__ __forceinline__ void load16(const void* x, int64_t at, float* v) {
-  if (kF32) {
-    const float4* p = reinterpret_cast<const float4*>(static_cast<const float*>(x) + at);
-#pragma unroll
-    for (int i = 0; i < 4; ++i) {
-      const float4 f = __ldg(p + i);
-      v[4 * i] = f.x;
-      v[4 * i + 1] = f.y;
-      v[4 * i + 2] = f.z;
-      v[4 * i + 3] = f.w;
-    }
+__device__ __forceinline__ void ldg256(const void* p, uint32_t* v) {
+  asm volatile("ld.global.nc.v8.b32 {%0,%1,%2,%3,%4,%5,%6,%7}, [%8];"
+               : "=r"(v[0]), "=r"(v[1]), "=r"(v[2]), "=r"(v[3]), "=r"(v[4]), "=r"(v[5]), "=r"(v[6]), "=r"(v[7])
+               : "l"(p));
+}
+
+// 32 bytes, in one load where the address allows.
+__device__ __forceinline__ void load32(const void* p, bool whole, uint32_t* w) {
+  if (whole) {
+    ldg256(p, w);
   } else {
-    const uint4* p = reinterpret_cast<const uint4*>(static_cast<const uint16_t*>(x) + at);
-#pragma unroll
-    for (int i = 0; i < 2; ++i) {
-      const uint4 u = __ldg(p + i);
-      const uint32_t w[4] = {u.x, u.y, u.z, u.w};
-#pragma unroll
-      for (int j = 0; j < 4; ++j) {
-        v[8 * i + 2 * j] = bf16lo_to_f32(w[j]);
-        v[8 * i + 2 * j + 1] = bf16hi_to_f32(w[j]);
-      }
-    }
+    const uint4 a = __ldg(static_cast<const uint4*>(p)), b = __ldg(static_cast<const uint4*>(p) + 1);
+    w[0] = a.x, w[1] = a.y, w[2] = a.z, w[3] = a.w, w[4] = b.x, w[5] = b.y, w[6] = b.z, w[7] = b.w;
   }
+}
+
+// 16 elements of a row as f32, and the bits of the largest magnitude.
+template <bool kF32>
+__device__ __forceinline__ uint32_t load16(const void* x, int64_t at, bool whole, float* v) {
+  if (kF32) {
+    uint32_t w[16], top = 0;
+    const float* p = static_cast<const float*>(x) + at;
+    load32(p, whole, w);
+    load32(p + 8, whole, w + 8);
+#pragma unroll
+    for (int i = 0; i < 16; ++i) {
+      v[i] = __uint_as_float(w[i]);
+      top = max(top, w[i] & 0x7FFFFFFFu);
+    }
+    return top;
+  }
+  uint32_t w[8], top = 0;  // two 16-bit maxima at a time: bits without the sign are ordered as magnitudes
+  load32(static_cast<const uint16_t*>(x) + at, whole, w);
+#pragma unroll
+  for (int i = 0; i < 8; ++i) {
+    top = __vmaxu2(top, w[i] & 0x7FFF7FFFu);
+    v[2 * i] = bf16lo_to_f32(w[i]);
+    v[2 * i + 1] = bf16hi_to_f32(w[i]);
+  }
+  return max(top << 16, top & 0xFFFF0000u);
+}
+
+// u / divisor for u < 2^31: umulhi(u, mul) >> shift.
+struct FastDiv {
+  uint32_t mul, shift, div;
+};
+inline FastDiv fast_div(uint32_t d) {
+  if (d == 1) return FastDiv{0, 0, 1};
+  uint32_t l = 1;
+  while ((uint64_t{1} << l) < d) ++l;
+  return FastDiv{static_cast<uint32_t>(((uint64_t{1} << (31 + l)) + d - 1) / d), l - 1, d};
+}
+__device__ __forceinline__ uint32_t divide(uint32_t u, const FastDiv& f) {
+  return f.div == 1 ? u : __umulhi(u, f.mul) >> f.shift;
 }
 
 // x [rows, k] -> codes [rows, k/2] and scales [rows, k/block] (kRecords: the
@@ -50,24 +80,24 @@ __device__ __forceinline__ void load16(const void* x, int64_t at, float* v) {
 // rows * upr < 2^31 (the host slices).
 template <int kFormat, bool kF32, bool kRecords>
 __global__ void __launch_bounds__(kThreads) quantize_kernel(const void* __restrict__ x, int64_t ldx, int rows, int k,
-                                                            uint32_t upr, float tensor_scale, float inv_6ts,
+                                                            FastDiv upr, int whole, float tensor_scale, float inv_6ts,
                                                             uint8_t* __restrict__ codes,
                                                             uint8_t* __restrict__ scales) {
   const uint32_t u = blockIdx.x * kThreads + threadIdx.x;
-  const uint32_t row = u / upr, c = u % upr;  // an mxfp4 pair (u even, u + 1) is one row's
+  const uint32_t row = divide(u, upr), c = u - row * upr.div;  // an mxfp4 pair (u even, u + 1) is one row's
   const bool live = row < static_cast<uint32_t>(rows);
   const int col = static_cast<int>(c) * 16;
   float v[16];
 #pragma unroll
   for (int i = 0; i < 16; ++i) v[i] = 0.f;
-  if (live && col < k) load16<kF32>(x, static_cast<int64_t>(row) * ldx + col, v);
-  float q[16];
-  const uint32_t sb = quantize_cols<kFormat, 16>(v, tensor_scale, inv_6ts, q);
-  const uint32_t w[2] = {code_word<kRecords>(q), code_word<kRecords>(q + 8)};
+  uint32_t top = 0;
+  if (live && col < k) top = load16<kF32>(x, static_cast<int64_t>(row) * ldx + col, whole != 0, v);
+  uint32_t w[2];
+  const uint32_t sb = quantize_cols<kFormat, 16, kRecords>(v, top, tensor_scale, inv_6ts, w);
   if (!live) return;
   if (kRecords) {
     const int r = static_cast<int>(row % kRecRows);
-    uint8_t* rec = codes + (static_cast<size_t>(row / kRecRows) * (upr / 16) + c / 16) * rec_bytes(kFormat);
+    uint8_t* rec = codes + (static_cast<size_t>(row / kRecRows) * (upr.div / 16) + c / 16) * rec_bytes(kFormat);
     const int cu = static_cast<int>(c % 16);  // unit inside the record
     *reinterpret_cast<uint2*>(rec + r * 128 + (((cu >> 1) ^ (r & 7)) << 4) + (cu & 1) * 8) = make_uint2(w[0], w[1]);
     if (kFormat == AEX_FP4_NV)
@@ -101,10 +131,10 @@ __device__ __forceinline__ float scaled(float cs, float tensor_scale) {
 template <int kFormat, bool kF32, bool kRecords>
 __global__ void __launch_bounds__(kThreads) dequantize_kernel(const uint8_t* __restrict__ codes,
                                                               const uint8_t* __restrict__ scales, int rows,
-                                                              uint32_t upr, int k_blocks, float tensor_scale,
-                                                              void* __restrict__ out, int64_t ldo) {
+                                                              FastDiv upr, int k_blocks, float tensor_scale,
+                                                              void* __restrict__ out, int64_t ldo, int whole) {
   const uint32_t u = blockIdx.x * kThreads + threadIdx.x;
-  const uint32_t row = u / upr, c = u % upr;
+  const uint32_t row = divide(u, upr), c = u - row * upr.div;
   if (row >= static_cast<uint32_t>(rows)) return;
   uint2 w;
   uint32_t sb;
@@ -122,26 +152,33 @@ __global__ void __launch_bounds__(kThreads) dequantize_kernel(const uint8_t* __r
   float v[16];
 #pragma unroll
   for (int h = 0; h < 2; ++h) {
-    const uint32_t word = h ? w.y : w.x;
+    uint32_t d[4];
+    decode_f16(h ? w.y : w.x, d);
 #pragma unroll
     for (int i = 0; i < 8; ++i) {
-      const int nib = kRecords ? ((i & 1) ? 4 + (i >> 1) : (i >> 1)) : i;
-      const uint32_t cd = word >> (4 * nib);
-      const float mag = __uint_as_float((cd & 7u) << 22) * 0x1p126f;
-      v[8 * h + i] = scaled<kF32>(__uint_as_float(__float_as_uint(mag) | ((cd & 8u) << 28)) * s, tensor_scale);
+      // byte b of a record word holds columns (0, 2), (4, 6), (1, 3), (5, 7) of its eight
+      const int b = kRecords ? (i & 1) * 2 + (i >> 2) : i >> 1, hi = kRecords ? (i >> 1) & 1 : i & 1;
+      const float cv = __half2float(__ushort_as_half(static_cast<uint16_t>(hi ? d[b] >> 16 : d[b] & 0xFFFFu)));
+      v[8 * h + i] = scaled<kF32>(cv * s, tensor_scale);
     }
   }
   const int64_t at = static_cast<int64_t>(row) * ldo + static_cast<int64_t>(c) * 16;
-  if (kF32) {
-    float4* o = reinterpret_cast<float4*>(static_cast<float*>(out) + at);
+  uint32_t o[16];
 #pragma unroll
-    for (int i = 0; i < 4; ++i) o[i] = make_float4(v[4 * i], v[4 * i + 1], v[4 * i + 2], v[4 * i + 3]);
-  } else {
-    uint4* o = reinterpret_cast<uint4*>(static_cast<uint16_t*>(out) + at);
+  for (int i = 0; i < 16; ++i) o[i] = __float_as_uint(v[i]);
+  if (!kF32) {
 #pragma unroll
-    for (int i = 0; i < 2; ++i)
-      o[i] = make_uint4(pack_bf16x2(v[8 * i], v[8 * i + 1]), pack_bf16x2(v[8 * i + 2], v[8 * i + 3]),
-                        pack_bf16x2(v[8 * i + 4], v[8 * i + 5]), pack_bf16x2(v[8 * i + 6], v[8 * i + 7]));
+    for (int i = 0; i < 8; ++i) o[i] = pack_bf16x2(v[2 * i], v[2 * i + 1]);
+  }
+  uint8_t* dst = static_cast<uint8_t*>(out) + at * (kF32 ? 4 : 2);
+#pragma unroll
+  for (int i = 0; i < (kF32 ? 16 : 8); i += 8) {
+    if (whole) {
+      st_global_32(dst + 4 * i, o + i);
+    } else {
+      *reinterpret_cast<uint4*>(dst + 4 * i) = make_uint4(o[i], o[i + 1], o[i + 2], o[i + 3]);
+      *reinterpret_cast<uint4*>(dst + 4 * i + 16) = make_uint4(o[i + 4], o[i + 5], o[i + 6], o[i + 7]);
+    }
   }
 }
 
@@ -198,7 +235,9 @@ int launch_quantize(aex_ctx* ctx, const void* x, int64_t ldx, int rows, int k, f
     uint8_t* cs = kRecords ? codes + static_cast<size_t>(r0 / kRecRows) * (upr / 16) * rec_bytes(kFormat)
                            : codes + static_cast<size_t>(r0) * upr * 8;
     uint8_t* ss = kRecords ? nullptr : scales + static_cast<size_t>(r0) * (k / block_of(kFormat));
-    quantize_kernel<kFormat, kF32, kRecords><<<blocks, kThreads, 0, s>>>(xs, ldx, nr, k, upr, ts, inv, cs, ss);
+    const int whole = (reinterpret_cast<uintptr_t>(xs) | static_cast<uint64_t>(ldx * (kF32 ? 4 : 2))) % 32 == 0;
+    quantize_kernel<kFormat, kF32, kRecords>
+        <<<blocks, kThreads, 0, s>>>(xs, ldx, nr, k, fast_div(upr), whole, ts, inv, cs, ss);
     if (int r = check_launch(ctx, "fp4 quantize_kernel")) return r;
   }
   return AEX_OK;
@@ -216,8 +255,10 @@ int launch_dequantize(aex_ctx* ctx, const uint8_t* codes, const uint8_t* scales,
     const uint8_t* cs = kRecords ? codes + static_cast<size_t>(r0 / kRecRows) * k_blocks * rec_bytes(kFormat)
                                  : codes + static_cast<size_t>(r0) * upr * 8;
     const uint8_t* ss = kRecords ? nullptr : scales + static_cast<size_t>(r0) * (k / block_of(kFormat));
-    dequantize_kernel<kFormat, kF32, kRecords><<<blocks, kThreads, 0, s>>>(
-        cs, ss, nr, upr, k_blocks, ts, static_cast<uint8_t*>(out) + r0 * ldo * (kF32 ? 4 : 2), ldo);
+    uint8_t* os = static_cast<uint8_t*>(out) + r0 * ldo * (kF32 ? 4 : 2);
+    const int whole = (reinterpret_cast<uintptr_t>(os) | static_cast<uint64_t>(ldo * (kF32 ? 4 : 2))) % 32 == 0;
+    dequantize_kernel<kFormat, kF32, kRecords>
+        <<<blocks, kThreads, 0, s>>>(cs, ss, nr, fast_div(upr), k_blocks, ts, os, ldo, whole);
     if (int r = check_launch(ctx, "fp4 dequantize_kernel")) return r;
   }
   return AEX_OK;

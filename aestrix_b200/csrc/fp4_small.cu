@@ -64,6 +64,7 @@ struct SmallParams {
   void* y;
   int64_t ldy;
   int y_f32;
+  uint32_t zero;  // 0 (arrive_after_loads)
   int* status;
 };
 
@@ -111,18 +112,6 @@ __device__ __forceinline__ uint32_t lds32(uint32_t a) {
   return v;
 }
 __device__ __forceinline__ float lds_f32(uint32_t a) { return __uint_as_float(lds32(a)); }
-
-// The eight codes of a word as four f16 pairs: byte b of a record word holds
-// columns (0, 2), (4, 6), (1, 3), (5, 7) of its eight. An operand only has to
-// pair the same columns on both sides, so the staged activations follow.
-__device__ __forceinline__ void decode_f16(uint32_t w, uint32_t* d) {
-  asm("{\n\t.reg .b8 t0, t1, t2, t3;\n\t"
-      "mov.b32 {t0, t1, t2, t3}, %4;\n\t"
-      "cvt.rn.f16x2.e2m1x2 %0, t0;\n\tcvt.rn.f16x2.e2m1x2 %1, t1;\n\t"
-      "cvt.rn.f16x2.e2m1x2 %2, t2;\n\tcvt.rn.f16x2.e2m1x2 %3, t3;\n\t}"
-      : "=r"(d[0]), "=r"(d[1]), "=r"(d[2]), "=r"(d[3])
-      : "r"(w));
-}
 
 __device__ __forceinline__ uint32_t mul_f16x2(uint32_t a, uint32_t b) {
   uint32_t d;
@@ -193,10 +182,11 @@ __device__ __forceinline__ void sm_stage(const SmallParams& p, const SmStage& st
       }
     }
     if (p.quantize) {
-      float q[8];
-      const float s = scale_to_f32<kFormat>(quantize_cols<kFormat, 8>(v, p.x_scale, p.inv_6ts, q));
-      uint32_t d[4];
-      decode_f16(code_word<false>(q), d);
+      uint32_t top = 0, w, d[4];
+#pragma unroll
+      for (int e = 0; e < 8; ++e) top = max(top, __float_as_uint(v[e]) & 0x7FFFFFFFu);
+      const float s = scale_to_f32<kFormat>(quantize_cols<kFormat, 8, false>(v, top, p.x_scale, p.inv_6ts, &w));
+      decode_f16(w, d);
 #pragma unroll
       for (int j = 0; j < 4; ++j) {
         v[2 * j] = f16_value(d[j] & 0xFFFFu) * s;  // exact
@@ -510,14 +500,18 @@ __global__ void __launch_bounds__(sm_threads(kT)) small_kernel(const __grid_cons
       if (!ok) continue;  // the barriers above still see every warp
       const uint32_t off = in_phase * 512, foff = in_phase * cols * 4;
       const bool narrow = !((wide_now >> in_phase) & 1u);
+      uint32_t all = 0;
 #pragma unroll
       for (int q = 0; q < (kGated ? 2 : 1); ++q) {
         uint4 codes[4];
         uint32_t sc[kFormat == AEX_FP4_NV ? 2 : 4];
         sm_load<kFormat>(ring0 + cs * kSlot + q * kRec, at, codes, sc);
+#pragma unroll
+        for (int i = 0; i < 4; ++i) all |= codes[i].x | codes[i].y | codes[i].z | codes[i].w;
+#pragma unroll
+        for (int i = 0; i < (kFormat == AEX_FP4_NV ? 2 : 4); ++i) all |= sc[i];
         if (q == (kGated ? 1 : 0)) {
-          __syncwarp();
-          if (lane == 0) mbar_arrive_addr(empty0 + 8 * cs);  // the warp's reads of the slot are done
+          arrive_after_loads(empty0 + 8 * cs, all, p.zero, lane);  // the warp's reads of the slot are done
         }
         if (narrow)
           sm_record<kFormat, kT, false>(codes, sc, xb, off, fb, foff, q ? acc1 : acc0);

@@ -30,7 +30,7 @@ struct TilePiece {
 // piece to the next, either c or r goes up by one).
 struct TileWork {
   int m_tiles, whole, split;
-  int rows;  // rows of a slot
+  int rows;  // rows of a slot (stored in bands of 32)
   float* pieces;
 
   // First record of cluster c's share; split * recs * clusters < 2^31 (plan_tiles), since 64-bit divisions at the
@@ -65,12 +65,6 @@ struct TileWork {
     return true;
   }
 };
-
-__device__ __forceinline__ void st_global_32(void* p, const uint32_t* v) {
-  asm volatile("st.global.v8.b32 [%0], {%1,%2,%3,%4,%5,%6,%7,%8};" ::"l"(p), "r"(v[0]), "r"(v[1]), "r"(v[2]), "r"(v[3]),
-               "r"(v[4]), "r"(v[5]), "r"(v[6]), "r"(v[7])
-               : "memory");
-}
 
 // kN (8 or 16) columns [c, c + kN) of a tile's row from their f32 sums (gated:
 // v of the gate, u of the up projection), columns 256 nt + c (gated: 128 nt + c)
@@ -169,51 +163,90 @@ __device__ __forceinline__ void tile_half(const TileOut& p, int64_t row, int nt,
 }
 
 // ------------------------------------------------------------- split tiles
-// Half of the raw accumulators of a piece's row `in_tile` into its slot, columns
-// first (a warp's 32 rows of a column are one 128-byte line).
+// A slot holds a piece's raw accumulators as [32 rows' band][8 columns'
+// group][row][8 columns]: a warp's rows of a group are one kilobyte, written
+// and read 32 bytes a lane.
+__device__ __forceinline__ float* piece_at(const TileWork& w, int slot, int in_tile, int group) {
+  const int bands = (w.rows + 31) >> 5;
+  return w.pieces + ((((static_cast<size_t>(slot) * bands + (in_tile >> 5)) * 32 + group) * 32) + (in_tile & 31)) * 8;
+}
+
+// Columns [c, c + 16) of a row.
+__device__ __forceinline__ void store_piece16(const TileWork& w, int slot, int in_tile, int c, const float* v) {
+  st_global_32(piece_at(w, slot, in_tile, c >> 3), reinterpret_cast<const uint32_t*>(v));
+  st_global_32(piece_at(w, slot, in_tile, (c >> 3) + 1), reinterpret_cast<const uint32_t*>(v + 8));
+}
+
+// Half of a piece's row.
 __device__ __forceinline__ void store_piece(const TileWork& w, int slot, int in_tile, bool live, int half,
                                             uint32_t tbase) {
-  float* dst = w.pieces + static_cast<size_t>(slot) * w.rows * 256 + in_tile;
 #pragma unroll 1
-  for (int c = 128 * half; c < 128 * half + 128; c += 32) {
-    float v[32];
-    tmem_read<32>(tbase + c, v);
-    if (live) {
-#pragma unroll
-      for (int e = 0; e < 32; ++e) dst[static_cast<size_t>(c + e) * w.rows] = v[e];
-    }
+  for (int c = 128 * half; c < 128 * half + 128; c += 16) {
+    float v[16];
+    tmem_read<16>(tbase + c, v);
+    if (live) store_piece16(w, slot, in_tile, c, v);
   }
 }
 
 // Adds the pieces of the split tiles in the order of the clusters that wrote
 // them and hands eight columns of a row at a time to `emit(row, nt, c, v, u)`
-// (gated: v of columns [c, c + 8), u of [128 + c, ..)). One thread each.
+// (gated: v of columns [c, c + 8), u of [128 + c, ..)). One thread each, a warp
+// for 32 rows, four pieces in flight.
+constexpr int kJoinThreads = 256;
+inline int join_blocks(const TileWork& w, bool gated) {
+  return (w.split * ((w.rows + 31) / 32) * (gated ? 16 : 32) + kJoinThreads / 32 - 1) / (kJoinThreads / 32);
+}
+
 template <bool kGated, typename F>
 __device__ __forceinline__ void join_tile(const TileWork& w, int recs, int clusters, int m, F emit) {
-  constexpr int kGroups = kGated ? 16 : 32;
-  const int idx = static_cast<int>(blockIdx.x * blockDim.x + threadIdx.x);
-  const int in_tile = idx % w.rows, c8 = idx / w.rows % kGroups * 8, r = idx / (kGroups * w.rows);
+  constexpr int kGroups = kGated ? 16 : 32, kSums = kGated ? 2 : 1;
+  const int wid = static_cast<int>(blockIdx.x) * (kJoinThreads / 32) + (threadIdx.x >> 5);
+  const int bands = (w.rows + 31) / 32;
+  const int group = wid % kGroups, band = wid / kGroups % bands, r = wid / (kGroups * bands);
   if (r >= w.split) return;
   const int t = w.whole + r;
+  const int in_tile = band * 32 + (threadIdx.x & 31);
   const int64_t row = static_cast<int64_t>(t % w.m_tiles) * 256 + in_tile;
-  if (row >= m) return;
   const int lo = r * recs, hi = lo + recs;
   int c = r * clusters / w.split;
   while (c > 0 && w.start(c, clusters, recs) > lo) --c;
   while (w.start(c + 1, clusters, recs) <= lo) ++c;
-  float v[8], u[8];
+  wait_dependency();  // the pieces are written
+  if (in_tile >= w.rows || row >= m) return;
+  float v[kSums][8];
 #pragma unroll
-  for (int e = 0; e < 8; ++e) v[e] = u[e] = 0.f;
-  for (; c < clusters && w.start(c, clusters, recs) < hi; ++c) {
-    if (w.start(c, clusters, recs) == w.start(c + 1, clusters, recs)) continue;  // nothing fell to this cluster
-    const float* src = w.pieces + (static_cast<size_t>(c + r) * 256 + c8) * w.rows + in_tile;
+  for (int q = 0; q < kSums; ++q)
 #pragma unroll
-    for (int e = 0; e < 8; ++e) {
-      v[e] += src[static_cast<size_t>(e) * w.rows];
-      if (kGated) u[e] += src[static_cast<size_t>(128 + e) * w.rows];
+    for (int e = 0; e < 8; ++e) v[q][e] = 0.f;
+  bool more = true;
+  while (more) {
+    float4 x[4][kSums][2];
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      // (a cluster to which nothing fell has no piece)
+      const int s0 = c + i < clusters ? w.start(c + i, clusters, recs) : hi;
+      more = s0 < hi;
+      const bool have = more && s0 != w.start(c + i + 1, clusters, recs);
+#pragma unroll
+      for (int q = 0; q < kSums; ++q) {
+        x[i][q][0] = x[i][q][1] = make_float4(0.f, 0.f, 0.f, 0.f);
+        if (have) {
+          const float4* src = reinterpret_cast<const float4*>(piece_at(w, c + i + r, in_tile, group + 16 * q));
+          x[i][q][0] = src[0];
+          x[i][q][1] = src[1];
+        }
+      }
     }
+    c += 4;
+#pragma unroll
+    for (int i = 0; i < 4; ++i)
+#pragma unroll
+      for (int q = 0; q < kSums; ++q) {
+        v[q][0] += x[i][q][0].x, v[q][1] += x[i][q][0].y, v[q][2] += x[i][q][0].z, v[q][3] += x[i][q][0].w;
+        v[q][4] += x[i][q][1].x, v[q][5] += x[i][q][1].y, v[q][6] += x[i][q][1].z, v[q][7] += x[i][q][1].w;
+      }
   }
-  emit(row, t / w.m_tiles, c8, v, u);
+  emit(row, t / w.m_tiles, group * 8, v[0], v[kSums - 1]);
 }
 
 // 2: rows of whole 32-byte sectors, 1: of 16-byte vectors, 0: neither.

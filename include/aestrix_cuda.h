@@ -233,8 +233,8 @@ typedef struct aex_fp4weight aex_fp4weight;
  * amax below 2^-125; AEX_FP4_NV amax / (6 tensor_scale) rounded to e4m3 (to
  * nearest even, at most 448). Codes: x / (scale * tensor_scale) to the nearest
  * e2m1 value, ties to the even code, at most 6; both roundings are those of
- * the exact quotient. A block with scale 0 has codes 0; a block that holds an
- * infinity or NaN gets a NaN scale. No reference counterpart (its packs are
+ * the exact quotient. A zero code keeps the sign; a block that holds an
+ * infinity or NaN gets a NaN scale and zero codes. No reference counterpart (its packs are
  * quantized offline). */
 int aex_fp4_quantize(aex_ctx* ctx, const void* x, int x_dtype, int64_t ldx, int rows, int k, int format,
                      float tensor_scale, uint8_t* codes, uint8_t* scales, aex_stream stream);

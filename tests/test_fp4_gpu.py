@@ -331,3 +331,29 @@ def test_gated_dgrad_against_differences(cuda_ctx, act):
         slope = (loss(X + h * d) - loss(X - h * d)) / (2 * h)
         # dg, du and dx are rounded to bf16 (2^-8 each of what they sum); the difference is good to h^2
         assert (np.abs(dx @ d - slope) <= 2.1 * 2.0**-8 * (size @ np.abs(d)) + 1e-6).all()
+
+
+# ---------------------------------------------------------------------------------- repeatability
+
+@pytest.mark.parametrize("mode", MODES)
+@pytest.mark.parametrize("m,n,k", [(1, 2048, 7680), (16, 1000, 4096), (257, 2048, 7680), (1024, 1024, 4096)])
+def test_same_bits_every_time(cuda_ctx, mode, m, n, k):
+    """No sum depends on which warp or CTA is first, and no slot of a ring is filled again before it is
+    read: every one of many calls in a row, queued without a gap, gives the same bits."""
+    x, dh = activations(m, k, 1), activations(m, n, 2)
+    wg, _ = make_weight(n, k, mode, 1, 0.00011)
+    wu, _ = make_weight(n, k, mode, 2, 0.00037)
+    calls = {
+        "mm": lambda: fp4.fp4_mm(x, wg),
+        "gated": lambda: fp4.fp4_gated_mm(x, wg, wu),
+        "quantized": lambda: fp4.fp4_mm(x, wg, quantize_x=True),
+        "gated quantized": lambda: fp4.fp4_gated_mm(x, wg, wu, quantize_x=True),
+        "dgrad": lambda: fp4.fp4_mm_dgrad(dh, wg),
+        "gated dgrad": lambda: fp4.fp4_gated_mm_dgrad(dh, x, wg, wu),
+    }
+    for name, call in calls.items():
+        first = call()
+        differ = torch.zeros((), dtype=torch.int64, device="cuda")
+        for _ in range(100):
+            differ += (call() != first).sum()
+        assert differ.item() == 0, name
