@@ -83,6 +83,7 @@ __global__ void __launch_bounds__(kThreads) quantize_kernel(const void* __restri
                                                             FastDiv upr, int whole, float tensor_scale, float inv_6ts,
                                                             uint8_t* __restrict__ codes,
                                                             uint8_t* __restrict__ scales) {
+  if (kRecords) launch_dependents();  // the product that reads the records waits for them itself
   const uint32_t u = blockIdx.x * kThreads + threadIdx.x;
   const uint32_t row = divide(u, upr), c = u - row * upr.div;  // an mxfp4 pair (u even, u + 1) is one row's
   const bool live = row < static_cast<uint32_t>(rows);

@@ -4,11 +4,11 @@
 // HBM-bound: the weight is read once. A CTA owns 128 weight rows (one column of
 // records; the gated form one of each weight) and one K split of a
 // thread-block cluster; a producer warp streams its records through a ring of
-// shared-memory slots by bulk copies, sixteen compute warps take 16 rows of
-// every other record each (eight, with every record, left the SM's schedulers
-// idle over half of the time: two warps each). The number of slots is even, or
-// enough for every record: a slot's records then all belong to one of the two
-// halves of the warps, which so sees every phase of the slot's barriers.
+// shared-memory slots by bulk copies, compute warps take 16 rows each, three
+// sets of eight warps every third record (one set left the SM's schedulers idle
+// over half of the time). The number of slots is a multiple of the sets, or
+// enough for every record: a slot's records then all belong to one set, which
+// so sees every phase of the slot's barriers.
 // The codes are decoded in registers and multiplied on the tensor cores by
 // mma.sync.m16n8k16 with the activations as the 8-column operand: at 1 to 8
 // rows the work on a decoded pair is the same, and the decoding is what the
@@ -42,11 +42,13 @@
 namespace aex {
 namespace fp4 {
 
-// Compute warps: sixteen for up to 16 activation columns, eight beyond (registers: 8 kT sums and more a thread).
-__host__ __device__ constexpr int sm_warps(int kT) { return kT <= 2 ? 16 : 8; }
+// Sets of eight compute warps: three for up to 16 activation columns, one beyond (registers: 8 kT sums and more a
+// thread).
+__host__ __device__ constexpr int sm_ways(int kT) { return kT <= 2 ? 3 : 1; }
+__host__ __device__ constexpr int sm_warps(int kT) { return 8 * sm_ways(kT); }
 __host__ __device__ constexpr int sm_threads(int kT) { return sm_warps(kT) * 32 + 32; }
 constexpr int kSmMaxSplit = 8;
-constexpr size_t kSmXBudget = 68 * 1024;  // staged activations of one phase
+constexpr int kSmSmem = 226 * 1024;
 
 struct SmallParams {
   const uint8_t* w0;
@@ -159,26 +161,39 @@ struct SmStage {
 template <int kFormat>
 __device__ __forceinline__ void sm_stage(const SmallParams& p, const SmStage& st, int kb0, int nkb, uint32_t only,
                                          int warp, int warps, int lane) {
-  for (int i = warp; i < p.m * nkb; i += warps) {
-    const int b = i / p.m, mr = i % p.m;
-    if (only && !((only >> b) & 1u)) continue;
-    const int col = (kb0 + b) * kRecK + lane * 8;
-    float v[8];
-#pragma unroll
-    for (int e = 0; e < 8; ++e) v[e] = 0.f;
+  // The next item's loads are on their way while one is worked on.
+  const int items = p.m * nkb;
+  uint4 n0 = make_uint4(0, 0, 0, 0), n1 = n0;
+  auto fetch = [&](int i) {
+    const int b = i / p.m, mr = i - b * p.m, col = (kb0 + b) * kRecK + lane * 8;
+    n0 = n1 = make_uint4(0, 0, 0, 0);
     if (col < p.k) {
       if (p.x_f32) {
-        const float4* s = reinterpret_cast<const float4*>(static_cast<const float*>(p.x) + mr * p.ldx + col);
-        const float4 f0 = __ldg(s), f1 = __ldg(s + 1);
-        v[0] = f0.x, v[1] = f0.y, v[2] = f0.z, v[3] = f0.w, v[4] = f1.x, v[5] = f1.y, v[6] = f1.z, v[7] = f1.w;
+        const uint4* s = reinterpret_cast<const uint4*>(static_cast<const float*>(p.x) + mr * p.ldx + col);
+        n0 = __ldg(s);
+        n1 = __ldg(s + 1);
       } else {
-        const uint4 u = __ldg(reinterpret_cast<const uint4*>(static_cast<const uint16_t*>(p.x) + mr * p.ldx + col));
-        const uint32_t w[4] = {u.x, u.y, u.z, u.w};
+        n0 = __ldg(reinterpret_cast<const uint4*>(static_cast<const uint16_t*>(p.x) + mr * p.ldx + col));
+      }
+    }
+  };
+  if (warp < items) fetch(warp);
+  for (int i = warp; i < items; i += warps) {
+    const uint4 r0 = n0, r1 = n1;
+    if (i + warps < items) fetch(i + warps);
+    const int b = i / p.m, mr = i - b * p.m;
+    if (only && !((only >> b) & 1u)) continue;
+    float v[8];
+    if (p.x_f32) {
+      const uint32_t w[8] = {r0.x, r0.y, r0.z, r0.w, r1.x, r1.y, r1.z, r1.w};
 #pragma unroll
-        for (int j = 0; j < 4; ++j) {
-          v[2 * j] = bf16lo_to_f32(w[j]);
-          v[2 * j + 1] = bf16hi_to_f32(w[j]);
-        }
+      for (int e = 0; e < 8; ++e) v[e] = __uint_as_float(w[e]);
+    } else {
+      const uint32_t w[4] = {r0.x, r0.y, r0.z, r0.w};
+#pragma unroll
+      for (int j = 0; j < 4; ++j) {
+        v[2 * j] = bf16lo_to_f32(w[j]);
+        v[2 * j + 1] = bf16hi_to_f32(w[j]);
       }
     }
     if (p.quantize) {
@@ -401,7 +416,7 @@ __global__ void __launch_bounds__(sm_threads(kT)) small_kernel(const __grid_cons
   constexpr int kSlot = sm_slot_bytes(kFormat, kGated);
   constexpr int kRec = rec_bytes(kFormat);
   constexpr int kSmWarps = sm_warps(kT), kSmCompute = kSmWarps * 32, kSmThreads = sm_threads(kT);
-  constexpr int kWays = kSmWarps / 8;  // the warps that share 16 rows take turns at the records
+  constexpr int kWays = sm_ways(kT);  // the warps that share 16 rows take turns at the records
   const int slots = p.slots;
   uint8_t* ring = smem;
   uint64_t* full = reinterpret_cast<uint64_t*>(smem + slots * kSlot);
@@ -421,6 +436,7 @@ __global__ void __launch_bounds__(sm_threads(kT)) small_kernel(const __grid_cons
   st.wide = &wide;
   st.cols = cols;
   st.parts = parts;
+  launch_dependents();
   if (tid == 0) {
     abort_flag = 0;
     wide = 0;
@@ -430,6 +446,7 @@ __global__ void __launch_bounds__(sm_threads(kT)) small_kernel(const __grid_cons
     }
     fence_barrier_init();
   }
+  wait_dependency();  // x, and the weight, may be the previous kernel's
   __syncthreads();
   float acc0[kT][4], acc1[kGated ? kT : 1][4];
 #pragma unroll
@@ -456,7 +473,7 @@ __global__ void __launch_bounds__(sm_threads(kT)) small_kernel(const __grid_cons
     __syncwarp();
   } else {
     const int g = lane >> 2, t = lane & 3;
-    const int row0 = (warp & 7) * 16, odd = warp >> 3;
+    const int row0 = (warp & 7) * 16, set = warp >> 3;
     const SmLane at = sm_lane<kFormat>(row0, g, t, lane);
     // A column past the last reads the last one's: its sums are not stored.
     uint32_t xb[kT], fb[kT][2];
@@ -471,7 +488,7 @@ __global__ void __launch_bounds__(sm_threads(kT)) small_kernel(const __grid_cons
     uint32_t wide_now = 0;
     // slot s and its phase bit, and the record's place in the staged columns, advance with b
     uint32_t s = 0, ph = 0;
-    int in_phase = 0;
+    int in_phase = 0, turn = 0;
 #pragma unroll 1
     for (int b = 0; b < nkb; ++b, ++in_phase) {
       if (in_phase == p.kb_phase) in_phase = 0;
@@ -495,7 +512,9 @@ __global__ void __launch_bounds__(sm_threads(kT)) small_kernel(const __grid_cons
         s = 0;
         ph ^= 1;
       }
-      if (kWays == 2 && (b & 1) != odd) continue;
+      const bool mine = turn == set;
+      if (++turn == kWays) turn = 0;
+      if (!mine) continue;
       if (ok) ok = mbar_wait_warp_addr(full0 + 8 * cs, cph, &abort_flag, p.status, kDevTimeoutTma);
       if (!ok) continue;  // the barriers above still see every warp
       const uint32_t off = in_phase * 512, foff = in_phase * cols * 4;
@@ -534,12 +553,12 @@ __global__ void __launch_bounds__(sm_threads(kT)) small_kernel(const __grid_cons
   float* part0 = reinterpret_cast<float*>(ring);
   float* part1 = part0 + kWays * cols * kRecRows;
   if (warp < kSmWarps) {
-    const int g = lane >> 2, t = lane & 3, row = (warp & 7) * 16 + g, odd = warp >> 3;
+    const int g = lane >> 2, t = lane & 3, row = (warp & 7) * 16 + g, set = warp >> 3;
 #pragma unroll
     for (int i = 0; i < kT; ++i)
 #pragma unroll
       for (int e = 0; e < 4; ++e) {
-        const int c0 = 8 * i + 2 * t + (e & 1), c = odd * cols + c0, r = row + (e >> 1) * 8;
+        const int c0 = 8 * i + 2 * t + (e & 1), c = set * cols + c0, r = row + (e >> 1) * 8;
         if (c0 < cols) {
           part0[c * kRecRows + r] = acc0[i][e];
           if (kGated) part1[c * kRecRows + r] = acc1[i][e];
@@ -605,9 +624,8 @@ int launch_small(aex_ctx* ctx, const Job& j, cudaStream_t s) {
 
   auto kern = small_kernel<kFormat, kT, kGated>;
   constexpr int kSlot = sm_slot_bytes(kFormat, kGated);
-  constexpr int kMaxSmem = 226 * 1024;
   static SmemOptIn opt_in;
-  if (int r = opt_in(ctx, reinterpret_cast<const void*>(kern), kMaxSmem)) return r;
+  if (int r = opt_in(ctx, reinterpret_cast<const void*>(kern), kSmSmem)) return r;
   // K split: the one that leaves the busiest SM the fewest records (CTAs that share an SM share its schedulers), the
   // smallest of those (less to add up). 72 row tiles of 16 records (B200, one row): split 2, 144 CTAs.
   int best_split = 1;
@@ -622,14 +640,15 @@ int launch_small(aex_ctx* ctx, const Job& j, cudaStream_t s) {
     }
   }
   const int kb = (w->k_blocks + best_split - 1) / best_split;
-  const int best_slots = std::min(kb, kGated ? 4 : 6);
+  const int best_slots = std::min(kb, kGated ? 3 : 6);
+  const size_t x_budget = kSmSmem - static_cast<size_t>(best_slots) * kSlot - 128;
   int best_phase = std::min(kb, 32);  // a bit each in the mask of wide records
-  while (best_phase > 1 && static_cast<size_t>(cols) * (best_phase * 516 + 64) > kSmXBudget)
+  while (best_phase > 1 && static_cast<size_t>(cols) * (best_phase * 516 + 64) > x_budget)
     best_phase = (best_phase + 1) / 2;
   // the partial sums take the ring's place
   const size_t best_smem =
       std::max(static_cast<size_t>(best_slots) * kSlot + 128 + static_cast<size_t>(cols) * (best_phase * 516 + 64),
-               static_cast<size_t>(cols) * kRecRows * 4 * (sm_warps(kT) / 8) * (kGated ? 2 : 1));
+               static_cast<size_t>(cols) * kRecRows * 4 * sm_ways(kT) * (kGated ? 2 : 1));
   p.kb_per_split = (w->k_blocks + best_split - 1) / best_split;
   p.kb_phase = best_phase;
   p.slots = best_slots;
@@ -638,13 +657,15 @@ int launch_small(aex_ctx* ctx, const Job& j, cudaStream_t s) {
   cfg.blockDim = dim3(sm_threads(kT), 1, 1);
   cfg.dynamicSmemBytes = best_smem;
   cfg.stream = s;
-  cudaLaunchAttribute attr[1];
+  cudaLaunchAttribute attr[2];
   attr[0].id = cudaLaunchAttributeClusterDimension;
   attr[0].val.clusterDim.x = 1;
   attr[0].val.clusterDim.y = best_split;
   attr[0].val.clusterDim.z = 1;
+  attr[1].id = cudaLaunchAttributeProgrammaticStreamSerialization;  // set up behind the previous kernel
+  attr[1].val.programmaticStreamSerializationAllowed = 1;
   cfg.attrs = attr;
-  cfg.numAttrs = 1;
+  cfg.numAttrs = 2;
   AEX_CUDA_TRY(ctx, cudaLaunchKernelEx(&cfg, kern, p));
   return check_launch(ctx, "fp4 small_kernel");
 }
