@@ -4,9 +4,9 @@
 // HBM-bound: the weight is read once. A CTA owns 128 weight rows (one column of
 // records; the gated form one of each weight) and one K split of a
 // thread-block cluster; a producer warp streams its records through a ring of
-// shared-memory slots by bulk copies, compute warps take 16 rows each, three
-// sets of eight warps every third record (one set left the SM's schedulers idle
-// over half of the time). The number of slots is a multiple of the sets, or
+// shared-memory slots by bulk copies, compute warps take 16 rows each, up to
+// three sets of eight warps that take turns at the records (one set left the
+// SM's schedulers idle over half of the time). The number of slots is a multiple of the sets, or
 // enough for every record: a slot's records then all belong to one set, which
 // so sees every phase of the slot's barriers.
 // The codes are decoded in registers and multiplied on the tensor cores by
@@ -42,9 +42,8 @@
 namespace aex {
 namespace fp4 {
 
-// Sets of eight compute warps: three for up to 16 activation columns, one beyond (registers: 8 kT sums and more a
-// thread).
-__host__ __device__ constexpr int sm_ways(int kT) { return kT <= 2 ? 3 : 1; }
+// Sets of eight compute warps, by the registers that 8 kT activation columns take.
+__host__ __device__ constexpr int sm_ways(int kT) { return kT == 1 ? 3 : kT == 2 ? 2 : 1; }
 __host__ __device__ constexpr int sm_warps(int kT) { return 8 * sm_ways(kT); }
 __host__ __device__ constexpr int sm_threads(int kT) { return sm_warps(kT) * 32 + 32; }
 constexpr int kSmMaxSplit = 8;
@@ -266,7 +265,12 @@ __device__ __forceinline__ void sm_stage(const SmallParams& p, const SmStage& st
 template <int kFormat, int kT, bool kWide>
 __device__ __forceinline__ void sm_record(const uint4* codes, const uint32_t* scales, const uint32_t* xb, uint32_t off,
                                           const uint32_t (*fb)[2], uint32_t foff, float (*acc)[4]) {
-  float c[kT][4];
+  float c[kT][4], f[kT][2];
+#pragma unroll
+  for (int i = 0; i < kT; ++i) {
+    f[i][0] = lds_f32(fb[i][0] + foff);
+    f[i][1] = lds_f32(fb[i][1] + foff);
+  }
   if (kFormat == AEX_FP4_NV) {
     float d[kT][4];  // a second chain of sums: the products of one chain wait for one another
 #pragma unroll
@@ -346,19 +350,18 @@ __device__ __forceinline__ void sm_record(const uint4* codes, const uint32_t* sc
         mma16816<kWide>(d, pa + 2, pb + 2, b.z, b.w);
 #pragma unroll
         for (int e = 0; e < 4; ++e) {
-          const float s = e < 2 ? sa : sb;
-          c[i][e] = ch == 0 ? d[e] * s : fmaf(d[e], s, c[i][e]);
+          // the column's own scale first: what is then multiplied is the f32 product's size, whatever the exponents
+          const float s = e < 2 ? sa : sb, v = d[e] * f[i][e & 1];
+          c[i][e] = ch == 0 ? v * s : fmaf(v, s, c[i][e]);
         }
       }
     }
   }
 #pragma unroll
   for (int i = 0; i < kT; ++i) {
-    const float f0 = lds_f32(fb[i][0] + foff), f1 = lds_f32(fb[i][1] + foff);
-    acc[i][0] = fmaf(c[i][0], f0, acc[i][0]);
-    acc[i][1] = fmaf(c[i][1], f1, acc[i][1]);
-    acc[i][2] = fmaf(c[i][2], f0, acc[i][2]);
-    acc[i][3] = fmaf(c[i][3], f1, acc[i][3]);
+#pragma unroll
+    for (int e = 0; e < 4; ++e)
+      acc[i][e] = kFormat == AEX_FP4_NV ? fmaf(c[i][e], f[i][e & 1], acc[i][e]) : acc[i][e] + c[i][e];
   }
 }
 
@@ -640,7 +643,9 @@ int launch_small(aex_ctx* ctx, const Job& j, cudaStream_t s) {
     }
   }
   const int kb = (w->k_blocks + best_split - 1) / best_split;
-  const int best_slots = std::min(kb, kGated ? 3 : 6);
+  constexpr int kSlots = !kGated ? 6 : sm_ways(kT) == 3 ? 3 : 4;
+  static_assert(kSlots % sm_ways(kT) == 0, "a slot's records belong to one set of warps");
+  const int best_slots = std::min(kb, kSlots);
   const size_t x_budget = kSmSmem - static_cast<size_t>(best_slots) * kSlot - 128;
   int best_phase = std::min(kb, 32);  // a bit each in the mask of wide records
   while (best_phase > 1 && static_cast<size_t>(cols) * (best_phase * 516 + 64) > x_budget)

@@ -357,3 +357,350 @@ def test_same_bits_every_time(cuda_ctx, mode, m, n, k):
         for _ in range(100):
             differ += (call() != first).sum()
         assert differ.item() == 0, name
+
+
+# ------------------------------------------------------------- values that need care
+
+def wide_rows(m, k, seed):
+    """f32 rows whose 256-column stretches span more binades than f16 holds: huge and tiny values side by
+    side, the huge ones where it matters next to zeros."""
+    g = np.random.default_rng(seed)
+    x = g.standard_normal((m, k)) * np.ldexp(1.0, g.integers(-60, 60, (m, k)))
+    x[:, ::5] = 0.0
+    return torch.from_numpy(x.astype(np.float32))
+
+
+@pytest.mark.parametrize("mode", MODES)
+@pytest.mark.parametrize("dtype", ["bf16", "f32"])
+@pytest.mark.parametrize("m,k", [(1, 512), (3, 1120), (7, 2048), (16, 544)])
+def test_few_rows_wide_range(cuda_ctx, mode, dtype, m, k):
+    """The few-rows kernel's f16 staging does not hold these; every element still counts in full: the
+    tolerance is that of the f32 sums, and a row whose large values meet zero weights keeps its small
+    ones."""
+    x = wide_rows(m, k, m + k).to(DT[dtype]).cuda()
+    w, ref_w = make_weight(136, k, mode, k)
+    y = fp4.fp4_mm(x, w, out_dtype=torch.float32)
+    close(y, f64(x) @ ref_w.T, 2.0**-24 * np.abs(f64(x) @ ref_w.T) + sum_bound(f64(x), ref_w, steps_of(m, k, False)))
+    # one huge value against a weight column of zeros, tiny ones elsewhere
+    codes = np.ones((130, k), np.uint8)  # 0.5
+    codes[:, 7] = 0
+    scales = np.full((130, k // R.BLOCK[mode]), 127 if mode == "mxfp4" else 56, np.uint8)  # 1.0
+    w = fp4.FP4Weight(torch.from_numpy(R.pack(codes)).cuda(), torch.from_numpy(scales).cuda(), mode)
+    x = torch.full((m, k), 2.0**-40, dtype=DT[dtype], device="cuda")
+    x[:, 7] = 2.0**100
+    y = fp4.fp4_mm(x, w, out_dtype=torch.float32)
+    ref = (k - 1) * 2.0**-41
+    assert np.abs(f64(y) - ref).max() <= ref * (steps_of(m, k, False) + 8) * 2.0**-22
+
+
+@pytest.mark.parametrize("mode", MODES)
+@pytest.mark.parametrize("m", [2, 20, 40, 300])
+@pytest.mark.parametrize("quantize_x", [False, True])
+def test_infinities_and_nan_stay_where_they_are(cuda_ctx, mode, m, quantize_x):
+    """A row that holds an infinity or NaN, and a weight row with a NaN scale, spoil their own outputs
+    only. Without quantization an infinity gives infinities of the right sign."""
+    k, n = 544, 264
+    x = activations(m, k, 3)
+    g = np.random.default_rng(5)
+    codes = g.integers(1, 8, (n, k)).astype(np.uint8)  # positive, none zero
+    scales = np.full((n, k // R.BLOCK[mode]), 120 if mode == "mxfp4" else 40, np.uint8)
+    scales[100, 3] = 255 if mode == "mxfp4" else 127
+    w = fp4.FP4Weight(torch.from_numpy(R.pack(codes)).cuda(), torch.from_numpy(scales).cuda(), mode)
+    clean = fp4.fp4_mm(x, w, quantize_x=quantize_x, x_scale=1.0)
+    assert torch.isnan(clean[:, 100]).all() and torch.isfinite(clean[:, :100]).all()
+    assert torch.isfinite(clean[:, 101:]).all()
+    y = x.clone()
+    y[0, 17] = float("-inf")
+    y[m - 1, 300] = float("nan")
+    got = fp4.fp4_mm(y, w, quantize_x=quantize_x, x_scale=1.0)
+    keep = [c for c in range(n) if c != 100]
+    assert torch.equal(got[1:m - 1, keep], clean[1:m - 1, keep])
+    assert torch.isnan(got[m - 1]).all()
+    if quantize_x:
+        assert torch.isnan(got[0]).all()
+    else:
+        assert (got[0, keep] == float("-inf")).all()
+
+
+def test_mx_scale_extremes(cuda_ctx):
+    """mxfp4 scale bytes from 0 (2^-127) to 250, in every kernel: the value is code * 2^(byte - 127)."""
+    n, k = 272, 256
+    g = np.random.default_rng(9)
+    codes = g.integers(0, 16, (n, k)).astype(np.uint8)
+    scales = np.repeat(np.linspace(0, 250, n).astype(np.uint8)[:, None], k // 32, 1)
+    w = fp4.FP4Weight(torch.from_numpy(R.pack(codes)).cuda(), torch.from_numpy(scales).cuda(), "mxfp4")
+    ref_w = R.values(codes, scales, "mxfp4")
+    for m in (3, 20, 50):
+        x = (activations(m, k, m).float() * 2.0**-10).to(torch.bfloat16)
+        y = fp4.fp4_mm(x, w, out_dtype=torch.float32)
+        ref = f64(x) @ ref_w.T
+        fits = np.abs(ref) < 1e38
+        # products below the smallest normal f32 may be flushed by the tensor cores: k of them a sum
+        bound = 2.0**-24 * np.abs(ref) + sum_bound(f64(x), ref_w, steps_of(m, k, False)) + k * 2.0**-125
+        assert (np.abs(f64(y) - ref)[fits] <= bound[fits]).all()
+
+
+def test_zero_rows_and_zero_weights(cuda_ctx):
+    for m in (1, 9, 40, 200):
+        x = activations(m, 544, 1)
+        x[0] = 0
+        codes, scales = np.zeros((136, 544), np.uint8), np.zeros((136, 34), np.uint8)
+        w = fp4.FP4Weight(torch.from_numpy(R.pack(codes)).cuda(), torch.from_numpy(scales).cuda(), "nvfp4")
+        assert not fp4.fp4_mm(x, w).any()
+        w, _ = make_weight(136, 544, "nvfp4", 1)
+        for q in (False, True):
+            assert not fp4.fp4_mm(x, w, quantize_x=q, x_scale=0.01)[0].any()
+
+
+# -------------------------------------------------------- layouts, streams, graphs, long inputs
+
+@pytest.mark.parametrize("m", [5, 20, 150])
+@pytest.mark.parametrize("offset,pitch", [(0, 264), (1, 263), (3, 257), (8, 304), (16, 272)])
+def test_output_pitch_and_surroundings(cuda_ctx, m, offset, pitch):
+    """Any pitch and element-aligned start of the result; what lies around it is left as it was."""
+    n, k = 257, 288
+    x = activations(m, k, 2)
+    w, _ = make_weight(n, k, "nvfp4", 3)
+    for dtype in (torch.bfloat16, torch.float32):
+        for q in (False, True):
+            want = fp4.fp4_mm(x, w, quantize_x=q, x_scale=0.02, out_dtype=dtype)
+            buf = torch.full(((m + 2) * pitch + offset + n,), 7.0, dtype=dtype, device="cuda")
+            out = buf[offset:].as_strided((m, n), (pitch, 1))
+            fp4.fp4_mm(x, w, quantize_x=q, x_scale=0.02, out=out)
+            assert torch.equal(out, want)
+            mask = torch.ones_like(buf, dtype=torch.bool)
+            mask[offset:].as_strided((m, n), (pitch, 1)).fill_(False)
+            assert (buf[mask] == 7.0).all()
+            want = fp4.fp4_gated_mm(x, w, w, quantize_x=q, x_scale=0.02, out_dtype=dtype)
+            fp4.fp4_gated_mm(x, w, w, quantize_x=q, x_scale=0.02, out=out)
+            assert torch.equal(out, want) and (buf[mask] == 7.0).all()
+
+
+@pytest.mark.parametrize("m", [4, 24, 140])
+def test_input_pitch_and_start(cuda_ctx, m):
+    """Rows of a wider tensor, starting 16 (not 32) bytes into it."""
+    n, k = 136, 288
+    base = activations(m, 512, 4)
+    x = base[:, 8:8 + k]
+    w, _ = make_weight(n, k, "mxfp4", 3)
+    for q in (False, True):
+        assert torch.equal(fp4.fp4_mm(x, w, quantize_x=q), fp4.fp4_mm(x.contiguous(), w, quantize_x=q))
+    dy = base[:, 8:8 + n]
+    assert torch.equal(fp4.fp4_mm_dgrad(dy, w), fp4.fp4_mm_dgrad(dy.contiguous(), w))
+    a = fp4.fp4_gated_mm_dgrad(dy, x, w, w)
+    assert torch.equal(a, fp4.fp4_gated_mm_dgrad(dy.contiguous(), x.contiguous(), w, w))
+
+
+@pytest.mark.parametrize("m,n,k,dtype", [(2, 20000, 9216, "bf16"), (16, 130, 24576, "f32"), (32, 1000, 9216, "bf16"),
+                                         (13, 5000, 7680, "f32")])
+def test_few_rows_long_columns(cuda_ctx, m, n, k, dtype):
+    """More columns than a CTA stages at once."""
+    x = activations(m, k, 6, DT[dtype])
+    w, ref_w = make_weight(n, k, "nvfp4", 8)
+    y = fp4.fp4_mm(x, w, out_dtype=torch.float32)
+    ref = f64(x) @ ref_w.T
+    close(y, ref, 2.0**-24 * np.abs(ref) + sum_bound(f64(x), ref_w, 19 + k // 256))
+
+
+def test_more_than_2_to_31_elements(cuda_ctx):
+    """Offsets past 32 bits: the last rows of a matrix of 2.2 billion elements, against the same rows alone."""
+    m, k = 270000, 8192
+    x = torch.empty(m, k, dtype=torch.bfloat16, device="cuda")
+    x.normal_()
+    codes, scales = fp4.quantize(x, "nvfp4", tensor_scale=0.002)
+    tail = x[-300:].clone()
+    c, s = fp4.quantize(tail, "nvfp4", tensor_scale=0.002)
+    assert torch.equal(codes[-300:], c) and torch.equal(scales[-300:], s)
+    back = fp4.dequantize(codes, scales, "nvfp4", tensor_scale=0.002)
+    assert torch.equal(back[-300:], fp4.dequantize(c, s, "nvfp4", tensor_scale=0.002))
+    del back, codes, scales
+    w, _ = make_weight(40, k, "nvfp4", 1)
+    # tiles are summed whole or in pieces by their number: the f32 sums may differ by their rounding
+    for q in (False, True):
+        a = fp4.fp4_mm(x, w, quantize_x=q, x_scale=0.002)[-300:].float()
+        b = fp4.fp4_mm(tail, w, quantize_x=q, x_scale=0.002).float()
+        assert (a - b).abs().max() <= 2.0**-7 * b.abs().max()
+    dx = fp4.fp4_mm_dgrad(x[:, :40], w)[-300:].float()
+    ref = fp4.fp4_mm_dgrad(tail[:, :40], w).float()
+    assert (dx - ref).abs().max() <= 2.0**-7 * ref.abs().max()
+
+
+def feed_forward(x, ws, quantize_x, scale):
+    """The block as a transformer runs it: gated projection, then down."""
+    h = fp4.fp4_gated_mm(x, ws["gate"], ws["up"], quantize_x=quantize_x, x_scale=scale)
+    return h, fp4.fp4_mm(h, ws["down"], quantize_x=quantize_x, x_scale=scale)
+
+
+def feed_forward_weights(hidden, width, mode):
+    out, ref = {}, {}
+    for i, (name, n, k) in enumerate((("gate", width, hidden), ("up", width, hidden), ("down", hidden, width))):
+        out[name], ref[name] = make_weight(n, k, mode, 11 + i, 0.0002)
+    return out, ref
+
+
+@pytest.mark.parametrize("mode", MODES)
+@pytest.mark.parametrize("m", [1, 20, 150])
+def test_feed_forward_and_its_gradient(cuda_ctx, mode, m):
+    """The operators as they are used together: forward through the gated block and down, the gradient
+    back through both, against float64 with h rounded to bf16 between (as it is handed over)."""
+    hidden, width = 512, 1120
+    ws, ref = feed_forward_weights(hidden, width, mode)
+    x, dy = activations(m, hidden, 1), activations(m, hidden, 2)
+    h, y = feed_forward(x, ws, False, 1.0)
+    want_h, bound_h = gated_bound(f64(x), ref["gate"], ref["up"], "silu", steps_of(m, hidden, False), 2.0**-8)
+    close(h, want_h, bound_h)
+    H = f64(h)
+    want = H @ ref["down"].T
+    close(y, want, 2.0**-8 * np.abs(want) + sum_bound(H, ref["down"], steps_of(m, width, False)))
+    dh = fp4.fp4_mm_dgrad(dy, ws["down"])
+    want = f64(dy) @ ref["down"]
+    close(dh, want, 2.0**-8 * np.abs(want) + sum_bound(f64(dy), ref["down"].T, -(-hidden // 128) * 8))
+    dx = fp4.fp4_gated_mm_dgrad(dh, x, ws["gate"], ws["up"])
+    dg, du, *_ = gated_grad_ref(f64(x), f64(dh), ref["gate"], ref["up"], "silu")
+    want = dg @ ref["gate"] + du @ ref["up"]
+    size = np.abs(dg) @ np.abs(ref["gate"]) + np.abs(du) @ np.abs(ref["up"])
+    close(dx, want, 2.0**-8 * np.abs(want) + 1.1 * 2.0**-8 * size)
+
+
+@pytest.mark.parametrize("m", [1, 40, 300])
+@pytest.mark.parametrize("quantize_x", [False, True])
+def test_captured_and_replayed(cuda_ctx, m, quantize_x):
+    """Two graphs of the block, replayed in turn and at once on two streams with new inputs: each has its
+    own workspaces, and each replay reads what its input holds then."""
+    hidden, width = 512, 2048
+    ws, _ = feed_forward_weights(hidden, width, "nvfp4")
+    s1, s2 = torch.cuda.Stream(), torch.cuda.Stream()
+    graphs = []
+    for s in (s1, s2):
+        x = activations(m, hidden, 1)
+        torch.cuda.synchronize()
+        with torch.cuda.stream(s):
+            feed_forward(x, ws, quantize_x, 0.02)
+            fp4.fp4_gated_mm_dgrad(torch.zeros(m, width, dtype=torch.bfloat16, device="cuda"), x, ws["gate"], ws["up"])
+        torch.cuda.synchronize()
+        g = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(g, stream=s):
+            h, y = feed_forward(x, ws, quantize_x, 0.02)
+            dx = fp4.fp4_gated_mm_dgrad(h, x, ws["gate"], ws["up"])
+        graphs.append((g, x, y, dx))
+    for r in range(3):
+        ins = [activations(m, hidden, 10 + 2 * r + i) for i in range(2)]
+        want = []
+        for x in ins:
+            h, y = feed_forward(x, ws, quantize_x, 0.02)
+            want.append((y, fp4.fp4_gated_mm_dgrad(h, x, ws["gate"], ws["up"])))
+        for (g, x, _, _), new in zip(graphs, ins):
+            x.copy_(new)
+        torch.cuda.synchronize()
+        for s, (g, *_rest) in zip((s1, s2), graphs):
+            with torch.cuda.stream(s):
+                g.replay()
+                g.replay()
+        torch.cuda.synchronize()
+        for (g, x, y, dx), (wy, wdx) in zip(graphs, want):
+            assert torch.equal(y, wy) and torch.equal(dx, wdx)
+    assert cuda_ctx.device_status() == 0
+
+
+@pytest.mark.parametrize("m", [3, 60, 260])
+def test_given_stream_and_two_streams_at_once(cuda_ctx, m):
+    """The stream argument is the one the kernels run on; calls on two streams that share a weight do not
+    touch one another's scratch."""
+    n, k = 1000, 2080
+    w, _ = make_weight(n, k, "mxfp4", 1)
+    xs = [activations(m, k, i) for i in range(2)]
+    want = [[fp4.fp4_mm(x, w), fp4.fp4_mm(x, w, quantize_x=True), fp4.quantize(x, "mxfp4")[0]] for x in xs]
+    streams = [torch.cuda.Stream(), torch.cuda.Stream()]
+    torch.cuda.synchronize()
+    got = [[], []]
+    for _ in range(10):
+        for i, s in enumerate(streams):
+            got[i].append([fp4.fp4_mm(xs[i], w, stream=s), fp4.fp4_mm(xs[i], w, quantize_x=True, stream=s),
+                           fp4.quantize(xs[i], "mxfp4", stream=s)[0]])
+    torch.cuda.synchronize()
+    for i in range(2):
+        for row in got[i]:
+            assert all(torch.equal(a, b) for a, b in zip(row, want[i]))
+
+
+def test_current_device_is_left_alone(cuda_ctx):
+    before = torch.cuda.current_device()
+    w, _ = make_weight(40, 64, "mxfp4", 1)
+    fp4.fp4_mm(activations(2, 64, 1), w)
+    assert torch.cuda.current_device() == before
+
+
+# ------------------------------------------------------------------------------------- refusals
+
+def test_refusals(cuda_ctx):
+    x = activations(40, 288, 1)
+    w, _ = make_weight(136, 288, "mxfp4", 1)
+    v, _ = make_weight(136, 288, "nvfp4", 1)
+    t, _ = make_weight(128, 288, "mxfp4", 1)
+    E = _lib.AexError
+    with pytest.raises(ValueError, match="columns"):
+        fp4.fp4_mm(x[:, :256], w)
+    with pytest.raises(E, match="multiple of 16 bytes"):
+        fp4.fp4_mm(torch.empty(40, 292, dtype=torch.bfloat16, device="cuda")[:, :288], w)
+    with pytest.raises(E, match="16-byte aligned"):
+        fp4.fp4_mm(torch.empty(40, 296, dtype=torch.bfloat16, device="cuda")[:, 4:292], w)
+    with pytest.raises(ValueError, match="contiguous rows"):
+        fp4.fp4_mm(torch.empty(288, 40, dtype=torch.bfloat16, device="cuda").t(), w)
+    with pytest.raises(TypeError):
+        fp4.fp4_mm(x.half(), w)
+    with pytest.raises(E, match="m <= 16"):
+        fp4.fp4_mm(x.float(), w)
+    with pytest.raises(E, match="no tensor scale"):
+        fp4.fp4_mm(x, w, quantize_x=True, x_scale=0.5)
+    for bad in (0.0, -1.0, float("nan"), float("inf"), 1e-35):
+        with pytest.raises(E, match="tensor_scale"):
+            fp4.fp4_mm(x, v, quantize_x=True, x_scale=bad)
+        with pytest.raises(E, match="tensor_scale"):
+            fp4.quantize(x, "nvfp4", tensor_scale=bad)
+    with pytest.raises(ValueError, match="multiple of 32"):
+        fp4.quantize(x[:, :48], "mxfp4")
+    with pytest.raises(ValueError, match="no rows"):
+        fp4.fp4_mm(x[:0], w)
+    with pytest.raises(TypeError, match="out_dtype"):
+        fp4.fp4_mm(x, w, out_dtype=torch.float16)
+    with pytest.raises(ValueError, match="rows"):
+        fp4.fp4_mm(x, w, out=torch.empty(39, 136, dtype=torch.bfloat16, device="cuda"))
+    with pytest.raises(E, match="row pitch"):
+        fp4.fp4_mm(x, w, out=torch.empty(1, 136, dtype=torch.bfloat16, device="cuda").expand(40, 136))
+    for other in (v, t):
+        with pytest.raises(E, match="one shape and format"):
+            fp4.fp4_gated_mm(x, w, other)
+    with pytest.raises(ValueError, match="activation"):
+        fp4.fp4_gated_mm(x, w, w, activation="relu")
+    with pytest.raises(TypeError):
+        fp4.fp4_mm_dgrad(x.float()[:, :136], w)
+    with pytest.raises(ValueError, match="same number of rows"):
+        fp4.fp4_gated_mm_dgrad(x[:39, :136].contiguous(), x, w, w)
+    with pytest.raises(TypeError, match="bfloat16"):
+        fp4.fp4_gated_mm_dgrad(x[:, :136].contiguous(), x, w, w, out_dtype=torch.float32)
+    codes, scales = fp4.quantize(x, "mxfp4")
+    with pytest.raises(ValueError, match="scales"):
+        fp4.FP4Weight(codes, scales, "nvfp4")
+    with pytest.raises(ValueError, match="contiguous"):
+        fp4.FP4Weight(codes.t().contiguous().t(), scales, "mxfp4")
+    w.close()
+    with pytest.raises(ValueError, match="closed"):
+        fp4.fp4_mm(x, w)
+    # the workspace of the C call: too small, misaligned, missing
+    a = _lib.aex_fp4_mm_args()
+    y = torch.empty(40, 136, dtype=torch.bfloat16, device="cuda")
+    a.x, a.x_dtype, a.ldx, a.m = x.data_ptr(), _lib.AEX_DTYPE_BF16, 288, 40
+    a.quantize_x, a.x_scale, a.y, a.y_dtype, a.ldy = 1, 1.0, y.data_ptr(), _lib.AEX_DTYPE_BF16, 136
+    L = _lib.lib()
+    need = L.aex_fp4_mm_workspace_bytes(v.handle, 40, 1)
+    ws = torch.empty(need + 256, dtype=torch.uint8, device="cuda")
+    for p, n in ((None, 0), (ws.data_ptr(), need - 1), (ws.data_ptr() + 16, need)):
+        a.workspace, a.workspace_bytes = p, n
+        assert L.aex_fp4_mm(cuda_ctx.handle, v.handle, a, None) == _lib.AEX_ERR_INVALID_ARG
+        assert b"workspace" in L.aex_last_error_string(cuda_ctx.handle)
+    for field, value in (("quantize_x", 2), ("m", 0), ("y_dtype", 5), ("x_dtype", -1)):
+        old = getattr(a, field)
+        setattr(a, field, value)
+        assert L.aex_fp4_mm(cuda_ctx.handle, v.handle, a, None) == _lib.AEX_ERR_INVALID_ARG
+        setattr(a, field, old)
+    assert cuda_ctx.device_status() == 0
