@@ -102,9 +102,8 @@ __device__ __forceinline__ float rcp_approx(float x) {
 // unit has 4 significant bits, and a quotient that is rounded correctly (a
 // reciprocal rounded to nearest, one residual) is a border only if v is. Any
 // other tensor_scale: v is multiplied by the reciprocal 2^-21 above and below;
-// the approximations are off by at most 2^-22, so where both give the same code
-// it is the quotient's, and where not (a value in some hundred thousand) the
-// border is settled exactly. (Settling every value cost 21 us for 4608 x 4096.)
+// the approximations are off by at most 2^-22, so where both give the same codes
+// they are the quotients', and where not the eight borders are settled exactly. (Settling every value cost 21 us for 4608 x 4096.)
 template <int kFormat, int kN, bool kPermute>
 __device__ __forceinline__ uint32_t quantize_cols(const float* v, uint32_t top, float tensor_scale, float inv_6ts,
                                                   uint32_t* codes) {
@@ -138,7 +137,6 @@ __device__ __forceinline__ uint32_t quantize_cols(const float* v, uint32_t top, 
   } else {
     const float inv = rcp_approx(unit);
     const float up = inv * (1.f + 0x1p-21f), down = inv * (1.f - 0x1p-21f);
-    bool near = false;
 #pragma unroll
     for (int h = 0; h < kN / 8; ++h) {
       float a[8], b[8];
@@ -148,13 +146,14 @@ __device__ __forceinline__ uint32_t quantize_cols(const float* v, uint32_t top, 
         b[i] = v[8 * h + i] * down;
       }
       codes[h] = code_word<kPermute>(a);
-      near |= codes[h] != code_word<kPermute>(b);
-    }
-    if (near && sb) {
+      if (codes[h] != code_word<kPermute>(b) && sb) {
 #pragma unroll
-      for (int i = 0; i < kN; ++i) q[i] = copysignf(settle(fabsf(v[i]) * inv, s, tensor_scale, fabsf(v[i])), v[i]);
-#pragma unroll
-      for (int h = 0; h < kN / 8; ++h) codes[h] = code_word<kPermute>(q + 8 * h);
+        for (int i = 0; i < 8; ++i) {
+          const float x = v[8 * h + i];
+          a[i] = copysignf(settle(fabsf(x) * inv, s, tensor_scale, fabsf(x)), x);
+        }
+        codes[h] = code_word<kPermute>(a);
+      }
     }
   }
   if (bad || sb == 0) {

@@ -79,7 +79,7 @@ __device__ __forceinline__ uint32_t divide(uint32_t u, const FastDiv& f) {
 // past the last are left as they are). `upr` units of 16 columns a row (even);
 // rows * upr < 2^31 (the host slices).
 template <int kFormat, bool kF32, bool kRecords>
-__global__ void __launch_bounds__(kThreads) quantize_kernel(const void* __restrict__ x, int64_t ldx, int rows, int k,
+__global__ void __launch_bounds__(kThreads, 8) quantize_kernel(const void* __restrict__ x, int64_t ldx, int rows, int k,
                                                             FastDiv upr, int whole, float tensor_scale, float inv_6ts,
                                                             uint8_t* __restrict__ codes,
                                                             uint8_t* __restrict__ scales) {
@@ -114,17 +114,62 @@ __global__ void __launch_bounds__(kThreads) quantize_kernel(const void* __restri
   }
 }
 
-// Two codes' product with the block scale is exact in f32 (2 + 4 bits); the
-// tensor scale is then one rounding for an f32 output. For bf16 that f32 is
-// rounded to odd first, so that the second rounding sees which side of a tie
-// the product is on.
-template <bool kF32>
-__device__ __forceinline__ float scaled(float cs, float tensor_scale) {
-  if (kF32) return cs * tensor_scale;
-  const float p = __fmul_rz(cs, tensor_scale);
-  return __fmaf_rn(cs, tensor_scale, -p) != 0.f && fabsf(p) <= 3.402823466e38f
-             ? __uint_as_float(__float_as_uint(p) | 1u)
-             : p;
+__device__ __forceinline__ uint32_t nibble_compress(uint32_t x) {  // 4 bytes < 16 -> 4 nibbles
+  x = (x | (x >> 4)) & 0x00FF00FFu;
+  return (x | (x >> 8)) & 0x0000FFFFu;
+}
+__device__ __forceinline__ uint32_t permute_word(uint32_t w) {
+  return nibble_compress(w & 0x0F0F0F0Fu) | (nibble_compress((w >> 4) & 0x0F0F0F0Fu) << 16);
+}
+__device__ __forceinline__ uint32_t nibble_spread(uint32_t x) {  // 4 nibbles -> the low nibbles of 4 bytes
+  x = (x | (x << 8)) & 0x00FF00FFu;
+  return (x | (x << 4)) & 0x0F0F0F0Fu;
+}
+__device__ __forceinline__ uint32_t restore_word(uint32_t w) {  // inverse of permute_word
+  return nibble_spread(w & 0xFFFFu) | (nibble_spread(w >> 16) << 4);
+}
+
+// x rounded so that one more rounding, to bf16, is that of the exact product
+// c * tensor_scale: to odd, which keeps the side of every bf16 tie.
+__device__ __forceinline__ float product_to_odd(float c, float tensor_scale) {
+  const float p = __fmul_rz(c, tensor_scale);
+  return __fmaf_rn(c, tensor_scale, -p) != 0.f ? __uint_as_float(__float_as_uint(p) | 1u) : p;
+}
+
+// Four bytes of a and b by the nibbles of sel's low half (__byte_perm without its masking of bit 3).
+__device__ __forceinline__ uint32_t prmt(uint32_t a, uint32_t b, uint32_t sel) {
+  uint32_t d;
+  asm("prmt.b32 %0, %1, %2, %3;" : "=r"(d) : "r"(a), "r"(b), "r"(sel));
+  return d;
+}
+
+// The values of 16 codes as bf16 pairs in the order of the columns. A block has
+// eight magnitudes: s and 1.5 s times the tensor scale, each rounded once, and
+// powers of two of them (exact: tensor scales and block scales leave room). The
+// codes select their bytes (a third of the instructions of a product and a
+// rounding for each).
+__device__ __forceinline__ void bf16_by_table(uint2 codes, float s, float tensor_scale, uint32_t* o) {
+  const float a = __bfloat162float(__float2bfloat16_rn(product_to_odd(s, tensor_scale)));
+  const float b = __bfloat162float(__float2bfloat16_rn(product_to_odd(1.5f * s, tensor_scale)));
+  const float m[8] = {a * 0.f, a * 0.5f, a, b, a * 2.f, b * 2.f, a * 4.f, b * 4.f};
+  uint32_t lo[2], hi[2];
+#pragma unroll
+  for (int h = 0; h < 2; ++h) {
+    const uint32_t p = __byte_perm(__float_as_uint(m[4 * h]), __float_as_uint(m[4 * h + 1]), 0x7362);
+    const uint32_t q = __byte_perm(__float_as_uint(m[4 * h + 2]), __float_as_uint(m[4 * h + 3]), 0x7362);
+    lo[h] = __byte_perm(p, q, 0x5410);
+    hi[h] = __byte_perm(p, q, 0x7632);
+  }
+#pragma unroll
+  for (int q = 0; q < 4; ++q) {
+    const uint32_t w = (q & 2 ? codes.y : codes.x) >> (16 * (q & 1)), idx = w & 0x7777u;
+    // a selector with bit 3 set repeats the sign of the selected byte: 0xFF for a negative code, 0x80 for others
+    const uint32_t sign = prmt(0x80808080u, 0x80808080u, w) << 1;
+    const uint32_t l4 = prmt(lo[0], lo[1], idx);
+    const uint32_t h4 = prmt(hi[0], hi[1], idx) | (sign & 0x80808080u);
+    o[2 * q] = __byte_perm(l4, h4, 0x5140);
+    o[2 * q + 1] = __byte_perm(l4, h4, 0x7362);
+  }
 }
 
 // Codes -> values, out [rows, k] (row pitch ldo). kRecords: from the record
@@ -150,26 +195,24 @@ __global__ void __launch_bounds__(kThreads) dequantize_kernel(const uint8_t* __r
     sb = __ldg(scales + (kFormat == AEX_FP4_NV ? u : u >> 1));
   }
   const float s = scale_to_f32<kFormat>(sb);
-  float v[16];
-#pragma unroll
-  for (int h = 0; h < 2; ++h) {
-    uint32_t d[4];
-    decode_f16(h ? w.y : w.x, d);
-#pragma unroll
-    for (int i = 0; i < 8; ++i) {
-      // byte b of a record word holds columns (0, 2), (4, 6), (1, 3), (5, 7) of its eight
-      const int b = kRecords ? (i & 1) * 2 + (i >> 2) : i >> 1, hi = kRecords ? (i >> 1) & 1 : i & 1;
-      const float cv = __half2float(__ushort_as_half(static_cast<uint16_t>(hi ? d[b] >> 16 : d[b] & 0xFFFFu)));
-      v[8 * h + i] = scaled<kF32>(cv * s, tensor_scale);
-    }
-  }
+  if (kRecords) w = make_uint2(restore_word(w.x), restore_word(w.y));
   const int64_t at = static_cast<int64_t>(row) * ldo + static_cast<int64_t>(c) * 16;
   uint32_t o[16];
+  if (kF32) {
 #pragma unroll
-  for (int i = 0; i < 16; ++i) o[i] = __float_as_uint(v[i]);
-  if (!kF32) {
+    for (int h = 0; h < 2; ++h) {
+      uint32_t d[4];
+      decode_f16(h ? w.y : w.x, d);
 #pragma unroll
-    for (int i = 0; i < 8; ++i) o[i] = pack_bf16x2(v[2 * i], v[2 * i + 1]);
+      for (int i = 0; i < 8; ++i) {
+        const uint32_t half = i & 1 ? d[i >> 1] >> 16 : d[i >> 1] & 0xFFFFu;
+        // code * scale is exact (2 + 4 bits), so this is one rounding
+        o[8 * h + i] =
+            __float_as_uint(__half2float(__ushort_as_half(static_cast<uint16_t>(half))) * s * tensor_scale);
+      }
+    }
+  } else {
+    bf16_by_table(w, s, tensor_scale, o);
   }
   uint8_t* dst = static_cast<uint8_t*>(out) + at * (kF32 ? 4 : 2);
 #pragma unroll
@@ -181,14 +224,6 @@ __global__ void __launch_bounds__(kThreads) dequantize_kernel(const uint8_t* __r
       *reinterpret_cast<uint4*>(dst + 4 * i + 16) = make_uint4(o[i + 4], o[i + 5], o[i + 6], o[i + 7]);
     }
   }
-}
-
-__device__ __forceinline__ uint32_t nibble_compress(uint32_t x) {  // 4 bytes < 16 -> 4 nibbles
-  x = (x | (x >> 4)) & 0x00FF00FFu;
-  return (x | (x >> 8)) & 0x0000FFFFu;
-}
-__device__ __forceinline__ uint32_t permute_word(uint32_t w) {
-  return nibble_compress(w & 0x0F0F0F0Fu) | (nibble_compress((w >> 4) & 0x0F0F0F0Fu) << 16);
 }
 
 // Rows as stored (codes, scales) -> records, zero past n and k. One CTA per
