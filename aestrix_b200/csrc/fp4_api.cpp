@@ -65,9 +65,9 @@ int run(aex_ctx* ctx, const aex_fp4weight* w0, const aex_fp4weight* w1, int acti
     return set_error(ctx, AEX_ERR_INVALID_ARG, "quantize_x must be 0 or 1");
   if (a->quantize_x)
     if (int r = fp4::check_format(ctx, w0->format, a->x_scale)) return r;
-  if (f32 && !a->quantize_x && a->m > fp4::kSmallRowsF32)
+  if (f32 && !a->quantize_x && a->m > fp4::kSmallRows)
     return set_error(ctx, AEX_ERR_UNSUPPORTED, "f32 activations without quantize_x are supported for m <= %d",
-                     fp4::kSmallRowsF32);
+                     fp4::kSmallRows);
   const bool gated = w1 != nullptr;
   if (a->m > fp4::kSmallRows)
     if (int r = check_tiles(ctx, a->quantize_x ? fp4::plan_block(w0, gated, a->m) : fp4::plan_gemm(w0, gated, a->m)))

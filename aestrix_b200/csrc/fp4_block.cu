@@ -161,7 +161,7 @@ __global__ void __launch_bounds__(kBThreads, 1) block_kernel(const __grid_consta
       int g = 0;
       bool ok = true;
       TilePiece t;
-      for (int i = 0; ok && p.work.piece(cluster, clusters, p.k_blocks, i, &t); ++i) {
+      for (int i = 0; ok && p.work.piece(cluster, clusters, i, &t); ++i) {
         const int mt = t.mt, nt = t.nt;
         const size_t step = static_cast<size_t>(kRec);
         // past the last tile of rows or outputs: any record, its results are not stored
@@ -209,7 +209,7 @@ __global__ void __launch_bounds__(kBThreads, 1) block_kernel(const __grid_consta
       uint32_t s = 0, ph = 0;
       bool ok = true;
       TilePiece t;
-      for (int i = 0; ok && p.work.piece(cluster, clusters, p.k_blocks, i, &t); ++i)
+      for (int i = 0; ok && p.work.piece(cluster, clusters, i, &t); ++i)
         for (int k = t.r0; k < t.r1; ++k) {
           if (!mbar_wait_cl(smem_u32(&full[s]), ph, &abort_flag, p.status, kDevTimeoutTma)) {
             ok = false;
@@ -231,7 +231,7 @@ __global__ void __launch_bounds__(kBThreads, 1) block_kernel(const __grid_consta
       uint32_t s = 0, ph = 0;
       bool ok = true;
       TilePiece t;
-      for (int i = 0; ok && p.work.piece(cluster, clusters, p.k_blocks, i, &t); ++i) {
+      for (int i = 0; ok && p.work.piece(cluster, clusters, i, &t); ++i) {
         // this accumulator's previous tile is read, and of the other's the columns they share
         const int b = i & 1;
         if ((i >= 2 && !mbar_wait_cl(smem_u32(&acce[b]), ((i >> 1) + 1) & 1, &abort_flag, p.status, kDevTimeoutMma)) ||
@@ -281,7 +281,7 @@ __global__ void __launch_bounds__(kBThreads, 1) block_kernel(const __grid_consta
     const int quad = warp & 3, half = (warp - 4) >> 2;
     const uint32_t ovl_lead = mapa_shared(smem_u32(ovl), 0);
     TilePiece t;
-    for (int i = 0; p.work.piece(cluster, clusters, p.k_blocks, i, &t); ++i) {
+    for (int i = 0; p.work.piece(cluster, clusters, i, &t); ++i) {
       const int b = i & 1;
       if (!mbar_wait_warp_cl(smem_u32(&accf[b]), (i >> 1) & 1, &abort_flag, p.status, kDevTimeoutEpilogue)) break;
       tc_fence_after();
@@ -356,11 +356,10 @@ __global__ void __launch_bounds__(kBThreads, 1) block_kernel(const __grid_consta
 }
 
 template <bool kGated>
-__global__ void __launch_bounds__(kJoinThreads) block_join_kernel(const __grid_constant__ BlockParams p, int clusters) {
-  join_tile<kGated>(p.work, p.k_blocks, clusters, p.o.m,
-                    [&](int64_t row, int nt, int c, const float* v, const float* u) {
-                      finish<kGated, 8>(p.o, row, nt, c, v, u);
-                    });
+__global__ void __launch_bounds__(kJoinThreads) block_join_kernel(const __grid_constant__ BlockParams p) {
+  join_tile<kGated>(p.work, p.o.m, [&](int64_t row, int nt, int c, const float* v, const float* u) {
+    finish<kGated, 8>(p.o, row, nt, c, v, u);
+  });
 }
 
 namespace {
@@ -376,11 +375,7 @@ int launch_block(aex_ctx* ctx, const Job& j, cudaStream_t s) {
   p.k_blocks = w->k_blocks;
   p.x_tiles = (j.m - 1) / kRecRows + 1;
   p.n_tiles = w->n_tiles;
-  p.work.m_tiles = plan.m_tiles;
-  p.work.whole = plan.whole;
-  p.work.split = plan.split;
-  p.work.rows = plan.rows;
-  p.work.pieces = static_cast<float*>(j.pieces);
+  p.work = tile_work(plan, j.pieces);
   p.o.m = j.m;
   p.o.cols = w->n;
   p.o.alpha0 = static_cast<float>(static_cast<double>(j.x_scale) * w->tensor_scale);
@@ -398,7 +393,7 @@ int launch_block(aex_ctx* ctx, const Job& j, cudaStream_t s) {
     return r;
   if (plan.split)
     return launch_after(ctx, reinterpret_cast<const void*>(block_join_kernel<kGated>), join_blocks(p.work, kGated),
-                        kJoinThreads, s, &p, const_cast<int*>(&plan.clusters));
+                        kJoinThreads, s, &p);
   return AEX_OK;
 }
 

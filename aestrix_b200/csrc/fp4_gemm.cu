@@ -77,7 +77,6 @@ struct GemmParams {
   const uint8_t* w1;
   int k_blocks;  // records along the columns of a weight
   int n_tiles;   // records along its rows
-  int recs;      // records per tile and CTA (dgrad: of both weights)
   TileWork work;
   TileOut o;
   GradOut grad;
@@ -187,7 +186,7 @@ __global__ void __launch_bounds__(kGThreads, 1)
       int g = 0;  // K steps so far
       bool ok = true;
       TilePiece t;
-      for (int i = 0; ok && p.work.piece(cluster, clusters, p.recs, i, &t); ++i) {
+      for (int i = 0; ok && p.work.piece(cluster, clusters, i, &t); ++i) {
         const int row0 = t.mt * 256 + static_cast<int>(rank) * 128;
         for (int k = t.r0 * kUnits * 2; k < t.r1 * kUnits * 2; ++k, ++g) {
           if (g >= kGA) {
@@ -223,7 +222,7 @@ __global__ void __launch_bounds__(kGThreads, 1)
       int g = 0;
       bool ok = true;
       TilePiece t;
-      for (int i = 0; ok && p.work.piece(cluster, clusters, p.recs, i, &t); ++i) {
+      for (int i = 0; ok && p.work.piece(cluster, clusters, i, &t); ++i) {
         for (int r = t.r0; r < t.r1; ++r, ++g) {
           if (g >= kGRecs && !mbar_wait(&rempty[s], ph ^ 1, &abort_flag, p.status, kDevTimeoutProducer)) {
             ok = false;
@@ -273,7 +272,7 @@ __global__ void __launch_bounds__(kGThreads, 1)
       uint32_t as = 0, aph = 0, bs = 0;
       bool ok = true;
       TilePiece t;
-      for (int i = 0; ok && p.work.piece(cluster, clusters, p.recs, i, &t); ++i)
+      for (int i = 0; ok && p.work.piece(cluster, clusters, i, &t); ++i)
         for (int u = t.r0 * kUnits; u < t.r1 * kUnits && ok; ++u) {
 #pragma unroll
           for (int h = 0; h < 2; ++h) {
@@ -297,7 +296,7 @@ __global__ void __launch_bounds__(kGThreads, 1)
       uint32_t as = 0, aph = 0, bs = 0, bph = 0, ds = 0;
       bool ok = true;
       TilePiece t;
-      for (int i = 0; ok && p.work.piece(cluster, clusters, p.recs, i, &t); ++i) {
+      for (int i = 0; ok && p.work.piece(cluster, clusters, i, &t); ++i) {
         const int b = i & 1;
         if (i >= 2 && !mbar_wait_cl(smem_u32(&acce[b]), ((i >> 1) + 1) & 1, &abort_flag, p.status, kDevTimeoutMma)) {
           ok = false;
@@ -347,7 +346,7 @@ __global__ void __launch_bounds__(kGThreads, 1)
     // ------------------------------------------------------------ epilogue
     const int quad = warp & 3, half = (warp - 4) >> 2;
     TilePiece t;
-    for (int i = 0; p.work.piece(cluster, clusters, p.recs, i, &t); ++i) {
+    for (int i = 0; p.work.piece(cluster, clusters, i, &t); ++i) {
       const int b = i & 1;
       if (!mbar_wait_warp_cl(smem_u32(&accf[b]), (i >> 1) & 1, &abort_flag, p.status, kDevTimeoutEpilogue)) break;
       tc_fence_after();
@@ -389,7 +388,7 @@ __global__ void __launch_bounds__(kGThreads, 1)
     int g = 0;                                                     // units so far
     bool ok = true;
     TilePiece t;
-    for (int i = 0; ok && p.work.piece(cluster, clusters, p.recs, i, &t); ++i) {
+    for (int i = 0; ok && p.work.piece(cluster, clusters, i, &t); ++i) {
       const int n = (t.r1 - t.r0) * kUnits;
       for (int u = 0; u < n; ++u, ++g) {
         const uint32_t cb = bs, cds = ds, cdph = dph, crs = rs, crph = rph;
@@ -472,9 +471,9 @@ __global__ void __launch_bounds__(kGThreads, 1)
 }
 
 template <int kMode>
-__global__ void __launch_bounds__(kJoinThreads) join_kernel(const __grid_constant__ GemmParams p, int clusters) {
+__global__ void __launch_bounds__(kJoinThreads) join_kernel(const __grid_constant__ GemmParams p) {
   constexpr bool kGated = kMode == kGatedFwd || kMode == kGatedGrad;
-  join_tile<kGated>(p.work, p.recs, clusters, p.o.m, [&](int64_t row, int nt, int c, const float* v, const float* u) {
+  join_tile<kGated>(p.work, p.o.m, [&](int64_t row, int nt, int c, const float* v, const float* u) {
     if (kMode == kGatedGrad) {
       float g[8], h[8];
 #pragma unroll
@@ -501,11 +500,7 @@ int x_map(aex_ctx* ctx, CUtensorMap* tm, const void* x, int64_t ldx, int rows, i
 template <int kFormat, int kMode>
 int launch_gemm(aex_ctx* ctx, const CUtensorMap& tm0, const CUtensorMap& tm1, GemmParams p, const TilePlan& plan,
                 void* pieces, cudaStream_t s) {
-  p.work.m_tiles = plan.m_tiles;
-  p.work.whole = plan.whole;
-  p.work.split = plan.split;
-  p.work.rows = plan.rows;
-  p.work.pieces = static_cast<float*>(pieces);
+  p.work = tile_work(plan, pieces);
   p.status = ctx->d_status;
   auto kern = gemm_kernel<kFormat, kMode>;
   static SmemOptIn opt_in;
@@ -515,8 +510,7 @@ int launch_gemm(aex_ctx* ctx, const CUtensorMap& tm0, const CUtensorMap& tm1, Ge
     return r;
   if (plan.split)
     return launch_after(ctx, reinterpret_cast<const void*>(join_kernel<kMode>),
-                        join_blocks(p.work, kMode == kGatedFwd || kMode == kGatedGrad), kJoinThreads, s, &p,
-                        const_cast<int*>(&plan.clusters));
+                        join_blocks(p.work, kMode == kGatedFwd || kMode == kGatedGrad), kJoinThreads, s, &p);
   return AEX_OK;
 }
 
@@ -578,7 +572,6 @@ int run_gemm(aex_ctx* ctx, const Job& j, cudaStream_t s) {
   CUtensorMap tm;
   if (int r = x_map(ctx, &tm, j.x, j.ldx, j.m, w->k)) return r;
   GemmParams p = weight_params(w, j.w1);
-  p.recs = w->k_blocks;
   p.o.m = j.m;
   p.o.cols = w->n;
   p.o.alpha0 = unit_of(w->format) * w->tensor_scale;
@@ -599,7 +592,6 @@ int run_gated_grad(aex_ctx* ctx, const aex_fp4weight* wg, const aex_fp4weight* w
   CUtensorMap tm;
   if (int r = x_map(ctx, &tm, x, ldx, m, wg->k)) return r;
   GemmParams p = weight_params(wg, wu);
-  p.recs = wg->k_blocks;
   p.o.m = m;
   p.o.cols = wg->n;
   p.o.alpha0 = unit_of(wg->format) * wg->tensor_scale;
@@ -624,7 +616,6 @@ int run_dgrad(aex_ctx* ctx, const aex_fp4weight* w0, const aex_fp4weight* w1, co
   if (w1)
     if (int r = x_map(ctx, &tm1, d1, ld1, m, w1->n)) return r;
   GemmParams p = weight_params(w0, w1);
-  p.recs = w0->n_tiles * (w1 ? 2 : 1);
   p.o.m = m;
   p.o.cols = w0->k;
   p.o.alpha0 = unit_of(w0->format) * alpha;

@@ -6,6 +6,7 @@
 #else
 #define AEX_HD
 #endif
+#include <algorithm>
 #include <atomic>
 
 #include "internal.h"
@@ -100,30 +101,38 @@ struct Job {
 // How a GEMM's 256 x 256 output tiles go to `clusters` CTA pairs (TileWork).
 struct TilePlan {
   int clusters = 0;  // of the launch
-  int m_tiles = 0, whole = 0, split = 0;
+  int m_tiles = 0, whole = 0, split = 0, parts = 0, recs = 0;
   int rows = 0;       // of a piece
   size_t bytes = 0;   // of all pieces
 };
 
 // `recs` records along K per tile, `rec_us` microseconds each in the main loop. Tiles that do not fill a last wave of
-// the clusters are split when that wave's records, dealt out over all clusters, and the join take less than the wave.
-// The join: 3 us, and the pieces written and read (B200, measured: 4 us for 6 MB, 8 us for 20 MB; 77 rows through
-// 7680 -> 4096 51 us whole, 22 us split; 512 rows back through 4096 -> 7680 30.8 us whole, 32.0 us split).
+// the clusters are split when that wave's records, dealt out over the clusters (32 pieces a tile at most), and the
+// join take less than the wave. The join: 2.5 us, 1 us for every eight pieces of a tile, and the pieces written and
+// read (B200, measured: 4 us for 6 MB, 8 us for 20 MB; 77 rows through 7680 -> 4096 51 us whole, 22 us split; 512
+// rows back through 4096 -> 7680 30.8 us whole, 32.0 us split).
 inline TilePlan plan_tiles(int clusters, int m, int64_t col_tiles, int recs, double rec_us) {
   TilePlan p;
   p.m_tiles = (m - 1) / 256 + 1;
   p.rows = m < 256 ? m : 256;
+  p.recs = recs;
   const int64_t tiles = p.m_tiles * col_tiles;
   if (tiles > 0x3FFFFFFF) return p;  // refused by the caller
   const int64_t left = tiles % clusters;
-  const size_t bytes = static_cast<size_t>(clusters + left) * ((p.rows + 31) / 32 * 32) * 256 * sizeof(float);
-  const double saved = rec_us * static_cast<double>(recs - (left * recs + clusters - 1) / clusters);
-  if (left && saved > 3.0 + 2.0 * static_cast<double>(bytes) / 6.5e6 && left * recs * clusters < 0x7FFFFFFF) {
-    p.split = static_cast<int>(left);
-    p.bytes = bytes;
+  p.whole = static_cast<int>(tiles);
+  if (left && left * recs < 0x7FFFFFFF / (clusters + 1)) {
+    const int64_t parts = std::min<int64_t>(clusters, left * std::min(recs, 32));
+    const int64_t share = (left * recs + parts - 1) / parts;
+    const size_t bytes = static_cast<size_t>(parts + left) * ((p.rows + 31) / 32 * 32) * 256 * sizeof(float);
+    const double join = 2.5 + 1.0 * static_cast<double>(parts / left / 8 + 1) + 2.0 * static_cast<double>(bytes) / 6.5e6;
+    if (rec_us * static_cast<double>(recs - share) > join) {
+      p.split = static_cast<int>(left);
+      p.parts = static_cast<int>(parts);
+      p.whole -= p.split;
+      p.bytes = bytes;
+    }
   }
-  p.whole = static_cast<int>(tiles) - p.split;
-  p.clusters = p.split || tiles > clusters ? clusters : static_cast<int>(tiles);
+  p.clusters = std::max(p.parts, std::min(p.whole, clusters));
   return p;
 }
 TilePlan plan_gemm(const aex_fp4weight* w, bool gated, int m);
@@ -170,10 +179,10 @@ int launch_after(aex_ctx* ctx, const void* kernel, int blocks, int threads, cuda
   return check_launch(ctx, "fp4 join");
 }
 
-// The few-rows kernel takes up to 48 columns of its 8-column operand: rows that are bf16 or quantized, or f32 rows at
-// three columns each. No workspace.
-constexpr int kSmallRows = 32;
-constexpr int kSmallRowsF32 = 16;
+// The few-rows kernel takes a row as one column of its 8-column operand where it is bf16 or quantized, f32 rows as
+// three columns each. No workspace. More rows go to the GEMMs: 19 rows, 7520 -> 5376, take 37 us as four times 8
+// columns and 24 us there.
+constexpr int kSmallRows = 16;
 int run_small(aex_ctx* ctx, const Job& j, cudaStream_t s);
 // Any number of bf16 rows: dequantizing GEMM.
 int run_gemm(aex_ctx* ctx, const Job& j, cudaStream_t s);

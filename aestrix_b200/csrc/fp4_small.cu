@@ -1,5 +1,5 @@
-// fp4_small.cu — products of few rows (at most 32; f32 rows 16) with microscaled
-// 4-bit weights: y = x W^T, or act(x Wg^T) * (x Wu^T).
+// fp4_small.cu — products of few rows (at most 16) with microscaled 4-bit
+// weights: y = x W^T, or act(x Wg^T) * (x Wu^T).
 //
 // HBM-bound: the weight is read once. A CTA owns 128 weight rows (one column of
 // records; the gated form one of each weight) and one K split of a

@@ -24,38 +24,37 @@ struct TilePiece {
 
 // The output tiles and who computes them. Tiles are numbered with the rows'
 // tiles fastest. The first `whole` go to the clusters in turn, one cluster
-// each; the records of the `split` others are dealt out evenly, in order, so
-// that a cluster gets at most the end of one tile and the start of the next.
-// The piece of split tile r that cluster c computes has slot c + r (from one
-// piece to the next, either c or r goes up by one).
+// each; the records of the `split` others are dealt out evenly, in order, over
+// the first `parts` clusters (at least one record each), so that a cluster gets
+// at most the end of one tile and the start of the next. The piece of split
+// tile r that cluster c computes has slot c + r (from one piece to the next,
+// either c or r goes up by one).
 struct TileWork {
-  int m_tiles, whole, split;
+  int m_tiles, whole, split, parts, recs;
   int rows;  // rows of a slot (stored in bands of 32)
   float* pieces;
 
-  // First record of cluster c's share; split * recs * clusters < 2^31 (plan_tiles), since 64-bit divisions at the
+  // First record of cluster c's share; split * recs * (parts + 1) < 2^31 (plan_tiles), since 64-bit divisions at the
   // start of every role cost over a microsecond.
-  __device__ int start(int c, int clusters, int recs) const { return split * recs * c / clusters; }
+  __device__ int start(int c) const { return split * recs * c / parts; }
   // The i-th piece of cluster c; false past the last.
-  __device__ bool piece(int c, int clusters, int recs, int i, TilePiece* t) const {
+  __device__ bool piece(int c, int clusters, int i, TilePiece* t) const {
     int n = 0;
     t->r0 = 0;
     t->r1 = recs;
     t->slot = -1;
-    if (split > 0) {
-      const int u0 = start(c, clusters, recs), u1 = start(c + 1, clusters, recs);
-      if (u1 > u0) {
-        const int first = u0 / recs, last = (u1 - 1) / recs;
-        n = last - first + 1;
-        if (i < n) {
-          const int r = first + i;
-          if (i == 0) t->r0 = u0 - r * recs;
-          if (r == last) t->r1 = u1 - r * recs;
-          t->slot = c + r;
-          t->mt = (whole + r) % m_tiles;
-          t->nt = (whole + r) / m_tiles;
-          return true;
-        }
+    if (c < parts) {
+      const int u0 = start(c), u1 = start(c + 1);
+      const int first = u0 / recs, last = (u1 - 1) / recs;
+      n = last - first + 1;
+      if (i < n) {
+        const int r = first + i;
+        if (i == 0) t->r0 = u0 - r * recs;
+        if (r == last) t->r1 = u1 - r * recs;
+        t->slot = c + r;
+        t->mt = (whole + r) % m_tiles;
+        t->nt = (whole + r) / m_tiles;
+        return true;
       }
     }
     const int at = c + (i - n) * clusters;
@@ -65,6 +64,25 @@ struct TileWork {
     return true;
   }
 };
+
+// kN pairs of bf16 to an address of which only the type's alignment is known:
+// whole words, where it is odd those between the pairs (a store of one element
+// takes a request of its own; 3412 x 1344 -> 225 gated 32 -> 20 us). Going
+// through shared memory, 32 rows at a time, took 4 us less at 356 x
+// 288 -> 599, but its warp barriers in the epilogue cost the block-scaled
+// GEMM's aligned rows 40 of 130 us.
+template <int kN>
+__device__ __forceinline__ void store_words(uint16_t* y, const uint32_t* pk) {
+  const bool odd = reinterpret_cast<uintptr_t>(y) & 2;
+  uint32_t* w = reinterpret_cast<uint32_t*>(y - (odd ? 1 : 0));
+  if (odd)
+    y[0] = static_cast<uint16_t>(pk[0] & 0xFFFFu);
+  else
+    w[0] = pk[0];
+#pragma unroll
+  for (int e = 1; e < kN; ++e) w[e] = odd ? pk[e - 1] >> 16 | pk[e] << 16 : pk[e];
+  if (odd) y[2 * kN - 1] = static_cast<uint16_t>(pk[kN - 1] >> 16);
+}
 
 // kN (8 or 16) columns [c, c + kN) of a tile's row from their f32 sums (gated:
 // v of the gate, u of the up projection), columns 256 nt + c (gated: 128 nt + c)
@@ -117,6 +135,8 @@ __device__ __forceinline__ void finish(const TileOut& p, int64_t row, int nt, in
 #pragma unroll
       for (int e = 0; e < kN / 2; e += 4)
         *reinterpret_cast<uint4*>(y + 2 * e) = make_uint4(pk[e], pk[e + 1], pk[e + 2], pk[e + 3]);
+    } else if (col + kN <= p.cols) {
+      store_words<kN / 2>(y, pk);
     } else {
 #pragma unroll
       for (int e = 0; e < kN; ++e)
@@ -198,8 +218,8 @@ inline int join_blocks(const TileWork& w, bool gated) {
 }
 
 template <bool kGated, typename F>
-__device__ __forceinline__ void join_tile(const TileWork& w, int recs, int clusters, int m, F emit) {
-  constexpr int kGroups = kGated ? 16 : 32, kSums = kGated ? 2 : 1;
+__device__ __forceinline__ void join_tile(const TileWork& w, int m, F emit) {
+  constexpr int kGroups = kGated ? 16 : 32, kSums = kGated ? 2 : 1, kAhead = 4;
   const int wid = static_cast<int>(blockIdx.x) * (kJoinThreads / 32) + (threadIdx.x >> 5);
   const int bands = (w.rows + 31) / 32;
   const int group = wid % kGroups, band = wid / kGroups % bands, r = wid / (kGroups * bands);
@@ -207,39 +227,32 @@ __device__ __forceinline__ void join_tile(const TileWork& w, int recs, int clust
   const int t = w.whole + r;
   const int in_tile = band * 32 + (threadIdx.x & 31);
   const int64_t row = static_cast<int64_t>(t % w.m_tiles) * 256 + in_tile;
-  const int lo = r * recs, hi = lo + recs;
-  int c = r * clusters / w.split;
-  while (c > 0 && w.start(c, clusters, recs) > lo) --c;
-  while (w.start(c + 1, clusters, recs) <= lo) ++c;
-  wait_dependency();  // the pieces are written
   if (in_tile >= w.rows || row >= m) return;
+  // Clusters c with records of tile r: start(c + 1) > r * recs and start(c) < (r + 1) * recs.
+  const int total = w.split * w.recs;
+  int c = ((r * w.recs + 1) * w.parts + total - 1) / total - 1;
+  const int end = ((r + 1) * w.parts + w.split - 1) / w.split;
+  wait_dependency();  // the pieces are written
   float v[kSums][8];
 #pragma unroll
   for (int q = 0; q < kSums; ++q)
 #pragma unroll
     for (int e = 0; e < 8; ++e) v[q][e] = 0.f;
-  bool more = true;
-  while (more) {
-    float4 x[4][kSums][2];
+  for (; c < end; c += kAhead) {
+    float4 x[kAhead][kSums][2];
 #pragma unroll
-    for (int i = 0; i < 4; ++i) {
-      // (a cluster to which nothing fell has no piece)
-      const int s0 = c + i < clusters ? w.start(c + i, clusters, recs) : hi;
-      more = s0 < hi;
-      const bool have = more && s0 != w.start(c + i + 1, clusters, recs);
+    for (int i = 0; i < kAhead; ++i)
 #pragma unroll
       for (int q = 0; q < kSums; ++q) {
         x[i][q][0] = x[i][q][1] = make_float4(0.f, 0.f, 0.f, 0.f);
-        if (have) {
+        if (c + i < end) {
           const float4* src = reinterpret_cast<const float4*>(piece_at(w, c + i + r, in_tile, group + 16 * q));
           x[i][q][0] = src[0];
           x[i][q][1] = src[1];
         }
       }
-    }
-    c += 4;
 #pragma unroll
-    for (int i = 0; i < 4; ++i)
+    for (int i = 0; i < kAhead; ++i)
 #pragma unroll
       for (int q = 0; q < kSums; ++q) {
         v[q][0] += x[i][q][0].x, v[q][1] += x[i][q][0].y, v[q][2] += x[i][q][0].z, v[q][3] += x[i][q][0].w;
@@ -247,6 +260,10 @@ __device__ __forceinline__ void join_tile(const TileWork& w, int recs, int clust
       }
   }
   emit(row, t / w.m_tiles, group * 8, v[0], v[kSums - 1]);
+}
+
+inline TileWork tile_work(const TilePlan& plan, void* pieces) {
+  return TileWork{plan.m_tiles, plan.whole, plan.split, plan.parts, plan.recs, plan.rows, static_cast<float*>(pieces)};
 }
 
 // 2: rows of whole 32-byte sectors, 1: of 16-byte vectors, 0: neither.
