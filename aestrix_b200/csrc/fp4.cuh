@@ -103,7 +103,8 @@ __device__ __forceinline__ float rcp_approx(float x) {
 // reciprocal rounded to nearest, one residual) is a border only if v is. Any
 // other tensor_scale: v is multiplied by the reciprocal 2^-21 above and below;
 // the approximations are off by at most 2^-22, so where both give the same codes
-// they are the quotients', and where not the eight borders are settled exactly. (Settling every value cost 21 us for 4608 x 4096.)
+// they are the quotients', and where not the eight borders are settled
+// exactly. (Settling every value cost 21 us for 4608 x 4096.)
 template <int kFormat, int kN, bool kPermute>
 __device__ __forceinline__ uint32_t quantize_cols(const float* v, uint32_t top, float tensor_scale, float inv_6ts,
                                                   uint32_t* codes) {
@@ -251,9 +252,12 @@ __device__ __forceinline__ float sigmoid_arg(float g, int activation) {
 }
 __device__ __forceinline__ float sigmoid_arg_slope(float g, int activation) {
   constexpr float kA = 1.5957691216057308f;
-  return activation == AEX_ACT_SILU ? 1.f : kA * fmaf(3.f * 0.044715f * g, g, 1.f);
+  // It is multiplied by g s (1 - s), which is 0 long before |g| = 64: a square that overflowed would make that a NaN.
+  const float c = fminf(fabsf(g), 64.f);
+  return activation == AEX_ACT_SILU ? 1.f : kA * fmaf(3.f * 0.044715f * c, c, 1.f);
 }
 
+// kFast: to about 2^-20 of the value; 0 where z is below -87 (the quotient's divisor is above 2^126).
 template <bool kFast>
 __device__ __forceinline__ float sigmoid(float z) {
   return kFast ? __fdividef(1.f, 1.f + __expf(-z)) : 1.f / (1.f + expf(-z));

@@ -1,5 +1,7 @@
 // fp4_api.cpp — argument checks and dispatch of the products with microscaled
 // 4-bit weights.
+#include <cmath>
+
 #include "fp4_internal.h"
 
 namespace aex {
@@ -65,6 +67,10 @@ int run(aex_ctx* ctx, const aex_fp4weight* w0, const aex_fp4weight* w1, int acti
     return set_error(ctx, AEX_ERR_INVALID_ARG, "quantize_x must be 0 or 1");
   if (a->quantize_x)
     if (int r = fp4::check_format(ctx, w0->format, a->x_scale)) return r;
+  // The sums are multiplied by both tensor scales at once.
+  for (const aex_fp4weight* w : {w0, w1})
+    if (a->quantize_x && w && !std::isnormal(a->x_scale * w->tensor_scale))
+      return set_error(ctx, AEX_ERR_INVALID_ARG, "x_scale times the weight's tensor scale must be a normal f32");
   if (f32 && !a->quantize_x && a->m > fp4::kSmallRows)
     return set_error(ctx, AEX_ERR_UNSUPPORTED, "f32 activations without quantize_x are supported for m <= %d",
                      fp4::kSmallRows);

@@ -400,6 +400,10 @@ int aex_fp4weight_create(aex_ctx* ctx, const uint8_t* codes, const uint8_t* scal
     return set_error(ctx, AEX_ERR_UNSUPPORTED, "fp4 weight of %d x %d is too large", n, k);
   DeviceGuard dev(ctx);
   if (dev.rc) return dev.rc;
+  cudaStreamCaptureStatus capture = cudaStreamCaptureStatusNone;
+  AEX_CUDA_TRY(ctx, cudaStreamIsCapturing(static_cast<cudaStream_t>(stream), &capture));
+  if (capture != cudaStreamCaptureStatusNone)  // a graph would lay the weight out at its replays only
+    return set_error(ctx, AEX_ERR_UNSUPPORTED, "a weight cannot be created on a stream that is being captured");
   int clusters = 0;
   if (int r = fp4::gemm_clusters(ctx, &clusters)) return r;
   auto* w = new (std::nothrow) aex_fp4weight();

@@ -30,6 +30,7 @@ from . import _lib
 MODES = {"mxfp4": _lib.AEX_FP4_MX, "nvfp4": _lib.AEX_FP4_NV}
 BLOCK = {"mxfp4": 32, "nvfp4": 16}
 ACTIVATIONS = {"silu": _lib.AEX_ACT_SILU, "gelu_tanh": _lib.AEX_ACT_GELU_TANH}
+_MAX = 2**31 - 1  # the C calls count rows and columns in 32 bits
 _DTYPES = {torch.bfloat16: _lib.AEX_DTYPE_BF16, torch.float32: _lib.AEX_DTYPE_F32}
 
 
@@ -57,6 +58,8 @@ def _matrix(name, t, dtypes, cols=None, device=None):
         raise ValueError(f"{name} must have {cols} columns, has {have}")
     if rows < 1:
         raise ValueError(f"{name} has no rows")
+    if rows > _MAX or have > _MAX:
+        raise ValueError(f"{name} has more than {_MAX} rows or columns")
     if t.stride(1) != 1 and have != 1:
         raise ValueError(f"{name} must have contiguous rows")
     return at
@@ -92,6 +95,8 @@ _OPEN = {}  # device index -> (library, default context), looked up without the 
 
 def _handles(ctx, device):
     if ctx is not None:
+        if ctx.device != device:
+            raise ValueError(f"the tensors are on cuda:{device}, the context on cuda:{ctx.device}")
         return _lib.lib(), ctx
     got = _OPEN.get(device)
     if got is None:
@@ -113,6 +118,8 @@ def _check_codes(codes, scales, mode):
     if not codes.is_contiguous() or not scales.is_contiguous():
         raise ValueError("codes and scales must be contiguous")
     rows, k = codes.shape[0], codes.shape[1] * 2
+    if k > _MAX:
+        raise ValueError(f"codes has more than {_MAX} columns")
     if tuple(scales.shape) != (rows, k // BLOCK[mode]) or k % 32:
         raise ValueError(f"codes [rows, k/2] and scales [rows, k/{BLOCK[mode]}] with k a multiple of 32")
     return rows, k, device
@@ -154,7 +161,9 @@ def dequantize(codes, scales, mode="nvfp4", tensor_scale=1.0, out_dtype=torch.bf
 
 class FP4Weight:
     """Device-resident microscaled 4-bit weight [n, k] (owns an aex_fp4weight handle). codes and scales
-    as :func:`quantize` returns them, or as they stand in a pack (uint32 words viewed as uint8)."""
+    as :func:`quantize` returns them, or as they stand in a pack (uint32 words viewed as uint8). Laid
+    out on ``stream``; products on other streams are the caller's to order behind it. Not while a
+    stream is being captured."""
 
     def __init__(self, codes, scales, mode="nvfp4", tensor_scale=1.0, ctx=None, stream=None):
         fmt = _mode(mode)

@@ -234,8 +234,8 @@ typedef struct aex_fp4weight aex_fp4weight;
  * nearest even, at most 448). Codes: x / (scale * tensor_scale) to the nearest
  * e2m1 value, ties to the even code, at most 6; both roundings are those of
  * the exact quotient. A zero code keeps the sign; a block that holds an
- * infinity or NaN gets a NaN scale and zero codes. No reference counterpart (its packs are
- * quantized offline). */
+ * infinity or NaN gets a NaN scale and zero codes. No reference counterpart (its
+ * packs are quantized offline). */
 int aex_fp4_quantize(aex_ctx* ctx, const void* x, int x_dtype, int64_t ldx, int rows, int k, int format,
                      float tensor_scale, uint8_t* codes, uint8_t* scales, aex_stream stream);
 
@@ -247,7 +247,9 @@ int aex_fp4_dequantize(aex_ctx* ctx, const uint8_t* codes, const uint8_t* scales
 /* Lay a weight [n, k] out for the products below (device pointers as
  * aex_fp4_quantize writes them, or as they stand in a pack). The handle owns
  * its device memory until aex_fp4weight_destroy; the arrays may be freed once
- * the stream has passed the call. The microscaled sibling of
+ * the stream has passed the call, and products on other streams are the
+ * caller's to order behind it. Neither call is for a time at which a stream is
+ * being captured (create refuses a stream that is). The microscaled sibling of
  * aex_qweight_create. */
 int aex_fp4weight_create(aex_ctx* ctx, const uint8_t* codes, const uint8_t* scales, int n, int k, int format,
                          float tensor_scale, aex_fp4weight** out, aex_stream stream);
@@ -264,7 +266,8 @@ typedef struct aex_fp4_mm_args {
   int64_t ldx;         /* row pitch in elements, a multiple of 16 bytes, >= k */
   int m;
   int quantize_x;      /* 1: x goes through aex_fp4_quantize's rounding in the weight's format first */
-  float x_scale;       /* its tensor scale (AEX_FP4_NV; 1 for AEX_FP4_MX); unused without quantize_x */
+  float x_scale;       /* its tensor scale (AEX_FP4_NV; 1 for AEX_FP4_MX), whose product with the weight's is to be a
+                        * normal f32; unused without quantize_x */
   void* y;             /* [m, n], aligned to its element */
   int y_dtype;         /* AEX_DTYPE_BF16 or AEX_DTYPE_F32 */
   int64_t ldy;         /* row pitch in elements, >= n */

@@ -704,3 +704,102 @@ def test_refusals(cuda_ctx):
         assert L.aex_fp4_mm(cuda_ctx.handle, v.handle, a, None) == _lib.AEX_ERR_INVALID_ARG
         setattr(a, field, old)
     assert cuda_ctx.device_status() == 0
+
+
+def test_refuses_what_32_bits_do_not_count(cuda_ctx):
+    w, _ = make_weight(128, 288, "mxfp4", 1)
+    row = torch.zeros(1, 288, dtype=torch.bfloat16, device="cuda")
+    with pytest.raises(ValueError, match="2147483647"):
+        fp4.fp4_mm(row.expand(2**32 + 1, 288), w)
+    with pytest.raises(ValueError, match="2147483647"):
+        fp4.quantize(row.expand(2**31, 288), "mxfp4")
+    codes = torch.zeros(1, 16, dtype=torch.uint8, device="cuda").expand(2**32 + 128, 16)
+    scales = torch.zeros(1, 1, dtype=torch.uint8, device="cuda").expand(2**32 + 128, 1)
+    with pytest.raises(ValueError, match="2147483647"):
+        fp4.FP4Weight(codes, scales, "mxfp4")
+
+
+def test_refuses_another_devices_context(cuda_ctx):
+    class Other:
+        device = 1
+
+    x = activations(3, 64, 1)
+    with pytest.raises(ValueError, match="context on cuda:1"):
+        fp4.quantize(x, "mxfp4", ctx=Other())
+    codes, scales = fp4.quantize(x, "mxfp4")
+    with pytest.raises(ValueError, match="context on cuda:1"):
+        fp4.FP4Weight(codes, scales, "mxfp4", ctx=Other())
+
+
+@pytest.mark.parametrize("m", [2, 40])
+def test_refuses_tensor_scales_whose_product_leaves_f32(cuda_ctx, m):
+    x = activations(m, 288, 1)
+    for ts, xs in ((2.0**90, 2.0**90), (2.0**-90, 2.0**-90)):
+        w, _ = make_weight(128, 288, "nvfp4", 1, ts)
+        v, _ = make_weight(128, 288, "nvfp4", 1, 1.0)
+        for call in (lambda: fp4.fp4_mm(x, w, quantize_x=True, x_scale=xs),
+                     lambda: fp4.fp4_gated_mm(x, v, w, quantize_x=True, x_scale=xs)):
+            with pytest.raises(_lib.AexError, match="normal f32"):
+                call()
+        fp4.fp4_mm(x, v, quantize_x=True, x_scale=xs)
+    cuda_ctx.sync()
+
+
+def test_a_weight_is_not_created_under_capture(cuda_ctx):
+    x = activations(5, 288, 1)
+    codes, scales = fp4.quantize(activations(64, 288, 2), "mxfp4")
+    w = fp4.FP4Weight(codes, scales, "mxfp4")
+    s = torch.cuda.Stream()
+    fp4.fp4_mm(x, w, stream=s)
+    torch.cuda.synchronize()
+    g = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(g, stream=s):
+        with pytest.raises(_lib.AexError, match="captured"):
+            fp4.FP4Weight(codes, scales, "mxfp4")
+        y = fp4.fp4_mm(x, w)  # the capture goes on
+    g.replay()
+    torch.cuda.synchronize()
+    assert torch.equal(y, fp4.fp4_mm(x, w))
+
+
+# ------------------------------------------------------------------- gates far out, tiles of many pieces
+
+@pytest.mark.parametrize("mode", MODES)
+@pytest.mark.parametrize("act", ["silu", "gelu_tanh"])
+def test_gated_dgrad_of_gates_far_out(cuda_ctx, mode, act):
+    """Gates of 1e20 and more, whose squares leave f32: the slope is 1 on one side and 0 on the other.
+    All terms have one sign, so the roundings bound the result relative to itself: dg and du (2^-8, and
+    2^-18 for what they are computed from), dx (2^-8), the sums."""
+    m, n, k = 4, 136, 96
+    g = np.random.default_rng(3)
+    pair = []
+    for _ in range(2):
+        codes = g.integers(1, 8, (n, k)).astype(np.uint8)  # positive, none zero
+        scales = np.full((n, k // R.BLOCK[mode]), 124 if mode == "mxfp4" else 40, np.uint8)
+        pair.append((fp4.FP4Weight(torch.from_numpy(R.pack(codes)).cuda(), torch.from_numpy(scales).cuda(), mode),
+                     R.values(codes, scales, mode, 1.0)))
+    (wg, rg), (wu, ru) = pair
+    x = (torch.rand(m, k, generator=torch.Generator().manual_seed(1)) + 0.5).bfloat16().cuda() * 2.0**70
+    x[m // 2:] *= -1
+    dh = (torch.rand(m, n, generator=torch.Generator().manual_seed(2)) + 0.5).bfloat16().cuda() * 2.0**-40
+    dx = f64(fp4.fp4_gated_mm_dgrad(dh, x, wg, wu, activation=act))
+    X, D = f64(x)[:m // 2], f64(dh)[:m // 2]
+    ref = (D * (X @ ru.T)) @ rg + (D * (X @ rg.T)) @ ru
+    steps = 16 + 2 * 2 * 8 + 16
+    assert (np.abs(dx[:m // 2] - ref) <= ref * (2.0**-8 + 1.01 * (2.0**-8 + 2.0**-18 + steps * 2.0**-22))).all()
+    assert (dx[m // 2:] == 0).all()
+
+
+@pytest.mark.parametrize("mode", MODES)
+@pytest.mark.parametrize("m,n,k", [(95, 128, 2336), (33, 256, 8256), (300, 100, 1056)])
+def test_few_tiles_of_many_pieces(cuda_ctx, mode, m, n, k):
+    """One or two output tiles, split along a long axis over more clusters than they have records."""
+    x = activations(m, k, m)
+    w, ref_w = make_weight(n, k, mode, n)
+    close(fp4.fp4_mm(x, w), f64(x) @ ref_w.T,
+          HALF[torch.bfloat16] * np.abs(f64(x) @ ref_w.T) + sum_bound(f64(x), ref_w, steps_of(m, k, False)))
+    dy = activations(m, k, m + 1)  # the same lengths, summed over the weight's rows
+    v, ref_v = make_weight(k, n // 32 * 32, mode, k)
+    ref = f64(dy) @ ref_v
+    close(fp4.fp4_mm_dgrad(dy, v), ref,
+          HALF[torch.bfloat16] * np.abs(ref) + sum_bound(f64(dy), ref_v.T, -(-k // 128) * 8))
