@@ -45,7 +45,7 @@ def _mode(mode):
 # by get_device() and plain integers, not by torch.device objects.
 
 def _matrix(name, t, dtypes, cols=None, device=None):
-    """The checks of a 2-D input with contiguous rows; its AEX_DTYPE (None for uint8), and device index."""
+    """The checks of a 2-D input with contiguous rows; its device's index."""
     if not isinstance(t, torch.Tensor) or t.dtype not in dtypes or t.dim() != 2:
         raise TypeError(f"{name} must be a 2-D tensor of {' or '.join(str(d) for d in dtypes)}")
     at = t.get_device()
@@ -56,11 +56,9 @@ def _matrix(name, t, dtypes, cols=None, device=None):
     rows, have = t.shape
     if cols is not None and have != cols:
         raise ValueError(f"{name} must have {cols} columns, has {have}")
-    if rows < 1:
-        raise ValueError(f"{name} has no rows")
-    if rows > _MAX or have > _MAX:
-        raise ValueError(f"{name} has more than {_MAX} rows or columns")
-    if t.stride(1) != 1 and have != 1:
+    if not 0 < rows <= _MAX or have > _MAX:
+        raise ValueError(f"{name} has more than {_MAX} rows or columns" if rows else f"{name} has no rows")
+    if have != 1 and t.stride(1) != 1:
         raise ValueError(f"{name} must have contiguous rows")
     return at
 
@@ -117,10 +115,11 @@ def _check_codes(codes, scales, mode):
     _matrix("scales", scales, _UINT8, device=device)
     if not codes.is_contiguous() or not scales.is_contiguous():
         raise ValueError("codes and scales must be contiguous")
-    rows, k = codes.shape[0], codes.shape[1] * 2
+    rows, k = codes.shape
+    k *= 2
     if k > _MAX:
         raise ValueError(f"codes has more than {_MAX} columns")
-    if tuple(scales.shape) != (rows, k // BLOCK[mode]) or k % 32:
+    if k % 32 or scales.shape != (rows, k // BLOCK[mode]):
         raise ValueError(f"codes [rows, k/2] and scales [rows, k/{BLOCK[mode]}] with k a multiple of 32")
     return rows, k, device
 
@@ -138,7 +137,7 @@ def quantize(x, mode="nvfp4", tensor_scale=1.0, ctx=None, stream=None):
     lib, ctx = _handles(ctx, device)
     codes = _empty((rows, k // 2), torch.uint8, x, stream)
     scales = _empty((rows, k // BLOCK[mode]), torch.uint8, x, stream)
-    rc = lib.aex_fp4_quantize(ctx.handle, x.data_ptr(), _DTYPES[x.dtype], _pitch(x), rows, k, fmt,
+    rc = lib.aex_fp4_quantize(ctx.handle, x.data_ptr(), _DTYPES[x.dtype], x.stride(0) if rows > 1 else k, rows, k, fmt,
                               tensor_scale, codes.data_ptr(), scales.data_ptr(), _stream(stream, device))
     if rc:
         ctx.check(rc)
@@ -153,7 +152,8 @@ def dequantize(codes, scales, mode="nvfp4", tensor_scale=1.0, out_dtype=torch.bf
     out = _out(out, rows, k, out_dtype, codes, device, stream)
     lib, ctx = _handles(ctx, device)
     rc = lib.aex_fp4_dequantize(ctx.handle, codes.data_ptr(), scales.data_ptr(), rows, k, fmt, tensor_scale,
-                                out.data_ptr(), _DTYPES[out.dtype], _pitch(out), _stream(stream, device))
+                                out.data_ptr(), _DTYPES[out.dtype], out.stride(0) if rows > 1 else k,
+                                _stream(stream, device))
     if rc:
         ctx.check(rc)
     return out
@@ -228,7 +228,7 @@ def _product(x, w, w_up, activation, quantize_x, x_scale, out_dtype, out, stream
         need = w.lib.aex_fp4_mm_workspace_bytes if w_up is None else w.lib.aex_fp4_gated_mm_workspace_bytes
         n_ws = need(w.handle, m, q)
     ws = _empty((n_ws,), torch.uint8, x, stream) if n_ws else None
-    a = _lib.aex_fp4_mm_args(x.data_ptr(), _DTYPES[x.dtype], _pitch(x), m, q, x_scale, out.data_ptr(),
+    a = _lib.aex_fp4_mm_args(x.data_ptr(), _DTYPES[x.dtype], x.stride(0) if m > 1 else w.k, m, q, x_scale, out.data_ptr(),
                              _DTYPES[out.dtype], out.stride(0) if m > 1 else w.n, ws.data_ptr() if n_ws else None,
                              n_ws)
     if w_up is None:
