@@ -180,7 +180,7 @@ int launch_after(aex_ctx* ctx, const void* kernel, int blocks, int threads, cuda
 }
 
 // The few-rows kernel takes a row as one column of its 8-column operand where it is bf16 or quantized, f32 rows as
-// three columns each. No workspace. More rows go to the GEMMs: 19 rows, 7520 -> 5376, take 37 us as four times 8
+// two columns each. No workspace. More rows go to the GEMMs: 19 rows, 7520 -> 5376, take 37 us as four times 8
 // columns and 24 us there.
 constexpr int kSmallRows = 16;
 int run_small(aex_ctx* ctx, const Job& j, cudaStream_t s);

@@ -6,9 +6,9 @@
 // thread-block cluster; a producer warp streams its records through a ring of
 // shared-memory slots by bulk copies, compute warps take 16 rows each, up to
 // three sets of eight warps that take turns at the records (one set left the
-// SM's schedulers idle over half of the time). The number of slots is a multiple of the sets, or
-// enough for every record: a slot's records then all belong to one set, which
-// so sees every phase of the slot's barriers.
+// SM's schedulers idle over half of the time). The number of slots is a multiple
+// of the sets, or enough for every record: a slot's records then all belong to
+// one set, which so sees every phase of the slot's barriers.
 // The codes are decoded in registers and multiplied on the tensor cores by
 // mma.sync.m16n8k16 with the activations as the 8-column operand: at 1 to 8
 // rows the work on a decoded pair is the same, and the decoding is what the
@@ -24,8 +24,11 @@
 // value by value as they are staged; a record's columns for which they do not
 // (or that hold an infinity or NaN) are staged as bf16 and take the integer
 // decoding, which covers every value. Both products are exact.
-// f32 rows take three columns: 11 + 11 + 2 bits of the significand, each with a
-// scale of its own (bf16: 8 + 8 + 8 bits, by truncation).
+// f32 rows take two columns, 11 + 11 bits and the sign between them, each with a
+// scale of its own: a value is held to within 2^-23 of itself, less than its
+// f32 products' sums lose, and checked as well (a third column for the last bit
+// cost 3 rows, 4096 -> 18431, 19.8 us against 15.1). As bf16: 8 + 8 + 8 bits, by
+// truncation, the last 8 in a second product.
 // Scales: nvfp4, 16 columns: into the decoded pair (2 + 4 bits, exact in f16);
 // mxfp4, 32 columns: exponents that f16 does not hold, so one column block is
 // summed over two products and enters the f32 sum times its scale.
@@ -43,7 +46,7 @@ namespace aex {
 namespace fp4 {
 
 // Sets of eight compute warps, by the registers that 8 kT activation columns take.
-__host__ __device__ constexpr int sm_ways(int kT) { return kT == 1 ? 3 : kT == 2 ? 2 : 1; }
+__host__ __device__ constexpr int sm_ways(int kT) { return kT == 1 ? 3 : 2; }
 __host__ __device__ constexpr int sm_warps(int kT) { return 8 * sm_ways(kT); }
 __host__ __device__ constexpr int sm_threads(int kT) { return sm_warps(kT) * 32 + 32; }
 constexpr int kSmMaxSplit = 8;
@@ -57,6 +60,7 @@ struct SmallParams {
   int x_f32, quantize;
   float x_scale, inv_6ts;
   int m, k, n, k_blocks;
+  int m_inv;     // i / m = i * m_inv >> 16 for i <= 512
   int kb_per_split;
   int kb_phase;  // records' worth of columns staged at a time
   int slots;
@@ -127,15 +131,7 @@ __device__ __forceinline__ uint32_t e4m3_pair_f16(uint32_t v) {
   return d;
 }
 
-__device__ __forceinline__ uint32_t f16_bits(float v) { return __half_as_ushort(__float2half_rn(v)); }
 __device__ __forceinline__ float f16_value(uint32_t b) { return __half2float(__ushort_as_half(static_cast<uint16_t>(b))); }
-
-// The eight halves h of adjacent columns as the 16 bytes the lanes multiply by:
-// in the order of decode_f16's pairs, or (wide) of adjacent columns.
-__device__ __forceinline__ uint4 operand16(const uint32_t* h, bool wide) {
-  return wide ? make_uint4(h[0] | h[1] << 16, h[2] | h[3] << 16, h[4] | h[5] << 16, h[6] | h[7] << 16)
-              : make_uint4(h[0] | h[2] << 16, h[4] | h[6] << 16, h[1] | h[3] << 16, h[5] | h[7] << 16);
-}
 
 // Where a lane quad finds its operand: the 16-byte unit u (8 columns) of a
 // record's 256 columns sits at unit sm_pos(u) of its staged column, so that the
@@ -146,115 +142,213 @@ __device__ __forceinline__ int sm_pos(int u) {
   return kFormat == AEX_FP4_MX ? u : ((u & 7) << 2) | (u >> 3);
 }
 
-// Staged activations of a phase: columns of `pitch` bytes at xs, then per
-// column and record the factor that undoes its scale; *wide: a bit per record.
+// Staged activations of a phase: columns of `pitch` bytes at xs, f32 rows' third
+// parts (wide records only) `third` bytes on, then per column and record the
+// factor that undoes its scale; *wide: a bit per record.
 struct SmStage {
   uint8_t* xs;
   float* factor;  // [kb_phase][cols]
   uint32_t* wide;
-  int pitch, cols, parts;
+  int pitch, cols, third;
 };
 
-// One warp per row and record: lane l stages columns 8l..8l+7. `only`: the
-// records to stage as bf16 (0: all, as f16, noting in *wide which need bf16).
-template <int kFormat>
-__device__ __forceinline__ void sm_stage(const SmallParams& p, const SmStage& st, int kb0, int nkb, uint32_t only,
-                                         int warp, int warps, int lane) {
-  // The next item's loads are on their way while one is worked on.
-  const int items = p.m * nkb;
-  uint4 n0 = make_uint4(0, 0, 0, 0), n1 = n0;
-  auto fetch = [&](int i) {
-    const int b = i / p.m, mr = i - b * p.m, col = (kb0 + b) * kRecK + lane * 8;
-    n0 = n1 = make_uint4(0, 0, 0, 0);
-    if (col < p.k) {
-      if (p.x_f32) {
-        const uint4* s = reinterpret_cast<const uint4*>(static_cast<const float*>(p.x) + mr * p.ldx + col);
-        n0 = __ldg(s);
-        n1 = __ldg(s + 1);
-      } else {
-        n0 = __ldg(reinterpret_cast<const uint4*>(static_cast<const uint16_t*>(p.x) + mr * p.ldx + col));
-      }
+__device__ __forceinline__ uint32_t cvt_f16x2(float lo, float hi) {
+  uint32_t d;
+  asm("cvt.rn.f16x2.f32 %0, %1, %2;" : "=r"(d) : "f"(hi), "f"(lo));
+  return d;
+}
+
+// Stages columns 8l..8l+7 of a row and record as f16 halves: bf16 rows, eight
+// values w. False unless every value is held exactly. 2^k takes the largest of
+// the record into [2^14, 2^15); f16 then holds all of a value's 8 bits down to
+// 2^-17, which is 31 binades below.
+__device__ __forceinline__ bool sm_stage_bf16(const uint4& q, uint8_t* dst, float* factor, int lane) {
+  const uint32_t w[4] = {q.x, q.y, q.z, q.w};
+  uint32_t top2 = 0, low2 = 0xFFFFFFFFu;  // of the two halves: the largest magnitude, the smallest less one
+#pragma unroll
+  for (int j = 0; j < 4; ++j) {
+    const uint32_t mag = w[j] & 0x7FFF7FFFu;
+    top2 = __vmaxu2(top2, mag);
+    low2 = __vminu2(low2, (mag + 0x7FFF7FFFu) ^ 0x80008000u);  // a zero becomes 0xFFFF
+  }
+  const uint32_t top = __reduce_max_sync(0xffffffffu, max(top2 & 0xFFFFu, top2 >> 16));
+  const int e0 = top ? static_cast<int>(top >> 7) - 127 : 14;
+  const bool fits = e0 >= -48 && e0 <= 62;
+  const int k = fits ? 14 - e0 : 0;
+  const float up = __uint_as_float(static_cast<uint32_t>(127 + k) << 23);
+  float v[8];
+#pragma unroll
+  for (int j = 0; j < 4; ++j) {
+    v[2 * j] = bf16lo_to_f32(w[j]) * up;
+    v[2 * j + 1] = bf16hi_to_f32(w[j]) * up;
+  }
+  *reinterpret_cast<uint4*>(dst) =
+      make_uint4(cvt_f16x2(v[0], v[2]), cvt_f16x2(v[4], v[6]), cvt_f16x2(v[1], v[3]), cvt_f16x2(v[5], v[7]));
+  if (lane == 0) *factor = __uint_as_float(static_cast<uint32_t>(127 - k) << 23);
+  return fits && min(low2 & 0xFFFFu, low2 >> 16) + 1 >= static_cast<uint32_t>(e0 + 127 - 31) << 7;
+}
+
+// The same of f32 values v in kParts halves: one holds them exactly (quantized
+// ones) or the record is wide, two to within 2^-23 of each value.
+template <int kParts>
+__device__ __forceinline__ bool sm_stage_f32(const float* v, uint8_t* dst, int pitch, float* factor, int lane) {
+  uint32_t top = 0;
+#pragma unroll
+  for (int e = 0; e < 8; ++e) top = max(top, __float_as_uint(v[e]) & 0x7FFFFFFFu);
+  top = __reduce_max_sync(0xffffffffu, top);
+  // outside 2^-48 .. 2^62 (and for what is not finite) bf16
+  const int e0 = top ? static_cast<int>(top >> 23) - 127 : 14;
+  bool held = e0 >= -48 && e0 <= 62;
+  const int k = held ? 14 - e0 : 0;
+  const float up = __uint_as_float(static_cast<uint32_t>(127 + k) << 23);
+  float r[8];
+#pragma unroll
+  for (int e = 0; e < 8; ++e) {
+    r[e] = v[e] * up;
+    held &= !(r[e] == 0.f && v[e] != 0.f);
+  }
+  float down = __uint_as_float(static_cast<uint32_t>(127 - k) << 23);
+#pragma unroll
+  for (int part = 0; part < kParts; ++part) {
+    constexpr int kFirst[4] = {0, 4, 1, 5};
+    uint32_t h[4];
+#pragma unroll
+    for (int j = 0; j < 4; ++j) {
+      const int e = kFirst[j];
+      h[j] = cvt_f16x2(r[e], r[e + 2]);
+      r[e] = (r[e] - f16_value(h[j] & 0xFFFFu)) * 2048.f;  // what is left, to the next part's scale
+      r[e + 2] = (r[e + 2] - f16_value(h[j] >> 16)) * 2048.f;
     }
-  };
-  if (warp < items) fetch(warp);
-  for (int i = warp; i < items; i += warps) {
-    const uint4 r0 = n0, r1 = n1;
-    if (i + warps < items) fetch(i + warps);
-    const int b = i / p.m, mr = i - b * p.m;
-    if (only && !((only >> b) & 1u)) continue;
-    float v[8];
+    *reinterpret_cast<uint4*>(dst + part * pitch) = make_uint4(h[0], h[1], h[2], h[3]);
+    if (lane == 0) factor[part] = down;
+    down *= 1.f / 2048.f;
+  }
+  constexpr float most = kParts == 2 ? 0.5f : 0.f;  // what two parts leave stands 2^22 too high
+#pragma unroll
+  for (int e = 0; e < 8; ++e) held &= fabsf(r[e]) <= most * fabsf(v[e] * up);
+  return held;
+}
+
+// Columns 8l..8l+7 of item i's row and record, as they stand (zeros past the last column and item).
+struct SmItem {
+  int b, mr;
+  uint4 lo, hi;
+};
+__device__ __forceinline__ SmItem sm_fetch(const SmallParams& p, int kb0, int i, int items, int lane) {
+  SmItem t;
+  t.b = i * p.m_inv >> 16;
+  t.mr = i - t.b * p.m;
+  t.lo = t.hi = make_uint4(0, 0, 0, 0);
+  const int col = (kb0 + t.b) * kRecK + lane * 8;
+  if (i < items && col < p.k) {
     if (p.x_f32) {
-      const uint32_t w[8] = {r0.x, r0.y, r0.z, r0.w, r1.x, r1.y, r1.z, r1.w};
-#pragma unroll
-      for (int e = 0; e < 8; ++e) v[e] = __uint_as_float(w[e]);
+      const uint4* s = reinterpret_cast<const uint4*>(static_cast<const float*>(p.x) + t.mr * p.ldx + col);
+      t.lo = __ldg(s);
+      t.hi = __ldg(s + 1);
     } else {
-      const uint32_t w[4] = {r0.x, r0.y, r0.z, r0.w};
-#pragma unroll
-      for (int j = 0; j < 4; ++j) {
-        v[2 * j] = bf16lo_to_f32(w[j]);
-        v[2 * j + 1] = bf16hi_to_f32(w[j]);
-      }
+      t.lo = __ldg(reinterpret_cast<const uint4*>(static_cast<const uint16_t*>(p.x) + t.mr * p.ldx + col));
     }
-    if (p.quantize) {
-      uint32_t top = 0, w, d[4];
+  }
+  return t;
+}
+// Its values, quantized where that is asked for.
+template <int kFormat>
+__device__ __forceinline__ void sm_values(const SmallParams& p, const SmItem& t, float* v) {
+  if (p.x_f32) {
+    const uint32_t w[8] = {t.lo.x, t.lo.y, t.lo.z, t.lo.w, t.hi.x, t.hi.y, t.hi.z, t.hi.w};
 #pragma unroll
-      for (int e = 0; e < 8; ++e) top = max(top, __float_as_uint(v[e]) & 0x7FFFFFFFu);
-      const float s = scale_to_f32<kFormat>(quantize_cols<kFormat, 8, false>(v, top, p.x_scale, p.inv_6ts, &w));
-      decode_f16(w, d);
+    for (int e = 0; e < 8; ++e) v[e] = __uint_as_float(w[e]);
+  } else {
+    const uint32_t w[4] = {t.lo.x, t.lo.y, t.lo.z, t.lo.w};
 #pragma unroll
-      for (int j = 0; j < 4; ++j) {
-        v[2 * j] = f16_value(d[j] & 0xFFFFu) * s;  // exact
-        v[2 * j + 1] = f16_value(d[j] >> 16) * s;
-      }
+    for (int j = 0; j < 4; ++j) {
+      v[2 * j] = bf16lo_to_f32(w[j]);
+      v[2 * j + 1] = bf16hi_to_f32(w[j]);
     }
-    uint8_t* dst = st.xs + (mr * st.parts) * st.pitch + b * 512 + sm_pos<kFormat>(lane) * 16;
-    uint32_t h[8];
-    if (only) {
-#pragma unroll 1
-      for (int part = 0; part < st.parts; ++part) {
-#pragma unroll
-        for (int e = 0; e < 8; ++e) {
-          // the top 8 bits, exactly what there is where x has no more; an infinity or NaN is in the first part alone
-          const uint32_t u = __float_as_uint(v[e]);
-          const bool special = (u & 0x7F800000u) == 0x7F800000u;
-          h[e] = special && (u & 0x007FFFFFu) ? 0x7FC0u : u >> 16;
-          v[e] = special ? 0.f : v[e] - __uint_as_float(u & 0xFFFF0000u);
-        }
-        *reinterpret_cast<uint4*>(dst + part * st.pitch) = operand16(h, true);
-        if (lane == 0) st.factor[b * st.cols + mr * st.parts + part] = kFormat == AEX_FP4_NV ? 128.f : 1.f;
-      }
-      continue;
-    }
-    uint32_t top = 0;
+  }
+  if (p.quantize) {
+    uint32_t top = 0, w, d[4];
 #pragma unroll
     for (int e = 0; e < 8; ++e) top = max(top, __float_as_uint(v[e]) & 0x7FFFFFFFu);
-    top = __reduce_max_sync(0xffffffffu, top);
-    // 2^k takes the largest into [2^14, 2^15); outside 2^-48 .. 2^62 (and for what is not finite) bf16
-    const int e0 = top ? static_cast<int>(top >> 23) - 127 : 14;
-    bool exact = e0 >= -48 && e0 <= 62;
-    const int k = exact ? 14 - e0 : 0;
-    const float up = __uint_as_float(static_cast<uint32_t>(127 + k) << 23);
-    float r[8];
+    const float s = scale_to_f32<kFormat>(quantize_cols<kFormat, 8, false>(v, top, p.x_scale, p.inv_6ts, &w));
+    decode_f16(w, d);
 #pragma unroll
-    for (int e = 0; e < 8; ++e) {
-      r[e] = v[e] * up;
-      exact &= !(r[e] == 0.f && v[e] != 0.f);
+    for (int j = 0; j < 4; ++j) {
+      v[2 * j] = f16_value(d[j] & 0xFFFFu) * s;  // exact
+      v[2 * j + 1] = f16_value(d[j] >> 16) * s;
     }
-    float down = __uint_as_float(static_cast<uint32_t>(127 - k) << 23);
+  }
+}
+
+// One warp per row and record; notes in *wide which records need bf16.
+template <int kFormat, int kParts>
+__device__ __forceinline__ void sm_stage(const SmallParams& p, const SmStage& st, int kb0, int nkb, int warp, int warps,
+                                         int lane) {
+  const int items = p.m * nkb;
+  const auto place = [&](const SmItem& t) {
+    return st.xs + t.mr * kParts * st.pitch + t.b * 512 + sm_pos<kFormat>(lane) * 16;
+  };
+  const auto note = [&](const SmItem& t, bool held) {
+    if (!__all_sync(0xffffffffu, held) && lane == 0) atomicOr(st.wide, 1u << t.b);
+  };
+  if (kParts == 1 && !p.x_f32 && !p.quantize) {
+    constexpr int kAhead = 4;  // items whose loads are on their way at once
 #pragma unroll 1
-    for (int part = 0; part < st.parts; ++part) {
+    for (int i = warp; i < items; i += kAhead * warps) {
+      SmItem t[kAhead];
+#pragma unroll
+      for (int j = 0; j < kAhead; ++j) t[j] = sm_fetch(p, kb0, i + j * warps, items, lane);
+#pragma unroll
+      for (int j = 0; j < kAhead; ++j)
+        if (i + j * warps < items)
+          note(t[j], sm_stage_bf16(t[j].lo, place(t[j]), st.factor + t[j].b * st.cols + t[j].mr, lane));
+    }
+    return;
+  }
+  SmItem next = sm_fetch(p, kb0, warp, items, lane);
+#pragma unroll 1
+  for (int i = warp; i < items; i += warps) {
+    const SmItem t = next;
+    next = sm_fetch(p, kb0, i + warps, items, lane);
+    float v[8];
+    sm_values<kFormat>(p, t, v);
+    note(t, sm_stage_f32<kParts>(v, place(t), st.pitch, st.factor + t.b * st.cols + t.mr * kParts, lane));
+  }
+}
+
+// Stages the records of `only` again, as bf16 (not inlined: it is rare, and its registers cost the main loop some).
+template <int kFormat, int kParts>
+__device__ __noinline__ void sm_stage_wide(const SmallParams& p, SmStage st, int kb0, int nkb, uint32_t only,
+                                           int warp, int warps, int lane) {
+  const int items = p.m * nkb;
+#pragma unroll 1
+  for (int i = warp; i < items; i += warps) {
+    const SmItem t = sm_fetch(p, kb0, i, items, lane);
+    if (!((only >> t.b) & 1u)) continue;
+    float v[8];
+    sm_values<kFormat>(p, t, v);
+    uint8_t* dst = st.xs + t.mr * kParts * st.pitch + t.b * 512 + sm_pos<kFormat>(lane) * 16;
+    uint32_t h[8];
+#pragma unroll 1
+    for (int part = 0; part < (kParts == 2 ? 3 : 1); ++part) {
 #pragma unroll
       for (int e = 0; e < 8; ++e) {
-        h[e] = f16_bits(r[e]);
-        r[e] = (r[e] - f16_value(h[e])) * 2048.f;  // what is left, to the next part's scale
+        // the top 8 bits, exactly what there is where x has no more; an infinity or NaN is in the first part alone
+        const uint32_t u = __float_as_uint(v[e]);
+        const bool special = (u & 0x7F800000u) == 0x7F800000u;
+        h[e] = special && (u & 0x007FFFFFu) ? 0x7FC0u : u >> 16;
+        v[e] = special ? 0.f : v[e] - __uint_as_float(u & 0xFFFF0000u);
       }
-      *reinterpret_cast<uint4*>(dst + part * st.pitch) = operand16(h, false);
-      if (lane == 0) st.factor[b * st.cols + mr * st.parts + part] = down;
-      down *= 1.f / 2048.f;
+      const uint4 o = make_uint4(h[0] | h[1] << 16, h[2] | h[3] << 16, h[4] | h[5] << 16, h[6] | h[7] << 16);
+      if (part < 2) {
+        *reinterpret_cast<uint4*>(dst + part * st.pitch) = o;
+        if (lane == 0)
+          st.factor[t.b * st.cols + t.mr * kParts + part] = kFormat == AEX_FP4_NV ? 128.f : 1.f;
+      } else {
+        *reinterpret_cast<uint4*>(dst + st.third) = o;
+        *reinterpret_cast<uint4*>(dst + st.third + st.pitch) = make_uint4(0, 0, 0, 0);
+      }
     }
-#pragma unroll
-    for (int e = 0; e < 8; ++e) exact &= r[e] == 0.f;
-    if (!__all_sync(0xffffffffu, exact) && lane == 0) atomicOr(st.wide, 1u << b);
   }
 }
 
@@ -413,7 +507,7 @@ __device__ __forceinline__ void sm_load(uint32_t rec, const SmLane& o, uint4* co
   }
 }
 
-template <int kFormat, int kT, bool kGated>
+template <int kFormat, int kT, bool kGated, int kParts>
 __global__ void __launch_bounds__(sm_threads(kT)) small_kernel(const __grid_constant__ SmallParams p) {
   extern __shared__ __align__(128) uint8_t smem[];
   constexpr int kSlot = sm_slot_bytes(kFormat, kGated);
@@ -430,15 +524,14 @@ __global__ void __launch_bounds__(sm_threads(kT)) small_kernel(const __grid_cons
   const int rt = blockIdx.x, split = blockIdx.y;
   const int kb0 = split * p.kb_per_split;
   const int nkb = max(0, min(p.k_blocks, kb0 + p.kb_per_split) - kb0);
-  const int parts = p.x_f32 && !p.quantize ? 3 : 1;
-  const int cols = p.m * parts;
+  const int cols = p.m * kParts;
   SmStage st;
   st.xs = reinterpret_cast<uint8_t*>(full) + 128;  // at most 8 slots
   st.pitch = p.kb_phase * 512 + 64;
-  st.factor = reinterpret_cast<float*>(st.xs + cols * st.pitch);
+  st.third = cols * st.pitch;
+  st.factor = reinterpret_cast<float*>(st.xs + kParts * cols * st.pitch);  // two parts: a third's columns in between
   st.wide = &wide;
   st.cols = cols;
-  st.parts = parts;
   launch_dependents();
   if (tid == 0) {
     abort_flag = 0;
@@ -502,11 +595,11 @@ __global__ void __launch_bounds__(sm_threads(kT)) small_kernel(const __grid_cons
           if (tid == 0) wide = 0;
           asm volatile("bar.sync 1, %0;" ::"n"(kSmCompute) : "memory");
         }
-        sm_stage<kFormat>(p, st, kb0 + b, count, 0, warp, kSmWarps, lane);
+        sm_stage<kFormat, kParts>(p, st, kb0 + b, count, warp, kSmWarps, lane);
         asm volatile("bar.sync 1, %0;" ::"n"(kSmCompute) : "memory");
         wide_now = *reinterpret_cast<volatile uint32_t*>(&wide);
         if (wide_now) {
-          sm_stage<kFormat>(p, st, kb0 + b, count, wide_now, warp, kSmWarps, lane);
+          sm_stage_wide<kFormat, kParts>(p, st, kb0 + b, count, wide_now, warp, kSmWarps, lane);
           asm volatile("bar.sync 1, %0;" ::"n"(kSmCompute) : "memory");
         }
       }
@@ -522,23 +615,26 @@ __global__ void __launch_bounds__(sm_threads(kT)) small_kernel(const __grid_cons
       if (!ok) continue;  // the barriers above still see every warp
       const uint32_t off = in_phase * 512, foff = in_phase * cols * 4;
       const bool narrow = !((wide_now >> in_phase) & 1u);
-      uint32_t all = 0;
+      const int passes = kParts == 1 || narrow ? 1 : kParts;  // the second: the third parts of f32 rows
+#pragma unroll 1
+      for (int pass = 0; pass < passes; ++pass) {
+        uint32_t all = 0;
 #pragma unroll
-      for (int q = 0; q < (kGated ? 2 : 1); ++q) {
-        uint4 codes[4];
-        uint32_t sc[kFormat == AEX_FP4_NV ? 2 : 4];
-        sm_load<kFormat>(ring0 + cs * kSlot + q * kRec, at, codes, sc);
+        for (int q = 0; q < (kGated ? 2 : 1); ++q) {
+          uint4 codes[4];
+          uint32_t sc[kFormat == AEX_FP4_NV ? 2 : 4];
+          sm_load<kFormat>(ring0 + cs * kSlot + q * kRec, at, codes, sc);
 #pragma unroll
-        for (int i = 0; i < 4; ++i) all |= codes[i].x | codes[i].y | codes[i].z | codes[i].w;
+          for (int i = 0; i < 4; ++i) all |= codes[i].x | codes[i].y | codes[i].z | codes[i].w;
 #pragma unroll
-        for (int i = 0; i < (kFormat == AEX_FP4_NV ? 2 : 4); ++i) all |= sc[i];
-        if (q == (kGated ? 1 : 0)) {
-          arrive_after_loads(empty0 + 8 * cs, all, p.zero, lane);  // the warp's reads of the slot are done
+          for (int i = 0; i < (kFormat == AEX_FP4_NV ? 2 : 4); ++i) all |= sc[i];
+          if (q == (kGated ? 1 : 0) && pass == passes - 1)
+            arrive_after_loads(empty0 + 8 * cs, all, p.zero, lane);  // the warp's reads of the slot are done
+          if (narrow)
+            sm_record<kFormat, kT, false>(codes, sc, xb, off, fb, foff, q ? acc1 : acc0);
+          else
+            sm_record<kFormat, kT, true>(codes, sc, xb, off + pass * st.third, fb, foff, q ? acc1 : acc0);
         }
-        if (narrow)
-          sm_record<kFormat, kT, false>(codes, sc, xb, off, fb, foff, q ? acc1 : acc0);
-        else
-          sm_record<kFormat, kT, true>(codes, sc, xb, off, fb, foff, q ? acc1 : acc0);
       }
     }
   }
@@ -577,8 +673,8 @@ __global__ void __launch_bounds__(sm_threads(kT)) small_kernel(const __grid_cons
     if (col >= p.n) continue;
     float v0 = 0.f, v1 = 0.f;
     for (int c = 0; c < nsplit; ++c)
-      for (int q = 0; q < kWays * parts; ++q) {
-        const uint32_t off = (((q % kWays) * cols + mr * parts + q / kWays) * kRecRows + r) * 4;
+      for (int q = 0; q < kWays * kParts; ++q) {
+        const uint32_t off = (((q % kWays) * cols + mr * kParts + q / kWays) * kRecRows + r) * 4;
         v0 += ld_shared_cluster_f32(mapa_shared(a0 + off, c));
         if (kGated) v1 += ld_shared_cluster_f32(mapa_shared(a1 + off, c));
       }
@@ -599,10 +695,10 @@ __global__ void __launch_bounds__(sm_threads(kT)) small_kernel(const __grid_cons
 
 namespace {
 
-template <int kFormat, int kT, bool kGated>
+template <int kFormat, int kT, bool kGated, int kParts>
 int launch_small(aex_ctx* ctx, const Job& j, cudaStream_t s) {
   const aex_fp4weight* w = j.w0;
-  const int cols = j.m * (j.x_f32 && !j.quantize ? 3 : 1);
+  const int cols = j.m * kParts;
   SmallParams p{};
   p.w0 = w->records;
   p.w1 = kGated ? j.w1->records : nullptr;
@@ -613,6 +709,7 @@ int launch_small(aex_ctx* ctx, const Job& j, cudaStream_t s) {
   p.x_scale = j.x_scale;
   p.inv_6ts = static_cast<float>(1.0 / (6.0 * static_cast<double>(j.x_scale)));
   p.m = j.m;
+  p.m_inv = 65536 / j.m + 1;
   p.k = w->k;
   p.n = w->n;
   p.k_blocks = w->k_blocks;
@@ -625,7 +722,7 @@ int launch_small(aex_ctx* ctx, const Job& j, cudaStream_t s) {
   p.y_f32 = j.y_f32;
   p.status = ctx->d_status;
 
-  auto kern = small_kernel<kFormat, kT, kGated>;
+  auto kern = small_kernel<kFormat, kT, kGated, kParts>;
   constexpr int kSlot = sm_slot_bytes(kFormat, kGated);
   static SmemOptIn opt_in;
   if (int r = opt_in(ctx, reinterpret_cast<const void*>(kern), kSmSmem)) return r;
@@ -648,11 +745,11 @@ int launch_small(aex_ctx* ctx, const Job& j, cudaStream_t s) {
   const int best_slots = std::min(kb, kSlots);
   const size_t x_budget = kSmSmem - static_cast<size_t>(best_slots) * kSlot - 128;
   int best_phase = std::min(kb, 32);  // a bit each in the mask of wide records
-  while (best_phase > 1 && static_cast<size_t>(cols) * (best_phase * 516 + 64) > x_budget)
-    best_phase = (best_phase + 1) / 2;
+  const auto staged = [&](int phase) { return static_cast<size_t>(cols) * (kParts * (phase * 512 + 64) + phase * 4); };
+  while (best_phase > 1 && staged(best_phase) > x_budget) best_phase = (best_phase + 1) / 2;
   // the partial sums take the ring's place
   const size_t best_smem =
-      std::max(static_cast<size_t>(best_slots) * kSlot + 128 + static_cast<size_t>(cols) * (best_phase * 516 + 64),
+      std::max(static_cast<size_t>(best_slots) * kSlot + 128 + staged(best_phase),
                static_cast<size_t>(cols) * kRecRows * 4 * sm_ways(kT) * (kGated ? 2 : 1));
   p.kb_per_split = (w->k_blocks + best_split - 1) / best_split;
   p.kb_phase = best_phase;
@@ -677,11 +774,20 @@ int launch_small(aex_ctx* ctx, const Job& j, cudaStream_t s) {
 
 template <int kFormat, bool kGated>
 int pick_tiles(aex_ctx* ctx, const Job& j, cudaStream_t s) {
-  const int cols = j.m * (j.x_f32 && !j.quantize ? 3 : 1);
-  if (cols <= 8) return launch_small<kFormat, 1, kGated>(ctx, j, s);
-  if (cols <= 16) return launch_small<kFormat, 2, kGated>(ctx, j, s);
-  if (cols <= 32) return launch_small<kFormat, 4, kGated>(ctx, j, s);
-  return launch_small<kFormat, 6, kGated>(ctx, j, s);  // 33..48 columns: f32 rows
+  if (!j.x_f32 || j.quantize)
+    return j.m <= 8 ? launch_small<kFormat, 1, kGated, 1>(ctx, j, s) : launch_small<kFormat, 2, kGated, 1>(ctx, j, s);
+  // f32 rows: eight a launch, sixteen columns (32 columns leave registers for one set of warps: 51 us for 16 rows,
+  // 4096 -> 18431, against 48 for two launches)
+  for (int r = 0; r < j.m; r += 8) {
+    Job part = j;
+    part.m = std::min(8, j.m - r);
+    part.x = static_cast<const float*>(j.x) + r * j.ldx;
+    part.y = static_cast<uint8_t*>(j.y) + r * j.ldy * (j.y_f32 ? 4 : 2);
+    if (int rc = part.m <= 4 ? launch_small<kFormat, 1, kGated, 2>(ctx, part, s)
+                             : launch_small<kFormat, 2, kGated, 2>(ctx, part, s))
+      return rc;
+  }
+  return AEX_OK;
 }
 
 }  // namespace

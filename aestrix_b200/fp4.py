@@ -241,7 +241,8 @@ def _product(x, w, w_up, activation, quantize_x, x_scale, out_dtype, out, stream
 
 
 def fp4_mm(x, w: FP4Weight, quantize_x=False, x_scale=1.0, out_dtype=torch.bfloat16, out=None, stream=None):
-    """y[m, n] = x[m, k] . W[n, k]^T, f32 sums, rounded once to bf16 or f32. x is bf16, or f32 for m <= 16.
+    """y[m, n] = x[m, k] . W[n, k]^T, f32 sums, rounded once to bf16 or f32. x is bf16, or f32 for m <= 16
+    (each value held to within 2^-23 of itself).
     With quantize_x, x (bf16 or f32, any m) goes through :func:`quantize`'s rounding in the weight's
     mode first, with x_scale as its tensor scale, and both operands are multiplied in 4 bits. f32
     results of more than 16 rows carry the tensor core's truncating f32 sums (about 1e-5 of their

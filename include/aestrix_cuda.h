@@ -262,7 +262,8 @@ int aex_fp4weight_dequantize(aex_ctx* ctx, const aex_fp4weight* w, void* out, in
 /* Activations and result of one product. */
 typedef struct aex_fp4_mm_args {
   const void* x;       /* [m, k], 16-byte aligned */
-  int x_dtype;         /* AEX_DTYPE_BF16, or AEX_DTYPE_F32 where m <= 16 or quantize_x */
+  int x_dtype;         /* AEX_DTYPE_BF16, or AEX_DTYPE_F32 where m <= 16 (a value is held to within 2^-23 of itself) or
+                        * quantize_x */
   int64_t ldx;         /* row pitch in elements, a multiple of 16 bytes, >= k */
   int m;
   int quantize_x;      /* 1: x goes through aex_fp4_quantize's rounding in the weight's format first */

@@ -200,7 +200,7 @@ def test_mm(cuda_ctx, mode, out, m, n, k):
 @pytest.mark.parametrize("mode", MODES)
 @pytest.mark.parametrize("m", [1, 2, 3, 5, 6, 16])
 def test_mm_f32_rows(cuda_ctx, mode, m):
-    """f32 activations keep all 24 bits."""
+    """f32 activations count to within 2^-23 of themselves."""
     n, k = 300, 4512
     x = activations(m, k, m, torch.float32) * 1.000123
     w, ref_w = make_weight(n, k, mode, m)
