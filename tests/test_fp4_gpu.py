@@ -803,3 +803,25 @@ def test_few_tiles_of_many_pieces(cuda_ctx, mode, m, n, k):
     ref = f64(dy) @ ref_v
     close(fp4.fp4_mm_dgrad(dy, v), ref,
           HALF[torch.bfloat16] * np.abs(ref) + sum_bound(f64(dy), ref_v.T, -(-k // 128) * 8))
+
+
+@pytest.mark.parametrize("mode", MODES)
+@pytest.mark.parametrize("wide", [False, True])
+@pytest.mark.parametrize("m", [1, 4, 7, 16])
+def test_f32_rows_to_the_last_bits(cuda_ctx, mode, wide, m):
+    """One value a row, so that nothing but its own rounding (2^-23) and that of the sums counts: the
+    products of its two parts (or three, in a record that also holds a huge value against zero weights)
+    are exact, added in f32 and scaled (at most six roundings or truncations, 2^-23 each)."""
+    k, n = 544, 130
+    g = np.random.default_rng(m)
+    codes = g.integers(1, 8, (n, k)).astype(np.uint8)  # positive, none zero
+    codes[:, 7] = 0
+    scales = np.full((n, k // R.BLOCK[mode]), 127 if mode == "mxfp4" else 56, np.uint8)  # 1.0
+    w = fp4.FP4Weight(torch.from_numpy(R.pack(codes)).cuda(), torch.from_numpy(scales).cuda(), mode)
+    x = np.zeros((m, k), np.float32)
+    x[np.arange(m), g.integers(8, 256, m)] = g.uniform(1, 2, m).astype(np.float32) * np.float32(2.0**-40)
+    if wide:
+        x[:, 7] = 2.0**50
+    ref = x.astype(np.float64) @ R.values(codes, scales, mode, 1.0).T
+    y = f64(fp4.fp4_mm(torch.from_numpy(x).cuda(), w, out_dtype=torch.float32))
+    assert (np.abs(y - ref) <= 7 * 2.0**-23 * ref).all()
