@@ -35,8 +35,11 @@
 // knows its phase although a group sees every other unit. A record is released
 // (rempty) by the decode warps that read it.
 // Tiles that would leave a last wave of the clusters mostly empty are split
-// along K evenly over all clusters; their f32 pieces go to the workspace and
+// along K evenly over the clusters; their f32 pieces go to the workspace and
 // join_kernel adds them in order and applies the epilogue.
+// Each kernel lets the stream's next one set up behind it (0.5 to 1 us a call).
+// Tensor memory is taken after the wait for the previous kernel: that one may
+// hold some, or not have taken its own yet.
 #include <algorithm>
 
 #include "fp4_internal.h"
@@ -163,13 +166,14 @@ __global__ void __launch_bounds__(kGThreads, 1)
     mbar_init(drain, 1);
     fence_barrier_init();
   }
-  if (warp == 2) {
-    tmem_alloc_pair(tmem_slot, 512);
-    tmem_relinquish_pair();
-  }
   if (warp == 0 && lane == 0) {
     prefetch_tmap(&tm0);
     if (kBack) prefetch_tmap(&tm1);
+  }
+  wait_dependency();  // what it reads may be the previous kernel's, and so may the tensor memory
+  if (warp == 2) {
+    tmem_alloc_pair(tmem_slot, 512);
+    tmem_relinquish_pair();
   }
   tc_fence_before();
   __syncthreads();
@@ -505,7 +509,7 @@ int launch_gemm(aex_ctx* ctx, const CUtensorMap& tm0, const CUtensorMap& tm1, Ge
   auto kern = gemm_kernel<kFormat, kMode>;
   static SmemOptIn opt_in;
   if (int r = opt_in(ctx, reinterpret_cast<const void*>(kern), kGSmem)) return r;
-  if (int r = launch_pairs(ctx, reinterpret_cast<const void*>(kern), plan.clusters, kGThreads, kGSmem, false, s,
+  if (int r = launch_pairs(ctx, reinterpret_cast<const void*>(kern), plan.clusters, kGThreads, kGSmem, true, s,
                            const_cast<CUtensorMap*>(&tm0), const_cast<CUtensorMap*>(&tm1), &p))
     return r;
   if (plan.split)

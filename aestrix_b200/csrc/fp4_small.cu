@@ -23,7 +23,7 @@
 // then hold bf16 values over 31 binades exactly. Whether they do is checked
 // value by value as they are staged; a record's columns for which they do not
 // (or that hold an infinity or NaN) are staged as bf16 and take the integer
-// decoding, which covers every value. Both products are exact.
+// decoding, which covers every value. Both products of bf16 rows are exact.
 // f32 rows take two columns, 11 + 11 bits and the sign between them, each with a
 // scale of its own: a value is held to within 2^-23 of itself, less than its
 // f32 products' sums lose, and checked as well (a third column for the last bit

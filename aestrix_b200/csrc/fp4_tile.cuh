@@ -220,6 +220,7 @@ inline int join_blocks(const TileWork& w, bool gated) {
 template <bool kGated, typename F>
 __device__ __forceinline__ void join_tile(const TileWork& w, int m, F emit) {
   constexpr int kGroups = kGated ? 16 : 32, kSums = kGated ? 2 : 1, kAhead = 4;
+  launch_dependents();
   const int wid = static_cast<int>(blockIdx.x) * (kJoinThreads / 32) + (threadIdx.x >> 5);
   const int bands = (w.rows + 31) / 32;
   const int group = wid % kGroups, band = wid / kGroups % bands, r = wid / (kGroups * bands);
