@@ -65,23 +65,57 @@ struct TileWork {
   }
 };
 
-// kN pairs of bf16 to an address of which only the type's alignment is known:
-// whole words, where it is odd those between the pairs (a store of one element
-// takes a request of its own; 3412 x 1344 -> 225 gated 32 -> 20 us). Going
-// through shared memory, 32 rows at a time, took 4 us less at 356 x
-// 288 -> 599, but its warp barriers in the epilogue cost the block-scaled
-// GEMM's aligned rows 40 of 130 us.
+// kN pairs of bf16 to an address of which only the type's alignment is known. A
+// store takes a request of its own whatever its size, so sixteen values are
+// turned to the 16-byte vector that lies whole within them and what is left
+// before and behind: 356 x 288 -> 599 12.5 us, in words 17.7, one by one 41.8;
+// 3412 x 1344 -> 225 gated 18.9, 21.0 and 32. (Through shared memory, 32 rows at
+// a time: 13.3, but the warp barriers that takes in the epilogue cost the
+// block-scaled GEMM's aligned rows 40 of 130 us.)
 template <int kN>
 __device__ __forceinline__ void store_words(uint16_t* y, const uint32_t* pk) {
   const bool odd = reinterpret_cast<uintptr_t>(y) & 2;
   uint32_t* w = reinterpret_cast<uint32_t*>(y - (odd ? 1 : 0));
-  if (odd)
-    y[0] = static_cast<uint16_t>(pk[0] & 0xFFFFu);
-  else
-    w[0] = pk[0];
+  if (kN != 8) {
+    if (odd)
+      y[0] = static_cast<uint16_t>(pk[0] & 0xFFFFu);
+    else
+      w[0] = pk[0];
 #pragma unroll
-  for (int e = 1; e < kN; ++e) w[e] = odd ? pk[e - 1] >> 16 | pk[e] << 16 : pk[e];
-  if (odd) y[2 * kN - 1] = static_cast<uint16_t>(pk[kN - 1] >> 16);
+    for (int e = 1; e < kN; ++e) w[e] = odd ? pk[e - 1] >> 16 | pk[e] << 16 : pk[e];
+    if (odd) y[2 * kN - 1] = static_cast<uint16_t>(pk[kN - 1] >> 16);
+    return;
+  }
+  // r[q ..): the words from w on, w being word q of its vector; the first and the last are halves where y is odd
+  const uint32_t q = static_cast<uint32_t>(reinterpret_cast<uintptr_t>(w) >> 2) & 3;
+  uint32_t r[12];
+#pragma unroll
+  for (int e = 0; e < 9; ++e) {
+    const uint32_t lo = e ? pk[e - 1] : 0u, hi = e < 8 ? pk[e] : 0u;
+    r[e] = odd ? __funnelshift_r(lo, hi, 16) : hi;
+  }
+  r[9] = r[10] = r[11] = 0;
+#pragma unroll
+  for (int e = 9; e > 0; --e) r[e] = q & 1 ? r[e - 1] : r[e];
+#pragma unroll
+  for (int e = 11; e > 1; --e) r[e] = q & 2 ? r[e - 2] : r[e];
+  uint32_t* v = w - q;
+  const uint32_t first = q + (odd ? 1 : 0);  // the first whole word
+  if (first == 0) {
+    *reinterpret_cast<uint4*>(v) = make_uint4(r[0], r[1], r[2], r[3]);
+  } else {
+    if (first == 1) v[1] = r[1];
+    if (first <= 2) *reinterpret_cast<uint2*>(v + 2) = make_uint2(r[2], r[3]);
+    if (first == 3) v[3] = r[3];
+  }
+  *reinterpret_cast<uint4*>(v + 4) = make_uint4(r[4], r[5], r[6], r[7]);
+  if (q >= 2) *reinterpret_cast<uint2*>(v + 8) = make_uint2(r[8], r[9]);
+  if (q == 1) v[8] = r[8];
+  if (q == 3) v[10] = r[10];
+  if (odd) {
+    y[0] = static_cast<uint16_t>(pk[0] & 0xFFFFu);
+    y[15] = static_cast<uint16_t>(pk[7] >> 16);
+  }
 }
 
 // kN (8 or 16) columns [c, c + kN) of a tile's row from their f32 sums (gated:
