@@ -87,20 +87,23 @@ struct GemmParams {
   int* status;
 };
 
-// dg, du of 8 columns (col a multiple of 8) from g, u (already scaled).
-__device__ __forceinline__ void grad8(const TileOut& o, const GradOut& p, int64_t row, int col, const float* g, const float* u) {
+// dh of 8 columns (col a multiple of 8), zeros past the last.
+__device__ __forceinline__ uint4 grad_load(const TileOut& o, const GradOut& p, int64_t row, int col) {
   const int left = o.cols - col;
-  if (left <= 0) return;
+  uint32_t d[4] = {0, 0, 0, 0};
   const uint16_t* src = p.dh + row * p.lddh + col;
-  uint32_t d[4];
-  if (left >= 8) {
-    const uint4 q = __ldg(reinterpret_cast<const uint4*>(src));
-    d[0] = q.x, d[1] = q.y, d[2] = q.z, d[3] = q.w;
-  } else {
+  if (left >= 8) return __ldg(reinterpret_cast<const uint4*>(src));
 #pragma unroll
-    for (int i = 0; i < 4; ++i)
-      d[i] = (2 * i < left ? src[2 * i] : 0u) | ((2 * i + 1 < left ? static_cast<uint32_t>(src[2 * i + 1]) : 0u) << 16);
-  }
+  for (int i = 0; i < 4; ++i)
+    d[i] = (2 * i < left ? src[2 * i] : 0u) | ((2 * i + 1 < left ? static_cast<uint32_t>(src[2 * i + 1]) : 0u) << 16);
+  return make_uint4(d[0], d[1], d[2], d[3]);
+}
+
+// dg, du of 8 columns from g, u (already scaled) and dh.
+__device__ __forceinline__ void grad8(const TileOut& o, const GradOut& p, int64_t row, int col, const float* g,
+                                      const float* u, const uint4& dh) {
+  if (col >= o.cols) return;
+  const uint32_t d[4] = {dh.x, dh.y, dh.z, dh.w};
   uint32_t og[4], ou[4];
 #pragma unroll
   for (int i = 0; i < 4; ++i) {
@@ -352,10 +355,18 @@ __global__ void __launch_bounds__(kGThreads, 1)
     TilePiece t;
     for (int i = 0; p.work.piece(cluster, clusters, i, &t); ++i) {
       const int b = i & 1;
-      if (!mbar_wait_warp_cl(smem_u32(&accf[b]), (i >> 1) & 1, &abort_flag, p.status, kDevTimeoutEpilogue)) break;
-      tc_fence_after();
       const int in_tile = static_cast<int>(rank) * 128 + quad * 32 + lane;
       const int64_t row = static_cast<int64_t>(t.mt) * 256 + in_tile;
+      // dh is loaded sixteen columns ahead (1411 rows, 160 -> 9008: 73.9 us when it was loaded where it is used, 69.3)
+      uint4 dh[2];
+      const int dcol = t.nt * 128 + 64 * half;
+      const bool grad = kMode == kGatedGrad && t.slot < 0 && row < p.o.m;
+      if (kMode == kGatedGrad) {
+        dh[0] = dh[1] = make_uint4(0, 0, 0, 0);
+        if (grad) dh[0] = grad_load(p.o, p.grad, row, dcol), dh[1] = grad_load(p.o, p.grad, row, dcol + 8);
+      }
+      if (!mbar_wait_warp_cl(smem_u32(&accf[b]), (i >> 1) & 1, &abort_flag, p.status, kDevTimeoutEpilogue)) break;
+      tc_fence_after();
       const uint32_t tbase = tmem + (static_cast<uint32_t>(quad * 32) << 16) + b * 256;
       if (t.slot >= 0) {
         store_piece(p.work, t.slot, in_tile, row < p.o.m, half, tbase);
@@ -363,18 +374,23 @@ __global__ void __launch_bounds__(kGThreads, 1)
         tile_half<kMode == kGatedFwd>(p.o, row, t.nt, half, tbase);
       } else {
 #pragma unroll 1
-        for (int c = 64 * half; c < 64 * half + 64; c += 16) {
+        for (int c = 0; c < 64; c += 16) {
           float g[16], u[16];
-          tmem_read<16>(tbase + c, g);
-          tmem_read<16>(tbase + 128 + c, u);
-          if (row < p.o.m) {
+          const uint4 d0 = dh[0], d1 = dh[1];
+          if (grad && c + 16 < 64) {
+            dh[0] = grad_load(p.o, p.grad, row, dcol + c + 16);
+            dh[1] = grad_load(p.o, p.grad, row, dcol + c + 24);
+          }
+          tmem_read<16>(tbase + 64 * half + c, g);
+          tmem_read<16>(tbase + 128 + 64 * half + c, u);
+          if (grad) {
 #pragma unroll
             for (int e = 0; e < 16; ++e) {
               g[e] *= p.o.alpha0;
               u[e] *= p.o.alpha1;
             }
-            grad8(p.o, p.grad, row, t.nt * 128 + c, g, u);
-            grad8(p.o, p.grad, row, t.nt * 128 + c + 8, g + 8, u + 8);
+            grad8(p.o, p.grad, row, dcol + c, g, u, d0);
+            grad8(p.o, p.grad, row, dcol + c + 8, g + 8, u + 8, d1);
           }
         }
       }
@@ -485,7 +501,7 @@ __global__ void __launch_bounds__(kJoinThreads) join_kernel(const __grid_constan
         g[e] = v[e] * p.o.alpha0;
         h[e] = u[e] * p.o.alpha1;
       }
-      grad8(p.o, p.grad, row, nt * 128 + c, g, h);
+      grad8(p.o, p.grad, row, nt * 128 + c, g, h, grad_load(p.o, p.grad, row, nt * 128 + c));
     } else {
       finish<kGated, 8>(p.o, row, nt, c, v, u);
     }
