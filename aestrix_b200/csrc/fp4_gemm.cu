@@ -87,12 +87,13 @@ struct GemmParams {
   int* status;
 };
 
-// dh of 8 columns (col a multiple of 8), zeros past the last.
+// dh of 8 columns (col a multiple of 8), zeros past the last. Plain loads: the previous kernel, which may have written
+// it, ran when this one was set up, and the read-only path is for what nobody writes meanwhile.
 __device__ __forceinline__ uint4 grad_load(const TileOut& o, const GradOut& p, int64_t row, int col) {
   const int left = o.cols - col;
   uint32_t d[4] = {0, 0, 0, 0};
   const uint16_t* src = p.dh + row * p.lddh + col;
-  if (left >= 8) return __ldg(reinterpret_cast<const uint4*>(src));
+  if (left >= 8) return *reinterpret_cast<const uint4*>(src);
 #pragma unroll
   for (int i = 0; i < 4; ++i)
     d[i] = (2 * i < left ? src[2 * i] : 0u) | ((2 * i + 1 < left ? static_cast<uint32_t>(src[2 * i + 1]) : 0u) << 16);

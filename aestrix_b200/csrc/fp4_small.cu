@@ -229,7 +229,8 @@ __device__ __forceinline__ bool sm_stage_f32(const float* v, uint8_t* dst, int p
   return held;
 }
 
-// Columns 8l..8l+7 of item i's row and record, as they stand (zeros past the last column and item).
+// Columns 8l..8l+7 of item i's row and record, as they stand (zeros past the last column and item). Plain loads: the
+// read-only path is for what nobody writes while the kernel runs, and this one is set up while the previous runs.
 struct SmItem {
   int b, mr;
   uint4 lo, hi;
@@ -243,10 +244,10 @@ __device__ __forceinline__ SmItem sm_fetch(const SmallParams& p, int kb0, int i,
   if (i < items && col < p.k) {
     if (p.x_f32) {
       const uint4* s = reinterpret_cast<const uint4*>(static_cast<const float*>(p.x) + t.mr * p.ldx + col);
-      t.lo = __ldg(s);
-      t.hi = __ldg(s + 1);
+      t.lo = s[0];
+      t.hi = s[1];
     } else {
-      t.lo = __ldg(reinterpret_cast<const uint4*>(static_cast<const uint16_t*>(p.x) + t.mr * p.ldx + col));
+      t.lo = *reinterpret_cast<const uint4*>(static_cast<const uint16_t*>(p.x) + t.mr * p.ldx + col);
     }
   }
   return t;

@@ -825,3 +825,36 @@ def test_f32_rows_to_the_last_bits(cuda_ctx, mode, wide, m):
     ref = x.astype(np.float64) @ R.values(codes, scales, mode, 1.0).T
     y = f64(fp4.fp4_mm(torch.from_numpy(x).cuda(), w, out_dtype=torch.float32))
     assert (np.abs(y - ref) <= 7 * 2.0**-23 * ref).all()
+
+
+@pytest.mark.parametrize("mode", MODES)
+@pytest.mark.parametrize("quantize_x", [False, True])
+@pytest.mark.parametrize("m", [1, 9, 40, 300])
+def test_chain_over_the_same_buffers(cuda_ctx, mode, quantize_x, m):
+    """Calls that read what the call before wrote, over and over the same buffers, against the same
+    calls one at a time: a kernel that is set up while the one before it runs must not see old rows."""
+    n = 768
+    w, _ = make_weight(n, n, mode, 1, 0.00011)
+    v, _ = make_weight(n, n, mode, 2, 0.00011)
+    x0 = activations(m, n, 1)
+
+    def chain(each):
+        a, b, c, rows = x0.clone(), torch.empty_like(x0), torch.empty_like(x0), []
+        for i in range(12):
+            fp4.fp4_mm(a, w, quantize_x=quantize_x, out=b)
+            each()
+            fp4.fp4_gated_mm_dgrad(b, a, w, v, out=c)
+            each()
+            fp4.fp4_mm_dgrad(c, v, out=b)
+            each()
+            rows.append(b.clone())
+            fp4.fp4_gated_mm(b.clamp_(-4, 4), v, w, quantize_x=quantize_x, out=a)
+            each()
+            a.copy_(x0 * (1 + i % 3)) if i % 2 else a.clamp_(-4, 4)
+        return rows
+
+    one_by_one = chain(torch.cuda.synchronize)
+    assert all(torch.isfinite(r).all() and r.any() for r in one_by_one)
+    for _ in range(5):
+        for got, ref in zip(chain(lambda: None), one_by_one):
+            assert torch.equal(got.view(torch.int16), ref.view(torch.int16))
