@@ -19,11 +19,14 @@
 // step (48) do not fit: the accumulators overlap by 48 columns, [0, 256) and
 // [208, 464). The epilogue reads those first and hands them back (`ovl`), so
 // that the next tile's products wait for a fifth of the epilogue only (with one
-// accumulator they waited for all of it: 157 us for the largest listed case).
+// accumulator they waited for all of it: 157 us for 4608 rows gated, 129 now).
 // Barriers per 256-column step (stage s): the copies land on each CTA's full[s];
 // the odd CTA's forwarder arrives on the even CTA's peer[s]; the MMA thread
 // waits for both, issues the copies of scales and four products, and commits to
 // both CTAs' empty[s]. Tiles are dealt out as in the dequantizing GEMM.
+// Measured, the rows' quantisation included: 4608 rows 4096 -> 12288 nvfp4 99 us
+// (4.7 PFLOP/s), gated 4096 -> 9216 mxfp4 129 us (5.4), the tensor pipe busy 70
+// and 74 % of the kernel at the 1.57 GHz that the power cap leaves.
 #include <algorithm>
 
 #include "fp4_internal.h"

@@ -1,7 +1,9 @@
 // fp4_small.cu — products of few rows (at most 16) with microscaled 4-bit
 // weights: y = x W^T, or act(x Wg^T) * (x Wu^T).
 //
-// HBM-bound: the weight is read once. A CTA owns 128 weight rows (one column of
+// The weight is read once, and the work on its codes takes longer than that: one
+// row 4096 -> 9216 nvfp4 8.1 us (2.6 TB/s), 3 f32 rows 4096 -> 18431 mxfp4 15.1 us
+// (2.7), half to two thirds of the issue slots taken. A CTA owns 128 weight rows (one column of
 // records; the gated form one of each weight) and one K split of a
 // thread-block cluster; a producer warp streams its records through a ring of
 // shared-memory slots by bulk copies, compute warps take 16 rows each, up to
