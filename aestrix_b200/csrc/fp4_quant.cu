@@ -1,9 +1,10 @@
 // fp4_quant.cu — to the microscaled 4-bit form and back, and the weight handle
 // of the fp4 products.
 //
-// All three kernels are streams: a thread owns 16 columns of a row, which is one nvfp4 block or, with its neighbouring lane, one mxfp4 block, so
-// the block's largest magnitude needs no shared memory and every element is
-// read and written once. 4608 x 9216 bf16 -> nvfp4 takes 23 us (4.7 TB/s; bound by
+// All three kernels are streams: a thread owns 16 columns of a row, which is one
+// nvfp4 block or, with its neighbouring lane, one mxfp4 block, so the block's
+// largest magnitude needs no shared memory and every element is read and
+// written once. 4608 x 9216 bf16 -> nvfp4 takes 23 us (4.7 TB/s; bound by
 // the rounding's instructions, three quarters of the issue slots), back 18.2 us
 // (6.0 TB/s, HBM).
 #include <cuda_fp16.h>
