@@ -4,9 +4,10 @@
 // All three kernels are streams: a thread owns 16 columns of a row, which is one
 // nvfp4 block or, with its neighbouring lane, one mxfp4 block, so the block's
 // largest magnitude needs no shared memory and every element is read and
-// written once. 4608 x 9216 bf16 -> nvfp4 takes 23 us (4.7 TB/s; bound by
-// the rounding's instructions, three quarters of the issue slots), back 18.2 us
-// (6.0 TB/s, HBM).
+// written once. 4608 x 9216 bf16 -> nvfp4 takes 21.5 us (5.1 TB/s; bound by the
+// rounding's instructions, three quarters of the issue slots; two values a
+// multiplication gained 0.9 us here and nothing in the products), -> mxfp4 17.1 us
+// (6.3 TB/s, HBM), back from nvfp4 18.2 us (6.0 TB/s, HBM).
 #include <cuda_fp16.h>
 
 #include <algorithm>
