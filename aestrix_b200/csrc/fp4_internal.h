@@ -71,6 +71,29 @@ AEX_HD constexpr int scale_off(int r, int g) {
   return kRecCodes + g * 512 + (r & 31) * 16 + (r >> 5) * 4;
 }
 
+// Records along k columns (k + 255 may leave 32 bits).
+constexpr int records_along(int k) { return (k - 1) / kRecK + 1; }
+
+// The conversions count their units of 16 columns (`upr` a row) in 32 bits and
+// find a unit's row by a division that is exact below 2^31.
+struct FastDiv {  // u / div = umulhi(u, mul) >> shift for u < 2^31
+  uint32_t mul, shift, div;
+};
+inline FastDiv fast_div(uint32_t d) {
+  if (d == 1) return FastDiv{0, 0, 1};
+  uint32_t l = 1;
+  while ((uint64_t{1} << l) < d) ++l;
+  return FastDiv{static_cast<uint32_t>(((uint64_t{1} << (31 + l)) + d - 1) / d), l - 1, d};
+}
+// Rows of one launch: at most 2^30 units, in whole tiles of 128 rows, or (rows of more than 2^23 units) a power of two
+// of rows, so that a slice lies within one tile. A row has at most 2^27 units, k being below 2^31.
+inline int64_t slice_rows(uint32_t upr) {
+  const int64_t most = (int64_t{1} << 30) / upr;
+  if (most >= kRecRows) return most / kRecRows * kRecRows;
+  int64_t rows = 1;
+  while (2 * rows <= most) rows *= 2;
+  return rows;
+}
 
 int check_format(aex_ctx* ctx, int format, float tensor_scale);
 // A row-major matrix that is read or written in 16-byte vectors.

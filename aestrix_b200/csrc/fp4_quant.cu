@@ -63,27 +63,19 @@ __device__ __forceinline__ uint32_t load16(const void* x, int64_t at, bool whole
   return max(top << 16, top & 0xFFFF0000u);
 }
 
-// u / divisor for u < 2^31: umulhi(u, mul) >> shift.
-struct FastDiv {
-  uint32_t mul, shift, div;
-};
-inline FastDiv fast_div(uint32_t d) {
-  if (d == 1) return FastDiv{0, 0, 1};
-  uint32_t l = 1;
-  while ((uint64_t{1} << l) < d) ++l;
-  return FastDiv{static_cast<uint32_t>(((uint64_t{1} << (31 + l)) + d - 1) / d), l - 1, d};
-}
 __device__ __forceinline__ uint32_t divide(uint32_t u, const FastDiv& f) {
   return f.div == 1 ? u : __umulhi(u, f.mul) >> f.shift;
 }
 
 // x [rows, k] -> codes [rows, k/2] and scales [rows, k/block] (kRecords: the
 // record layout in `codes`, columns padded with zeros to whole records; rows
-// past the last are left as they are). `upr` units of 16 columns a row (even);
-// rows * upr < 2^31 (the host slices).
+// past the last are left as they are; x starts at row `first` of the first
+// records). `upr` units of 16 columns a row (even); rows * upr < 2^31
+// (slice_rows).
 template <int kFormat, bool kF32, bool kRecords>
 __global__ void __launch_bounds__(kThreads, 8) quantize_kernel(const void* __restrict__ x, int64_t ldx, int rows, int k,
-                                                            FastDiv upr, int whole, float tensor_scale, float inv_6ts,
+                                                            uint32_t first, FastDiv upr, int whole,
+                                                            float tensor_scale, float inv_6ts,
                                                             uint8_t* __restrict__ codes,
                                                             uint8_t* __restrict__ scales) {
   if (kRecords) launch_dependents();  // the product that reads the records waits for them itself
@@ -100,8 +92,9 @@ __global__ void __launch_bounds__(kThreads, 8) quantize_kernel(const void* __res
   const uint32_t sb = quantize_cols<kFormat, 16, kRecords>(v, top, tensor_scale, inv_6ts, w);
   if (!live) return;
   if (kRecords) {
-    const int r = static_cast<int>(row % kRecRows);
-    uint8_t* rec = codes + (static_cast<size_t>(row / kRecRows) * (upr.div / 16) + c / 16) * rec_bytes(kFormat);
+    const uint32_t at = first + row;
+    const int r = static_cast<int>(at % kRecRows);
+    uint8_t* rec = codes + (static_cast<size_t>(at / kRecRows) * (upr.div / 16) + c / 16) * rec_bytes(kFormat);
     const int cu = static_cast<int>(c % 16);  // unit inside the record
     *reinterpret_cast<uint2*>(rec + r * 128 + (((cu >> 1) ^ (r & 7)) << 4) + (cu & 1) * 8) = make_uint2(w[0], w[1]);
     if (kFormat == AEX_FP4_NV)
@@ -176,11 +169,11 @@ __device__ __forceinline__ void bf16_by_table(uint2 codes, float s, float tensor
 }
 
 // Codes -> values, out [rows, k] (row pitch ldo). kRecords: from the record
-// layout. One thread per 16 columns.
+// layout, from row `first` of the first records on. One thread per 16 columns.
 template <int kFormat, bool kF32, bool kRecords>
 __global__ void __launch_bounds__(kThreads) dequantize_kernel(const uint8_t* __restrict__ codes,
                                                               const uint8_t* __restrict__ scales, int rows,
-                                                              FastDiv upr, int k_blocks, float tensor_scale,
+                                                              uint32_t first, FastDiv upr, int k_blocks, float tensor_scale,
                                                               void* __restrict__ out, int64_t ldo, int whole) {
   const uint32_t u = blockIdx.x * kThreads + threadIdx.x;
   const uint32_t row = divide(u, upr), c = u - row * upr.div;
@@ -188,9 +181,9 @@ __global__ void __launch_bounds__(kThreads) dequantize_kernel(const uint8_t* __r
   uint2 w;
   uint32_t sb;
   if (kRecords) {
-    const int r = static_cast<int>(row % kRecRows), cu = static_cast<int>(c % 16);
-    const uint8_t* rec =
-        codes + (static_cast<size_t>(row / kRecRows) * k_blocks + c / 16) * rec_bytes(kFormat);
+    const uint32_t in = first + row;
+    const int r = static_cast<int>(in % kRecRows), cu = static_cast<int>(c % 16);
+    const uint8_t* rec = codes + (static_cast<size_t>(in / kRecRows) * k_blocks + c / 16) * rec_bytes(kFormat);
     w = *reinterpret_cast<const uint2*>(rec + r * 128 + (((cu >> 1) ^ (r & 7)) << 4) + (cu & 1) * 8);
     sb = kFormat == AEX_FP4_NV ? rec[scale_off(r, cu >> 2) + (cu & 3)] : rec[scale_off(r, cu >> 3) + ((cu >> 1) & 3)];
   } else {
@@ -263,9 +256,8 @@ namespace {
 template <int kFormat, bool kF32, bool kRecords>
 int launch_quantize(aex_ctx* ctx, const void* x, int64_t ldx, int rows, int k, float ts, uint8_t* codes,
                     uint8_t* scales, cudaStream_t s) {
-  const uint32_t upr = kRecords ? static_cast<uint32_t>((k + kRecK - 1) / kRecK * 16) : static_cast<uint32_t>(k / 16);
-  // 32-bit unit indices: slices of whole 128-row tiles below 2^31 units each
-  const int64_t step = std::max<int64_t>(kRecRows, (int64_t{1} << 30) / upr / kRecRows * kRecRows);
+  const uint32_t upr = kRecords ? static_cast<uint32_t>(records_along(k)) * 16 : static_cast<uint32_t>(k / 16);
+  const int64_t step = slice_rows(upr);
   const float inv = static_cast<float>(1.0 / (6.0 * static_cast<double>(ts)));
   for (int64_t r0 = 0; r0 < rows; r0 += step) {
     const int nr = static_cast<int>(std::min<int64_t>(step, rows - r0));
@@ -275,8 +267,9 @@ int launch_quantize(aex_ctx* ctx, const void* x, int64_t ldx, int rows, int k, f
                            : codes + static_cast<size_t>(r0) * upr * 8;
     uint8_t* ss = kRecords ? nullptr : scales + static_cast<size_t>(r0) * (k / block_of(kFormat));
     const int whole = (reinterpret_cast<uintptr_t>(xs) | static_cast<uint64_t>(ldx * (kF32 ? 4 : 2))) % 32 == 0;
+    const auto first = static_cast<uint32_t>(r0 % kRecRows);
     quantize_kernel<kFormat, kF32, kRecords>
-        <<<blocks, kThreads, 0, s>>>(xs, ldx, nr, k, fast_div(upr), whole, ts, inv, cs, ss);
+        <<<blocks, kThreads, 0, s>>>(xs, ldx, nr, k, first, fast_div(upr), whole, ts, inv, cs, ss);
     if (int r = check_launch(ctx, "fp4 quantize_kernel")) return r;
   }
   return AEX_OK;
@@ -286,8 +279,8 @@ template <int kFormat, bool kF32, bool kRecords>
 int launch_dequantize(aex_ctx* ctx, const uint8_t* codes, const uint8_t* scales, int rows, int k, float ts, void* out,
                       int64_t ldo, cudaStream_t s) {
   const uint32_t upr = static_cast<uint32_t>(k / 16);
-  const int k_blocks = (k + kRecK - 1) / kRecK;
-  const int64_t step = std::max<int64_t>(kRecRows, (int64_t{1} << 30) / upr / kRecRows * kRecRows);
+  const int k_blocks = records_along(k);
+  const int64_t step = slice_rows(upr);
   for (int64_t r0 = 0; r0 < rows; r0 += step) {
     const int nr = static_cast<int>(std::min<int64_t>(step, rows - r0));
     const uint32_t blocks = static_cast<uint32_t>((static_cast<int64_t>(nr) * upr + kThreads - 1) / kThreads);
@@ -296,8 +289,9 @@ int launch_dequantize(aex_ctx* ctx, const uint8_t* codes, const uint8_t* scales,
     const uint8_t* ss = kRecords ? nullptr : scales + static_cast<size_t>(r0) * (k / block_of(kFormat));
     uint8_t* os = static_cast<uint8_t*>(out) + r0 * ldo * (kF32 ? 4 : 2);
     const int whole = (reinterpret_cast<uintptr_t>(os) | static_cast<uint64_t>(ldo * (kF32 ? 4 : 2))) % 32 == 0;
+    const auto first = static_cast<uint32_t>(r0 % kRecRows);
     dequantize_kernel<kFormat, kF32, kRecords>
-        <<<blocks, kThreads, 0, s>>>(cs, ss, nr, fast_div(upr), k_blocks, ts, os, ldo, whole);
+        <<<blocks, kThreads, 0, s>>>(cs, ss, nr, first, fast_div(upr), k_blocks, ts, os, ldo, whole);
     if (int r = check_launch(ctx, "fp4 dequantize_kernel")) return r;
   }
   return AEX_OK;
@@ -398,7 +392,7 @@ int aex_fp4weight_create(aex_ctx* ctx, const uint8_t* codes, const uint8_t* scal
   if (!codes || !scales || (reinterpret_cast<uintptr_t>(codes) & 15))
     return set_error(ctx, AEX_ERR_INVALID_ARG, "codes (16-byte aligned) and scales must not be NULL");
   const int64_t n_tiles = (static_cast<int64_t>(n) + fp4::kRecRows - 1) / fp4::kRecRows;
-  const int64_t k_blocks = (static_cast<int64_t>(k) + fp4::kRecK - 1) / fp4::kRecK;
+  const int64_t k_blocks = fp4::records_along(k);
   if (n_tiles * k_blocks > 0x7FFFFFFF)
     return set_error(ctx, AEX_ERR_UNSUPPORTED, "fp4 weight of %d x %d is too large", n, k);
   DeviceGuard dev(ctx);

@@ -1,6 +1,8 @@
 """CPU side of the microscaled 4-bit operators: the float64 checker against values worked out by
 hand, and the refusals that need no device."""
 import ctypes as C
+import os
+import subprocess
 
 import numpy as np
 import pytest
@@ -111,3 +113,45 @@ def test_args_struct_matches_the_header():
     f = _lib.aex_fp4_mm_args
     assert [getattr(f, n).offset for n, _ in f._fields_] == [0, 8, 16, 24, 28, 32, 40, 48, 56, 64, 72]
     assert C.sizeof(f) == 80
+
+
+# ---------------------------------------------------------------- host arithmetic of the library
+
+ROOT = os.path.dirname(os.path.dirname(os.path.abspath(__file__)))
+
+
+def compiled(tmp_path, body):
+    """What a program prints that includes the fp4 operators' host header."""
+    src, exe = tmp_path / "t.cpp", tmp_path / "t"
+    src.write_text('#include <cstdio>\n#include "fp4_internal.h"\nusing namespace aex::fp4;\n'
+                   "int main() {\n" + body + "\nreturn 0; }\n")
+    cuda = os.environ.get("CUDA_HOME", "/usr/local/cuda")
+    include = [os.path.join(ROOT, "aestrix_b200", "csrc"), os.path.join(cuda, "include")]
+    subprocess.run(["g++", "-std=c++17", "-O1", str(src), "-o", str(exe)] + ["-I" + d for d in include], check=True)
+    return subprocess.run([str(exe)], check=True, capture_output=True, text=True).stdout.split()
+
+
+LONGEST = 2**31 - 32  # columns: the largest multiple of 32 that an int holds
+
+
+@pytest.mark.parametrize("k", [32, 8192, 2**27 - 32, 2**27, 2**28, 406039616, 2**30 + 32, LONGEST])
+def test_conversions_count_their_units_in_range(tmp_path, k):
+    """The conversions' kernels find a unit's row by a division that is exact below 2^31: every launch's
+    units have to stay below that (124 rows of 406,039,616 columns in one launch left their last
+    columns unwritten), a launch lies in whole tiles of 128 rows or within one, and the division is
+    exact at either end of every row of a launch."""
+    uprs = {k // 16, ((k - 1) // 256 + 1) * 16}  # of a plain matrix and of records
+    got = compiled(tmp_path, f"""
+        std::printf("%d\\n", records_along({k}));
+        for (uint32_t upr : {{{", ".join(f"{u}u" for u in sorted(uprs))}}}) {{
+          const FastDiv f = fast_div(upr);
+          std::printf("%u %lld %u %u\\n", upr, (long long)slice_rows(upr), f.mul, f.shift);
+        }}""")
+    assert int(got[0]) == -(-k // 256)
+    for i in range(1, len(got), 4):
+        upr, rows, mul, shift = map(int, got[i:i + 4])
+        assert rows >= 1 and rows * upr + 256 < 2**31
+        assert rows % 128 == 0 or 128 % rows == 0
+        for row in {0, 1, rows // 2, rows - 1} & set(range(rows)):
+            for u in (row * upr, row * upr + upr - 1):
+                assert (u if upr == 1 else (u * mul >> 32) >> shift) == row
