@@ -71,6 +71,8 @@ AEX_HD constexpr int scale_off(int r, int g) {
   return kRecCodes + g * 512 + (r & 31) * 16 + (r >> 5) * 4;
 }
 
+// How many of the columns [col, col + count) a matrix of `cols` has (col + count may leave 32 bits).
+AEX_HD constexpr int columns_within(int col, int count, int cols) { return cols - col < count ? cols - col : count; }
 // Records along k columns (k + 255 may leave 32 bits).
 constexpr int records_along(int k) { return (k - 1) / kRecK + 1; }
 

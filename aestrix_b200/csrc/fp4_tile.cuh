@@ -124,7 +124,9 @@ __device__ __forceinline__ void store_words(uint16_t* y, const uint32_t* pk) {
 template <bool kGated, int kN>
 __device__ __forceinline__ void finish(const TileOut& p, int64_t row, int nt, int c, const float* v, const float* u) {
   const int col = nt * (kGated ? 128 : 256) + c;
-  if (col >= p.cols) return;
+  const int have = columns_within(col, kN, p.cols);
+  if (have <= 0) return;
+  const bool all = have == kN;
   float o[kN];
   if (!kGated) {
 #pragma unroll
@@ -150,31 +152,31 @@ __device__ __forceinline__ void finish(const TileOut& p, int64_t row, int nt, in
   }
   if (p.y_f32) {
     float* y = static_cast<float*>(p.y) + row * p.ldy + col;
-    if (p.vec && col + kN <= p.cols) {
+    if (p.vec && all) {
 #pragma unroll
       for (int e = 0; e < kN; e += 4) *reinterpret_cast<float4*>(y + e) = make_float4(o[e], o[e + 1], o[e + 2], o[e + 3]);
     } else {
 #pragma unroll
       for (int e = 0; e < kN; ++e)
-        if (col + e < p.cols) y[e] = o[e];
+        if (e < have) y[e] = o[e];
     }
   } else {
     uint16_t* y = static_cast<uint16_t*>(p.y) + row * p.ldy + col;
     uint32_t pk[kN / 2];
 #pragma unroll
     for (int e = 0; e < kN / 2; ++e) pk[e] = pack_bf16x2(o[2 * e], o[2 * e + 1]);
-    if (kN == 16 && p.vec == 2 && col + kN <= p.cols) {
+    if (kN == 16 && p.vec == 2 && all) {
       st_global_32(y, pk);
-    } else if (p.vec && col + kN <= p.cols) {
+    } else if (p.vec && all) {
 #pragma unroll
       for (int e = 0; e < kN / 2; e += 4)
         *reinterpret_cast<uint4*>(y + 2 * e) = make_uint4(pk[e], pk[e + 1], pk[e + 2], pk[e + 3]);
-    } else if (col + kN <= p.cols) {
+    } else if (all) {
       store_words<kN / 2>(y, pk);
     } else {
 #pragma unroll
       for (int e = 0; e < kN; ++e)
-        if (col + e < p.cols) y[e] = static_cast<uint16_t>((e & 1) ? pk[e >> 1] >> 16 : pk[e >> 1] & 0xFFFFu);
+        if (e < have) y[e] = static_cast<uint16_t>((e & 1) ? pk[e >> 1] >> 16 : pk[e >> 1] & 0xFFFFu);
     }
   }
 }

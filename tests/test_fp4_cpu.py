@@ -155,3 +155,12 @@ def test_conversions_count_their_units_in_range(tmp_path, k):
         for row in {0, 1, rows // 2, rows - 1} & set(range(rows)):
             for u in (row * upr, row * upr + upr - 1):
                 assert (u if upr == 1 else (u * mul >> 32) >> shift) == row
+
+
+def test_last_columns_of_the_widest_results(tmp_path):
+    """A tile's columns past the last are told without leaving 32 bits: the end of the group that the
+    last columns of a result of nearly 2^31 are in does (col + 16 > cols has no meaning there)."""
+    cases = [(0, 16, 40), (32, 16, 40), (48, 16, 40), (LONGEST - 16, 16, LONGEST), (LONGEST, 16, LONGEST),
+             (LONGEST + 16, 16, LONGEST), (2**31 - 16, 16, 2**31 - 1), (2**31 - 8, 8, 2**31 - 3)]
+    got = compiled(tmp_path, "\n".join(f'std::printf("%d\\n", columns_within({a}, {b}, {c}));' for a, b, c in cases))
+    assert [max(0, int(g)) for g in got] == [max(0, min(b, c - a)) for a, b, c in cases]
