@@ -42,6 +42,7 @@ int set_error(aex_ctx* ctx, int code, const char* fmt, ...) {
 }
 
 int cuda_error(aex_ctx* ctx, cudaError_t e, const char* what) {
+  cudaGetLastError();  // reported here: check_launch of a later call must not find it again
   const int code = (e == cudaErrorMemoryAllocation) ? AEX_ERR_OOM : AEX_ERR_CUDA;
   return set_error(ctx, code, "%s failed: %s (%s)", what, cudaGetErrorName(e), cudaGetErrorString(e));
 }

@@ -34,6 +34,7 @@ struct aex_qweight {
 namespace aex {
 
 int set_error(aex_ctx* ctx, int code, const char* fmt, ...);
+// Reports a failed runtime call, and takes its error from the runtime, which keeps it until it is read.
 int cuda_error(aex_ctx* ctx, cudaError_t e, const char* what);
 
 #define AEX_CUDA_TRY(ctx, expr)                                   \

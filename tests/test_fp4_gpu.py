@@ -5,6 +5,8 @@ f32 sums on the tensor cores truncate: every one of the accumulation steps (K/16
 4-bit operands; 16 for each 256 columns in the few-rows kernel, which adds those in f32) can lose
 a unit of the last place of a partial sum, which no partial sum's terms' magnitudes S = sum |x w|
 exceed, and aligning the terms of a step the same again: at most (steps + 8) 2^-22 S."""
+import ctypes as C
+
 import numpy as np
 import pytest
 import torch
@@ -858,3 +860,19 @@ def test_chain_over_the_same_buffers(cuda_ctx, mode, quantize_x, m):
     for _ in range(5):
         for got, ref in zip(chain(lambda: None), one_by_one):
             assert torch.equal(got.view(torch.int16), ref.view(torch.int16))
+
+
+# ------------------------------------------------------------------------------- errors of a call
+
+def test_a_failed_call_leaves_no_error_for_the_next(cuda_ctx):
+    """The runtime keeps a call's error until it is read: a weight that does not fit (309 GB) is refused,
+    and the launch after it, which looks whether it failed itself, has no part in that."""
+    x = activations(3, 64, 1)
+    want = fp4.quantize(x, "nvfp4")
+    codes, scales = want
+    h = C.c_void_p()
+    rc = _lib.lib().aex_fp4weight_create(cuda_ctx.handle, codes.data_ptr(), scales.data_ptr(), 2**30, 512,
+                                         _lib.AEX_FP4_NV, 1.0, C.byref(h), None)
+    assert rc == _lib.AEX_ERR_OOM and not h.value
+    got = fp4.quantize(x, "nvfp4")
+    assert torch.equal(got[0], want[0]) and torch.equal(got[1], want[1])
