@@ -876,3 +876,153 @@ def test_a_failed_call_leaves_no_error_for_the_next(cuda_ctx):
     assert rc == _lib.AEX_ERR_OOM and not h.value
     got = fp4.quantize(x, "nvfp4")
     assert torch.equal(got[0], want[0]) and torch.equal(got[1], want[1])
+
+
+# ------------------------------------------------------------- several tiles to a pair of CTAs
+
+def on_gpu(ref):
+    return torch.from_numpy(ref).cuda()
+
+
+def near(got, ref, bound, what):
+    """close(), for float64 tensors on the GPU (all of a large result)."""
+    got = got.double()
+    assert torch.isfinite(got).all(), f"{what}: not finite"
+    over = ((got - ref).abs() - bound).flatten()
+    at = int(over.argmax())
+    assert over[at] <= 0, (f"{what} at {divmod(at, ref.shape[1])}: got {got.flatten()[at].item()!r}, exact "
+                           f"{ref.flatten()[at].item()!r}, allowed {bound.flatten()[at].item():.3e}")
+
+
+def gpu_sum_bound(x, w, steps):
+    return (steps + 8) * 2.0**-22 * (x.abs() @ w.abs().T)
+
+
+def gpu_act(g, name):
+    """R.act on the GPU."""
+    if name == "silu":
+        s = torch.sigmoid(g)
+        return g * s, s * (1.0 + g * (1.0 - s))
+    c = (2.0 / np.pi) ** 0.5
+    t = torch.tanh(c * (g + 0.044715 * g**3))
+    return 0.5 * g * (1.0 + t), 0.5 * (1.0 + t) + 0.5 * g * (1.0 - t * t) * c * (1.0 + 3 * 0.044715 * g**2)
+
+
+# Of 2309 rows (ten tiles) and 128 (gated) or 256 columns a tile: 270 tiles, three to four for each of 74 pairs; 150,
+# two each and two more, which are split along their 9 or 33 records over many pairs that then take whole ones.
+MANY = [(2309, 27 * 128 - 116, 96), (2309, 27 * 128 - 116, 544), (2309, 15 * 128 - 72, 2080),
+        (2309, 15 * 128 - 72, 8256)]
+X_SCALE = 2.0**-8  # a power of two: the 4-bit form of x is exact in f32
+
+
+@pytest.mark.parametrize("mode", MODES)
+@pytest.mark.parametrize("quantize_x", [False, True])
+@pytest.mark.parametrize("m,n,k", MANY)
+def test_gated_of_many_tiles(cuda_ctx, mode, quantize_x, m, n, k):
+    """Pairs that go from tile to tile: both accumulators, again and again, and whole tiles after a piece
+    of a split one. Every element against float64."""
+    ts = X_SCALE if mode == "nvfp4" else 1.0
+    x = activations(m, k, m + k)
+    wg, rg = make_weight(n, k, mode, 1, 0.00011)
+    wu, ru = make_weight(n, k, mode, 2, 0.00037)
+    rg, ru = on_gpu(rg), on_gpu(ru)
+    if quantize_x:
+        X = fp4.dequantize(*fp4.quantize(x, mode, tensor_scale=ts), mode, tensor_scale=ts,
+                           out_dtype=torch.float32).double()
+    else:
+        X = x.double()
+    steps = steps_of(m, k, quantize_x)
+    g, u = X @ rg.T, X @ ru.T
+    eg, eu = gpu_sum_bound(X, rg, steps), gpu_sum_bound(X, ru, steps)
+    for act in ("silu", "gelu_tanh"):
+        a, _ = gpu_act(g, act)
+        z = (g.abs() if act == "silu" else 1.6 * (g + 0.045 * g**3).abs()).clamp(max=90.0)
+        bound = 1.2 * u.abs() * eg + a.abs() * eu + 1.2 * eg * eu  # as gated_bound
+        bound += ((6 + 1.2 * z) * 2.0**-23 + 2.0**-8) * (a * u).abs() + 2.0**-126
+        near(fp4.fp4_gated_mm(x, wg, wu, activation=act, quantize_x=quantize_x, x_scale=ts), a * u, bound, act)
+    cuda_ctx.sync()
+
+
+@pytest.mark.parametrize("mode", MODES)
+@pytest.mark.parametrize("quantize_x", [False, True])
+@pytest.mark.parametrize("m,n,k", [(m, 2 * n + 1, k) for m, n, k in MANY])
+def test_mm_of_many_tiles(cuda_ctx, mode, quantize_x, m, n, k):
+    ts = X_SCALE if mode == "nvfp4" else 1.0
+    x = activations(m, k, m + k)
+    w, ref_w = make_weight(n, k, mode, 1)
+    ref_w = on_gpu(ref_w)
+    X = x.double()
+    if quantize_x:
+        X = fp4.dequantize(*fp4.quantize(x, mode, tensor_scale=ts), mode, tensor_scale=ts,
+                           out_dtype=torch.float32).double()
+    ref, bound = X @ ref_w.T, gpu_sum_bound(X, ref_w, steps_of(m, k, quantize_x))
+    for out in (torch.bfloat16, torch.float32):
+        near(fp4.fp4_mm(x, w, quantize_x=quantize_x, x_scale=ts, out_dtype=out), ref, HALF[out] * ref.abs() + bound,
+             str(out))
+    cuda_ctx.sync()
+
+
+@pytest.mark.parametrize("mode", MODES)
+@pytest.mark.parametrize("act", ["silu", "gelu_tanh"])
+@pytest.mark.parametrize("m,n,k", [(m, n // 8 * 8, k) for m, n, k in MANY])
+def test_gated_dgrad_of_many_tiles(cuda_ctx, mode, act, m, n, k):
+    x, dh = activations(m, k, m + k), activations(m, n, m + n + 1)
+    wg, rg = make_weight(n, k, mode, 1, 0.00011)
+    wu, ru = make_weight(n, k, mode, 2, 0.00037)
+    rg, ru, X, D = on_gpu(rg), on_gpu(ru), x.double(), dh.double()
+    g, u = X @ rg.T, X @ ru.T
+    a, slope = gpu_act(g, act)
+    dg, du = D * u * slope, D * a
+    steps = -(-k // 256) * 16
+    eg, eu = gpu_sum_bound(X, rg, steps), gpu_sum_bound(X, ru, steps)
+    # as test_gated_dgrad
+    e_dg = (2.0**-8 + 2.0**-18) * dg.abs() + D.abs() * (slope.abs() * eu + 1.2 * u.abs() * eg) * 1.01 \
+        + 2.0**-18 * (D * u).abs()
+    e_du = (2.0**-8 + 2.0**-18) * du.abs() + 1.2 * D.abs() * eg * 1.01
+    ref = dg @ rg + du @ ru
+    bound = e_dg @ rg.abs() + e_du @ ru.abs() + 2.0**-8 * ref.abs() \
+        + (2 * -(-n // 128) * 8 + 8) * 2.0**-22 * 1.01 * (dg.abs() @ rg.abs() + du.abs() @ ru.abs())
+    near(fp4.fp4_gated_mm_dgrad(dh, x, wg, wu, activation=act), ref, bound, act)
+    cuda_ctx.sync()
+
+
+@pytest.mark.parametrize("mode", MODES)
+@pytest.mark.parametrize("m,n,k", [(2309, 96, 27 * 256 - 96), (2309, 2080, 15 * 256 - 160), (2309, 8256, 15 * 256 - 160)])
+def test_mm_dgrad_of_many_tiles(cuda_ctx, mode, m, n, k):
+    dy = activations(m, n, m + n)
+    w, ref_w = make_weight(n, k, mode, n + k)
+    ref_w, D = on_gpu(ref_w), dy.double()
+    ref, bound = D @ ref_w, gpu_sum_bound(D, ref_w.T, -(-n // 128) * 8)
+    for out in (torch.bfloat16, torch.float32):
+        near(fp4.fp4_mm_dgrad(dy, w, out_dtype=out), ref, HALF[out] * ref.abs() + bound, str(out))
+    cuda_ctx.sync()
+
+
+# ------------------------------------------------------------------------------ rows on their own
+
+@pytest.mark.parametrize("mode", MODES)
+@pytest.mark.parametrize("dtype", ["bf16", "f32"])
+@pytest.mark.parametrize("quantize_x", [False, True])
+@pytest.mark.parametrize("m", [3, 8, 9, 16])
+def test_few_rows_beside_a_row_of_infinities(cuda_ctx, mode, dtype, quantize_x, m):
+    """A row that holds an infinity or NaN sends its 256 columns of every row through the other staging:
+    the clean rows' results, in one and in two 8-column operands, are those of the formula all the same."""
+    k, n = 544, 264
+    g = np.random.default_rng(5)
+    codes = g.integers(1, 8, (n, k)).astype(np.uint8)  # positive, none zero
+    scales = np.full((n, k // R.BLOCK[mode]), 120 if mode == "mxfp4" else 40, np.uint8)
+    w = fp4.FP4Weight(torch.from_numpy(R.pack(codes)).cuda(), torch.from_numpy(scales).cuda(), mode)
+    ref_w = R.values(codes, scales, mode)
+    x = activations(m, k, 3, DT[dtype])
+    x[0, 17] = float("-inf")
+    x[m - 1, 300] = float("nan")
+    ts = 2.0**-6 if mode == "nvfp4" else 1.0
+    X = f64(x)[1:m - 1]
+    if quantize_x:
+        X = R.values(*R.quantize(X, mode, ts), mode, ts)
+    ref = X @ ref_w.T
+    for out in (torch.bfloat16, torch.float32):
+        y = fp4.fp4_mm(x, w, quantize_x=quantize_x, x_scale=ts, out_dtype=out)
+        close(y[1:m - 1], ref, HALF[out] * np.abs(ref) + sum_bound(X, ref_w, steps_of(m, k, quantize_x)))
+        assert torch.isnan(y[m - 1]).all()
+        assert (torch.isnan(y[0]) if quantize_x else y[0] == float("-inf")).all()
