@@ -17,7 +17,9 @@ of an MLX pack of mode "mxfp4" or "nvfp4", unchanged) and one scale byte per blo
 
 Tensors are 2-D CUDA tensors with contiguous rows whose pitch is a multiple of 16 bytes. Every call
 runs on ``stream`` (default: the current stream of the tensors' device); scratch comes from torch's
-allocator, so calls on different streams and captured graphs do not share any.
+allocator, so calls on different streams and captured graphs do not share any. Tensors handed to a
+call with a ``stream`` of its own are recorded on it, so they may be dropped at once; to order that
+stream behind whatever wrote them is the caller's.
 """
 from __future__ import annotations
 
@@ -75,6 +77,14 @@ def _empty(shape, dtype, like, stream):
         return like.new_empty(shape, dtype=dtype)
     with torch.cuda.stream(stream):
         return like.new_empty(shape, dtype=dtype)
+
+
+def _used(stream, *tensors):
+    """Tells torch's allocator of tensors that the given stream uses, so that their memory is handed to nobody
+    before it has passed the call."""
+    if stream is not None:
+        for t in tensors:
+            t.record_stream(stream)
 
 
 def _out(out, rows, cols, dtype, like, device, stream):
@@ -139,6 +149,7 @@ def quantize(x, mode="nvfp4", tensor_scale=1.0, ctx=None, stream=None):
     scales = _empty((rows, k // BLOCK[mode]), torch.uint8, x, stream)
     rc = lib.aex_fp4_quantize(ctx.handle, x.data_ptr(), _DTYPES[x.dtype], x.stride(0) if rows > 1 else k, rows, k, fmt,
                               tensor_scale, codes.data_ptr(), scales.data_ptr(), _stream(stream, device))
+    _used(stream, x)
     if rc:
         ctx.check(rc)
     return codes, scales
@@ -154,6 +165,7 @@ def dequantize(codes, scales, mode="nvfp4", tensor_scale=1.0, out_dtype=torch.bf
     rc = lib.aex_fp4_dequantize(ctx.handle, codes.data_ptr(), scales.data_ptr(), rows, k, fmt, tensor_scale,
                                 out.data_ptr(), _DTYPES[out.dtype], out.stride(0) if rows > 1 else k,
                                 _stream(stream, device))
+    _used(stream, codes, scales, out)
     if rc:
         ctx.check(rc)
     return out
@@ -177,6 +189,7 @@ class FP4Weight:
                                                      self.k, fmt, tensor_scale, C.byref(h),
                                                      _stream(stream, self.index)))
         self.handle = h
+        _used(stream, codes, scales)
 
     def close(self):
         if getattr(self, "handle", None):
@@ -235,6 +248,7 @@ def _product(x, w, w_up, activation, quantize_x, x_scale, out_dtype, out, stream
         rc = w.lib.aex_fp4_mm(w.ctx.handle, w.handle, a, _stream(stream, device))
     else:
         rc = w.lib.aex_fp4_gated_mm(w.ctx.handle, w.handle, w_up.handle, activation, a, _stream(stream, device))
+    _used(stream, x, out)
     if rc:
         w.ctx.check(rc)
     return out
@@ -273,6 +287,7 @@ def fp4_mm_dgrad(dy, w: FP4Weight, out_dtype=torch.bfloat16, out=None, stream=No
     rc = w.lib.aex_fp4_mm_dgrad(w.ctx.handle, w.handle, dy.data_ptr(), _pitch(dy), m, out.data_ptr(),
                                 _DTYPES[out.dtype], out.stride(0) if m > 1 else w.k, ws.data_ptr() if n_ws else None,
                                 n_ws, _stream(stream, w.index))
+    _used(stream, dy, out)
     if rc:
         w.ctx.check(rc)
     return out
@@ -301,6 +316,7 @@ def fp4_gated_mm_dgrad(dh, x, w_gate: FP4Weight, w_up: FP4Weight, activation="si
                                       dh.data_ptr(), _pitch(dh), m, out.data_ptr(),
                                       out.stride(0) if m > 1 else w.k, ws.data_ptr(), n_ws,
                                       _stream(stream, w.index))
+    _used(stream, x, dh, out)
     if rc:
         w.ctx.check(rc)
     return out

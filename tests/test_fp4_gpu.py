@@ -1026,3 +1026,41 @@ def test_few_rows_beside_a_row_of_infinities(cuda_ctx, mode, dtype, quantize_x, 
         close(y[1:m - 1], ref, HALF[out] * np.abs(ref) + sum_bound(X, ref_w, steps_of(m, k, quantize_x)))
         assert torch.isnan(y[m - 1]).all()
         assert (torch.isnan(y[0]) if quantize_x else y[0] == float("-inf")).all()
+
+
+# --------------------------------------------------------------- tensors dropped after a call
+
+def test_tensors_given_to_another_stream_may_be_dropped(cuda_ctx):
+    """With a stream of its own that is behind, a call's tensors are not handed to new work on the stream
+    they came from (a pack's arrays are usually dropped as soon as the weight is made)."""
+    m, n, k = 200, 520, 544
+    s = torch.cuda.Stream()
+    wg, _ = make_weight(n, k, "nvfp4", 1)
+    wu, _ = make_weight(n, k, "nvfp4", 2)
+    x0, dh0 = activations(m, k, 1), activations(m, n, 2)
+    c0, s0 = fp4.quantize(activations(n, k, 3), "nvfp4")
+    calls = {
+        "weight": ([c0, s0], lambda c, sc: fp4.FP4Weight(c, sc, "nvfp4", stream=s)),
+        "quantize": ([x0], lambda x: fp4.quantize(x, "nvfp4", stream=s)),
+        "dequantize": ([c0, s0], lambda c, sc: fp4.dequantize(c, sc, "nvfp4", stream=s)),
+        "mm": ([x0, dh0], lambda x, out: fp4.fp4_mm(x, wg, out=out, stream=s)),
+        "gated": ([x0], lambda x: fp4.fp4_gated_mm(x, wg, wu, quantize_x=True, stream=s)),
+        "dgrad": ([dh0], lambda dh: fp4.fp4_mm_dgrad(dh, wg, stream=s)),
+        "gated dgrad": ([dh0, x0], lambda dh, x: fp4.fp4_gated_mm_dgrad(dh, x, wg, wu, stream=s)),
+    }
+    for name, (given, call) in calls.items():
+        call(*[t.clone() for t in given])  # whatever a first call sets up
+        torch.cuda.synchronize()
+        mine = [t.clone() for t in given]
+        at = {t.data_ptr() for t in mine}
+        torch.cuda.synchronize()
+        with torch.cuda.stream(s):
+            torch.cuda._sleep(200_000_000)  # some 0.1 s
+        got = call(*mine)
+        del mine
+        new = [torch.full_like(t, 1) for t in given for _ in range(4)]
+        assert not at & {t.data_ptr() for t in new}, name
+        torch.cuda.synchronize()
+        if name == "weight":
+            assert torch.equal(got.dequantize(), fp4.dequantize(c0, s0, "nvfp4"))
+        del got, new
