@@ -987,7 +987,8 @@ def test_gated_dgrad_of_many_tiles(cuda_ctx, mode, act, m, n, k):
 
 
 @pytest.mark.parametrize("mode", MODES)
-@pytest.mark.parametrize("m,n,k", [(2309, 96, 27 * 256 - 96), (2309, 2080, 15 * 256 - 160), (2309, 8256, 15 * 256 - 160)])
+@pytest.mark.parametrize("m,n,k", [(2309, 96, 27 * 256 - 96), (2309, 2080, 15 * 256 - 160),
+                                   (2309, 8256, 15 * 256 - 160)])
 def test_mm_dgrad_of_many_tiles(cuda_ctx, mode, m, n, k):
     dy = activations(m, n, m + n)
     w, ref_w = make_weight(n, k, mode, n + k)
@@ -1030,9 +1031,10 @@ def test_few_rows_beside_a_row_of_infinities(cuda_ctx, mode, dtype, quantize_x, 
 
 # --------------------------------------------------------------- tensors dropped after a call
 
-def test_tensors_given_to_another_stream_may_be_dropped(cuda_ctx):
-    """With a stream of its own that is behind, a call's tensors are not handed to new work on the stream
-    they came from (a pack's arrays are usually dropped as soon as the weight is made)."""
+def test_tensors_given_to_another_stream_may_be_dropped(cuda_ctx, monkeypatch):
+    """A call's tensors are recorded on a stream of its own, and while that is behind they are not handed
+    to new work on the stream they came from (a pack's arrays are usually dropped as soon as the weight
+    is made; making it allocates, which may wait for the device, so there only the recording is seen)."""
     m, n, k = 200, 520, 544
     s = torch.cuda.Stream()
     wg, _ = make_weight(n, k, "nvfp4", 1)
@@ -1048,18 +1050,28 @@ def test_tensors_given_to_another_stream_may_be_dropped(cuda_ctx):
         "dgrad": ([dh0], lambda dh: fp4.fp4_mm_dgrad(dh, wg, stream=s)),
         "gated dgrad": ([dh0, x0], lambda dh, x: fp4.fp4_gated_mm_dgrad(dh, x, wg, wu, stream=s)),
     }
+    seen, record = set(), torch.Tensor.record_stream
+
+    def spy(t, stream):
+        seen.add((t.data_ptr(), stream.cuda_stream))
+        record(t, stream)
+
+    monkeypatch.setattr(torch.Tensor, "record_stream", spy)
     for name, (given, call) in calls.items():
         call(*[t.clone() for t in given])  # whatever a first call sets up
         torch.cuda.synchronize()
         mine = [t.clone() for t in given]
         at = {t.data_ptr() for t in mine}
         torch.cuda.synchronize()
+        seen.clear()
         with torch.cuda.stream(s):
             torch.cuda._sleep(200_000_000)  # some 0.1 s
         got = call(*mine)
+        assert {(p, s.cuda_stream) for p in at} <= seen, name
         del mine
         new = [torch.full_like(t, 1) for t in given for _ in range(4)]
-        assert not at & {t.data_ptr() for t in new}, name
+        if name != "weight":
+            assert not at & {t.data_ptr() for t in new}, name
         torch.cuda.synchronize()
         if name == "weight":
             assert torch.equal(got.dequantize(), fp4.dequantize(c0, s0, "nvfp4"))
