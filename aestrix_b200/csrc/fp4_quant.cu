@@ -173,8 +173,9 @@ __device__ __forceinline__ void bf16_by_table(uint2 codes, float s, float tensor
 template <int kFormat, bool kF32, bool kRecords>
 __global__ void __launch_bounds__(kThreads) dequantize_kernel(const uint8_t* __restrict__ codes,
                                                               const uint8_t* __restrict__ scales, int rows,
-                                                              uint32_t first, FastDiv upr, int k_blocks, float tensor_scale,
-                                                              void* __restrict__ out, int64_t ldo, int whole) {
+                                                              uint32_t first, FastDiv upr, int k_blocks,
+                                                              float tensor_scale, void* __restrict__ out,
+                                                              int64_t ldo, int whole) {
   const uint32_t u = blockIdx.x * kThreads + threadIdx.x;
   const uint32_t row = divide(u, upr), c = u - row * upr.div;
   if (row >= static_cast<uint32_t>(rows)) return;

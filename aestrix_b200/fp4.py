@@ -15,11 +15,13 @@ of an MLX pack of mode "mxfp4" or "nvfp4", unchanged) and one scale byte per blo
 * :func:`fp4_mm_dgrad`, :func:`fp4_gated_mm_dgrad` — their gradients with respect to ``x`` (a 4-bit
   weight is frozen).
 
-Tensors are 2-D CUDA tensors with contiguous rows whose pitch is a multiple of 16 bytes. Every call
-runs on ``stream`` (default: the current stream of the tensors' device); scratch comes from torch's
-allocator, so calls on different streams and captured graphs do not share any. Tensors handed to a
-call with a ``stream`` of its own are recorded on it, so they may be dropped at once; to order that
-stream behind whatever wrote them is the caller's.
+Tensors are 2-D CUDA tensors with contiguous rows; inputs start on 16 bytes and have a pitch of a
+multiple of that (an incoming gradient of n columns, n no multiple of 8, may have any: it is copied
+first). Results may have any pitch and start. Every call runs on ``stream`` (default: the current
+stream of the tensors' device); scratch comes from torch's allocator, so calls on different streams
+and captured graphs do not share any. Tensors handed to a call with a ``stream`` of its own are
+recorded on it, so they may be dropped at once; to order that stream behind whatever wrote them is
+the caller's.
 """
 from __future__ import annotations
 
@@ -277,7 +279,8 @@ def fp4_gated_mm(x, w_gate: FP4Weight, w_up: FP4Weight, activation="silu", quant
 
 
 def fp4_mm_dgrad(dy, w: FP4Weight, out_dtype=torch.bfloat16, out=None, stream=None):
-    """dx[m, k] = dy[m, n] . W[n, k], the gradient of :func:`fp4_mm` (without quantize_x); dy bf16."""
+    """dx[m, k] = dy[m, n] . W[n, k], the gradient of :func:`fp4_mm` (without quantize_x); dy bf16, of any
+    pitch where n is no multiple of 8 (:func:`fp4_mm`'s own results, say)."""
     _open(w)
     _matrix("dy", dy, _BF16, w.n, w.index)
     m = dy.shape[0]

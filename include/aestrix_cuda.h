@@ -296,8 +296,10 @@ int aex_fp4_gated_mm(aex_ctx* ctx, const aex_fp4weight* w_gate, const aex_fp4wei
 
 /* Gradient of aex_fp4_mm (without quantize_x) with respect to x: dx[m, k] =
  * dy[m, n] . W[n, k]. dy bf16, 16-byte aligned, row pitch lddy a multiple of 8
- * elements; dx bf16 or f32, aligned to its element, row pitch lddx. A 4-bit
- * weight is frozen: it has no gradient. */
+ * elements; where n is no multiple of 8 also any lddy >= n and element-aligned
+ * start (a contiguous result's), which costs a copy of dy into the workspace.
+ * dx bf16 or f32, aligned to its element, row pitch lddx. A 4-bit weight is
+ * frozen: it has no gradient. */
 size_t aex_fp4_mm_dgrad_workspace_bytes(const aex_fp4weight* w, int m);
 int aex_fp4_mm_dgrad(aex_ctx* ctx, const aex_fp4weight* w, const void* dy, int64_t lddy, int m, void* dx,
                      int dx_dtype, int64_t lddx, void* workspace, size_t workspace_bytes, aex_stream stream);
@@ -305,7 +307,8 @@ int aex_fp4_mm_dgrad(aex_ctx* ctx, const aex_fp4weight* w, const void* dy, int64
 /* Gradient of aex_fp4_gated_mm (without quantize_x) with respect to x, from
  * dh[m, n]: g and u are computed again from x (nothing is kept from the forward
  * pass), dg = dh u act'(g) and du = dh act(g), each rounded to bf16 as operands
- * of dx = dg . Wg + du . Wu (f32 accumulation). x, dh bf16 as dy above; dx bf16. */
+ * of dx = dg . Wg + du . Wu (f32 accumulation). x bf16 as in aex_fp4_mm_args, dh
+ * as dy above; dx bf16. */
 size_t aex_fp4_gated_mm_dgrad_workspace_bytes(const aex_fp4weight* w_gate, int m);
 int aex_fp4_gated_mm_dgrad(aex_ctx* ctx, const aex_fp4weight* w_gate, const aex_fp4weight* w_up, int activation,
                            const void* x, int64_t ldx, const void* dh, int64_t lddh, int m, void* dx, int64_t lddx,

@@ -1076,3 +1076,80 @@ def test_tensors_given_to_another_stream_may_be_dropped(cuda_ctx, monkeypatch):
         if name == "weight":
             assert torch.equal(got.dequantize(), fp4.dequantize(c0, s0, "nvfp4"))
         del got, new
+
+
+# ------------------------------------------------------------------- gradients of odd widths
+
+def placed(t, how):
+    """t's values as a contiguous tensor, in rows of whole vectors with NaN behind them, or anywhere."""
+    m, n = t.shape
+    if how == "contiguous":
+        return t.contiguous()
+    pitch, start = (-(-n // 8) * 8 + 8, 0) if how == "padded" else (n + 3, 5)
+    buf = torch.full((m * pitch + start,), float("nan"), dtype=t.dtype, device=t.device)
+    out = buf[start:].as_strided((m, n), (pitch, 1))
+    out.copy_(t)
+    return out
+
+
+@pytest.mark.parametrize("mode", MODES)
+@pytest.mark.parametrize("how", ["contiguous", "padded", "anywhere"])
+@pytest.mark.parametrize("m,n,k", [(1, 1, 32), (5, 1, 544), (1, 257, 96), (3, 129, 288), (77, 257, 544),
+                                   (300, 1003, 1120), (33, 8251, 256)])
+def test_dgrads_of_odd_widths(cuda_ctx, mode, how, m, n, k):
+    """Incoming gradients as the products return them (contiguous rows of n), in rows of whole vectors
+    whose rest holds NaN, and at any start and pitch; several tiles, and tiles in pieces."""
+    x, d = activations(m, k, m + k), placed(activations(m, n, m + n + 1), how)
+    wg, rg = make_weight(n, k, mode, 1, 0.00011)
+    wu, ru = make_weight(n, k, mode, 2, 0.00037)
+    X, D = f64(x), f64(d)
+    ref, bound = D @ rg, sum_bound(D, rg.T, -(-n // 128) * 8)
+    for out in (torch.bfloat16, torch.float32):
+        close(fp4.fp4_mm_dgrad(d, wg, out_dtype=out), ref, HALF[out] * np.abs(ref) + bound)
+    dg, du, g, u, a, slope = gated_grad_ref(X, D, rg, ru, "silu")
+    eg, eu = (sum_bound(X, w, -(-k // 256) * 16) for w in (rg, ru))
+    # as test_gated_dgrad
+    e_dg = (2.0**-8 + 2.0**-18) * np.abs(dg) + np.abs(D) * (np.abs(slope) * eu + 1.2 * np.abs(u) * eg) * 1.01 \
+        + 2.0**-18 * np.abs(D * u)
+    e_du = (2.0**-8 + 2.0**-18) * np.abs(du) + 1.2 * np.abs(D) * eg * 1.01
+    ref = dg @ rg + du @ ru
+    bound = e_dg @ np.abs(rg) + e_du @ np.abs(ru) + 2.0**-8 * np.abs(ref) \
+        + (2 * -(-n // 128) * 8 + 8) * 2.0**-22 * 1.01 * (np.abs(dg) @ np.abs(rg) + np.abs(du) @ np.abs(ru))
+    close(fp4.fp4_gated_mm_dgrad(d, x, wg, wu), ref, bound)
+    cuda_ctx.sync()
+
+
+def test_a_products_own_result_goes_back(cuda_ctx):
+    """What fp4_mm and fp4_gated_mm return is a gradient that their gradients take, whatever the width."""
+    for n in (256, 257, 1003):
+        w, _ = make_weight(n, 288, "nvfp4", 1)
+        x = activations(20, 288, 1)
+        for y in (fp4.fp4_mm(x, w), fp4.fp4_gated_mm(x, w, w)):
+            whole = placed(y, "padded") if n % 8 else y
+            assert torch.equal(fp4.fp4_mm_dgrad(y, w), fp4.fp4_mm_dgrad(whole, w))
+            assert torch.equal(fp4.fp4_gated_mm_dgrad(y, x, w, w), fp4.fp4_gated_mm_dgrad(whole, x, w, w))
+
+
+def test_odd_gradient_rows_refusals(cuda_ctx):
+    E = _lib.AexError
+    w, _ = make_weight(264, 288, "nvfp4", 1)
+    dy = torch.zeros(5, 267, dtype=torch.bfloat16, device="cuda")[:, :264]
+    with pytest.raises(E, match="multiple of 16 bytes"):  # a width of whole vectors has them
+        fp4.fp4_mm_dgrad(dy, w)
+    v, _ = make_weight(257, 288, "nvfp4", 1)
+    with pytest.raises(E, match="row pitch of at least 257"):
+        fp4.fp4_mm_dgrad(torch.zeros(1, 257, dtype=torch.bfloat16, device="cuda").expand(5, 257), v)
+    dx = torch.empty(5, 288, dtype=torch.bfloat16, device="cuda")
+    d = torch.zeros(5, 257, dtype=torch.bfloat16, device="cuda")
+    L, h = _lib.lib(), cuda_ctx.handle
+    need = L.aex_fp4_mm_dgrad_workspace_bytes(v.handle, 5)
+    assert need >= 5 * 264 * 2
+    ws = torch.empty(need, dtype=torch.uint8, device="cuda")
+    for p, n in ((None, 0), (ws.data_ptr(), need - 1)):
+        assert L.aex_fp4_mm_dgrad(h, v.handle, d.data_ptr(), 257, 5, dx.data_ptr(), 0, 288, p, n,
+                                  None) == _lib.AEX_ERR_INVALID_ARG
+        assert b"workspace" in L.aex_last_error_string(h)
+    for ptr, ld, m in ((d.data_ptr() + 1, 257, 5), (d.data_ptr(), 256, 5), (d.data_ptr(), 257, 0), (None, 257, 5)):
+        assert L.aex_fp4_mm_dgrad(h, v.handle, ptr, ld, m, dx.data_ptr(), 0, 288, ws.data_ptr(), need,
+                                  None) == _lib.AEX_ERR_INVALID_ARG
+    assert cuda_ctx.device_status() == 0
