@@ -33,6 +33,16 @@ int check_out(aex_ctx* ctx, const char* name, const void* y, int dtype, int64_t 
   return AEX_OK;
 }
 
+// Other CTAs may still read the input when the first results are written.
+int check_apart(aex_ctx* ctx, const char* out, const void* y, int y_dtype, int64_t ldy, int cols, const char* in,
+                const void* x, int x_dtype, int64_t ldx, int x_cols, int rows) {
+  const int64_t sy = y_dtype == AEX_DTYPE_F32 ? 4 : 2, sx = x_dtype == AEX_DTYPE_F32 ? 4 : 2;
+  if (fp4::overlap(reinterpret_cast<uintptr_t>(y), cols * sy, ldy * sy, reinterpret_cast<uintptr_t>(x), x_cols * sx,
+                   ldx * sx, rows))
+    return set_error(ctx, AEX_ERR_INVALID_ARG, "%s must not overlap %s", out, in);
+  return AEX_OK;
+}
+
 int check_workspace(aex_ctx* ctx, const void* p, size_t have, size_t need) {
   if (need && (!p || have < need || (reinterpret_cast<uintptr_t>(p) & 255)))
     return set_error(ctx, AEX_ERR_INVALID_ARG, "workspace: %zu bytes, 256-byte aligned, are needed", need);
@@ -82,6 +92,8 @@ int run(aex_ctx* ctx, const aex_fp4weight* w0, const aex_fp4weight* w1, int acti
   if (a->m <= 0) return set_error(ctx, AEX_ERR_INVALID_ARG, "m must be positive");
   if (int r = fp4::check_matrix(ctx, "x", a->x, a->x_dtype, a->ldx, a->m, w0->k)) return r;
   if (int r = check_out(ctx, "y", a->y, a->y_dtype, a->ldy, w0->n)) return r;
+  if (int r = check_apart(ctx, "y", a->y, a->y_dtype, a->ldy, w0->n, "x", a->x, a->x_dtype, a->ldx, w0->k, a->m))
+    return r;
   const bool f32 = a->x_dtype == AEX_DTYPE_F32;
   if (a->quantize_x != 0 && a->quantize_x != 1)
     return set_error(ctx, AEX_ERR_INVALID_ARG, "quantize_x must be 0 or 1");
@@ -167,6 +179,7 @@ int aex_fp4_mm_dgrad(aex_ctx* ctx, const aex_fp4weight* w, const void* dy, int64
   if (int r = check_weight(ctx, w, "w")) return r;
   if (int r = check_grad(ctx, "dy", dy, lddy, m, w->n)) return r;
   if (int r = check_out(ctx, "dx", dx, dx_dtype, lddx, w->k)) return r;
+  if (int r = check_apart(ctx, "dx", dx, dx_dtype, lddx, w->k, "dy", dy, AEX_DTYPE_BF16, lddy, w->n, m)) return r;
   const fp4::TilePlan plan = fp4::plan_dgrad(w, false, m);
   if (int r = check_tiles(ctx, plan)) return r;
   const size_t copy = copy_bytes(m, w->n);

@@ -97,6 +97,19 @@ inline int64_t slice_rows(uint32_t upr) {
   return rows;
 }
 
+// Whether two matrices of `rows` rows at a and b, of so many bytes a row and from one row to the next, share memory.
+// Rows of one pitch may lie beside one another (columns of one buffer); of two pitches they are taken to share what
+// their ranges share.
+inline bool overlap(uintptr_t a, int64_t a_row, int64_t a_pitch, uintptr_t b, int64_t b_row, int64_t b_pitch, int rows) {
+  const uintptr_t a_end = a + static_cast<uintptr_t>((rows - 1) * a_pitch + a_row);
+  const uintptr_t b_end = b + static_cast<uintptr_t>((rows - 1) * b_pitch + b_row);
+  if (a >= b_end || b >= a_end) return false;
+  if (rows == 1 || a_pitch != b_pitch) return true;
+  const auto pitch = static_cast<uintptr_t>(a_pitch);
+  const auto d = static_cast<int64_t>(b >= a ? (b - a) % pitch : (pitch - (a - b) % pitch) % pitch);  // b's first column
+  return d < a_row || d + b_row > a_pitch;
+}
+
 int check_format(aex_ctx* ctx, int format, float tensor_scale);
 // A row-major matrix that is read or written in 16-byte vectors.
 int check_matrix(aex_ctx* ctx, const char* name, const void* p, int dtype, int64_t ld, int rows, int cols);

@@ -17,7 +17,7 @@ of an MLX pack of mode "mxfp4" or "nvfp4", unchanged) and one scale byte per blo
 
 Tensors are 2-D CUDA tensors with contiguous rows; inputs start on 16 bytes and have a pitch of a
 multiple of that (an incoming gradient of n columns, n no multiple of 8, may have any: it is copied
-first). Results may have any pitch and start. Every call runs on ``stream`` (default: the current
+first). Results may have any pitch and start, and may not overlap an input. Every call runs on ``stream`` (default: the current
 stream of the tensors' device); scratch comes from torch's allocator, so calls on different streams
 and captured graphs do not share any. Tensors handed to a call with a ``stream`` of its own are
 recorded on it, so they may be dropped at once; to order that stream behind whatever wrote them is

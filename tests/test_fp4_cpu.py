@@ -164,3 +164,23 @@ def test_last_columns_of_the_widest_results(tmp_path):
              (LONGEST + 16, 16, LONGEST), (2**31 - 16, 16, 2**31 - 1), (2**31 - 8, 8, 2**31 - 3)]
     got = compiled(tmp_path, "\n".join(f'std::printf("%d\\n", columns_within({a}, {b}, {c}));' for a, b, c in cases))
     assert [max(0, int(g)) for g in got] == [max(0, min(b, c - a)) for a, b, c in cases]
+
+
+def test_overlap_of_two_matrices(tmp_path):
+    """Byte by byte over small ones: never false where they share a byte, and true without one only
+    where the pitches differ."""
+    got = iter(compiled(tmp_path, """
+        for (int rows = 1; rows < 4; ++rows)
+          for (int aw = 1; aw < 5; ++aw) for (int ap = aw; ap < 7; ++ap)
+            for (int bw = 1; bw < 5; ++bw) for (int bp = bw; bp < 7; ++bp)
+              for (int b = 60; b < 120; ++b) std::putchar(overlap(80, aw, ap, b, bw, bp, rows) ? '1' : '0');""")[0])
+    for rows in range(1, 4):
+        for aw in range(1, 5):
+            for ap in range(aw, 7):
+                mine = {80 + r * ap + c for r in range(rows) for c in range(aw)}
+                for bw in range(1, 5):
+                    for bp in range(bw, 7):
+                        for b in range(60, 120):
+                            share = any(b + r * bp + c in mine for r in range(rows) for c in range(bw))
+                            said = next(got) == "1"
+                            assert said == share or (said and ap != bp), (rows, aw, ap, bw, bp, b)

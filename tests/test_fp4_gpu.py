@@ -1153,3 +1153,28 @@ def test_odd_gradient_rows_refusals(cuda_ctx):
         assert L.aex_fp4_mm_dgrad(h, v.handle, ptr, ld, m, dx.data_ptr(), 0, 288, ws.data_ptr(), need,
                                   None) == _lib.AEX_ERR_INVALID_ARG
     assert cuda_ctx.device_status() == 0
+
+
+# ------------------------------------------------------------------------ results over inputs
+
+@pytest.mark.parametrize("m", [1, 5, 40, 300])
+def test_a_result_may_not_lie_over_an_input(cuda_ctx, m):
+    """It would be read by one CTA while another writes it. Columns of one buffer, and rows behind one
+    another, are apart."""
+    n = k = 256
+    w, _ = make_weight(n, k, "nvfp4", 1)
+    buf = torch.zeros(2 * m * 3 * k, dtype=torch.bfloat16, device="cuda")
+    wide = buf.view(2 * m, 3 * k)
+    x = wide[:m, :k]
+    x.copy_(activations(m, k, 1))
+    before = buf.clone()
+    for out in (x, wide[:m, k // 2:k // 2 + n], wide[m - 1:2 * m - 1, :n], buf[k - 8:].as_strided((m, n), (n, 1))):
+        for call in (lambda: fp4.fp4_mm(x, w, out=out), lambda: fp4.fp4_mm(x, w, quantize_x=True, out=out),
+                     lambda: fp4.fp4_gated_mm(x, w, w, out=out), lambda: fp4.fp4_mm_dgrad(x, w, out=out)):
+            with pytest.raises(_lib.AexError, match="must not overlap"):
+                call()
+    assert torch.equal(buf, before)
+    for out in (wide[:m, k:k + n], wide[:m, 2 * k:2 * k + n], wide[m:, :n]):
+        assert torch.equal(fp4.fp4_mm(x, w, out=out), fp4.fp4_mm(x, w))
+        assert torch.equal(fp4.fp4_mm_dgrad(x, w, out=out), fp4.fp4_mm_dgrad(x, w))
+        assert torch.equal(fp4.fp4_gated_mm(x, w, w, out=out), fp4.fp4_gated_mm(x, w, w))
