@@ -199,17 +199,6 @@ __device__ __forceinline__ void st_global_32(void* p, const uint32_t* v) {
                : "memory");
 }
 
-// Arrives (lane 0) on the barrier at `bar` once the loads that `v` was made of
-// have returned in every lane of the warp. Program order is not enough: a load
-// whose value is used only after a later wait was seen to be carried out after
-// the arrive, and read what the producer had copied into the slot by then (the
-// address depends on the loaded values by way of a zero that only the host
-// knows to be one).
-__device__ __forceinline__ void arrive_after_loads(uint32_t bar, uint32_t v, uint32_t zero, int lane) {
-  const uint32_t all = __reduce_or_sync(0xffffffffu, v);
-  if (lane == 0) mbar_arrive_addr(bar + (all & zero));
-}
-
 constexpr uint32_t kBf16x2_2p126 = 0x7E807E80u;  // 2^126 in both halves
 
 // The scale as the bf16 pair that decode_pair multiplies by. nvfp4: s * 2^119

@@ -154,6 +154,17 @@ __device__ __forceinline__ void mbar_arrive_addr(uint32_t a) {
   asm volatile("mbarrier.arrive.shared::cta.b64 _, [%0];" ::"r"(a) : "memory");
 }
 
+// Arrives (lane 0) on the barrier at `bar` once the loads that `v` was made of
+// have returned in every lane of the warp. Program order is not enough: a load
+// whose value is used only after a later wait was seen to be carried out after
+// the arrive, and read what the producer had copied into the slot by then (the
+// address depends on the loaded values by way of a zero that only the host
+// knows to be one).
+__device__ __forceinline__ void arrive_after_loads(uint32_t bar, uint32_t v, uint32_t zero, int lane) {
+  const uint32_t all = __reduce_or_sync(0xffffffffu, v);
+  if (lane == 0) mbar_arrive_addr(bar + (all & zero));
+}
+
 // ---------------------------------------------- barriers shared by a CTA pair
 // Waits with cluster-scope acquire, for barriers that the peer CTA (or the
 // peer's tensor-core commits) arrive on.

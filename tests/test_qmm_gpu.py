@@ -186,3 +186,18 @@ def test_gemm_weights_bit_exact_identity(cuda_ctx):
     # A zero weight sums to +0 in the accumulator whatever its sign.
     ref = np.where(ref == 0x8000, np.uint16(0), ref)
     assert np.array_equal(got, ref), np.argwhere(got != ref)[:8]
+
+
+@pytest.mark.parametrize("m,n,k,dtype", [(1, 18432, 4096, "f32"), (1, 1000, 7680, "bf16"), (3, 4100, 4096, "f32"),
+                                         (8, 9216, 4096, "bf16"), (16, 1000, 12288, "bf16")])
+def test_gemv_same_bits_every_time(cuda_ctx, m, n, k, dtype):
+    """No slot of the weight ring is filled again before the whole warp has read it: every one of many
+    calls in a row, over several weights and queued without a gap, gives the same bits."""
+    ws = [qmm.QuantizedWeight(*qmm.synthetic_weight(n, k, s)) for s in range(3)]
+    g = torch.Generator().manual_seed(m)
+    x = torch.randn(m, k, generator=g).to(torch.float32 if dtype == "f32" else torch.bfloat16).cuda()
+    first = [qmm.quantized_mm(x, w, out_dtype=torch.float32) for w in ws]
+    differ = torch.zeros((), dtype=torch.int64, device="cuda")
+    for i in range(300):
+        differ += (qmm.quantized_mm(x, ws[i % 3], out_dtype=torch.float32) != first[i % 3]).sum()
+    assert differ.item() == 0
