@@ -24,9 +24,10 @@
 // the odd CTA's forwarder arrives on the even CTA's peer[s]; the MMA thread
 // waits for both, issues the copies of scales and four products, and commits to
 // both CTAs' empty[s]. Tiles are dealt out as in the dequantizing GEMM.
-// Measured, the rows' quantisation included: 4608 rows 4096 -> 12288 nvfp4 99 us
-// (4.7 PFLOP/s), gated 4096 -> 9216 mxfp4 129 us (5.4), the tensor pipe busy 70
-// and 74 % of the kernel at the 1.57 GHz that the power cap leaves.
+// Measured, the rows' quantisation included (17 and 12 us of it): 4608 rows 4096
+// -> 12288 nvfp4 99 us (4.7 PFLOP/s) in the 2 ms after a pause, 117 us (4.0) in a
+// loop, where the power cap leaves 1.43 GHz; gated 4096 -> 9216 mxfp4 132 us (5.3)
+// and 152 (4.6). The tensor pipe is busy 70 and 74 % of the kernel.
 #include <algorithm>
 
 #include "fp4_internal.h"
@@ -146,6 +147,8 @@ __global__ void __launch_bounds__(kBThreads, 1) block_kernel(const __grid_consta
     mbar_init(drain, 1);
     fence_barrier_init();
   }
+  // Before the wait, as the GEMM must not: the kernel before this one is always quantize_kernel, launched without
+  // setting up early and without tensor memory, so whatever held some on this stream has ended.
   if (warp == 2) {
     tmem_alloc_pair(tmem_slot, 512);
     tmem_relinquish_pair();

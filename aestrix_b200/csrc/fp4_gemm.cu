@@ -40,10 +40,11 @@
 // Each kernel lets the stream's next one set up behind it (0.5 to 1 us a call).
 // Tensor memory is taken after the wait for the previous kernel: that one may
 // hold some, or not have taken its own yet.
-// Measured: 512 rows gated 4096 -> 9216 54 to 57 us (1.4 PFLOP/s), 1111 rows 9216
-// -> 4104 79 to 89 us (tiles of 256 use 82 % of the products), 512 rows back
-// through 4096 -> 7680 30 us (60 tiles on 74 pairs); the tensor pipe is busy 63
-// to 66 % of the kernel at 1.6 GHz.
+// Measured in the 2 ms after a pause, and in a loop, where the power cap leaves
+// 1.6 GHz (1.75 the gradient): 512 rows gated 4096 -> 9216 56 us (1.4 PFLOP/s) and
+// 64, 1111 rows 9216 -> 4104 82 and 93 (tiles of 256 use 82 % of the products), 512
+// rows back through 4096 -> 7680 31.5 and 33 (60 tiles on 74 pairs). The tensor pipe
+// is busy 63 to 66 % of the kernel.
 #include <algorithm>
 
 #include "fp4_internal.h"
@@ -104,7 +105,9 @@ __device__ __forceinline__ uint4 grad_load(const TileOut& o, const GradOut& p, i
   return make_uint4(d[0], d[1], d[2], d[3]);
 }
 
-// dg, du of 8 columns from g, u (already scaled) and dh.
+// dg, du of 8 columns from g, u (already scaled) and dh. They are rounded to bf16 here, as operands of the tensor
+// core's next product (what bf16 leaves of them would take that product a second time). So dx is off by 0.0023 of its
+// size (1024 rows, 4096 -> 9216), where its own last rounding alone comes to 0.0017.
 __device__ __forceinline__ void grad8(const TileOut& o, const GradOut& p, int64_t row, int col, const float* g,
                                       const float* u, const uint4& dh) {
   if (col >= o.cols) return;

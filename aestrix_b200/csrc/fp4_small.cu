@@ -2,9 +2,10 @@
 // weights: y = x W^T, or act(x Wg^T) * (x Wu^T).
 //
 // The weight is read once, and the work on its codes takes longer than that: one
-// row 4096 -> 9216 nvfp4 8.1 us (2.6 TB/s), 3 f32 rows 4096 -> 18431 mxfp4 15.1 us
-// (2.7), half to two thirds of the issue slots taken. A CTA owns 128 weight rows (one column of
-// records; the gated form one of each weight) and one K split of a
+// row 4096 -> 9216 nvfp4 8.1 us (2.6 TB/s), 3 f32 rows 4096 -> 18431 mxfp4 15.7 us
+// (2.6). Half to two thirds of the issue slots are taken; the rest is latency (staging,
+// the first records, the sum over the cluster). A CTA owns 128 weight rows (one
+// column of records; the gated form one of each weight) and one K split of a
 // thread-block cluster; a producer warp streams its records through a ring of
 // shared-memory slots by bulk copies, compute warps take 16 rows each, up to
 // three sets of eight warps that take turns at the records (one set left the

@@ -10,10 +10,11 @@ of an MLX pack of mode "mxfp4" or "nvfp4", unchanged) and one scale byte per blo
 * :func:`quantize`, :func:`dequantize` — to this form and back;
 * :class:`FP4Weight` — a weight laid out on the device for the products;
 * :func:`fp4_mm` — ``y = x . W^T``, activations as they are or quantized within the call;
-* :func:`fp4_gated_mm` — ``act(x . Wg^T) * (x . Wu^T)`` in one kernel (linear_in -> silu(g) * u,
-  Sources/ImarelloDiT/FeedForward.swift:11-24);
+* :func:`fp4_gated_mm` — ``act(x . Wg^T) * (x . Wu^T)``, neither projection stored (linear_in ->
+  silu(g) * u, Sources/ImarelloDiT/FeedForward.swift:11-24);
 * :func:`fp4_mm_dgrad`, :func:`fp4_gated_mm_dgrad` — their gradients with respect to ``x`` (a 4-bit
-  weight is frozen).
+  weight is frozen). Autograd does not record the products: a result has no history, whatever x
+  requires, and a backward pass calls these.
 
 Tensors are 2-D CUDA tensors with contiguous rows; inputs start on 16 bytes and have a pitch of a
 multiple of that (an incoming gradient of n columns, n no multiple of 8, may have any: it is copied
@@ -270,7 +271,7 @@ def fp4_mm(x, w: FP4Weight, quantize_x=False, x_scale=1.0, out_dtype=torch.bfloa
 def fp4_gated_mm(x, w_gate: FP4Weight, w_up: FP4Weight, activation="silu", quantize_x=False, x_scale=1.0,
                  out_dtype=torch.bfloat16, out=None, stream=None):
     """h[m, n] = act(x . Wg^T) * (x . Wu^T): both projections, the activation ("silu" or "gelu_tanh") and
-    the product in one kernel, rounded once. x, quantize_x and x_scale as :func:`fp4_mm`."""
+    their product fused, rounded once. x, quantize_x and x_scale as :func:`fp4_mm`."""
     _open(w_gate, w_up)
     act = ACTIVATIONS.get(activation)
     if act is None:

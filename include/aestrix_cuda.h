@@ -215,11 +215,13 @@ int aex_qmm_ex(aex_ctx* ctx, const aex_qweight* w, const void* x, int x_dtype, i
  *               scale (pass 1).
  *   AEX_FP4_NV  blocks of 16, e4m3 scale (bit 7 ignored, 0x7F is NaN), times
  *               one f32 per tensor in [2^-100, 2^100].
- * k is a multiple of 32 throughout; codes are 16-byte aligned. None of these
- * calls uses memory of the context: what a call needs is in its arguments, so
- * calls on different streams, and graphs that hold them, do not touch one
- * another. They leave the calling thread's current device as it was. No output
- * may overlap an input or the workspace. */
+ * k is a multiple of 32 throughout; codes are 16-byte aligned. Of the context
+ * these calls use its status word alone (as every call does, so it outlives the
+ * graphs that hold them): what else a call needs is in its arguments, so calls
+ * on different streams, and graphs, do not touch one another. They leave the
+ * calling thread's current device as it was. No output may overlap an input or
+ * the workspace (a product's result over its activations, or a gradient over
+ * the one it comes from, is refused). */
 #define AEX_FP4_MX 0
 #define AEX_FP4_NV 1
 #define AEX_ACT_SILU 0
@@ -288,8 +290,10 @@ int aex_fp4_mm(aex_ctx* ctx, const aex_fp4weight* w, const aex_fp4_mm_args* args
 
 /* y[m, n] = act(x . Wg^T) * (x . Wu^T), the gated feed-forward projection:
  * both products, the activation (AEX_ACT_SILU, or AEX_ACT_GELU_TANH
- * g (1 + tanh(sqrt(2/pi) (g + 0.044715 g^3))) / 2) and the product in one
- * kernel, f32 until the one rounding of y. Wg and Wu have one shape and format.
+ * g (1 + tanh(sqrt(2/pi) (g + 0.044715 g^3))) / 2) and their product fused, f32
+ * until the one rounding of y: no g or u is stored. One kernel, and where they are
+ * called for one that quantizes x and one that adds the pieces of split tiles. Wg
+ * and Wu have one shape and format.
  * Reference: linear_in -> silu(g) * u, Sources/ImarelloDiT/FeedForward.swift:11-24. */
 int aex_fp4_gated_mm(aex_ctx* ctx, const aex_fp4weight* w_gate, const aex_fp4weight* w_up, int activation,
                      const aex_fp4_mm_args* args, aex_stream stream);
