@@ -74,13 +74,7 @@ int check_grad(aex_ctx* ctx, const char* name, const void* p, int64_t ld, int m,
   return check_out(ctx, name, p, AEX_DTYPE_BF16, ld, n);
 }
 
-int whole_rows(aex_ctx* ctx, const void** p, int64_t* ld, int m, int n, void* copy, cudaStream_t s) {
-  if (reinterpret_cast<uintptr_t>(*p) % 16 == 0 && *ld % 8 == 0) return AEX_OK;
-  if (int r = fp4::pad_rows(ctx, *p, *ld, m, n, copy, padded(n), s)) return r;
-  *p = copy;
-  *ld = padded(n);
-  return AEX_OK;
-}
+bool whole_rows(const void* p, int64_t ld) { return reinterpret_cast<uintptr_t>(p) % 16 == 0 && ld % 8 == 0; }
 
 int check_tiles(aex_ctx* ctx, const fp4::TilePlan& p) {
   return p.clusters ? AEX_OK : set_error(ctx, AEX_ERR_UNSUPPORTED, "the product has too many output tiles");
@@ -182,12 +176,16 @@ int aex_fp4_mm_dgrad(aex_ctx* ctx, const aex_fp4weight* w, const void* dy, int64
   if (int r = check_apart(ctx, "dx", dx, dx_dtype, lddx, w->k, "dy", dy, AEX_DTYPE_BF16, lddy, w->n, m)) return r;
   const fp4::TilePlan plan = fp4::plan_dgrad(w, false, m);
   if (int r = check_tiles(ctx, plan)) return r;
-  const size_t copy = copy_bytes(m, w->n);
+  const size_t copy = whole_rows(dy, lddy) ? 0 : copy_bytes(m, w->n);
   if (int r = check_workspace(ctx, workspace, workspace_bytes, copy + plan.bytes)) return r;
   DeviceGuard dev(ctx);
   if (dev.rc) return dev.rc;
   auto s = static_cast<cudaStream_t>(stream);
-  if (int r = whole_rows(ctx, &dy, &lddy, m, w->n, workspace, s)) return r;
+  if (copy) {
+    if (int r = fp4::pad_rows(ctx, dy, lddy, m, w->n, workspace, padded(w->n), s)) return r;
+    dy = workspace;
+    lddy = padded(w->n);
+  }
   return fp4::run_dgrad(ctx, w, nullptr, dy, lddy, nullptr, 0, m, w->tensor_scale, dx, dx_dtype == AEX_DTYPE_F32, lddx,
                         static_cast<uint8_t*>(workspace) + copy, s);
 }
@@ -211,7 +209,8 @@ int aex_fp4_gated_mm_dgrad(aex_ctx* ctx, const aex_fp4weight* w_gate, const aex_
   if (int r = check_out(ctx, "dx", dx, AEX_DTYPE_BF16, lddx, w_gate->k)) return r;
   if (int r = check_tiles(ctx, fp4::plan_gemm(w_gate, true, m))) return r;
   if (int r = check_tiles(ctx, fp4::plan_dgrad(w_gate, true, m))) return r;
-  const size_t need = aex_fp4_gated_mm_dgrad_workspace_bytes(w_gate, m);
+  const size_t copy = whole_rows(dh, lddh) ? 0 : copy_bytes(m, w_gate->n);
+  const size_t need = aex_fp4_gated_mm_dgrad_workspace_bytes(w_gate, m) - (copy_bytes(m, w_gate->n) - copy);
   if (int r = check_workspace(ctx, workspace, workspace_bytes, need)) return r;
   DeviceGuard dev(ctx);
   if (dev.rc) return dev.rc;
@@ -222,8 +221,12 @@ int aex_fp4_gated_mm_dgrad(aex_ctx* ctx, const aex_fp4weight* w_gate, const aex_
   auto* ws = static_cast<uint8_t*>(workspace);
   auto* dg = reinterpret_cast<uint16_t*>(ws);
   auto* du = reinterpret_cast<uint16_t*>(ws + d);
-  if (int r = whole_rows(ctx, &dh, &lddh, m, w_gate->n, ws + 2 * d, s)) return r;
-  void* pieces = ws + 2 * d + copy_bytes(m, w_gate->n);
+  if (copy) {
+    if (int r = fp4::pad_rows(ctx, dh, lddh, m, w_gate->n, ws + 2 * d, ld, s)) return r;
+    dh = ws + 2 * d;
+    lddh = ld;
+  }
+  void* pieces = ws + 2 * d + copy;
   if (int r = fp4::run_gated_grad(ctx, w_gate, w_up, activation, x, ldx, m, dh, lddh, dg, du, ld, pieces, s)) return r;
   return fp4::run_dgrad(ctx, w_gate, w_up, dg, ld, du, ld, m, 1.f, dx, false, lddx, pieces, s);
 }

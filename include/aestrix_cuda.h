@@ -220,8 +220,8 @@ int aex_qmm_ex(aex_ctx* ctx, const aex_qweight* w, const void* x, int x_dtype, i
  * graphs that hold them): what else a call needs is in its arguments, so calls
  * on different streams, and graphs, do not touch one another. They leave the
  * calling thread's current device as it was. No output may overlap an input or
- * the workspace (a product's result over its activations, or a gradient over
- * the one it comes from, is refused). */
+ * the workspace (aex_fp4_mm, aex_fp4_gated_mm and aex_fp4_mm_dgrad refuse a
+ * result that lies over their x or dy). */
 #define AEX_FP4_MX 0
 #define AEX_FP4_NV 1
 #define AEX_ACT_SILU 0
@@ -301,7 +301,8 @@ int aex_fp4_gated_mm(aex_ctx* ctx, const aex_fp4weight* w_gate, const aex_fp4wei
 /* Gradient of aex_fp4_mm (without quantize_x) with respect to x: dx[m, k] =
  * dy[m, n] . W[n, k]. dy bf16, 16-byte aligned, row pitch lddy a multiple of 8
  * elements; where n is no multiple of 8 also any lddy >= n and element-aligned
- * start (a contiguous result's), which costs a copy of dy into the workspace.
+ * start (a contiguous result's), which costs a copy of dy into the workspace
+ * (aex_fp4_mm_dgrad_workspace_bytes has room for it).
  * dx bf16 or f32, aligned to its element, row pitch lddx. A 4-bit weight is
  * frozen: it has no gradient. */
 size_t aex_fp4_mm_dgrad_workspace_bytes(const aex_fp4weight* w, int m);

@@ -1178,3 +1178,93 @@ def test_a_result_may_not_lie_over_an_input(cuda_ctx, m):
         assert torch.equal(fp4.fp4_mm(x, w, out=out), fp4.fp4_mm(x, w))
         assert torch.equal(fp4.fp4_mm_dgrad(x, w, out=out), fp4.fp4_mm_dgrad(x, w))
         assert torch.equal(fp4.fp4_gated_mm(x, w, w, out=out), fp4.fp4_gated_mm(x, w, w))
+
+
+def test_whole_rows_of_an_odd_width_need_no_copy(cuda_ctx):
+    """A C caller whose rows are of whole vectors needs the copy's part of the workspace neither."""
+    w, _ = make_weight(257, 288, "nvfp4", 1)
+    d = placed(activations(5, 257, 1), "padded")
+    dx, L = torch.empty(5, 288, dtype=torch.bfloat16, device="cuda"), _lib.lib()
+    assert L.aex_fp4_mm_dgrad_workspace_bytes(w.handle, 5) == -(-5 * 264 * 2 // 256) * 256
+    rc = L.aex_fp4_mm_dgrad(cuda_ctx.handle, w.handle, d.data_ptr(), d.stride(0), 5, dx.data_ptr(),
+                            _lib.AEX_DTYPE_BF16, 288, None, 0, None)
+    assert rc == _lib.AEX_OK
+    torch.cuda.synchronize()
+    assert torch.equal(dx, fp4.fp4_mm_dgrad(d, w))
+
+
+@pytest.mark.parametrize("m", [3, 70])
+def test_captured_with_streams_and_odd_widths(cuda_ctx, m):
+    """Calls given the capturing stream, over tensors that are dropped, and gradients that are copied
+    first: the graph replays what the calls compute, next to other work of the same pool."""
+    n, k = 257, 544
+    w, _ = make_weight(n, k, "mxfp4", 1)
+    x = activations(m, k, 1)
+
+    def calls(stream):
+        y = fp4.fp4_mm(x, w, quantize_x=True, stream=stream)
+        dx = fp4.fp4_mm_dgrad(y, w, stream=stream)
+        return fp4.fp4_gated_mm_dgrad(y, dx, w, w, stream=stream)  # y and dx are dropped here
+
+    s = torch.cuda.Stream()
+    want = calls(None)
+    torch.cuda.synchronize()
+    with torch.cuda.stream(s):
+        calls(s)
+    torch.cuda.synchronize()
+    g = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(g, stream=s):
+        got = calls(s)
+    for seed in (1, 2):
+        x.copy_(activations(m, k, seed))
+        want = calls(None)
+        torch.cuda.synchronize()
+        g.replay()
+        junk = [torch.full_like(x, 3.0) for _ in range(8)]
+        torch.cuda.synchronize()
+        assert torch.equal(got, want)
+        del junk
+
+
+# ------------------------------------------------------------------------ rows beyond 2^27 columns
+
+@pytest.mark.parametrize("mode", MODES)
+def test_rows_of_more_units_than_a_launch_holds_128_of(cuda_ctx, mode):
+    """2^27 and 32 columns: 64 rows a launch, so that the second starts inside a tile of 128. x is zero
+    but for forty columns, whose blocks say all there is to say."""
+    if torch.cuda.mem_get_info()[0] < 100e9:
+        pytest.skip("needs 100 GB of device memory")
+    m, k, block = 70, 2**27 + 32, R.BLOCK[mode]
+    g = np.random.default_rng(1)
+    blocks = np.unique(np.concatenate([[0, k // block - 1], g.integers(0, k // block, 38)]))
+    some = np.zeros((m, len(blocks), block), np.float32)
+    some[:, np.arange(len(blocks)), g.integers(0, block, len(blocks))] = g.choice([-3.0, -1.0, 0.5, 2.0, 6.0],
+                                                                                  (m, len(blocks)))
+    some = some.reshape(m, -1)
+    cols = torch.from_numpy((blocks[:, None] * block + np.arange(block)).reshape(-1)).cuda()
+    x = torch.zeros(m, k, dtype=torch.bfloat16, device="cuda")
+    x[:, cols] = torch.from_numpy(some).bfloat16().cuda()
+    ref_codes, ref_scales = R.quantize(some, mode)
+    ref = R.values(ref_codes, ref_scales, mode)
+    codes, scales = fp4.quantize(x, mode)
+    at = torch.from_numpy(blocks).cuda()
+    assert np.array_equal(scales[:, at].cpu().numpy(), ref_scales)
+    assert int(scales.count_nonzero()) == int((ref_scales != 0).sum())
+    assert np.array_equal(codes[:, cols[::2] // 2].cpu().numpy(), R.pack(ref_codes))
+    assert int(codes.count_nonzero()) == int((R.pack(ref_codes) != 0).sum())
+    y = torch.empty(m, 40, device="cuda")
+    w = fp4.FP4Weight(codes[:40], scales[:40], mode)
+    fp4.fp4_mm(x, w, quantize_x=True, out=y)
+    want = ref @ ref[:40].T
+    # the sums have at most forty terms, in as many steps
+    close(y, want, 2.0**-24 * np.abs(want) + (len(blocks) + 8) * 2.0**-22 * (np.abs(ref) @ np.abs(ref[:40]).T))
+    del w, x
+    torch.cuda.empty_cache()
+    back = fp4.dequantize(codes, scales, mode)
+    assert np.array_equal(f64(back[:, cols]), ref)
+    assert int(back.count_nonzero()) == int((ref != 0).sum())
+    w = fp4.FP4Weight(codes, scales, mode)
+    got = w.dequantize()
+    assert all(torch.equal(got[r], back[r]) for r in range(m))
+    del w, got, back, codes, scales
+    torch.cuda.empty_cache()
