@@ -1268,3 +1268,22 @@ def test_rows_of_more_units_than_a_launch_holds_128_of(cuda_ctx, mode):
     assert all(torch.equal(got[r], back[r]) for r in range(m))
     del w, got, back, codes, scales
     torch.cuda.empty_cache()
+
+
+def test_dequantize_rounds_once_next_to_ties(cuda_ctx):
+    """Tensor scales amax * 1.25 / 2688 = amax * 5 / (21 * 2^9) of bf16 amax, rounded to f32: a scale of 1.75 times a
+    code of 1.5 has the factor 21, so those products lie within 2^-24 of numbers of 11 bits, ties of bf16 among
+    them. Rounding them to f32 on the way would take some to the wrong side."""
+    codes = np.tile(np.arange(16, dtype=np.uint8), (127, 2))
+    scales = np.repeat(np.arange(127, dtype=np.uint8)[:, None], 2, 1)
+    c, s = torch.from_numpy(R.pack(codes)).cuda(), torch.from_numpy(scales).cuda()
+    twice = 0
+    for a in range(128):
+        ts = float(np.float32((1 + a / 128) * 1.25 / 2688))
+        ref = R.values(codes, scales, "nvfp4", ts)  # exact: 6 by 24 bits
+        _, e = np.frexp(ref)
+        step = np.ldexp(1.0, e - 8)
+        once = np.where(ref == 0, 0.0, np.round(ref / step) * step)
+        assert np.array_equal(f64(fp4.dequantize(c, s, "nvfp4", tensor_scale=ts)), once)
+        twice += (np.round(np.float32(ref).astype(np.float64) / step) * step != once).sum()
+    assert twice  # these scales do hold such products
