@@ -85,9 +85,8 @@ def _empty(shape, dtype, like, stream):
 def _used(stream, *tensors):
     """Tells torch's allocator of tensors that the given stream uses, so that their memory is handed to nobody
     before it has passed the call."""
-    if stream is not None:
-        for t in tensors:
-            t.record_stream(stream)
+    for t in tensors:
+        t.record_stream(stream)
 
 
 def _out(out, rows, cols, dtype, like, device, stream):
@@ -152,7 +151,8 @@ def quantize(x, mode="nvfp4", tensor_scale=1.0, ctx=None, stream=None):
     scales = _empty((rows, k // BLOCK[mode]), torch.uint8, x, stream)
     rc = lib.aex_fp4_quantize(ctx.handle, x.data_ptr(), _DTYPES[x.dtype], x.stride(0) if rows > 1 else k, rows, k, fmt,
                               tensor_scale, codes.data_ptr(), scales.data_ptr(), _stream(stream, device))
-    _used(stream, x)
+    if stream is not None:
+        _used(stream, x)
     if rc:
         ctx.check(rc)
     return codes, scales
@@ -168,7 +168,8 @@ def dequantize(codes, scales, mode="nvfp4", tensor_scale=1.0, out_dtype=torch.bf
     rc = lib.aex_fp4_dequantize(ctx.handle, codes.data_ptr(), scales.data_ptr(), rows, k, fmt, tensor_scale,
                                 out.data_ptr(), _DTYPES[out.dtype], out.stride(0) if rows > 1 else k,
                                 _stream(stream, device))
-    _used(stream, codes, scales, out)
+    if stream is not None:
+        _used(stream, codes, scales, out)
     if rc:
         ctx.check(rc)
     return out
@@ -192,7 +193,8 @@ class FP4Weight:
                                                      self.k, fmt, tensor_scale, C.byref(h),
                                                      _stream(stream, self.index)))
         self.handle = h
-        _used(stream, codes, scales)
+        if stream is not None:
+            _used(stream, codes, scales)
 
     def close(self):
         if getattr(self, "handle", None):
@@ -251,7 +253,8 @@ def _product(x, w, w_up, activation, quantize_x, x_scale, out_dtype, out, stream
         rc = w.lib.aex_fp4_mm(w.ctx.handle, w.handle, a, _stream(stream, device))
     else:
         rc = w.lib.aex_fp4_gated_mm(w.ctx.handle, w.handle, w_up.handle, activation, a, _stream(stream, device))
-    _used(stream, x, out)
+    if stream is not None:
+        _used(stream, x, out)
     if rc:
         w.ctx.check(rc)
     return out
@@ -291,7 +294,8 @@ def fp4_mm_dgrad(dy, w: FP4Weight, out_dtype=torch.bfloat16, out=None, stream=No
     rc = w.lib.aex_fp4_mm_dgrad(w.ctx.handle, w.handle, dy.data_ptr(), _pitch(dy), m, out.data_ptr(),
                                 _DTYPES[out.dtype], out.stride(0) if m > 1 else w.k, ws.data_ptr() if n_ws else None,
                                 n_ws, _stream(stream, w.index))
-    _used(stream, dy, out)
+    if stream is not None:
+        _used(stream, dy, out)
     if rc:
         w.ctx.check(rc)
     return out
@@ -320,7 +324,8 @@ def fp4_gated_mm_dgrad(dh, x, w_gate: FP4Weight, w_up: FP4Weight, activation="si
                                       dh.data_ptr(), _pitch(dh), m, out.data_ptr(),
                                       out.stride(0) if m > 1 else w.k, ws.data_ptr(), n_ws,
                                       _stream(stream, w.index))
-    _used(stream, x, dh, out)
+    if stream is not None:
+        _used(stream, x, dh, out)
     if rc:
         w.ctx.check(rc)
     return out
